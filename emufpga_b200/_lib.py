@@ -21,6 +21,7 @@ STATUS = {
 
 # GGML dtypes
 F32, F16, Q8_0, Q2_K, Q5_K, Q6_K = 0, 1, 8, 10, 13, 14
+BF16 = 30  # activations of the serving operators
 BLOCK = {F32: (1, 4), F16: (1, 2), Q8_0: (32, 34), Q2_K: (256, 84), Q5_K: (256, 176), Q6_K: (256, 210)}
 
 # families
@@ -85,6 +86,13 @@ class SweepInfo(C.Structure):
     """spm_sweep_info (spmgpu.h)."""
     _fields_ = [("streams", C.c_int32), ("position", C.c_int32), ("host_bytes", C.c_uint64),
                 ("device_bytes", C.c_uint64), ("copies", C.c_uint64), ("bytes_copied", C.c_uint64)]
+
+
+class Kv8(C.Structure):
+    """spm_kv8 (spmgpu.h)."""
+    _fields_ = [("device", C.c_int32), ("pages", C.c_int32), ("page_tokens", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("pad_", C.c_int32), ("k_codes", C.c_void_p), ("v_codes", C.c_void_p),
+                ("k_scales", C.c_void_p), ("v_scales", C.c_void_p), ("status", C.c_void_p)]
 
 
 PROTOTYPES = {
@@ -160,6 +168,17 @@ PROTOTYPES = {
     "spm_sweep_rewind": (C.c_int32, [_P]),
     "spm_sweep_plan": (C.c_int32, [_U64P, C.c_int32, C.c_uint64, _I32P, C.c_int32, C.POINTER(C.c_int64),
                                    C.c_int64, C.POINTER(C.c_int64)]),
+    "spm_page_plan": (C.c_int32, [C.c_int, _P, _P, _P, C.c_int32, C.c_int32, _P, C.c_int32, _P, C.c_int32, _P, _P,
+                                  C.c_int32, _P, _P, _P, _P, _P, _P]),
+    "spm_kv8_append": (C.c_int32, [C.POINTER(Kv8), C.c_uint32, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64,
+                                   C.c_int32, _P, _P]),
+    "spm_kv8_values": (C.c_int32, [C.POINTER(Kv8), C.c_uint32, _P, C.c_int32, _P, _P, _P]),
+    "spm_kv8_attention_workspace": (C.c_int32, [C.POINTER(Kv8), C.c_int32, C.c_int32, C.c_int32, C.c_int32, _U64P]),
+    "spm_kv8_attention": (C.c_int32, [C.POINTER(Kv8), C.c_uint32, _P, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _P,
+                                      _P, C.c_int32, C.c_int32, _P, C.c_int32, C.c_float, _P, C.c_int64, C.c_int64,
+                                      _P, C.c_uint64, _P]),
+    "spm_sample": (C.c_int32, [C.c_int, C.c_uint32, _P, C.c_int64, C.c_int32, C.c_int32, _P, _P, _P, _P, _P, _P, _P,
+                               _P, _P]),
 }
 
 _lib: C.CDLL | None = None

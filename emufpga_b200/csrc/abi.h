@@ -43,4 +43,47 @@ struct DeviceBuf {
     ~DeviceBuf() { if (p) cudaFree(p); }
 };
 
+// Makes `device` current for the life of the object and then puts back the
+// caller's.  SPM_E_NO_DEVICE where no device is visible.
+struct DeviceScope {
+    int before = -1;
+    explicit DeviceScope(int device) {
+        int n = 0;
+        if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
+            cudaGetLastError();
+            fail(SPM_E_NO_DEVICE, "no CUDA device is visible");
+        }
+        if (device < 0 || device >= n) fail(SPM_E_ARG, "device index out of range");
+        CUDA_OK(cudaGetDevice(&before));
+        if (before != device) CUDA_OK(cudaSetDevice(device));
+        else before = -1;
+    }
+    DeviceScope(const DeviceScope&) = delete;
+    DeviceScope& operator=(const DeviceScope&) = delete;
+    ~DeviceScope() { if (before >= 0) cudaSetDevice(before); }
+};
+
+// The multiprocessors of the current device (asked for once per device).
+inline int device_sms() {
+    static int sms[64] = {};
+    int d = 0;
+    CUDA_OK(cudaGetDevice(&d));
+    if (d < 64 && sms[d]) return sms[d];
+    int v = 0;
+    CUDA_OK(cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, d));
+    if (d < 64) sms[d] = v;
+    return v;
+}
+
+// Raises a kernel's dynamic shared memory limit on the current device, once
+// per device (`done` is the kernel's own bit per device).
+template <class K>
+void allow_smem(K kernel, size_t bytes, unsigned long long& done) {
+    int d = 0;
+    CUDA_OK(cudaGetDevice(&d));
+    if (d < 64 && (done >> d & 1)) return;
+    CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+    if (d < 64) done |= 1ull << d;
+}
+
 }  // namespace spm

@@ -1,0 +1,624 @@
+// Attention over the paged 8-bit KV cache (spm_kv8_attention), for decode ticks
+// and few queries per request.
+//
+// Per query row and kv head:  s_j = c 2^(e_j) (q . K_j),  c = scale log2(e),
+// out = sum_j 2^(s_j - m) 2^(f_j) V_j / sum_j 2^(s_j - m), with K_j, V_j the int8
+// codes and 2^(e_j), 2^(f_j) the scales of key j's page.  One pass with running
+// references, all integers, so that every rescaling is a power of two and exact:
+// m = ceil(max s) for the sum, and r = max(ceil(max s in a page's 16 rows) + f)
+// for the accumulator, which then holds sum_j 2^(s_j + f_j - r) V_j with every
+// weight at most 1: it fits fp16 whatever the pages' scales are.
+//
+// Products on the tensor cores (mma.sync m16n8k16, fp16 in, fp32 out): int8 codes
+// are exact in fp16.  Queries are scaled per row to 2^10 and split into fp16 high
+// and low parts where they are f32 (22 bits; one part holds a bf16 or f16), the
+// weights likewise.  The 16 rows of an mma are cached tokens (or, for the values,
+// head dimensions) and its 8 columns are query rows (tokens x heads of the group),
+// so that one conversion of the codes serves every query of a kv head:
+//   codes: ldmatrix brings 4 bytes of a row to each lane; byte permutes make
+//   0x6400 | (code + 128) = 1024 + 128 + code in fp16, and one subtraction of 1152
+//   the code.  The order of dimensions within an mma's k is free, so the queries
+//   are laid out to match the bytes; for the values (transposed by ldmatrix) the
+//   even and odd dimensions of a 16-byte column become rows g and g + 8.
+//
+// What bounds it is the cache's bytes.  Each warp streams its own 32 tokens at a
+// time through a ring in shared memory (16-byte asynchronous copies, no barrier
+// among warps).  Work is cut into units of 128 tokens of a (row tile, kv head),
+// and every CTA takes an equal run of the units of all requests, so that ragged
+// lengths load all SMs alike; where a run ends inside a (row tile, kv head) its
+// partial goes to the workspace and kv8_combine_kernel adds the parts in order.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "kv8.h"
+#include "kv8_attention.h"
+
+namespace spm {
+namespace {
+using namespace dev;
+
+constexpr int kDecThreads = 32 * kDecWarps;
+
+__device__ __forceinline__ void ldsm4(uint32_t (&a)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&a)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Bytes of x (already + 128) picked by SEL, as two fp16 codes.
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t codes2(uint32_t x) {
+    const uint32_t u = __byte_perm(x, 0x64646464u, SEL);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 half2_floats(uint32_t b) { return __half22float2(*reinterpret_cast<const __half2*>(&b)); }
+__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(saddr(dst)), "l"(src) : "memory");
+}
+// 2^(to - from) for integer-valued references; 0 where there was none yet.
+__device__ __forceinline__ float step_down(float from, float to) {
+    return from == -INFINITY ? 0.f : pow2i(int(fmaxf(from - to, -126.f)));
+}
+
+// The exponent of a scale (a power of two); -inf for 0, NaN for NaN.
+__device__ __forceinline__ float exponent_of(float s) {
+    return s > 0.f ? float((__float_as_int(s) >> 23) - 127) : s == 0.f ? -INFINITY : __int_as_float(0x7fffffff);
+}
+
+template <int HD, int NT, int NP>
+struct DecSmem {
+    // a token's codes: the eight rows that an ldmatrix reads lie on distinct banks,
+    // by an exclusive or of the 16-byte chunk with the row where a row fills whole
+    // bank sweeps, else by 16 bytes between the rows
+    static constexpr bool swizzled = HD == 64 || HD % 128 == 0;
+    static constexpr int row = swizzled ? HD : HD + 16;
+    static __device__ __forceinline__ int at(int r, int chunk) {
+        if (HD == 64) return r * row + ((chunk ^ ((r >> 1) & 3)) << 4);
+        if (HD % 128 == 0) return r * row + ((chunk ^ (r & 7)) << 4);
+        return r * row + (chunk << 4);
+    }
+    // CTAs that an SM's shared memory takes
+    static constexpr int per_sm() { return total * 2 + 2048 <= 227 * 1024 ? 2 : 1; }
+    static constexpr int stage = 2 * kDecSub * row + 16;      // keys, values, then 2 + 2 scales
+    static constexpr int q = 0;                               // [NP][NT][HD / 16][32 lanes][4 halves]
+    static constexpr int qbytes = NP * NT * HD * 16;
+    static constexpr int qscale = q + qbytes;                 // [8 NT] floats
+    static constexpr int ring = (qscale + 8 * NT * 4 + 15) & ~15;
+    static constexpr int state = HD + 4;                      // a row's accumulator, then m, r, l
+    static constexpr int ring_bytes = kDecWarps * kDecStages * stage;
+    static constexpr int state_bytes = kDecWarps * 8 * NT * state * 4;
+    static constexpr int total = ring + (ring_bytes > state_bytes ? ring_bytes : state_bytes);
+};
+
+template <int HD, int NT, int NP>
+__global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a) {
+    using L = DecSmem<HD, NT, NP>;
+    constexpr int NR = 8 * NT, KB = HD / 32;
+    extern __shared__ __align__(128) uint8_t sm[];
+    __shared__ long long wsum[kDecWarps], found[2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int V = a.requests * a.tiles;  // (request, row tile) pairs
+
+    // ---- this CTA's run of units ----
+    auto block_scan = [&](long long x, long long& before) {  // exclusive sum over threads, and the total
+        long long v = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long n = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += n;
+        }
+        __syncthreads();
+        if (lane == 31) wsum[warp] = v;
+        __syncthreads();
+        before = v - x;
+        long long total = 0;
+#pragma unroll
+        for (int w = 0; w < kDecWarps; w++) {
+            if (w < warp) before += wsum[w];
+            total += wsum[w];
+        }
+        return total;
+    };
+    long long total = 0;
+    for (int v0 = 0; v0 < V; v0 += kDecThreads) {
+        long long before;
+        const int v = v0 + tid;
+        const long long n = v < V ? (long long)kv8_units(a, v) * a.kv_heads : 0;
+        const long long sum = block_scan(n, before);
+        if (blockIdx.x == 0 && v < V) a.prefix[v] = total + before;
+        total += sum;
+    }
+    if (blockIdx.x == 0 && tid == 0) a.prefix[V] = total;
+    const long long share = (total + gridDim.x - 1) / gridDim.x;
+    const long long begin = min(total, share * (long long)blockIdx.x), end = min(total, begin + share);
+    if (begin >= end) return;
+    {
+        long long run = 0;
+        for (int v0 = 0; v0 < V; v0 += kDecThreads) {
+            long long before;
+            const int v = v0 + tid;
+        const long long n = v < V ? (long long)kv8_units(a, v) * a.kv_heads : 0;
+            const long long sum = block_scan(n, before);
+            if (n && run + before <= begin && begin < run + before + n) found[0] = v, found[1] = run + before;
+            run += sum;
+            if (run > begin) break;
+        }
+        __syncthreads();
+    }
+    int v = int(found[0]);
+    long long base = found[1], u = begin;  // base: the first unit of pair v
+
+    const int lrow = (lane & 7) + 8 * ((lane >> 3) & 1), lchunk = lane >> 4;  // this lane's ldmatrix row
+    uint8_t* ring = sm + L::ring + warp * kDecStages * L::stage;
+    float* qscale = reinterpret_cast<float*>(sm + L::qscale);
+    for (int piece = 0; u < end; piece++) {
+        int nu = kv8_units(a, v);
+        while (u >= base + (long long)nu * a.kv_heads) {
+            base += (long long)nu * a.kv_heads;
+            v++;
+            nu = kv8_units(a, v);
+        }
+        const int req = v / a.tiles, tile = v % a.tiles;
+        const int head = int((u - base) / nu), unit0 = int((u - base) % nu);
+        const int units = int(min((long long)(nu - unit0), end - u));
+        const int s0 = a.starts[req], nq = a.starts[req + 1] - s0, len = kv8_len(a, req);
+        const int row0 = tile * NR, rows = min(NR, nq * a.group - row0);
+        const int keys = kv8_keys(a, nq, len, tile);
+        const int k0 = unit0 * kDecUnit, k1 = min(keys, (unit0 + units) * kDecUnit);
+        u += units;
+        __syncthreads();  // the ring and the queries of the piece before are done with
+
+        // ---- tokens k0 .. k1 - 1, 32 at a time in turn among the warps ----
+        const int steps = max(0, (k1 - k0 - kDecSub * warp + kDecUnit - 1) / kDecUnit);
+        const int32_t* trow = a.table + size_t(req) * a.width;
+        auto page_of = [&](int j) {  // lanes 0, 1: the pages of step j's two blocks of 16 tokens
+            const int tok = k0 + kDecSub * (warp + kDecWarps * j) + 16 * (lane & 1);
+            int p = 0;
+            if (j < steps && tok < k1) {
+                p = __ldg(trow + (tok >> a.shift));
+                if (uint32_t(p) >= uint32_t(a.pages)) {
+                    flag(a.status, SPM_PAGE_ID);
+                    p = a.pages ? 0 : -1;
+                }
+            }
+            return p;
+        };
+        auto issue = [&](int j, int mine) {
+            if (j < steps) {
+                uint8_t* st = ring + (j % kDecStages) * L::stage;
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const int tok = k0 + kDecSub * (warp + kDecWarps * j) + 16 * b;
+                    const int p = __shfl_sync(0xffffffffu, mine, b);
+                    if (tok >= k1 || p < 0) continue;
+                    const size_t at = size_t(p) * a.kv_heads + head;
+                    const size_t from = (at * a.page + (tok & (a.page - 1))) * HD;
+#pragma unroll
+                    for (int i = 0; i < HD / 32; i++) {
+                        const int c = lane + 32 * i, r = c / (HD / 16), o = c % (HD / 16);
+                        cp_async16(st + L::at(16 * b + r, o), a.k_codes + from + 16 * c);
+                        cp_async16(st + kDecSub * L::row + L::at(16 * b + r, o), a.v_codes + from + 16 * c);
+                    }
+                    if (lane == 0) cp_async4(st + 2 * kDecSub * L::row + 4 * b, a.k_scales + at);
+                    if (lane == 1) cp_async4(st + 2 * kDecSub * L::row + 8 + 4 * b, a.v_scales + at);
+                }
+            }
+            cp_async_commit();
+        };
+        int ahead = page_of(0);
+#pragma unroll
+        for (int j = 0; j < kDecStages - 1; j++) {
+            const int next = page_of(j + 1);
+            issue(j, ahead);
+            ahead = next;
+        }
+
+        // ---- the queries, split into fp16 parts in the order of the codes' bytes ----
+        for (int r = warp; r < NR; r += kDecWarps) {
+            float x[HD / 32];
+            uint32_t big = 0;
+            const int qr = row0 + r, qi = qr / a.group, qh = head * a.group + qr % a.group;
+#pragma unroll
+            for (int i = 0; i < HD / 32; i++) {
+                x[i] = r < rows ? kv8_load(a, int64_t(s0 + qi) * a.q_token + qh * a.q_head + lane + 32 * i) : 0.f;
+                big = max(big, __float_as_uint(x[i]) & 0x7fffffffu);
+            }
+            big = __reduce_max_sync(0xffffffffu, big);
+            // to 2^10 .. 2^11; as it is where nothing or infinity stands there
+            const int up = big >= 0x00800000u && big < 0x7f800000u ? min(137 - int(big >> 23), 126) : 0;
+            const float mul = pow2i(up);
+            if (lane == 0) qscale[r] = a.scale_log2 * pow2i(-up);
+            __half* dst = reinterpret_cast<__half*>(sm + L::q);
+#pragma unroll
+            for (int i = 0; i < HD / 32; i++) {
+                const int d = lane + 32 * i, blk = d >> 4, tt = (d >> 2) & 3;
+                const float y = __fmul_rn(x[i], mul);
+                const __half hi = __float2half_rn(y);
+                const int at = (((r >> 3) * (HD / 16) + blk) * 32 + (r & 7) * 4 + tt) * 4 + (d & 3);
+                dst[at] = hi;
+                if (NP == 2) dst[NT * (HD / 16) * 128 + at] = __float2half_rn(__fsub_rn(y, __half2float(hi)));
+            }
+        }
+        __syncthreads();
+
+        float o[HD / 16][NT][4], m_run[NT][2], r_run[NT][2], l_run[NT][2], qs[NT][2];
+        int limit[NT][2];  // keys that the lane's columns see
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                m_run[n][c] = r_run[n][c] = -INFINITY;
+                l_run[n][c] = 0.f;
+                const int r = 8 * n + 2 * t + c;
+                qs[n][c] = qscale[r];
+                limit[n][c] = r < rows ? len - nq + (row0 + r) / a.group + 1 : 0;
+#pragma unroll
+                for (int d = 0; d < HD / 16; d++) o[d][n][c] = o[d][n][c + 2] = 0.f;
+            }
+        for (int j = 0; j < steps; j++) {
+            const int next = page_of(j + kDecStages);
+            issue(j + kDecStages - 1, ahead);
+            ahead = next;
+            cp_async_wait<kDecStages - 1>();
+            __syncwarp();
+            const uint8_t* st = ring + (j % kDecStages) * L::stage;
+            const uint32_t kb = saddr(st), vb = kb + kDecSub * L::row;
+            const float* scales = reinterpret_cast<const float*>(st + 2 * kDecSub * L::row);
+            const int tok0 = k0 + kDecSub * (warp + kDecWarps * j);
+            const bool two = tok0 + 16 < k1;  // the second block holds tokens
+            float s[2][NT][4];
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) s[b][n][0] = s[b][n][1] = s[b][n][2] = s[b][n][3] = 0.f;
+#pragma unroll
+            for (int d = 0; d < KB; d++) {
+                uint2 q[NP][NT][2];
+#pragma unroll
+                for (int p = 0; p < NP; p++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+                            q[p][n][e] = *reinterpret_cast<const uint2*>(
+                                sm + L::q + (((p * NT + n) * (HD / 16) + 2 * d + e) * 32 + lane) * 8);
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    if (b && !two) break;
+                    uint32_t x[4];
+                    ldsm4(x, kb + b * 16 * L::row + L::at(lrow, lchunk + 2 * d));
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const uint32_t lo = x[2 * e] ^ 0x80808080u, hi = x[2 * e + 1] ^ 0x80808080u;
+                        const uint32_t a0 = codes2<0x4140>(lo), a1 = codes2<0x4140>(hi), a2 = codes2<0x4342>(lo),
+                                       a3 = codes2<0x4342>(hi);
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+#pragma unroll
+                            for (int p = NP - 1; p >= 0; p--) mma_f16(s[b][n], a0, a1, a2, a3, q[p][n][e].x, q[p][n][e].y);
+                    }
+                }
+            }
+            // ---- softmax: s[b][n][0, 1] token 16 b + g, columns 2t, 2t + 1; [2, 3] token + 8 ----
+            uint32_t w[2][NT][NP][2];  // weights as B operands
+            const float ve[2] = {exponent_of(scales[2]), two ? exponent_of(scales[3]) : -INFINITY};
+            const float ks[2] = {scales[0], two ? scales[1] : 0.f};
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                float top[2][2];
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        const int tok = tok0 + 16 * b + g;
+                        const float f = ks[b] * qs[n][c];
+                        s[b][n][c] = tok < limit[n][c] && tok < k1 ? s[b][n][c] * f : -INFINITY;
+                        s[b][n][c + 2] = tok + 8 < limit[n][c] && tok + 8 < k1 ? s[b][n][c + 2] * f : -INFINITY;
+                        top[b][c] = fmaxf(s[b][n][c], s[b][n][c + 2]);
+                    }
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1)
+#pragma unroll
+                    for (int b = 0; b < 2; b++)
+#pragma unroll
+                        for (int c = 0; c < 2; c++) top[b][c] = fmaxf(top[b][c], __shfl_xor_sync(0xffffffffu, top[b][c], x));
+                float down[2];
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const float t0 = ceilf(top[0][c]), t1 = ceilf(top[1][c]);
+                    const float m = fmaxf(m_run[n][c], fmaxf(t0, t1));
+                    const float r = fmaxf(r_run[n][c], fmaxf(t0 + ve[0], t1 + ve[1]));
+                    l_run[n][c] *= step_down(m_run[n][c], m);
+                    down[c] = step_down(r_run[n][c], r);
+                    m_run[n][c] = m;
+                    r_run[n][c] = r;
+                    const float m0 = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                    for (int b = 0; b < 2; b++) {
+                        // 2^(m + f - r), at least 0 where the page's values are all zero
+                        const float f = ve[b] != ve[b] ? ve[b]
+                                        : ve[b] == -INFINITY || r == -INFINITY ? 0.f
+                                        : pow2i(int(fminf(fmaxf(m0 + ve[b] - r, -126.f), 126.f)));
+#pragma unroll
+                        for (int e = c; e < 4; e += 2) {
+                            const float p = exp2f(s[b][n][e] - m0);
+                            l_run[n][c] += p;
+                            // (a masked key adds nothing even to a page of NaN)
+                            s[b][n][e] = s[b][n][e] == -INFINITY ? 0.f : p * f;
+                        }
+                    }
+                }
+                if (__any_sync(0xffffffffu, down[0] != 1.f || down[1] != 1.f)) {
+#pragma unroll
+                    for (int d = 0; d < HD / 16; d++) {
+                        o[d][n][0] *= down[0];
+                        o[d][n][1] *= down[1];
+                        o[d][n][2] *= down[0];
+                        o[d][n][3] *= down[1];
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const uint32_t hi = half2_bits(s[b][n][2 * e], s[b][n][2 * e + 1]);
+                        w[b][n][0][e] = transposed(hi);
+                        if (NP == 2) {
+                            const float2 h = half2_floats(hi);
+                            w[b][n][NP - 1][e] = transposed(half2_bits(s[b][n][2 * e] - h.x, s[b][n][2 * e + 1] - h.y));
+                        }
+                    }
+            }
+            // ---- values ----
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                if (b && !two) break;
+#pragma unroll
+                for (int d = 0; d < KB; d++) {
+                    uint32_t x[4];
+                    ldsm4t(x, vb + b * 16 * L::row + L::at(lrow, lchunk + 2 * d));
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const uint32_t lo = x[2 * e] ^ 0x80808080u, hi = x[2 * e + 1] ^ 0x80808080u;
+                        const uint32_t a0 = codes2<0x4240>(lo), a1 = codes2<0x4341>(lo), a2 = codes2<0x4240>(hi),
+                                       a3 = codes2<0x4341>(hi);
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+#pragma unroll
+                            for (int p = NP - 1; p >= 0; p--)
+                                mma_f16(o[2 * d + e][n], a0, a1, a2, a3, w[b][n][p][0], w[b][n][p][1]);
+                    }
+                }
+            }
+            __syncwarp();
+        }
+        cp_async_wait<0>();
+        __syncthreads();
+        // ---- the warps' states through shared memory, added in warp order ----
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l_run[n][c] += __shfl_xor_sync(0xffffffffu, l_run[n][c], x);
+                float* st = reinterpret_cast<float*>(sm + L::ring) + (warp * NR + 8 * n + 2 * t + c) * L::state;
+#pragma unroll
+                for (int d = 0; d < HD / 16; d++) {
+                    st[16 * d + 2 * g] = o[d][n][c];
+                    st[16 * d + 2 * g + 1] = o[d][n][c + 2];
+                }
+                if (g == 0) {
+                    st[HD] = m_run[n][c];
+                    st[HD + 1] = r_run[n][c];
+                    st[HD + 2] = l_run[n][c];
+                }
+            }
+        __syncthreads();
+        const bool whole = units == nu;
+        // the run's first piece may be a pair's tail or middle, its last one a pair's head
+        float* part = a.parts + size_t(2 * blockIdx.x + (piece ? 1 : 0)) * NR * (HD + 4);
+        for (int e = tid; e < rows * HD; e += kDecThreads) {
+            const int r = e / HD, d = e % HD;
+            const float* st = reinterpret_cast<const float*>(sm + L::ring) + r * L::state;
+            float m = -INFINITY, ref = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < kDecWarps; x++) {
+                m = fmaxf(m, st[x * NR * L::state + HD]);
+                ref = fmaxf(ref, st[x * NR * L::state + HD + 1]);
+            }
+            float sum = 0.f, acc = 0.f;
+#pragma unroll
+            for (int x = 0; x < kDecWarps; x++) {
+                const float* sx = st + x * NR * L::state;
+                sum = fmaf(sx[HD + 2], step_down(sx[HD], m), sum);
+                acc = fmaf(sx[d], step_down(sx[HD + 1], ref), acc);
+            }
+            if (whole) {
+                const int qr = row0 + r, qi = qr / a.group, qh = head * a.group + qr % a.group;
+                kv8_store(a, int64_t(s0 + qi) * a.o_token + qh * a.o_head + d, kv8_finish(acc, ref, sum, m));
+            } else {
+                part[r * (HD + 4) + d] = acc;
+                if (d == 0) {
+                    part[r * (HD + 4) + HD] = m;
+                    part[r * (HD + 4) + HD + 1] = ref;
+                    part[r * (HD + 4) + HD + 2] = sum;
+                }
+            }
+        }
+    }
+}
+
+// Adds the parts of every (row tile, kv head) that the runs cut, in the order of
+// the runs: the part of run c is its second where the pair begins in it after
+// another (or after its own first piece), else its first.
+template <int NR>
+__global__ void __launch_bounds__(128) kv8_combine_kernel(const Kv8Args a, int grid, int hd) {
+    pdl_wait();
+    const int v = blockIdx.x, head = blockIdx.y, V = a.requests * a.tiles;
+    const long long p0 = a.prefix[v], p1 = a.prefix[v + 1], total = a.prefix[V];
+    const int nu = int((p1 - p0) / a.kv_heads);
+    if (nu == 0) return;
+    const long long share = (total + grid - 1) / grid, u0 = p0 + (long long)head * nu, u1 = u0 + nu;
+    const int c0 = int(u0 / share), c1 = int((u1 - 1) / share);
+    if (c0 == c1) return;  // one run held all of it and wrote the result
+    const int req = v / a.tiles, s0 = a.starts[req], nq = a.starts[req + 1] - s0, row0 = (v % a.tiles) * NR;
+    const int rows = min(NR, nq * a.group - row0), W = hd + 4;
+    auto part = [&](int c) {
+        const int second = u0 > share * c ? 1 : 0;
+        return a.parts + size_t(2 * c + second) * NR * W;
+    };
+    for (int e = threadIdx.x; e < rows * hd; e += 128) {
+        const int r = e / hd, d = e % hd;
+        float m = -INFINITY, ref = -INFINITY, sum = 0.f, acc = 0.f;
+        for (int c = c0; c <= c1; c++) {
+            const float* p = part(c) + r * W;
+            m = fmaxf(m, p[hd]);
+            ref = fmaxf(ref, p[hd + 1]);
+        }
+        for (int c = c0; c <= c1; c++) {
+            const float* p = part(c) + r * W;
+            sum = fmaf(p[hd + 2], step_down(p[hd], m), sum);
+            acc = fmaf(p[d], step_down(p[hd + 1], ref), acc);
+        }
+        const int qr = row0 + r, qi = qr / a.group, qh = head * a.group + qr % a.group;
+        kv8_store(a, int64_t(s0 + qi) * a.o_token + qh * a.o_head + d, kv8_finish(acc, ref, sum, m));
+    }
+}
+
+template <int HD, int NT, int NP>
+void launch_decode(const Kv8Args& a, int grid, cudaStream_t st) {
+    constexpr int smem = DecSmem<HD, NT, NP>::total;
+    static_assert(smem <= 227 * 1024, "a CTA's shared memory");
+    static_assert(DecSmem<HD, NT, NP>::per_sm() == (HD <= 128 ? 2 : 1), "plan_of's grid");
+    static unsigned long long done = 0;
+    allow_smem(kv8_decode_kernel<HD, NT, NP>, smem, done);
+    kv8_decode_kernel<HD, NT, NP><<<grid, kDecThreads, smem, st>>>(a);
+    CUDA_OK(cudaGetLastError());
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(a.requests * a.tiles), unsigned(a.kv_heads));
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    CUDA_OK(cudaLaunchKernelEx(&cfg, kv8_combine_kernel<8 * NT>, a, grid, HD));
+}
+
+template <int HD>
+void launch_dim(const Kv8Args& a, int nt, bool two, int grid, cudaStream_t st) {
+    if (nt == 1) two ? launch_decode<HD, 1, 2>(a, grid, st) : launch_decode<HD, 1, 1>(a, grid, st);
+    else two ? launch_decode<HD, 2, 2>(a, grid, st) : launch_decode<HD, 2, 1>(a, grid, st);
+}
+
+// How a call is cut, from what the host knows of it.
+struct Plan {
+    int nt, tiles, grid;
+    uint64_t prefix_bytes, parts_bytes;
+};
+
+Plan plan_of(const spm_kv8* c, int heads, int requests, int most, int width) {
+    Plan p;
+    const int sms = 148;  // of a B200; the grid need not match the device's for the result
+    const int group = heads / c->kv_heads;
+    const int64_t rows = int64_t(std::max(most, 1)) * group;
+    p.nt = rows <= 8 ? 1 : 2;
+    p.tiles = int((rows + 8 * p.nt - 1) / (8 * p.nt));
+    const int64_t pairs = int64_t(requests) * p.tiles;
+    if (pairs > INT32_MAX) fail(SPM_E_ARG, "too many requests and queries for one call");
+    const int per_sm = c->head_dim <= 128 ? 2 : 1;  // DecSmem's per_sm
+    const int64_t units = (int64_t(width) * c->page_tokens + kDecUnit - 1) / kDecUnit;
+    if (units * pairs > INT64_MAX / 65536) fail(SPM_E_ARG, "too many requests and queries for one call");
+    p.grid = int(std::max<int64_t>(1, std::min<int64_t>(int64_t(per_sm) * sms, std::max<int64_t>(units, 1) * pairs * c->kv_heads)));
+    p.prefix_bytes = (uint64_t(pairs + 1) * 8 + 15) & ~uint64_t(15);
+    p.parts_bytes = uint64_t(p.grid) * 2 * 8 * p.nt * (c->head_dim + 4) * 4;
+    return p;
+}
+
+void check_attention(const spm_kv8* c, int32_t heads, int32_t requests, int32_t most, int32_t width) {
+    kv8_check(c);
+    if (heads < 1 || heads % c->kv_heads) fail(SPM_E_ARG, "heads must be a multiple of kv_heads");
+    if (requests < 0 || most < 0 || width < 0) fail(SPM_E_ARG, "negative size");
+    if (int64_t(width) * c->page_tokens > INT32_MAX) fail(SPM_E_ARG, "positions are 32-bit: table_width * page_tokens must fit");
+    if (int64_t(most) * (heads / c->kv_heads) > INT32_MAX) fail(SPM_E_ARG, "too many queries");
+    if (c->kv_heads > 65535) fail(SPM_E_ARG, "too many kv heads");
+}
+
+}  // namespace
+}  // namespace spm
+
+using namespace spm;
+
+spm_status spm_kv8_attention_workspace(const spm_kv8* c, int32_t heads, int32_t requests, int32_t most,
+                                       int32_t table_width, uint64_t* bytes) {
+    return guarded([&] {
+        if (!bytes) fail(SPM_E_ARG, "null output");
+        check_attention(c, heads, requests, most, table_width);
+        const Plan p = plan_of(c, heads, requests, most, table_width);
+        *bytes = p.prefix_bytes + p.parts_bytes;
+    });
+}
+
+spm_status spm_kv8_attention(const spm_kv8* c, uint32_t dtype, const void* q, int64_t q_token, int64_t q_head,
+                             int32_t heads, int32_t rows, const int32_t* starts, const int32_t* lens,
+                             int32_t requests, int32_t most, const int32_t* table, int32_t table_width, float scale,
+                             void* out, int64_t out_token, int64_t out_head, void* workspace,
+                             uint64_t workspace_bytes, void* cuda_stream) {
+    return guarded([&] {
+        check_attention(c, heads, requests, most, table_width);
+        kv8_check_type(dtype);
+        if (rows < 0) fail(SPM_E_ARG, "negative row count");
+        if (requests == 0 || rows == 0 || most == 0) return;
+        if (!q || !out || !starts || !lens || (table_width && !table)) fail(SPM_E_ARG, "null argument");
+        const Plan p = plan_of(c, heads, requests, most, table_width);
+        if (!workspace || workspace_bytes < p.prefix_bytes + p.parts_bytes)
+            fail(SPM_E_ARG, "the workspace is smaller than spm_kv8_attention_workspace says");
+        if (reinterpret_cast<uintptr_t>(workspace) & 15) fail(SPM_E_ARG, "the workspace must be 16-byte aligned");
+        DeviceScope scope(c->device);
+        Kv8Args a{};
+        a.k_codes = c->k_codes, a.v_codes = c->v_codes;
+        a.k_scales = c->k_scales, a.v_scales = c->v_scales;
+        a.pages = c->pages, a.page = c->page_tokens, a.shift = __builtin_ctz(unsigned(c->page_tokens));
+        a.kv_heads = c->kv_heads, a.group = heads / c->kv_heads;
+        a.q = q, a.q_token = q_token, a.q_head = q_head, a.dtype = dtype, a.rows = rows;
+        a.starts = starts, a.lens = lens, a.requests = requests, a.most = most;
+        a.table = table, a.width = table_width, a.tile_rows = 8 * p.nt, a.tiles = p.tiles;
+        a.scale_log2 = float(double(scale) * 1.4426950408889634);
+        a.out = out, a.o_token = out_token, a.o_head = out_head;
+        a.prefix = static_cast<long long*>(workspace);
+        a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.prefix_bytes);
+        a.status = c->status;
+        const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+        const bool two = dtype == SPM_F32;
+        switch (c->head_dim) {
+            case 64: launch_dim<64>(a, p.nt, two, p.grid, st); break;
+            case 96: launch_dim<96>(a, p.nt, two, p.grid, st); break;
+            case 128: launch_dim<128>(a, p.nt, two, p.grid, st); break;
+            case 192: launch_dim<192>(a, p.nt, two, p.grid, st); break;
+            default: launch_dim<256>(a, p.nt, two, p.grid, st); break;
+        }
+    });
+}

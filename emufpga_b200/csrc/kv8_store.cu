@@ -1,0 +1,287 @@
+// Storing into the paged 8-bit KV cache (spm_kv8_append) and reading whole
+// pages back (spm_kv8_values).
+//
+// A (page, kv head) has one scale 2^e, the smallest with |x| <= 127 * 2^e over
+// the values written.  A power of two rather than amax / 127: x / scale, code *
+// scale and the rescaling of rows that are already there when e grows are then
+// exact up to the one rounding to an integer, so a page that is filled a token
+// at a time, its scale growing on the way, is never more than one step
+// (half + quarter + ...) away from its values, and a code is the same whatever
+// order sums run in.  It costs less than one of the eight bits.
+//
+// Bound: bytes (rows in, one byte a value out) for prompts; launch latency for
+// a decode tick.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "kv8.h"
+
+namespace spm {
+namespace {
+using namespace dev;
+
+constexpr int kStoreThreads = 256, kStoreWarps = kStoreThreads / 32;
+constexpr int kStoreWindow = 64;  // at most: tokens whose runs begin in a CTA's window
+
+struct StoreArgs {
+    const void* x[2];         // keys, values
+    int64_t token[2], head[2];
+    int8_t* codes[2];
+    float* scales[2];
+    int32_t pages, page, shift, kv_heads, dim;
+    const int32_t* slots;
+    int32_t tokens, window;
+    int32_t* status;
+    bool vec;                 // four elements at a time: strides and bases allow it
+};
+
+// Four consecutive elements of a row as f32.
+template <class T>
+__device__ __forceinline__ void load4(const T* p, bool vec, float (&v)[4]) {
+    if (vec) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 q = *reinterpret_cast<const float4*>(p);
+            v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+        } else {
+            const uint2 q = *reinterpret_cast<const uint2*>(p);
+            const T* h = reinterpret_cast<const T*>(&q);
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = to_f32(h[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = to_f32(p[j]);
+    }
+}
+
+__device__ __forceinline__ uint32_t code_of(float x, float inv) {
+    // rounds half to even; NaN (a value or scale that is not finite) is 0
+    return uint32_t(min(max(__float2int_rn(__fmul_rn(x, inv)), -127), 127)) & 0xffu;
+}
+
+// The smallest 2^e with amax <= 127 * 2^e, as amax's bits give it: amax =
+// m * 2^x with m in [1, 2) lies at or under 127 * 2^(x - 6) iff m <= 127/64.
+// 0 for no value but zeros, NaN where a value is not finite.
+__device__ __forceinline__ float scale_of(uint32_t amax) {
+    if (amax == 0) return 0.f;
+    if (amax >= 0x7f800000u) return __int_as_float(0x7fffffff);
+    const int x = int(amax >> 23) - 127;  // -127 for subnormals, which the clamp covers
+    return pow2i(x - 6 + ((amax & 0x7fffffu) > 0x7e0000u ? 1 : 0));
+}
+
+// Grid (window of tokens, kv head, keys or values).  A run is the tokens of
+// one page that follow one another in the call; a CTA takes the runs that begin
+// in its window, whose last may reach up to a page beyond it.
+template <class T>
+__global__ void __launch_bounds__(kStoreThreads) kv8_append_kernel(const StoreArgs a) {
+    __shared__ int32_t slot[kStoreWindow + 256];
+    __shared__ int16_t lead[kStoreWindow + 256];   // the first token of a token's run, within the window
+    __shared__ uint32_t amax[kStoreWindow];
+    __shared__ float inv[kStoreWindow], ratio[kStoreWindow];
+    __shared__ int own;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int w0 = blockIdx.x * a.window, h = blockIdx.y, kv = blockIdx.z;
+    const int P = a.page, D = a.dim;
+    const int win = min(a.window, a.tokens - w0), span = min(a.tokens - w0, win + P - 1);
+    for (int i = tid; i < span; i += kStoreThreads) slot[i] = a.slots[w0 + i];
+    if (tid < win) amax[tid] = 0;
+    __syncthreads();
+    if (warp == 0) {
+        int carry = -1, end = span;
+        for (int i0 = 0; i0 < end; i0 += 32) {
+            const int i = i0 + lane;
+            bool first = false;
+            if (i < span) {
+                const int s = slot[i], before = i ? slot[i - 1] : w0 ? a.slots[w0 - 1] : -2;
+                first = s < 0 || before < 0 || s != before + 1 || (s & (P - 1)) == 0;
+            }
+            const uint32_t m = __ballot_sync(0xffffffffu, first);
+            const uint32_t upto = m & (0xffffffffu >> (31 - lane));
+            const int l = upto ? i0 + 31 - __clz(upto) : carry;
+            if (i < span) lead[i] = int16_t(l);
+            // runs that begin behind the window are the next CTAs'
+            const uint32_t past = m & (i0 >= win ? 0xffffffffu : i0 + 32 <= win ? 0u : 0xffffffffu << (win - i0));
+            if (past) end = i0 + __ffs(past) - 1;
+            if (m) carry = i0 + 31 - __clz(m);
+        }
+        if (lane == 0) own = end;
+    }
+    __syncthreads();
+    const int n = own;
+    const uint32_t limit = uint32_t(a.pages) * uint32_t(P);
+    const T* x = static_cast<const T*>(a.x[kv]) + h * a.head[kv];
+    const int64_t stride = a.token[kv];
+    int8_t* codes = a.codes[kv];
+    float* scales = a.scales[kv];
+    for (int i = warp; i < n; i += kStoreWarps) {
+        const int l = lead[i], s = slot[i];
+        if (l < 0 || uint32_t(s) >= limit) {
+            if (l >= 0 && s != -1 && lane == 0) flag(a.status, SPM_PAGE_ID);
+            continue;
+        }
+        const T* row = x + (w0 + i) * stride;
+        uint32_t m = 0;
+        for (int c = 4 * lane; c < D; c += 128) {
+            float v[4];
+            load4(row + c, a.vec, v);
+#pragma unroll
+            for (int j = 0; j < 4; j++) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+        }
+        m = __reduce_max_sync(0xffffffffu, m);
+        if (lane == 0) atomicMax(&amax[l], m);
+    }
+    __syncthreads();
+    if (tid < win) {
+        inv[tid] = ratio[tid] = 0.f;
+        const int s = slot[tid];
+        if (lead[tid] == tid && uint32_t(s) < limit) {
+            float* p = scales + size_t(s >> a.shift) * a.kv_heads + h;
+            float sc = scale_of(amax[tid]);
+            if (s & (P - 1)) {
+                const float was = *p;
+                if (!(was == was)) sc = was;            // NaN stays
+                else if (was > sc) sc = was;
+                else if (was > 0.f && sc > was) ratio[tid] = __fdiv_rn(was, sc);
+            }
+            *p = sc;
+            inv[tid] = sc > 0.f ? __fdiv_rn(1.f, sc) : 0.f;
+        }
+    }
+    __syncthreads();
+    // rows that were there, where the scale has grown
+    for (int l = 0; l < win; l++) {
+        const float q = ratio[l];
+        if (q == 0.f) continue;
+        const int s = slot[l], rows = s & (P - 1);
+        uint32_t* w = reinterpret_cast<uint32_t*>(codes + ((size_t(s >> a.shift) * a.kv_heads + h) * P) * D);
+        for (int i = tid; i < rows * D / 4; i += kStoreThreads) {
+            const uint32_t c = w[i];
+            uint32_t o = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) o |= code_of(float(int8_t(c >> (8 * j))), q) << (8 * j);
+            w[i] = o;
+        }
+    }
+    for (int i = warp; i < n; i += kStoreWarps) {
+        const int l = lead[i], s = slot[i];
+        if (l < 0 || uint32_t(s) >= limit) continue;
+        const T* row = x + (w0 + i) * stride;
+        const float q = inv[l];
+        uint32_t* o = reinterpret_cast<uint32_t*>(
+            codes + ((size_t(s >> a.shift) * a.kv_heads + h) * P + (s & (P - 1))) * D);
+        for (int c = 4 * lane; c < D; c += 128) {
+            float v[4];
+            load4(row + c, a.vec, v);
+            o[c >> 2] = code_of(v[0], q) | code_of(v[1], q) << 8 | code_of(v[2], q) << 16 | code_of(v[3], q) << 24;
+        }
+    }
+}
+
+struct ValueArgs {
+    const int8_t* codes[2];
+    const float* scales[2];
+    void* out[2];
+    const int32_t* ids;
+    int32_t n, pages, kv_heads, words;  // words: 16-code pieces of a (page, head)
+    int32_t* status;
+};
+
+// 16 codes to a thread: 16 bytes in, 32 or 64 out.
+template <class T>
+__global__ void __launch_bounds__(256) kv8_values_kernel(const ValueArgs a) {
+    const int kv = blockIdx.y;
+    T* out = static_cast<T*>(a.out[kv]);
+    if (!out) return;
+    const size_t total = size_t(a.n) * a.kv_heads * a.words;
+    for (size_t i = size_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += size_t(gridDim.x) * 256) {
+        const size_t ph = i / a.words, w = i % a.words;
+        const int p = int(ph / a.kv_heads), h = int(ph % a.kv_heads);
+        const int id = a.ids ? a.ids[p] : p;
+        uint4 c = make_uint4(0, 0, 0, 0);
+        float s = 0.f;
+        if (uint32_t(id) < uint32_t(a.pages)) {
+            const size_t at = size_t(id) * a.kv_heads + h;
+            c = __ldg(reinterpret_cast<const uint4*>(a.codes[kv]) + at * a.words + w);
+            s = __ldg(a.scales[kv] + at);
+        } else if (w == 0) {
+            flag(a.status, SPM_PAGE_ID);
+        }
+        const uint32_t q[4] = {c.x, c.y, c.z, c.w};
+        __align__(16) T v[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) v[j] = from_f32<T>(__fmul_rn(float(int8_t(q[j >> 2] >> (8 * (j & 3)))), s));
+        uint4* o = reinterpret_cast<uint4*>(out + 16 * i);
+#pragma unroll
+        for (int j = 0; j < int(sizeof(T)); j++) o[j] = reinterpret_cast<const uint4*>(v)[j];
+    }
+}
+
+}  // namespace
+}  // namespace spm
+
+using namespace spm;
+
+spm_status spm_kv8_append(const spm_kv8* c, uint32_t dtype, const void* k, int64_t k_token, int64_t k_head,
+                          const void* v, int64_t v_token, int64_t v_head, int32_t tokens, const int32_t* slots,
+                          void* cuda_stream) {
+    return guarded([&] {
+        kv8_check(c);
+        kv8_check_type(dtype);
+        if (tokens < 0) fail(SPM_E_ARG, "negative token count");
+        if (c->kv_heads > 65535) fail(SPM_E_ARG, "too many kv heads");
+        if (tokens == 0) return;
+        if (!k || !v || !slots) fail(SPM_E_ARG, "null keys, values or slots");
+        DeviceScope scope(c->device);
+        const size_t size = dtype == SPM_F32 ? 4 : 2;
+        StoreArgs a{};
+        a.x[0] = k, a.x[1] = v;
+        a.token[0] = k_token, a.token[1] = v_token;
+        a.head[0] = k_head, a.head[1] = v_head;
+        a.codes[0] = c->k_codes, a.codes[1] = c->v_codes;
+        a.scales[0] = c->k_scales, a.scales[1] = c->v_scales;
+        a.pages = c->pages, a.page = c->page_tokens, a.shift = __builtin_ctz(unsigned(c->page_tokens));
+        a.kv_heads = c->kv_heads, a.dim = c->head_dim;
+        a.slots = slots, a.tokens = tokens, a.status = c->status;
+        a.vec = !((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % (4 * size)) &&
+                !((k_token | k_head | v_token | v_head) & 3);
+        // windows of a page of prompt tokens, cut down to a warp's token each
+        // while that leaves SMs without a CTA (a decode tick)
+        a.window = kStoreWindow;
+        while (a.window > kStoreWarps && int64_t((tokens + a.window - 1) / a.window) * c->kv_heads * 2 < 2 * device_sms())
+            a.window /= 2;
+        const dim3 grid(unsigned((tokens + a.window - 1) / a.window), unsigned(c->kv_heads), 2);
+        const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+        if (dtype == SPM_F32) kv8_append_kernel<float><<<grid, kStoreThreads, 0, st>>>(a);
+        else if (dtype == SPM_F16) kv8_append_kernel<__half><<<grid, kStoreThreads, 0, st>>>(a);
+        else kv8_append_kernel<__nv_bfloat16><<<grid, kStoreThreads, 0, st>>>(a);
+        CUDA_OK(cudaGetLastError());
+    });
+}
+
+spm_status spm_kv8_values(const spm_kv8* c, uint32_t dtype, const int32_t* page_ids, int32_t n, void* k_out,
+                          void* v_out, void* cuda_stream) {
+    return guarded([&] {
+        kv8_check(c);
+        kv8_check_type(dtype);
+        if (n < 0) fail(SPM_E_ARG, "negative page count");
+        if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15)
+            fail(SPM_E_ARG, "outputs must be 16-byte aligned");
+        if (n == 0 || (!k_out && !v_out)) return;
+        DeviceScope scope(c->device);
+        ValueArgs a{};
+        a.codes[0] = c->k_codes, a.codes[1] = c->v_codes;
+        a.scales[0] = c->k_scales, a.scales[1] = c->v_scales;
+        a.out[0] = k_out, a.out[1] = v_out;
+        a.ids = page_ids, a.n = n, a.pages = c->pages, a.kv_heads = c->kv_heads;
+        a.words = c->page_tokens * c->head_dim / 16;
+        a.status = c->status;
+        const size_t total = size_t(n) * c->kv_heads * a.words;
+        const dim3 grid(unsigned(std::min<size_t>((total + 255) / 256, size_t(device_sms()) * 8)), 2);
+        const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+        if (dtype == SPM_F32) kv8_values_kernel<float><<<grid, 256, 0, st>>>(a);
+        else if (dtype == SPM_F16) kv8_values_kernel<__half><<<grid, 256, 0, st>>>(a);
+        else kv8_values_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
+        CUDA_OK(cudaGetLastError());
+    });
+}

@@ -1,0 +1,209 @@
+// Block tables, slot maps and the stack of free pages of one serving tick, on
+// the device (spm_page_plan).
+//
+// With e_r = ceil(ended_r / P) pages back and f_r = ceil((cached_r + fresh_r) / P)
+// - ceil(cached_r / P) pages wanted, exclusive sums over the rows give every
+// page its place on the stack and every token its row:
+//   push i of row r  -> free[count + E_r + i]           (E: sums of e)
+//   page j of row r  <- free[count + E - 1 - (F_r + j)] (F: sums of f)
+//   token t          -> row r with S_r <= t < S_r+1     (S: sums of fresh)
+//
+// What bounds it is latency: a few kilobytes and three dependent phases (push,
+// pop, slots), so it is ONE launch of one cluster whose CTAs each form the sums
+// in their own shared memory and then share out rows and tokens.
+#include <cooperative_groups.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "abi.h"
+#include "device.cuh"
+
+namespace spm {
+namespace {
+using namespace dev;
+namespace cg = cooperative_groups;
+
+constexpr int kPlanThreads = 512, kPlanWarps = kPlanThreads / 32;
+constexpr int kPlanRequests = 8192;
+
+struct PlanArgs {
+    const int32_t *cached, *fresh, *ended;
+    int32_t requests, page, shift;
+    int32_t* table;
+    int32_t width;
+    int32_t* free_pages;
+    int32_t pages;
+    const int32_t* count;
+    int32_t* left;
+    int32_t tokens;
+    int32_t *starts, *lens, *positions, *slots, *status;
+};
+
+__device__ __forceinline__ long long warp_scan(long long v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long n = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += n;
+    }
+    return v;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanArgs a) {
+    extern __shared__ int32_t sm[];
+    __shared__ long long part[3][kPlanWarps];
+    __shared__ int bad;
+    cg::cluster_group cl = cg::this_cluster();
+    const int R = a.requests, P = a.page, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = int(cl.block_rank()), ranks = int(cl.num_blocks());
+    int32_t* S = sm;               // [R + 1] tokens before row r
+    int32_t* E = S + R + 1;        // pages back before row r
+    int32_t* F = E + R + 1;        // pages taken before row r
+    int32_t* C = F + R + 1;        // cached
+    if (tid == 0) bad = 0;
+    __syncthreads();
+    const int count = *a.count;
+    // a thread's share of the rows, then the exclusive sums over threads
+    const int per = (R + kPlanThreads - 1) / kPlanThreads, r0 = min(R, tid * per), r1 = min(R, r0 + per);
+    const long long cap = (long long)a.width << a.shift;
+    long long s = 0, e = 0, f = 0;
+    bool wrong = false;
+    for (int r = r0; r < r1; r++) {
+        const long long c = a.cached[r], n = a.fresh[r], d = a.ended ? a.ended[r] : 0;
+        C[r] = int32_t(c);
+        wrong |= c < 0 || n < 0 || d < 0 || c + n > cap || d > cap;
+        S[r] = int32_t(n);
+        E[r] = int32_t((d + P - 1) >> a.shift);
+        F[r] = int32_t(((c + n + P - 1) >> a.shift) - ((c + P - 1) >> a.shift));
+        s += n;
+        e += E[r];
+        f += F[r];
+    }
+    if (wrong) bad = 1;
+    const long long si = warp_scan(s, lane), ei = warp_scan(e, lane), fi = warp_scan(f, lane);
+    if (lane == 31) part[0][warp] = si, part[1][warp] = ei, part[2][warp] = fi;
+    __syncthreads();
+    if (warp < 3) {
+        const long long v = lane < kPlanWarps ? part[warp][lane] : 0;
+        const long long i = warp_scan(v, lane);
+        if (lane < kPlanWarps) part[warp][lane] = i;
+    }
+    __syncthreads();
+    const long long ts = part[0][kPlanWarps - 1], te = part[1][kPlanWarps - 1], tf = part[2][kPlanWarps - 1];
+    int code = 0;
+    if (bad) code = SPM_PAGE_LENGTH;
+    else if (count < 0 || count + te > a.pages) code = SPM_PAGE_STACK;
+    else if (tf > count + te) code = SPM_PAGE_FREE;
+    else if (ts > a.tokens) code = SPM_PAGE_TOKENS;
+    if (code) {
+        // nothing moves: no CTA of the cluster writes table or stack
+        for (int i = rank * kPlanThreads + tid; i < a.tokens; i += ranks * kPlanThreads) a.positions[i] = a.slots[i] = -1;
+        for (int i = rank * kPlanThreads + tid; i <= R; i += ranks * kPlanThreads) {
+            a.starts[i] = 0;
+            if (i < R) a.lens[i] = 0;
+        }
+        cl.sync();  // every CTA has read the count
+        if (rank == 0 && tid == 0) {
+            *a.left = count;
+            flag(a.status, code);
+        }
+        return;
+    }
+    s = si - s + (warp ? part[0][warp - 1] : 0);
+    e = ei - e + (warp ? part[1][warp - 1] : 0);
+    f = fi - f + (warp ? part[2][warp - 1] : 0);
+    for (int r = r0; r < r1; r++) {
+        const int n = S[r], b = E[r], w = F[r];
+        S[r] = int32_t(s);
+        E[r] = int32_t(e);
+        F[r] = int32_t(f);
+        if (rank == 0) {
+            a.starts[r] = int32_t(s);
+            a.lens[r] = C[r] + n;
+        }
+        s += n;
+        e += b;
+        f += w;
+    }
+    if (tid == 0) {
+        S[R] = int32_t(ts);
+        E[R] = int32_t(te);
+        F[R] = int32_t(tf);
+        if (rank == 0) a.starts[R] = int32_t(ts);
+    }
+    __syncthreads();
+    // pages of ended requests onto the stack, a warp to a row
+    for (int r = rank * kPlanWarps + warp; r < R; r += ranks * kPlanWarps)
+        for (int j = lane; j < E[r + 1] - E[r]; j += 32) a.free_pages[count + E[r] + j] = a.table[size_t(r) * a.width + j];
+    __threadfence();
+    cl.sync();  // the whole stack stands, and the rows' old entries have been read
+    if (rank == 0 && tid == 0) *a.left = int32_t(count + te - tf);
+    for (int r = rank * kPlanWarps + warp; r < R; r += ranks * kPlanWarps) {
+        const int old = int((uint32_t(C[r]) + P - 1) >> a.shift);
+        for (int j = lane; j < F[r + 1] - F[r]; j += 32)
+            a.table[size_t(r) * a.width + old + j] = __ldcg(a.free_pages + (count + te - 1 - F[r] - j));
+    }
+    __threadfence();
+    cl.sync();  // the table stands
+    for (int t = rank * kPlanThreads + tid; t < a.tokens; t += ranks * kPlanThreads) {
+        int pos = -1, slot = -1;
+        if (t < ts) {
+            int lo = 0, hi = R;  // S[lo] <= t < S[hi]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (S[mid] <= t) lo = mid;
+                else hi = mid;
+            }
+            pos = C[lo] + t - S[lo];
+            const int page = __ldcg(a.table + size_t(lo) * a.width + (pos >> a.shift));
+            if (uint32_t(page) < uint32_t(a.pages)) slot = page * P + (pos & (P - 1));
+            else flag(a.status, SPM_PAGE_ID);
+        }
+        a.positions[t] = pos;
+        a.slots[t] = slot;
+    }
+}
+
+}  // namespace
+}  // namespace spm
+
+using namespace spm;
+
+spm_status spm_page_plan(int device, const int32_t* cached, const int32_t* fresh, const int32_t* ended,
+                         int32_t requests, int32_t page_tokens, int32_t* table, int32_t table_width,
+                         int32_t* free_pages, int32_t pages, const int32_t* free_count, int32_t* free_left,
+                         int32_t tokens, int32_t* starts, int32_t* lens, int32_t* positions, int32_t* slots,
+                         int32_t* status, void* cuda_stream) {
+    return guarded([&] {
+        if (requests < 0 || requests > kPlanRequests) fail(SPM_E_ARG, "a plan takes 0 to 8192 requests");
+        if (page_tokens < 16 || page_tokens > 256 || (page_tokens & (page_tokens - 1)))
+            fail(SPM_E_ARG, "page_tokens is 16, 32, 64, 128 or 256");
+        if (tokens < 0 || pages < 0 || table_width < 0) fail(SPM_E_ARG, "negative size");
+        if (int64_t(table_width) * page_tokens > INT32_MAX || int64_t(pages) * page_tokens > INT32_MAX)
+            fail(SPM_E_ARG, "positions and slots are 32-bit: table_width and pages times page_tokens must fit");
+        if (!free_count || !free_left || !starts) fail(SPM_E_ARG, "null free_count, free_left or starts");
+        if (requests && (!cached || !fresh || !lens)) fail(SPM_E_ARG, "null lengths");
+        if ((requests && table_width && !table) || (pages && !free_pages)) fail(SPM_E_ARG, "null table or stack");
+        if (tokens && (!positions || !slots)) fail(SPM_E_ARG, "null positions or slots");
+        DeviceScope scope(device);
+        PlanArgs a{cached, fresh, ended, requests, page_tokens, __builtin_ctz(unsigned(page_tokens)), table, table_width,
+                   free_pages, pages, free_count, free_left, tokens, starts, lens, positions, slots, status};
+        const size_t smem = size_t(4 * requests + 3) * sizeof(int32_t);
+        static unsigned long long done = 0;
+        allow_smem(page_plan_kernel, size_t(4 * kPlanRequests + 3) * sizeof(int32_t), done);
+        // one CTA up to a few rows and tokens for each of its threads, else a cluster of eight
+        const unsigned ctas = requests <= 64 && tokens <= 4 * kPlanThreads ? 1 : 8;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(ctas);
+        cfg.blockDim = dim3(kPlanThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = static_cast<cudaStream_t>(cuda_stream);
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = ctas;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        CUDA_OK(cudaLaunchKernelEx(&cfg, page_plan_kernel, a));
+    });
+}

@@ -28,6 +28,10 @@
  *   spm_ternary_*         spm-gemv-ref/src/gemv.rs:39-126 (run_gemv)
  *   spm_sweep_*           spm-stream-file/src/prefetch.rs + spm-stream-groups rewind:
  *                         .spm files streamed from host memory through a device ring
+ *   spm_page_plan, spm_kv8_*  no counterpart: spm-kv/src/cache.rs:49-58 and
+ *                         attend.rs:37-94 hold f32 rows of one client
+ *   spm_sample            no counterpart: the reference picks greedily
+ *                         (spm-batch/examples/serve-demo.rs:74-79)
  */
 #ifndef SPMGPU_H
 #define SPMGPU_H
@@ -422,6 +426,111 @@ enum { SPM_PLAN_EVENTS = 1, SPM_PLAN_WAIT = 2, SPM_PLAN_COPY = 3, SPM_PLAN_LAUNC
 spm_status spm_sweep_plan(const uint64_t* region_bytes, int32_t streams, uint64_t device_bytes,
                           const int32_t* script, int32_t script_len, int64_t* log, int64_t log_cap,
                           int64_t* log_len);
+
+/* ---- serving: page tables, a paged 8-bit KV cache, sampling ----
+ * Operators of a serving tick on the caller's device memory, run one after the
+ * other: spm_page_plan, then per layer spm_kv8_append and spm_kv8_attention,
+ * then spm_sample on the head's logits.  All pointers are device pointers on
+ * `device`, everything is enqueued on cuda_stream (NULL = default stream), no
+ * call allocates, synchronises or reads device memory on the host, and every
+ * call can be captured into a CUDA graph; the caller's current device is put
+ * back.  What only the device can see (a length past its table, a page that is
+ * not one) is recorded in the call's `status` word, which keeps its first
+ * non-zero code until the caller clears it; such a call reads and writes
+ * nothing out of range.  Activation types: SPM_F32, SPM_F16, SPM_BF16. */
+enum { SPM_BF16 = 30 };  /* GGML's code */
+enum {
+    SPM_PAGE_LENGTH = 11,  /* a length is negative or past the table's width   */
+    SPM_PAGE_FREE = 12,    /* more pages wanted than free                     */
+    SPM_PAGE_TOKENS = 13,  /* more tokens than the slot map holds             */
+    SPM_PAGE_STACK = 14,   /* more pages back than the pool has               */
+    SPM_PAGE_ID = 15,      /* a page or slot that is not in the pool          */
+    SPM_PAGE_QUERIES = 16  /* a request with more queries than `most`, or
+                              starts that do not ascend within the rows       */
+};
+
+/* Block table, slot map and free stack of one tick, from the requests'
+ * lengths.  Row r (of `requests` <= 8192) of table[requests][table_width] holds
+ * the pages of cached[r] tokens, page_tokens to a page, and takes fresh[r] more;
+ * the pages of ended[r] tokens (ended may be NULL) of the row's former request
+ * go onto the stack free_pages[0 .. *free_count) first, row after row; the new
+ * pages then come off its top, row after row.  free_pages has room for `pages`
+ * entries; *free_left receives the stack's new height (free_count and free_left
+ * may be the same word).  Per request: starts[requests + 1], the first of its
+ * tokens in the call, and lens = cached + fresh; per token: its position in its
+ * request and its slot, page * page_tokens + offset, -1 behind the last token up
+ * to `tokens`.  A row whose request has ended keeps its entries until they are
+ * overwritten.  A plan that fails (status: SPM_PAGE_LENGTH, _FREE, _TOKENS,
+ * _STACK, in this order) leaves table and stack as they were and returns no
+ * tokens: starts and lens 0, positions and slots -1. */
+spm_status spm_page_plan(int device, const int32_t* cached, const int32_t* fresh, const int32_t* ended,
+                         int32_t requests, int32_t page_tokens, int32_t* table, int32_t table_width,
+                         int32_t* free_pages, int32_t pages, const int32_t* free_count, int32_t* free_left,
+                         int32_t tokens, int32_t* starts, int32_t* lens, int32_t* positions, int32_t* slots,
+                         int32_t* status, void* cuda_stream);
+
+/* One layer's keys and values in pages of page_tokens (16, 32, 64, 128 or 256)
+ * tokens: codes[pages][kv_heads][page_tokens][head_dim] in int8 and one f32
+ * scale for each (page, kv head), head_dim 64, 96, 128, 192 or 256.  A value is
+ * code * scale; scales are powers of two, so that storing is one rounding of
+ * x / scale to an integer and every product is exact. */
+typedef struct spm_kv8 {
+    int32_t device, pages, page_tokens, kv_heads, head_dim, pad_;
+    int8_t *k_codes, *v_codes;   /* 16-byte aligned */
+    float *k_scales, *v_scales;
+    int32_t* status;             /* may be NULL */
+} spm_kv8;
+
+/* Rows of keys and values into their slots.  k, v: `tokens` rows of
+ * [kv_heads][head_dim] of type dtype, *_token and *_head elements apart.  A
+ * slot of -1 is passed over.  The tokens of one page follow one another in a
+ * call, in ascending slots (as spm_page_plan gives them); a page is in one place
+ * of a call.  The scale is the smallest power of two with |x| <= 127 scale over
+ * the rows written; rows already in the page (those before the first slot
+ * written, if that is not the page's first) raise it, and are rounded again
+ * (half to even) where it grows.  A value that is not finite makes the scale of
+ * its page and head NaN, and so all its values. */
+spm_status spm_kv8_append(const spm_kv8* cache, uint32_t dtype, const void* k, int64_t k_token, int64_t k_head,
+                          const void* v, int64_t v_token, int64_t v_head, int32_t tokens, const int32_t* slots,
+                          void* cuda_stream);
+/* Whole pages' values: out [n][kv_heads][page_tokens][head_dim] of type dtype
+ * for the pages page_ids[0..n) (NULL: 0..n-1); a page that is not in the pool
+ * gives zeros.  k_out or v_out may be NULL. */
+spm_status spm_kv8_values(const spm_kv8* cache, uint32_t dtype, const int32_t* page_ids, int32_t n, void* k_out,
+                          void* v_out, void* cuda_stream);
+/* Attention over the cache: q and out are `rows` rows of [heads][head_dim], request
+ * r's rows starts[r] .. starts[r + 1] (at most `most` of them, the same number for
+ * none: 0), standing at its last positions: row i of n sees the keys up to position
+ * lens[r] - n + i, the cache holding lens[r] tokens in the pages of table row r.
+ * heads is a multiple of kv_heads, head h reads kv head h / (heads / kv_heads).
+ * A row that sees no key is zero; rows behind starts[requests] are left as they
+ * were.  `workspace` is scratch of spm_kv8_attention_workspace bytes (for the same
+ * arguments; 16-byte aligned), not shared by calls that may overlap. */
+spm_status spm_kv8_attention_workspace(const spm_kv8* cache, int32_t heads, int32_t requests, int32_t most,
+                                       int32_t table_width, uint64_t* bytes);
+spm_status spm_kv8_attention(const spm_kv8* cache, uint32_t dtype, const void* q, int64_t q_token, int64_t q_head,
+                             int32_t heads, int32_t rows, const int32_t* starts, const int32_t* lens,
+                             int32_t requests, int32_t most, const int32_t* table, int32_t table_width, float scale,
+                             void* out, int64_t out_token, int64_t out_head, void* workspace,
+                             uint64_t workspace_bytes, void* cuda_stream);
+
+/* A pick per row of logits[rows][vocab] (row_stride elements apart).  Tokens in
+ * the order (logit descending, index ascending), weights exp((logit - max) /
+ * temperature) in 64 bits; kept is the shortest of three prefixes: the top_k
+ * first; the smallest whose mass reaches top_p of the top_k's; those of weight >=
+ * min_p; at least one token.  The pick is the first token by index at which the
+ * kept mass exceeds u (in [0, 1)) times its total; kept (may be NULL) receives
+ * the number kept and prob (may be NULL) the pick's share of the kept mass.
+ * Per-row device arrays; NULL, top_k <= 0 or >= vocab, top_p >= 1 and min_p <= 0
+ * switch a filter off, temperature NULL is 1, and a temperature that is not
+ * above 0 takes the largest logit, the first by index (spm_decode_step's greedy
+ * pick takes the last, as the reference does).  -inf and NaN are never picked;
+ * where nothing else is left the token is -1, kept and prob 0.  Logits of +inf
+ * share all the mass.  vocab <= 2^19. */
+spm_status spm_sample(int device, uint32_t dtype, const void* logits, int64_t row_stride, int32_t rows,
+                      int32_t vocab, const float* temperature, const int32_t* top_k, const float* top_p,
+                      const float* min_p, const float* u, int32_t* token, int32_t* kept, float* prob,
+                      void* cuda_stream);
 
 #ifdef __cplusplus
 }
