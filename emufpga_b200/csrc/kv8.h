@@ -45,6 +45,25 @@ __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v);
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
 
+// Four consecutive elements as f32; in one load where `vec` says that they are aligned.
+template <class T>
+__device__ __forceinline__ void load4(const T* p, bool vec, float (&v)[4]) {
+    if (vec) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 q = *reinterpret_cast<const float4*>(p);
+            v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+        } else {
+            const uint2 q = *reinterpret_cast<const uint2*>(p);
+            const T* h = reinterpret_cast<const T*>(&q);
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = to_f32(h[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = to_f32(p[j]);
+    }
+}
+
 // 2^e for e clamped to the normal range.
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
 

@@ -36,25 +36,6 @@ struct StoreArgs {
     bool vec;                 // four elements at a time: strides and bases allow it
 };
 
-// Four consecutive elements of a row as f32.
-template <class T>
-__device__ __forceinline__ void load4(const T* p, bool vec, float (&v)[4]) {
-    if (vec) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 q = *reinterpret_cast<const float4*>(p);
-            v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
-        } else {
-            const uint2 q = *reinterpret_cast<const uint2*>(p);
-            const T* h = reinterpret_cast<const T*>(&q);
-#pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = to_f32(h[j]);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = to_f32(p[j]);
-    }
-}
-
 __device__ __forceinline__ uint32_t code_of(float x, float inv) {
     // rounds half to even; NaN (a value or scale that is not finite) is 0
     return uint32_t(min(max(__float2int_rn(__fmul_rn(x, inv)), -127), 127)) & 0xffu;

@@ -3,16 +3,23 @@
 // Every filter keeps a prefix of the tokens sorted by (logit descending, index
 // ascending), so the three together keep the shortest one, which a threshold
 // names: all keys above it and the first `ties` tokens by index that equal it.
-// No sort: the threshold is found by radix selection over the logits' ordered
-// 32-bit keys (11, 11 and 10 bits), by counts for top-k and by masses for top-p.
 //
 // Weights exp((x - max) / T) are formed in 64 bits and held as integers in units
-// of 2^-44 (a sum of 2^19 fits 64 bits), so sums are exact, independent of their order (shared memory atomics
-// included) and the same on every run; a neighbour at a border of top-p or u is
-// told apart at 2^-44 of the largest weight.
+// of 2^-44 (a sum of 2^19 fits 64 bits), so sums are exact, independent of their
+// order (shared memory atomics included) and the same on every run; a neighbour
+// at a border of top-p or u is told apart at 2^-44 of the largest weight.
 //
-// A row is one thread-block cluster: each CTA keeps its slice of the row in
-// shared memory, so the logits are read from HBM once, and the cluster's
+// The row is not sorted.  A histogram over 1024 bins of (max - x) / T, 1/32
+// wide, of counts (top-k) or masses (top-p) shows the bin in which the border
+// lies; only what lies there (for top-k: there and above) is listed and sorted,
+// a few hundred tokens as a rule.  Where a list would be longer than 2048 (long
+// runs of equal logits, a large top_k) the border is found by radix selection
+// over the logits' ordered 32-bit keys instead.
+//
+// What bounds it: the logits' bytes for many rows, and the 64-bit exponentials
+// where top-k does not spare them; for few rows the chain of dependent passes and
+// cluster barriers.  A row is one thread-block cluster whose CTAs keep its
+// slices in shared memory, so the logits are read from HBM once and the
 // histograms are added through distributed shared memory.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -26,16 +33,17 @@ namespace {
 using namespace dev;
 namespace cg = cooperative_groups;
 
-constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
-constexpr int kBins = 2048;
-constexpr int kSampleClusters = 8;       // CTAs of a row, at most
-constexpr int kSampleSlice = 40 * 1024;  // logits of a slice that shared memory holds
+constexpr int kBins = 1024;
+constexpr int kSampleClusters = 8;        // CTAs of a row, at most
+constexpr int kList = 2048;               // tokens that are sorted, at most
+constexpr int kSampleSlice = 160 * 1024;  // bytes of a slice that shared memory holds
+constexpr int kTable = 128;               // of the exponential
 typedef unsigned long long u64;
 
 struct SampleArgs {
     const void* logits;
     int64_t stride;
-    int32_t vocab, slice;   // slice: logits of a CTA, a multiple of the warps' 32
+    int32_t vocab, slice;   // slice: logits of a CTA, a multiple of four for each warp
     const float* temperature;
     const int32_t* top_k;
     const float *top_p, *min_p, *u;
@@ -53,56 +61,113 @@ __device__ __forceinline__ float value_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-struct Shared {
-    uint32_t hist[kBins];                 // counts, or the masses' low 16 bits
-    uint32_t mid[kBins], high[kBins];     // masses' next 16 bits, and the rest
-    u64 total[kBins];                     // the cluster's
-    u64 scan[kSampleWarps];
-    u64 need_out;
-    int bin_out;
+struct alignas(16) Shared {
+    union {
+        struct {
+            uint32_t low[kBins], mid[kBins], high[kBins];  // this CTA's: counts in low, or masses in 16 + 16 + the rest
+            u64 total[kBins];                              // the cluster's
+            u64 part[kBins];                      // sums of a share of the bins over some of the CTAs
+        };
+        struct {
+            u64 list[kList];    // this CTA's border tokens: key, then the index's complement
+            u64 sorted[kList];  // the cluster's
+        };
+    };
+    double table[kTable];                 // 2^(j / kTable)
+    u64 scan[32];
+    u64 need_out, seg_mass[kSampleClusters * 32];
+    uint32_t seg_count[kSampleClusters * 32], seg_ties[kSampleClusters * 32];
     uint32_t top[kSampleClusters];        // each CTA's largest key
-    u64 seg_mass[kSampleClusters * kSampleWarps];
-    uint32_t seg_count[kSampleClusters * kSampleWarps], seg_ties[kSampleClusters * kSampleWarps];
+    uint32_t listed;                      // length of this CTA's list
+    int bin_out;
+    u64 pick_before, pick_ties, pick_total, pick_count;
+    int pick_seg;
 };
 
 struct Row {
-    double top, inv;      // the largest logit, 1 / T
-    bool inf;             // it is +inf
-    __device__ __forceinline__ double weight(float x) const {
-        if (inf) return x == INFINITY ? 1.0 : 0.0;
-        return exp((double(x) - top) * inv);
+    double top, inv, slope;   // the largest logit, 1 / T, -128 log2(e) / T
+    float ftop, bins;         // 32 / T: bins of a logit's distance from the top
+    const double* table;
+    __device__ __forceinline__ double below(float x) const { return x == ftop ? 0.0 : top - double(x); }
+    __device__ __forceinline__ double weight(float x) const { return x == ftop ? 1.0 : exp(-below(x) * inv); }
+    // round(2^(44 - y)), y = (top - x) log2(e) / T: table-driven (P. T. P. Tang,
+    // ACM TOMS 15, 1989), 2^z = 2^e * 2^(j/128) * 2^(r/128), j and e integers, the
+    // last factor's series to r^4 (|r| <= 1/2: 2e-15 from the whole one).
+    // Without branches, so that several overlap; 0 for -inf and NaN.
+    __device__ __forceinline__ u64 mass(float x) const {
+        constexpr double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer in the low bits
+        constexpr double c = 0.69314718055994530942 / kTable;
+        const double s = fma(top - double(x), slope, 44.0 * kTable), k = s + magic;
+        const int n = __double2loint(k);
+        const double r = s - (k - magic);
+        const double p = fma(r, fma(r, fma(r, fma(r, c * c * c * c / 24, c * c * c / 6), c * c / 2), c), 1.0);
+        const double t = p * table[n & (kTable - 1)];  // in [1, 2) or a rounding beside it
+        // t 2^(n >> 7), at most 2^44, added to 2^52: its integer is the mantissa
+        const double w = __hiloint2double(__double2hiint(t) + ((n & ~(kTable - 1)) << 13), __double2loint(t)) + 4503599627370496.0;
+        // (2^-46 down the weight is 0, and its exponent above soon past a double's)
+        const u64 m = x > -INFINITY && distance(x) * bins < 46.f * 22.2f ? __double_as_longlong(w) & 0xfffffffffffffull : 0;
+        return x == INFINITY ? 1ull << 44 : m;
     }
-    __device__ __forceinline__ u64 mass(float x) const { return __double2ull_rn(weight(x) * 17592186044416.0); }
+    __device__ __forceinline__ float distance(float x) const { return fminf(ftop - x, 3.402823466e38f); }
+    // The bin of a candidate's distance from the top; ascending as x descends.
+    __device__ __forceinline__ float place(float x) const { return fminf(x == INFINITY ? 0.f : distance(x) * bins, float(kBins - 1)); }
+    __device__ __forceinline__ int bin(float x) const { return int(place(x)); }
+    // And the 1024th part of bin b.
+    __device__ __forceinline__ int part(float x, int b) const {
+        return int(fminf((place(x) - float(b)) * float(kBins), float(kBins - 1)));
+    }
 };
 
-// From the cluster's totals, bins descending: the bin in which the running sum
-// reaches `need` (>= 1), and what is still needed inside it.
-__device__ void select_bin(Shared& s, u64 need, int& bin, u64& left) {
-    constexpr int PER = kBins / kSampleThreads;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    u64 mine = 0;
-#pragma unroll
-    for (int j = 0; j < PER; j++) mine += s.total[kBins - 1 - (tid * PER + j)];
-    u64 incl = mine;
+// Inclusive sum over the block's threads on top of `base`; base becomes the total.
+template <int NT>
+__device__ __forceinline__ u64 block_sums(Shared& s, u64 w, u64& base) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const u64 n = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += n;
+        const u64 y = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += y;
     }
     __syncthreads();
-    if (lane == 31) s.scan[warp] = incl;
+    if (lane == 31) s.scan[warp] = w;
     __syncthreads();
-    u64 before = incl - mine;
-    for (int w = 0; w < warp; w++) before += s.scan[w];
+    u64 t = lane < NT / 32 ? s.scan[lane] : 0;  // a sum for each warp
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 y = __shfl_up_sync(0xffffffffu, t, o);
+        if (lane >= o) t += y;
+    }
+    const u64 before = __shfl_sync(0xffffffffu, t, (warp + 31) & 31);
+    w += base + (warp ? before : 0);
+    base += __shfl_sync(0xffffffffu, t, 31);
+    return w;
+}
+
+// From the cluster's totals, bins in the order FIRST (ascending or descending):
+// the bin in which the running sum reaches `need` (>= 1), and what is needed
+// inside it; -1 where the sum stays below.
+template <int NT, bool DOWN>
+__device__ void select_bin(Shared& s, u64 need, int& bin, u64& left, u64& all) {
+    constexpr int PER = kBins / NT;
+    static_assert(PER >= 1, "a bin for each thread");
+    const int tid = threadIdx.x;
+    auto at = [&](int i) { return s.total[DOWN ? kBins - 1 - i : i]; };
+    u64 mine = 0;
+#pragma unroll
+    for (int j = 0; j < PER; j++) mine += at(tid * PER + j);
+    all = 0;
+    u64 before = block_sums<NT>(s, mine, all) - mine;
+    if (tid == 0) s.bin_out = -1;
+    __syncthreads();
+    if (need == 0) return;  // the sum alone is asked for
     if (before < need && need <= before + mine) {
+#pragma unroll
         for (int j = 0; j < PER; j++) {
-            const int b = kBins - 1 - (tid * PER + j);
-            if (need <= before + s.total[b]) {
-                s.bin_out = b;
+            const u64 t = at(tid * PER + j);
+            if (before < need && need <= before + t) {
+                s.bin_out = DOWN ? kBins - 1 - (tid * PER + j) : tid * PER + j;
                 s.need_out = need - before;
-                break;
             }
-            before += s.total[b];
+            before += t;
         }
     }
     __syncthreads();
@@ -110,38 +175,143 @@ __device__ void select_bin(Shared& s, u64 need, int& bin, u64& left) {
     left = s.need_out;
 }
 
-template <class T>
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs a) {
+// Descending bitonic sort of n <= kList entries, padded with 0: E neighbours to a
+// thread, exchanges among them in registers, up to 32 E apart between lanes, and
+// the rest through shared memory.
+template <int NT>
+__device__ void sort_descending(u64* v, int n) {
+    constexpr int E = kList / NT;
+    const int tid = threadIdx.x, i = E * tid;
+    int size = 32 * E;
+    while (size < n) size *= 2;
+    const bool idle = i - E * (tid & 31) >= size;  // a warp of padding
+    u64 a[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) a[e] = i + e < n ? v[i + e] : 0;
+    for (int k = 2; k <= size; k *= 2) {
+        for (int j = k / 2; j >= E; j /= 2) {
+            u64 c[E];
+            if (j >= 32 * E) {
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (!idle) v[i + e] = a[e];
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < E; e++) c[e] = idle ? 0 : v[(i ^ j) + e];
+            } else {
+                if (idle) break;
+#pragma unroll
+                for (int e = 0; e < E; e++) c[e] = __shfl_xor_sync(0xffffffffu, a[e], j / E);
+            }
+            const bool larger = ((i & j) == 0) == ((i & k) == 0);  // this place takes the larger
+#pragma unroll
+            for (int e = 0; e < E; e++) a[e] = larger ? max(a[e], c[e]) : min(a[e], c[e]);
+        }
+#pragma unroll
+        for (int j = E / 2; j > 0; j /= 2) {
+            if (j >= k) continue;
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (!(e & j)) {
+                    const bool down = ((i + e) & k) == 0;
+                    const u64 lo = min(a[e], a[e + j]), hi = max(a[e], a[e + j]);
+                    a[e] = down ? hi : lo;
+                    a[e + j] = down ? lo : hi;
+                }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; e++)
+        if (!idle) v[i + e] = a[e];
+    __syncthreads();
+}
+
+template <class T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs a) {
+    constexpr int W = NT / 32;
     extern __shared__ __align__(16) uint8_t raw[];
     Shared& s = *reinterpret_cast<Shared*>(raw);
-    float* held = reinterpret_cast<float*>(raw + sizeof(Shared));
+    T* held = reinterpret_cast<T*>(raw + sizeof(Shared));
     cg::cluster_group cl = cg::this_cluster();
     const int C = int(cl.num_blocks()), rank = int(cl.block_rank());
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row = blockIdx.x / C;
     const T* x = static_cast<const T*>(a.logits) + row * a.stride;
     const int i0 = min(a.vocab, rank * a.slice), n = min(a.vocab, i0 + a.slice) - i0;
-    const bool holds = a.slice <= kSampleSlice;
-    auto at = [&](int i) { return holds ? held[i] : to_f32(x[i0 + i]); };
+    const bool holds = a.slice * int(sizeof(T)) <= kSampleSlice;
+    // four logits of the slice from i on (a multiple of four); -inf behind its end
+    auto four = [&](int i, float (&v)[4]) {
+        if (holds) {
+            load4(held + i, true, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = i + j < n ? to_f32(x[i0 + i + j]) : -INFINITY;
+        }
+    };
+    // f(four logits, the first's place) over the slice, by whole warps; -inf behind the end
+    auto quads = [&](auto&& f) {
+        for (int i0 = 128 * warp; i0 < n; i0 += 4 * NT) {
+            float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (i0 + 4 * lane < n) four(i0 + 4 * lane, v);
+            f(v, i0 + 4 * lane);
+        }
+    };
+    // f(logit, its place in the slice) for the candidates of this thread
+    auto each = [&](auto&& f) {
+        for (int i = 4 * tid; i < n; i += 4 * NT) {
+            float v[4];
+            four(i, v);
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (v[j] > -INFINITY) f(v[j], i + j);  // (not -inf, not NaN)
+        }
+    };
+    cg::cluster_group::arrival_token started = cl.barrier_arrive();
 
     // ---- the slice into shared memory; the largest key ----
     uint32_t top = 0;
-    for (int i = tid; i < n; i += kSampleThreads) {
-        const float v = to_f32(x[i0 + i]);
-        if (holds) held[i] = v;
-        top = max(top, key_of(v));
+    {
+        constexpr int V = 16 / sizeof(T);
+        const T* from = x + i0;
+        const int head = min(n, int((16 - (reinterpret_cast<uintptr_t>(from) & 15)) & 15) / int(sizeof(T)));
+        auto take = [&](int i, T v) {
+            if (holds) held[i] = v;
+            top = max(top, key_of(to_f32(v)));
+        };
+        if (tid < head) take(tid, from[tid]);
+        const int whole = (n - head) / V;
+        const uint4* wide = reinterpret_cast<const uint4*>(from + head);
+#pragma unroll 4
+        for (int i = tid; i < whole; i += NT) {
+            const uint4 q = __ldcs(wide + i);
+            const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+            for (int j = 0; j < V; j++) take(head + V * i + j, e[j]);
+        }
+        const int rest = head + V * whole;
+        if (tid < n - rest) take(rest + tid, from[rest + tid]);
+        if (holds && tid < 4 && n + tid < a.slice) held[n + tid] = from_f32<T>(-INFINITY);  // the last four's places
     }
+    if (tid < kTable) s.table[tid] = exp2(double(tid) / kTable);
+    for (int b = tid; b < kBins; b += NT) s.low[b] = s.mid[b] = s.high[b] = 0;
+    if (tid == 0) s.listed = 0;
     top = __reduce_max_sync(0xffffffffu, top);
-    if (tid < kSampleClusters) s.top[tid] = 0;
+    uint32_t* tops = reinterpret_cast<uint32_t*>(s.scan);
+    if (lane == 0) tops[warp] = top;
+    cl.barrier_wait(std::move(started));  // every CTA runs
     __syncthreads();
-    if (lane == 0) atomicMax(&s.top[rank], top);
-    __syncthreads();
-    cl.sync();  // (every CTA's array stands)
-    if (tid < C && tid != rank) s.top[tid] = cl.map_shared_rank(s.top, tid)[tid];
+    if (tid < C) {
+        top = 0;
+#pragma unroll 8
+        for (int w = 0; w < W; w++) top = max(top, tops[w]);
+        cl.map_shared_rank(s.top, tid)[rank] = top;
+    }
     cl.sync();
     top = 0;
     for (int c = 0; c < C; c++) top = max(top, s.top[c]);
-    if (top == 0) {
+    if (top == 0) {  // the same for the whole cluster
         if (rank == 0 && tid == 0) {
             a.token[row] = -1;
             if (a.kept) a.kept[row] = 0;
@@ -152,101 +322,281 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     const float temp = a.temperature ? a.temperature[row] : 1.f;
     const bool greedy = !(temp > 0.f);
     Row r;
-    r.top = double(value_of(top));
-    r.inf = value_of(top) == INFINITY;
+    r.ftop = value_of(top);
+    r.top = double(r.ftop);
     r.inv = greedy ? 1.0 : 1.0 / double(temp);
-    int k = greedy ? 1 : a.top_k ? a.top_k[row] : 0;
+    r.slope = r.inv * -1.4426950408889634074 * kTable;
+    r.bins = r.ftop == INFINITY ? 1e30f : fminf(float(32.0 * r.inv), 1e30f);
+    r.table = s.table;
+    int k = greedy ? 0 : a.top_k ? a.top_k[row] : 0;
     if (k <= 0 || k >= a.vocab) k = 0;
     if (greedy) k = 1;
     const float p = !greedy && a.top_p ? a.top_p[row] : 1.f;
     const bool nucleus = p < 1.f;
     const float least = !greedy && a.min_p ? a.min_p[row] : 0.f;
-    const float low = least > 1.f ? 1.f : least;  // (NaN compares as off below)
+    // weight >= min_p as a distance from the top; off (NaN too) at 0, 1 at most
+    const bool floored = least > 0.f;
+    const double reach = floored ? -log(fmin(double(least), 1.0)) : 0.0;
+    auto keeps = [&](float v) { return !floored || r.below(v) * r.inv <= reach; };
 
-    auto clear = [&](bool mass) {
-        for (int b = tid; b < kBins; b += kSampleThreads) {
-            s.hist[b] = 0;
-            if (mass) s.mid[b] = s.high[b] = 0;
-        }
+    auto clear = [&]() {
+        for (int b = tid; b < kBins; b += NT) s.low[b] = s.mid[b] = s.high[b] = 0;
         __syncthreads();
+    };
+    auto add_mass = [&](int b, u64 w) {
+        if (w & 0xffffu) atomicAdd(&s.low[b], uint32_t(w & 0xffffu));
+        if (w >> 16 & 0xffffu) atomicAdd(&s.mid[b], uint32_t(w >> 16 & 0xffffu));
+        if (w >> 32) atomicAdd(&s.high[b], uint32_t(w >> 32));
     };
     // the CTAs' histograms added into every CTA's total
     auto gather = [&](bool mass) {
-        __syncthreads();
         cl.sync();
-        const int share = kBins / C;
-        for (int b = rank * share + tid; b < (rank + 1) * share; b += kSampleThreads) {
+        const int share = kBins / C, parts = max(1, min(4, NT / share)), each = (C + parts - 1) / parts;
+        for (int e = tid; e < share * parts; e += NT) {
+            const int b = rank * share + e % share, q = e / share;
             u64 sum = 0;
-            for (int c = 0; c < C; c++) {
-                sum += cl.map_shared_rank(s.hist, c)[b];
+#pragma unroll 2
+            for (int c = q * each; c < min(C, (q + 1) * each); c++) {
+                sum += cl.map_shared_rank(s.low, c)[b];
                 if (mass)
                     sum += (u64(cl.map_shared_rank(s.mid, c)[b]) << 16) + (u64(cl.map_shared_rank(s.high, c)[b]) << 32);
             }
-            for (int c = 0; c < C; c++) cl.map_shared_rank(s.total, c)[b] = sum;
+            if (parts == 1) {
+                for (int c = 0; c < C; c++) cl.map_shared_rank(s.total, c)[b] = sum;
+            } else {
+                s.part[e] = sum;
+            }
+        }
+        if (parts > 1) {
+            __syncthreads();
+            for (int e = tid; e < share * parts; e += NT) {
+                const int i = e % share, q = e / share;
+                u64 sum = 0;
+                for (int g = 0; g < parts; g++) sum += s.part[g * share + i];
+#pragma unroll 2
+                for (int c = q * each; c < min(C, (q + 1) * each); c++)
+                    cl.map_shared_rank(s.total, c)[rank * share + i] = sum;
+            }
         }
         cl.sync();
     };
-    auto add_mass = [&](int b, u64 w) {
-        atomicAdd(&s.hist[b], uint32_t(w & 0xffffu));
-        atomicAdd(&s.mid[b], uint32_t(w >> 16 & 0xffffu));
-        atomicAdd(&s.high[b], uint32_t(w >> 32));
+    // the cluster's lists, whole, in this CTA's `sorted`; their length
+    auto collect = [&]() {
+        int len = 0;
+        for (int c = 0; c < C; c++) {
+            const int m = int(*cl.map_shared_rank(&s.listed, c));
+            const u64* from = cl.map_shared_rank(s.list, c);
+            for (int i = tid; i < m; i += NT) s.sorted[len + i] = from[i];
+            len += m;
+        }
+        __syncthreads();
+        return len;
     };
-    constexpr int shift[3] = {21, 10, 0};
-    constexpr uint32_t above[3] = {0u, 0xffe00000u, 0xfffffc00u};  // key bits that earlier levels have fixed
+    // lists the candidates that `in` takes; listed counts them even where the list is full
+    auto list = [&](auto&& in) {
+        quads([&](const float (&v)[4], int i) {
+            uint32_t take = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) take |= uint32_t(v[j] > -INFINITY && in(v[j])) << j;
+            const uint32_t some = __ballot_sync(0xffffffffu, take != 0);
+            if (!some) return;
+            const int mine = __popc(take);
+            int to = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, to, o);
+                if (lane >= o) to += y;
+            }
+            int at = 0;
+            if (lane == 31) at = int(atomicAdd(&s.listed, uint32_t(to)));
+            at = __shfl_sync(0xffffffffu, at, 31) + to - mine;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (take >> j & 1) {
+                    if (at < kList) s.list[at] = u64(key_of(v[j])) << 32 | (0xffffffffu - uint32_t(i0 + i + j));
+                    at++;
+                }
+        });
+    };
 
     uint32_t thr = 1;               // kept: keys above thr, and the first `ties` that equal it
     u64 ties = ~0ull;
+    bool radix_k = false, radix_p = false;
     if (k) {
-        u64 need = u64(k);
-        uint32_t prefix = 0;
-        bool all = false;           // fewer candidates than k: all are kept
-        for (int level = 0; level < 3 && !all; level++) {
-            clear(false);
-            for (int i = tid; i < n; i += kSampleThreads) {
-                const uint32_t key = key_of(at(i));
-                if (key && (key & above[level]) == prefix) atomicAdd(&s.hist[key >> shift[level] & (kBins - 1)], 1u);
-            }
-            gather(false);
-            if (level == 0) {
-                s.bin_out = -1;
+        each([&](float v, int) { atomicAdd(&s.low[r.bin(v)], 1u); });
+        gather(false);
+        int bin = 0;
+        u64 left = 0, all = 0;
+        select_bin<NT, false>(s, u64(k), bin, left, all);
+        if (bin >= 0) {
+            const u64 upto = k - left + s.total[bin];  // tokens of this bin and those before
+            __syncthreads();                           // (the list lies over the totals)
+            if (upto <= u64(kList)) {
+                // all of them sorted: the borders, and the pick among them, in the first CTA
+                list([&](float v) { return r.bin(v) <= bin; });
+                cl.sync();
+                int len = rank == 0 ? collect() : 0;
+                cl.sync();  // the others' lists have been read
+                if (rank) return;
+                sort_descending<NT>(s.sorted, len);
+                len = min(len, k);
+                // masses of the k first, and their running sum (over the list, which is done with)
+                u64* mass = s.list;
+                u64 total = 0;
+                for (int c0 = 0; c0 < len; c0 += NT) {
+                    const int i = c0 + tid;
+                    const u64 w = block_sums<NT>(s, i < len ? r.mass(value_of(uint32_t(s.sorted[i] >> 32))) : 0, total);
+                    if (i < len) mass[i] = w;
+                }
+                if (tid == 0) s.listed = 0;
                 __syncthreads();
+                const double want = ceil(double(p) * double(total));
+                const u64 need = !nucleus ? total : want < 1.0 ? 1 : min(total, __double2ull_rn(want));
+                for (int i = tid; i < len; i += NT)
+                    if (((i == 0 || mass[i - 1] < need) || !nucleus) && keeps(value_of(uint32_t(s.sorted[i] >> 32))))
+                        atomicAdd(&s.listed, 1u);  // a prefix: its length is its count
+                __syncthreads();
+                const int kept = max(1, int(s.listed));
+                total = mass[kept - 1];
+                const float u = a.u[row];
+                u64 target = u > 0.f ? __double2ull_rd(fmin(double(u), 1.0) * double(total)) : 0;
+                target = min(target, total - 1);
+                __syncthreads();
+                // by index: complement first, descending
+                for (int i = tid; i < kept; i += NT) s.sorted[i] = s.sorted[i] << 32 | s.sorted[i] >> 32;
+                __syncthreads();
+                sort_descending<NT>(s.sorted, kept);
+                u64 run = 0;
+                for (int c0 = 0; c0 < kept; c0 += NT) {
+                    const int i = c0 + tid;
+                    const u64 own = i < kept ? r.mass(value_of(uint32_t(s.sorted[i]))) : 0, w = block_sums<NT>(s, own, run);
+                    if (i < kept && w - own <= target && target < w) {
+                        a.token[row] = int32_t(0xffffffffu - uint32_t(s.sorted[i] >> 32));
+                        if (a.kept) a.kept[row] = kept;
+                        if (a.prob) a.prob[row] = float(r.weight(value_of(uint32_t(s.sorted[i]))) * 17592186044416.0 / double(total));
+                    }
+                }
+                return;
             }
-            int bin;
-            select_bin(s, need, bin, need);
-            if (level == 0 && bin < 0) all = true;
-            else prefix |= uint32_t(bin) << shift[level];
+            radix_k = true;
         }
-        if (!all) {
-            thr = prefix;
-            ties = need;
+        radix_p = nucleus;
+    } else if (nucleus) {
+        // The border lies above every weight under half of (1 - p) / vocab: all of those
+        // sum to less than 1 - p of the total.  They need no bins (a register holds their
+        // sum, which goes to the last bin).
+        const double edge = 0.5 * (1.0 - fmax(double(p), 0.0)) / double(a.vocab) * 17592186044416.0;
+        const u64 small = edge < 1.0 ? 0 : u64(edge);
+        u64 rest = 0;
+        quads([&](const float (&v)[4], int) {
+            u64 m[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) m[j] = r.mass(v[j]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (m[j] >= small) add_mass(r.bin(v[j]), m[j]);
+                else rest += m[j];
+            }
+        });
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
+        if (lane == 0) add_mass(kBins - 1, rest);
+        gather(true);
+        int bin = 0, sub = -1, m = 0;
+        u64 need = 0, left = 0, sum = 0;
+        select_bin<NT, false>(s, 0, bin, left, sum);
+        const double want = ceil(double(p) * double(sum));
+        need = want < 1.0 ? 1 : min(sum, __double2ull_rn(want));
+        select_bin<NT, false>(s, need, bin, left, sum);
+        auto inside = [&](float v) { return r.bin(v) == bin && (sub < 0 || r.part(v, bin) == sub); };
+        // what lies in the border's bin; in its part of the bin where that is too much
+        // to sort soon
+        constexpr int kSoon = 512;
+        while (true) {
+            __syncthreads();  // (the list lies over the totals)
+            list(inside);
+            cl.sync();
+            m = 0;
+            for (int c = 0; c < C; c++) m += int(*cl.map_shared_rank(&s.listed, c));
+            if (m <= (sub < 0 ? kSoon : kList) || sub >= 0) break;
+            cl.sync();  // the lists' lengths have been read
+            if (tid == 0) s.listed = 0;
+            clear();
+            each([&](float v, int) {
+                if (r.bin(v) == bin) add_mass(r.part(v, bin), r.mass(v));
+            });
+            gather(true);
+            select_bin<NT, false>(s, left, sub, left, sum);
+        }
+        if (m <= kList) {
+            collect();
+            cl.sync();  // every list has been read
+            sort_descending<NT>(s.sorted, m);
+            // the first whose running sum reaches what is needed inside the bin
+            u64 run = 0;
+            if (tid == 0) s.bin_out = m - 1;
+            for (int c0 = 0; c0 < m; c0 += NT) {
+                const int i = c0 + tid;
+                const u64 own = i < m ? r.mass(value_of(uint32_t(s.sorted[i] >> 32))) : 0, w = block_sums<NT>(s, own, run);
+                if (i < m && w - own < left && left <= w) s.bin_out = i;
+            }
+            __syncthreads();
+            const int last = max(0, s.bin_out);
+            thr = uint32_t(s.sorted[last] >> 32);
+            // its rank among the tokens that equal it (they lie side by side)
+            if (tid == 0) s.listed = 0;
+            __syncthreads();
+            for (int i = tid; i <= last; i += NT)
+                if (uint32_t(s.sorted[i] >> 32) == thr) atomicAdd(&s.listed, 1u);
+            __syncthreads();
+            ties = s.listed;
+        } else {
+            cl.sync();  // the lists' lengths have been read
+            radix_p = true;
         }
     }
-    if (nucleus) {
-        u64 need = 0;
+    // ---- radix selection, ten bits at a time from the top, where a list is too long ----
+    constexpr int shift[4] = {22, 12, 2, 0};
+    constexpr uint32_t above[4] = {0u, 0xffc00000u, 0xfffff000u, 0xfffffffcu};  // bits that earlier levels have fixed
+    constexpr uint32_t digits[4] = {1023u, 1023u, 1023u, 3u};
+    if (radix_k) {
+        u64 need = u64(k), all;
         uint32_t prefix = 0;
-        for (int level = 0; level < 3; level++) {
-            clear(true);
-            for (int i = tid; i < n; i += kSampleThreads) {
-                const float v = at(i);
+        for (int level = 0; level < 4; level++) {
+            clear();
+            each([&](float v, int) {
                 const uint32_t key = key_of(v);
-                if (key && (key & above[level]) == prefix && (key > thr || (key == thr && ties == ~0ull)))
-                    add_mass(key >> shift[level] & (kBins - 1), r.mass(v));
-            }
+                if ((key & above[level]) == prefix) atomicAdd(&s.low[key >> shift[level] & digits[level]], 1u);
+            });
+            gather(false);
+            int bin;
+            select_bin<NT, true>(s, need, bin, need, all);
+            prefix |= uint32_t(bin) << shift[level];
+        }
+        thr = prefix;
+        ties = need;
+    }
+    if (radix_p) {
+        u64 need = 0, all;
+        uint32_t prefix = 0;
+        int bin;
+        for (int level = 0; level < 4; level++) {
+            clear();
+            each([&](float v, int) {
+                const uint32_t key = key_of(v);
+                if ((key & above[level]) == prefix && (key > thr || (key == thr && ties == ~0ull)))
+                    add_mass(key >> shift[level] & digits[level], r.mass(v));
+            });
             // top-k's ties, once for the row
-            if (rank == 0 && tid == 0 && ties != ~0ull && (thr & above[level]) == prefix) {
-                add_mass(thr >> shift[level] & (kBins - 1), r.mass(value_of(thr)) * ties);
-            }
+            if (rank == 0 && tid == 0 && ties != ~0ull && (thr & above[level]) == prefix)
+                add_mass(thr >> shift[level] & digits[level], r.mass(value_of(thr)) * ties);
             gather(true);
             if (level == 0) {
-                u64 sum = 0;
-                for (int b = lane; b < kBins; b += 32) sum += s.total[b];
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                const double want = ceil(double(p) * double(sum));
-                need = want < 1.0 ? 1 : min(sum, __double2ull_rn(want));
+                select_bin<NT, true>(s, 0, bin, need, all);
+                const double want = ceil(double(p) * double(all));
+                need = want < 1.0 ? 1 : min(all, __double2ull_rn(want));
             }
-            int bin;
-            select_bin(s, need, bin, need);
+            select_bin<NT, true>(s, need, bin, need, all);
             prefix |= uint32_t(bin) << shift[level];
         }
         const u64 w = r.mass(value_of(prefix)), m = (need + w - 1) / w;
@@ -256,89 +606,117 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
         }
     }
     // ---- masses, counts and ties of the warps' segments, in index order ----
-    const int seg = a.slice / kSampleWarps, j0 = min(n, warp * seg), j1 = min(n, j0 + seg);
-    auto keeps = [&](float v) { return !(low > 0.f) || r.weight(v) >= double(low); };
+    const int seg = a.slice / W, j0 = min(n, warp * seg), j1 = min(n, j0 + seg);
     const u64 tie_mass = r.mass(value_of(thr));
     const bool tie_kept = keeps(value_of(thr));
     u64 mass = 0;
     uint32_t count = 0, tied = 0;
-    for (int i = j0 + lane; i < j1; i += 32) {
-        const float v = at(i);
-        const uint32_t key = key_of(v);
-        if (key > thr && keeps(v)) {
-            mass += r.mass(v);
-            count++;
+    for (int i = j0 + 4 * lane; i < j1; i += 128) {
+        float v[4];
+        four(i, v);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t key = i + j < j1 ? key_of(v[j]) : 0;
+            if (!(key > thr && keeps(v[j]))) v[j] = -INFINITY;
+            count += v[j] > -INFINITY;
+            tied += key == thr && tie_kept;
         }
-        tied += key == thr && tie_kept;
+        if (max(max(v[0], v[1]), max(v[2], v[3])) > -INFINITY) mass += r.mass(v[0]) + r.mass(v[1]) + r.mass(v[2]) + r.mass(v[3]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
     count = __reduce_add_sync(0xffffffffu, count);
     tied = __reduce_add_sync(0xffffffffu, tied);
     if (lane < C) {
-        const int to = rank * kSampleWarps + warp;
+        const int to = rank * W + warp;
         cl.map_shared_rank(s.seg_mass, lane)[to] = mass;
         cl.map_shared_rank(s.seg_count, lane)[to] = count;
         cl.map_shared_rank(s.seg_ties, lane)[to] = tied;
     }
     cl.sync();
-    u64 total = 0, before = 0;       // the row's kept mass; that of the segments before this warp's
-    u64 ties_before = 0, ties_all = 0, count_all = 0;
-    const int me = rank * kSampleWarps + warp;
-    for (int w = 0; w < C * kSampleWarps; w++) {
-        if (w == me) before = total, ties_before = ties_all;
-        const u64 t = s.seg_ties[w], taken = ties_all >= ties ? 0 : min(t, ties - ties_all);
-        total += s.seg_mass[w] + taken * tie_mass;
-        count_all += s.seg_count[w] + taken;
-        ties_all += t;
-    }
-    const float u = a.u[row];
-    // the first token with cumulated mass > target
-    u64 target = u > 0.f ? __double2ull_rd(fmin(double(u), 1.0) * double(total)) : 0;
-    target = min(target, total - 1);
-    u64 run = before, seen = ties_before;
-    const u64 mine = s.seg_mass[me] + (seen >= ties ? 0 : min(u64(s.seg_ties[me]), ties - seen)) * tie_mass;
-    if (before <= target && target < before + mine) {
-        for (int i = j0; i < j1; i += 32) {
-            u64 w = 0;
-            float v = 0.f;
-            uint32_t key = 0;
-            if (i + lane < j1) {
-                v = at(i + lane);
-                key = key_of(v);
-            }
-            const bool tie = key == thr && tie_kept && key;
-            const uint32_t b = __ballot_sync(0xffffffffu, tie);
-            if (tie && seen + __popc(b & ((1u << lane) - 1)) < ties) w = tie_mass;
-            else if (key > thr && keeps(v)) w = r.mass(v);
-            seen += __popc(b);
-            u64 incl = w;
+    // four segments to a lane of the first warp; ties go to the first by index
+    constexpr int PER = kSampleClusters * W / 32;
+    if (warp == 0) {
+        u64 t[PER], m[PER], c = 0, tsum = 0;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const u64 y = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += y;
-            }
-            const uint32_t over = __ballot_sync(0xffffffffu, run + incl > target);
-            if (over) {
-                if (lane == __ffs(over) - 1) {
-                    a.token[row] = i0 + i + lane;
-                    if (a.kept) a.kept[row] = int32_t(count_all);
-                    if (a.prob) a.prob[row] = float(r.weight(v) * 17592186044416.0 / double(total));
-                }
-                break;
-            }
-            run += __shfl_sync(0xffffffffu, incl, 31);
+        for (int j = 0; j < PER; j++) {
+            const int w = lane * PER + j;
+            t[j] = w < C * W ? s.seg_ties[w] : 0;
+            tsum += t[j];
         }
+        u64 tb = tsum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 y = __shfl_up_sync(0xffffffffu, tb, o);
+            if (lane >= o) tb += y;
+        }
+        tb -= tsum;
+        u64 msum = 0, before[PER];
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int w = lane * PER + j;
+            const u64 taken = tb >= ties ? 0 : min(t[j], ties - tb);
+            before[j] = tb;
+            tb += t[j];
+            m[j] = taken * tie_mass + (w < C * W ? s.seg_mass[w] : 0);
+            c += taken + (w < C * W ? s.seg_count[w] : 0);
+            msum += m[j];
+        }
+        u64 mb = msum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 y = __shfl_up_sync(0xffffffffu, mb, o);
+            if (lane >= o) mb += y;
+        }
+        const u64 total = __shfl_sync(0xffffffffu, mb, 31);
+        mb -= msum;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+        const float u = a.u[row];
+        // the first token with cumulated mass > target
+        u64 target = u > 0.f ? __double2ull_rd(fmin(double(u), 1.0) * double(total)) : 0;
+        target = min(target, total - 1);
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            if (mb <= target && target < mb + m[j]) {
+                s.pick_seg = lane * PER + j;
+                s.pick_before = target - mb;  // still to pass inside the segment
+                s.pick_ties = before[j];
+                s.pick_total = total;
+                s.pick_count = c;
+            }
+            mb += m[j];
+        }
+    }
+    __syncthreads();
+    if (s.pick_seg / W != rank) return;
+    const int from = min(n, s.pick_seg % W * seg), to = min(n, from + seg);
+    u64 run = 0, seen = s.pick_ties;
+    const u64 target = s.pick_before;
+    for (int c0 = from; c0 < to; c0 += NT) {
+        const int i = c0 + tid;
+        const float v = i < to ? to_f32(holds ? held[i] : x[i0 + i]) : 0.f;
+        const uint32_t key = i < to ? key_of(v) : 0;
+        const bool tie = key && key == thr && tie_kept;
+        const u64 rank_of = block_sums<NT>(s, tie, seen);  // this one counted
+        const u64 own = tie ? (rank_of <= ties ? tie_mass : 0) : key > thr && keeps(v) ? r.mass(v) : 0;
+        const u64 w = block_sums<NT>(s, own, run);
+        if (w - own <= target && target < w) {
+            a.token[row] = i0 + i;
+            if (a.kept) a.kept[row] = int32_t(s.pick_count);
+            if (a.prob) a.prob[row] = float(r.weight(v) * 17592186044416.0 / double(s.pick_total));
+        }
+        if (run > target) break;
     }
 }
 
-template <class T>
+template <class T, int NT>
 void launch_sample(const SampleArgs& a, int rows, int ctas, size_t smem, cudaStream_t st) {
     static unsigned long long done = 0;
-    allow_smem(sample_kernel<T>, sizeof(Shared) + kSampleSlice * sizeof(float), done);
+    allow_smem(sample_kernel<T, NT>, sizeof(Shared) + kSampleSlice, done);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(rows) * unsigned(ctas));
-    cfg.blockDim = dim3(kSampleThreads);
+    cfg.blockDim = dim3(NT);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -347,7 +725,15 @@ void launch_sample(const SampleArgs& a, int rows, int ctas, size_t smem, cudaStr
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    CUDA_OK(cudaLaunchKernelEx(&cfg, sample_kernel<T>, a));
+    CUDA_OK(cudaLaunchKernelEx(&cfg, sample_kernel<T, NT>, a));
+}
+
+template <class T>
+void launch_type(const SampleArgs& a, int rows, int ctas, size_t smem, cudaStream_t st) {
+    // While every CTA has an SM to itself, 1024 threads shorten its passes; beyond
+    // that two CTAs of 512 to an SM hide each other's barriers.
+    if (int64_t(rows) * ctas <= device_sms()) launch_sample<T, 1024>(a, rows, ctas, smem, st);
+    else launch_sample<T, 512>(a, rows, ctas, smem, st);
 }
 
 }  // namespace
@@ -371,12 +757,13 @@ spm_status spm_sample(int device, uint32_t dtype, const void* logits, int64_t ro
         // a CTA for every 2048 logits, eight at most
         int ctas = 1;
         while (ctas < kSampleClusters && vocab > 2048 * ctas) ctas *= 2;
-        const int per = kSampleThreads;  // 32 for each warp
+        const int per = 4 * 32;  // four for each warp, of 32 at most
         a.slice = ((vocab + ctas - 1) / ctas + per - 1) / per * per;
-        const size_t smem = sizeof(Shared) + (a.slice <= kSampleSlice ? size_t(a.slice) * sizeof(float) : 0);
+        const size_t bytes = size_t(a.slice) * (dtype == SPM_F32 ? 4 : 2);
+        const size_t smem = sizeof(Shared) + (bytes <= size_t(kSampleSlice) ? bytes : 0);
         const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
-        if (dtype == SPM_F32) launch_sample<float>(a, rows, ctas, smem, st);
-        else if (dtype == SPM_F16) launch_sample<__half>(a, rows, ctas, smem, st);
-        else launch_sample<__nv_bfloat16>(a, rows, ctas, smem, st);
+        if (dtype == SPM_F32) launch_type<float>(a, rows, ctas, smem, st);
+        else if (dtype == SPM_F16) launch_type<__half>(a, rows, ctas, smem, st);
+        else launch_type<__nv_bfloat16>(a, rows, ctas, smem, st);
     });
 }
