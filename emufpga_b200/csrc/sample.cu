@@ -77,7 +77,7 @@ struct alignas(16) Shared {
     u64 scan[32];
     u64 need_out, seg_mass[kSampleClusters * 32];
     uint32_t seg_count[kSampleClusters * 32], seg_ties[kSampleClusters * 32];
-    uint32_t top[kSampleClusters];        // each CTA's largest key
+    float top[kSampleClusters];           // each CTA's largest logit
     uint32_t listed;                      // length of this CTA's list
     int bin_out;
     u64 pick_before, pick_ties, pick_total, pick_count;
@@ -112,6 +112,10 @@ struct Row {
     // The bin of a candidate's distance from the top; ascending as x descends.
     __device__ __forceinline__ float place(float x) const { return fminf(x == INFINITY ? 0.f : distance(x) * bins, float(kBins - 1)); }
     __device__ __forceinline__ int bin(float x) const { return int(place(x)); }
+    __device__ __forceinline__ bool in_bin(float x, int b) const {
+        const float p = place(x);
+        return p >= float(b) && p < float(b + 1);
+    }
     // And the 1024th part of bin b.
     __device__ __forceinline__ int part(float x, int b) const {
         return int(fminf((place(x) - float(b)) * float(kBins), float(kBins - 1)));
@@ -270,15 +274,15 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     };
     cg::cluster_group::arrival_token started = cl.barrier_arrive();
 
-    // ---- the slice into shared memory; the largest key ----
-    uint32_t top = 0;
+    // ---- the slice into shared memory; the largest logit (NaN is none) ----
+    float top = -INFINITY;
     {
         constexpr int V = 16 / sizeof(T);
         const T* from = x + i0;
         const int head = min(n, int((16 - (reinterpret_cast<uintptr_t>(from) & 15)) & 15) / int(sizeof(T)));
         auto take = [&](int i, T v) {
             if (holds) held[i] = v;
-            top = max(top, key_of(to_f32(v)));
+            top = fmaxf(top, to_f32(v));
         };
         if (tid < head) take(tid, from[tid]);
         const int whole = (n - head) / V;
@@ -287,8 +291,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
         for (int i = tid; i < whole; i += NT) {
             const uint4 q = __ldcs(wide + i);
             const T* e = reinterpret_cast<const T*>(&q);
+            if (holds && head == 0) reinterpret_cast<uint4*>(held)[i] = q;
 #pragma unroll
-            for (int j = 0; j < V; j++) take(head + V * i + j, e[j]);
+            for (int j = 0; j < V; j++) {
+                if (head == 0) top = fmaxf(top, to_f32(e[j]));
+                else take(head + V * i + j, e[j]);
+            }
         }
         const int rest = head + V * whole;
         if (tid < n - rest) take(rest + tid, from[rest + tid]);
@@ -297,21 +305,20 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     if (tid < kTable) s.table[tid] = exp2(double(tid) / kTable);
     for (int b = tid; b < kBins; b += NT) s.low[b] = s.mid[b] = s.high[b] = 0;
     if (tid == 0) s.listed = 0;
-    top = __reduce_max_sync(0xffffffffu, top);
-    uint32_t* tops = reinterpret_cast<uint32_t*>(s.scan);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float* tops = reinterpret_cast<float*>(s.scan);
     if (lane == 0) tops[warp] = top;
     cl.barrier_wait(std::move(started));  // every CTA runs
     __syncthreads();
     if (tid < C) {
-        top = 0;
 #pragma unroll 8
-        for (int w = 0; w < W; w++) top = max(top, tops[w]);
+        for (int w = 0; w < W; w++) top = fmaxf(top, tops[w]);
         cl.map_shared_rank(s.top, tid)[rank] = top;
     }
     cl.sync();
-    top = 0;
-    for (int c = 0; c < C; c++) top = max(top, s.top[c]);
-    if (top == 0) {  // the same for the whole cluster
+    for (int c = 0; c < C; c++) top = fmaxf(top, s.top[c]);
+    if (top == -INFINITY) {  // the same for the whole cluster
         if (rank == 0 && tid == 0) {
             a.token[row] = -1;
             if (a.kept) a.kept[row] = 0;
@@ -322,7 +329,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     const float temp = a.temperature ? a.temperature[row] : 1.f;
     const bool greedy = !(temp > 0.f);
     Row r;
-    r.ftop = value_of(top);
+    r.ftop = top;
     r.top = double(r.ftop);
     r.inv = greedy ? 1.0 : 1.0 / double(temp);
     r.slope = r.inv * -1.4426950408889634074 * kTable;
@@ -433,7 +440,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
             __syncthreads();                           // (the list lies over the totals)
             if (upto <= u64(kList)) {
                 // all of them sorted: the borders, and the pick among them, in the first CTA
-                list([&](float v) { return r.bin(v) <= bin; });
+                list([&](float v) { return r.place(v) < float(bin + 1); });
                 cl.sync();
                 int len = rank == 0 ? collect() : 0;
                 cl.sync();  // the others' lists have been read
@@ -508,7 +515,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
         const double want = ceil(double(p) * double(sum));
         need = want < 1.0 ? 1 : min(sum, __double2ull_rn(want));
         select_bin<NT, false>(s, need, bin, left, sum);
-        auto inside = [&](float v) { return r.bin(v) == bin && (sub < 0 || r.part(v, bin) == sub); };
+        auto inside = [&](float v) { return r.in_bin(v, bin) && (sub < 0 || r.part(v, bin) == sub); };
         // what lies in the border's bin; in its part of the bin where that is too much
         // to sort soon
         constexpr int kSoon = 512;
@@ -523,7 +530,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
             if (tid == 0) s.listed = 0;
             clear();
             each([&](float v, int) {
-                if (r.bin(v) == bin) add_mass(r.part(v, bin), r.mass(v));
+                if (r.in_bin(v, bin)) add_mass(r.part(v, bin), r.mass(v));
             });
             gather(true);
             select_bin<NT, false>(s, left, sub, left, sum);
@@ -605,24 +612,46 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
             ties = m;
         }
     }
+    // ---- min-p as a threshold of its own: the least logit that keeps() takes ----
+    float cut = thr == 1 ? -INFINITY : value_of(thr);  // kept: above it, and `ties` of its equals
+    if (floored) {
+        // by bisection over the keys, from a few around the rounded border where they hold it
+        const float near = fminf(fmaxf(float(r.top - reach * double(temp)), -3.402823466e38f), r.ftop);
+        uint32_t no = 0x007fffffu, yes = key_of(r.ftop);  // below every finite key; the top is kept
+        const uint32_t mid = key_of(near);
+        if (mid > no + 4 && !keeps(value_of(mid - 4))) no = mid - 4;
+        if (mid + 4 < yes && keeps(value_of(mid + 4))) yes = mid + 4;
+        while (yes - no > 1) {
+            const uint32_t k = no + (yes - no) / 2;
+            if (keeps(value_of(k))) yes = k;
+            else no = k;
+        }
+        const float v = value_of(yes);
+        if (v > cut) {
+            cut = v;
+            ties = ~0ull;
+        }
+    }
     // ---- masses, counts and ties of the warps' segments, in index order ----
     const int seg = a.slice / W, j0 = min(n, warp * seg), j1 = min(n, j0 + seg);
-    const u64 tie_mass = r.mass(value_of(thr));
-    const bool tie_kept = keeps(value_of(thr));
+    const u64 tie_mass = r.mass(cut);
     u64 mass = 0;
     uint32_t count = 0, tied = 0;
     for (int i = j0 + 4 * lane; i < j1; i += 128) {
         float v[4];
         four(i, v);
+        bool some = false;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const uint32_t key = i + j < j1 ? key_of(v[j]) : 0;
-            if (!(key > thr && keeps(v[j]))) v[j] = -INFINITY;
+            const bool in = i + j < j1;
+            tied += in && v[j] == cut;
+            v[j] = in && v[j] > cut ? v[j] : -INFINITY;
             count += v[j] > -INFINITY;
-            tied += key == thr && tie_kept;
+            some |= v[j] > -INFINITY;
         }
-        if (max(max(v[0], v[1]), max(v[2], v[3])) > -INFINITY) mass += r.mass(v[0]) + r.mass(v[1]) + r.mass(v[2]) + r.mass(v[3]);
+        if (some) mass += r.mass(v[0]) + r.mass(v[1]) + r.mass(v[2]) + r.mass(v[3]);
     }
+    if (cut == -INFINITY) tied = 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
     count = __reduce_add_sync(0xffffffffu, count);
@@ -696,10 +725,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     for (int c0 = from; c0 < to; c0 += NT) {
         const int i = c0 + tid;
         const float v = i < to ? to_f32(holds ? held[i] : x[i0 + i]) : 0.f;
-        const uint32_t key = i < to ? key_of(v) : 0;
-        const bool tie = key && key == thr && tie_kept;
+        const bool tie = i < to && v == cut && cut > -INFINITY;
         const u64 rank_of = block_sums<NT>(s, tie, seen);  // this one counted
-        const u64 own = tie ? (rank_of <= ties ? tie_mass : 0) : key > thr && keeps(v) ? r.mass(v) : 0;
+        const u64 own = tie ? (rank_of <= ties ? tie_mass : 0) : i < to && v > cut ? r.mass(v) : 0;
         const u64 w = block_sums<NT>(s, own, run);
         if (w - own <= target && target < w) {
             a.token[row] = i0 + i;
