@@ -27,6 +27,11 @@ STATUS = {11: "a length is negative or past its table", 12: "more pages wanted t
           15: "a page or slot is not in the pool", 16: "a request's rows are not what the call says"}
 
 
+_I32 = torch.int32
+# the current stream's handle (torch.cuda.current_stream builds an object around it, 2 us)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _dtype(t: torch.Tensor, what: str) -> int:
     code = DTYPES.get(t.dtype)
     if code is None:
@@ -34,24 +39,26 @@ def _dtype(t: torch.Tensor, what: str) -> int:
     return code
 
 
-def _i32(t: torch.Tensor, what: str, device, shape=None) -> int:
-    if t.dtype is not torch.int32 or t.device != device or not t.is_contiguous():
-        raise SpmError(-1, f"{what} must be a contiguous int32 tensor on {device}")
-    if shape is not None and t.shape != shape:
-        raise SpmError(-1, f"{what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+def _i32(t: torch.Tensor, what: str, index: int, n: int | None = None) -> int:
+    """The address of a contiguous int32 tensor of n values on device `index`."""
+    if t.dtype is not _I32 or t.get_device() != index or not t.is_contiguous():
+        raise SpmError(-1, f"{what} must be a contiguous int32 tensor on cuda:{index}")
+    if n is not None and t.numel() != n:
+        raise SpmError(-1, f"{what} must have {n} values, got {t.numel()}")
     return t.data_ptr()
 
 
-def _cuda(t: torch.Tensor, what: str) -> torch.device:
-    if not t.is_cuda:
+def _cuda(t: torch.Tensor, what: str) -> int:
+    index = t.get_device()
+    if index < 0:
         raise SpmError(-1, f"{what} must be a CUDA tensor")
-    return t.device
+    return index
 
 
-def _on(device, stream):
+def _on(index: int, stream):
     """The raw stream to launch on, and a context in which scratch is allocated for it."""
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream, contextlib.nullcontext()
+        return _raw_stream(index), contextlib.nullcontext()
     return stream.cuda_stream, torch.cuda.stream(stream)
 
 
@@ -80,22 +87,21 @@ def plan(cached, new, table, free, count, page_tokens: int, tokens: int, ended=N
     back first.  ``free`` is the stack of free pages, ``count`` its height (one
     int32), ``left`` (default: ``count``) receives the new height.  ``tokens``
     is the length of the slot map, -1 behind the last token."""
-    device = _cuda(table, "table")
+    index = _cuda(table, "table")
     if table.dim() != 2:
         raise SpmError(-1, "table must be requests x width")
     R, width = table.shape
-    rows, one = torch.Size((R,)), torch.Size((1,))
     left = count if left is None else left
     if tokens < 0:
         raise SpmError(-1, "negative token count")
-    args = (device.index, _i32(cached, "cached", device, rows), _i32(new, "new", device, rows),
-            None if ended is None else _i32(ended, "ended", device, rows), R, page_tokens, _i32(table, "table", device),
-            width, _i32(free, "free", device), free.numel(), _i32(count, "count", device, one),
-            _i32(left, "left", device, one), tokens)
-    word = None if status is None else _i32(status, "status", device, one)
-    raw, scratch = _on(device, stream)
+    args = (index, _i32(cached, "cached", index, R), _i32(new, "new", index, R),
+            None if ended is None else _i32(ended, "ended", index, R), R, page_tokens, _i32(table, "table", index),
+            width, _i32(free, "free", index), free.numel(), _i32(count, "count", index, 1),
+            _i32(left, "left", index, 1), tokens)
+    word = None if status is None else _i32(status, "status", index, 1)
+    raw, scratch = _on(index, stream)
     with scratch:
-        maps = torch.empty(2 * R + 1 + 2 * tokens, dtype=torch.int32, device=device)
+        maps = table.new_empty(2 * R + 1 + 2 * tokens)
     starts, lens, positions, slots = maps.split((R + 1, R, tokens, tokens))
     at = maps.data_ptr()
     call("spm_page_plan", *args, at, at + 4 * (R + 1), at + 4 * (2 * R + 1), at + 4 * (2 * R + 1 + tokens), word, raw)
@@ -140,7 +146,8 @@ class Cache:
         return self
 
     def _take(self, k_codes, k_scales, v_codes, v_scales) -> None:
-        dev = _cuda(k_codes, "codes")
+        self._index = _cuda(k_codes, "codes")
+        dev = k_codes.device
         if k_codes.dim() != 4:
             raise SpmError(-1, "codes must be pages x kv_heads x page_tokens x head_dim")
         for c, s in ((k_codes, k_scales), (v_codes, v_scales)):
@@ -152,7 +159,7 @@ class Cache:
         self.pages, self.kv_heads, self.page_tokens, self.head_dim = k_codes.shape
         self.device = dev
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
-        self._c = Kv8(dev.index, self.pages, self.page_tokens, self.kv_heads, self.head_dim, 0, k_codes.data_ptr(),
+        self._c = Kv8(self._index, self.pages, self.page_tokens, self.kv_heads, self.head_dim, 0, k_codes.data_ptr(),
                       v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), self.status.data_ptr())
         self._ref = C.byref(self._c)
         self._work: dict = {}
@@ -169,7 +176,7 @@ class Cache:
 
     def _rows(self, t, what: str) -> int:
         """Checks [tokens, heads, head_dim] rows (any strides over tokens and heads)."""
-        if t.dim() != 3 or t.shape[2] != self.head_dim or t.device != self.device:
+        if t.dim() != 3 or t.shape[2] != self.head_dim or t.get_device() != self._index:
             raise SpmError(-1, f"{what} must be tokens x heads x {self.head_dim} on {self.device}")
         if t.stride(2) != 1 and t.numel():
             raise SpmError(-1, f"{what} must be contiguous along head_dim")
@@ -180,8 +187,8 @@ class Cache:
         kp, vp = self._rows(k, "k"), self._rows(v, "v")
         if k.shape != v.shape or k.dtype is not v.dtype or k.shape[1] != self.kv_heads:
             raise SpmError(-1, f"k and v must be of one type, tokens x {self.kv_heads} x {self.head_dim}")
-        sp = _i32(slots, "slots", self.device, k.shape[:1])
-        raw = (stream or torch.cuda.current_stream(self.device)).cuda_stream
+        sp = _i32(slots, "slots", self._index, k.shape[0])
+        raw = _raw_stream(self._index) if stream is None else stream.cuda_stream
         call("spm_kv8_append", self._ref, _dtype(k, "k"), kp, k.stride(0), k.stride(1), vp, v.stride(0), v.stride(1),
              k.shape[0], sp, raw)
 
@@ -189,10 +196,10 @@ class Cache:
         """The values (k, v) that whole pages stand for: [n, kv_heads, page_tokens, head_dim] for the int32
         page numbers ``pages``, or for all (spm_kv8_values)."""
         n = self.pages if pages is None else pages.numel()
-        ids = None if pages is None else _i32(pages, "pages", self.device)
+        ids = None if pages is None else _i32(pages, "pages", self._index)
         if dtype not in DTYPES:
             raise SpmError(-5, "values are float32, float16 or bfloat16")
-        raw, scratch = _on(self.device, stream)
+        raw, scratch = _on(self._index, stream)
         with scratch:
             out = torch.empty((2, n, self.kv_heads, self.page_tokens, self.head_dim), dtype=dtype, device=self.device)
         k, v = out.unbind(0)
@@ -211,9 +218,9 @@ class Cache:
         if table.dim() != 2:
             raise SpmError(-1, "table must be requests x width")
         R, width = table.shape
-        args = (_i32(starts, "starts", self.device, torch.Size((R + 1,))), _i32(lens, "lens", self.device, table.shape[:1]),
-                R, most, _i32(table, "table", self.device), width)
-        raw, scratch = _on(self.device, stream)
+        args = (_i32(starts, "starts", self._index, R + 1), _i32(lens, "lens", self._index, R), R, most,
+                _i32(table, "table", self._index), width)
+        raw, scratch = _on(self._index, stream)
         need = self._bytes(H, R, most, width)
         with scratch:
             if out is None:

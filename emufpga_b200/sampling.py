@@ -46,7 +46,7 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, stre
 
     temperature, top_p, min_p (float32) and top_k (int32) are tensors of one
     value per row, or None for off; see spm_sample for what they do."""
-    device = _cuda(logits, "logits")
+    index = _cuda(logits, "logits")
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise SpmError(-1, "logits must be rows x vocab, contiguous along vocab")
     n, vocab = logits.shape
@@ -54,8 +54,8 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, stre
     def per_row(t, what, dtype=torch.float32):
         if t is None:
             return None
-        if t.dtype is not dtype or t.device != device or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
-            raise SpmError(-1, f"{what} must be a contiguous {dtype} tensor of one value per row on {device}")
+        if t.dtype is not dtype or t.get_device() != index or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+            raise SpmError(-1, f"{what} must be a contiguous {dtype} tensor of one value per row on cuda:{index}")
         return t.data_ptr()
 
     if u is None:
@@ -63,11 +63,9 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, stre
     args = (per_row(temperature, "temperature"), per_row(top_k, "top_k", torch.int32), per_row(top_p, "top_p"),
             per_row(min_p, "min_p"), per_row(u, "u"))
     dt = _dtype(logits, "logits")
-    raw, scratch = _on(device, stream)
+    raw, scratch = _on(index, stream)
     with scratch:
-        out = torch.empty((3, n), dtype=torch.int32, device=device)
-    at = out.data_ptr()
-    call("spm_sample", device.index, dt, logits.data_ptr(), logits.stride(0), n, vocab, *args, at, at + 4 * n, at + 8 * n,
-         raw)
-    token, kept, prob = out.unbind(0)
-    return Picks(token, kept, prob.view(torch.float32))
+        token, kept, prob = (u.new_empty(n, dtype=t) for t in (torch.int32, torch.int32, torch.float32))
+    call("spm_sample", index, dt, logits.data_ptr(), logits.stride(0), n, vocab, *args, token.data_ptr(), kept.data_ptr(),
+         prob.data_ptr(), raw)
+    return Picks(token, kept, prob)
