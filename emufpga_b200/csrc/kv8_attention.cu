@@ -9,21 +9,22 @@
 // for the accumulator, which then holds sum_j 2^(s_j + f_j - r) V_j with every
 // weight at most 1: it fits fp16 whatever the pages' scales are.
 //
-// Products on the tensor cores (mma.sync m16n8k16, fp16 in, fp32 out): int8 codes
-// are exact in fp16.  Queries are scaled per row to 2^10 and split into fp16 high
-// and low parts where they are f32 (22 bits; one part holds a bf16 or f16), the
-// weights likewise.  The 16 rows of an mma are cached tokens (or, for the values,
-// head dimensions) and its 8 columns are query rows (tokens x heads of the group),
-// so that one conversion of the codes serves every query of a kv head:
-//   codes: ldmatrix brings 4 bytes of a row to each lane; byte permutes make
-//   0x6400 | (code + 128) = 1024 + 128 + code in fp16, and one subtraction of 1152
-//   the code.  The order of dimensions within an mma's k is free, so the queries
-//   are laid out to match the bytes; for the values (transposed by ldmatrix) the
-//   even and odd dimensions of a 16-byte column become rows g and g + 8.
+// Products on the tensor cores (mma.sync).  The 16 rows of an mma are cached tokens
+// (or, for the values, head dimensions) and its 8 columns are query rows (tokens x
+// heads of the group), so that one pass over the codes serves every query of a kv
+// head.
+//   Scores: int8 x int8 (m16n8k32).  The codes go in as they lie; a query row is
+//   fixed point to its largest value, 22 bits in three signed 8-bit digits (two, 14
+//   bits, would gain 2% of a long decode).  Sums are exact in int32.
+//   Values: fp16 x fp16 (m16n8k16), fp32 sums.  The codes are exact in fp16: byte
+//   permutes make 0x6400 | (code + 128) = 1024 + 128 + code and a subtraction of 1152
+//   the code.  Weights are fp16 (a floating type: a long tail of small ones counts),
+//   high and low part (22 bits) where the result is f32.  ldmatrix transposes pairs
+//   of bytes: the even and odd dimensions of a 16-byte column become rows g and g + 8.
 //
-// What bounds it is the cache's bytes.  Each warp streams its own 32 tokens at a
-// time through a ring in shared memory (16-byte asynchronous copies, no barrier
-// among warps).  Work is cut into units of 128 tokens of a (row tile, kv head),
+// What bounds it is the cache's bytes.  Each warp streams its own 32 tokens (16 where
+// head_dim is over 128) at a time through a ring in shared memory (16-byte asynchronous copies, no barrier
+// among warps).  Work is cut into units of four such steps of a (row tile, kv head),
 // and every CTA takes an equal run of the units of all requests, so that ragged
 // lengths load all SMs alike; where a run ends inside a (row tile, kv head) its
 // partial goes to the workspace and kv8_combine_kernel adds the parts in order.
@@ -62,6 +63,17 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_fast(float x) {  // to 2^-22
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // Bytes of x (already + 128) picked by SEL, as two fp16 codes.
 template <uint32_t SEL>
 __device__ __forceinline__ uint32_t codes2(uint32_t x) {
@@ -89,6 +101,7 @@ __device__ __forceinline__ float exponent_of(float s) {
 
 template <int HD, int NT, int NP>
 struct DecSmem {
+    static constexpr int sub = kv8_sub(HD);
     // a token's codes: the eight rows that an ldmatrix reads lie on distinct banks,
     // by an exclusive or of the 16-byte chunk with the row where a row fills whole
     // bank sweeps, else by 16 bytes between the rows
@@ -99,11 +112,10 @@ struct DecSmem {
         if (HD % 128 == 0) return r * row + ((chunk ^ (r & 7)) << 4);
         return r * row + (chunk << 4);
     }
-    // CTAs that an SM's shared memory takes
-    static constexpr int per_sm() { return total * 2 + 2048 <= 227 * 1024 ? 2 : 1; }
-    static constexpr int stage = 2 * kDecSub * row + 16;      // keys, values, then 2 + 2 scales
-    static constexpr int q = 0;                               // [NP][NT][HD / 16][32 lanes][4 halves]
-    static constexpr int qbytes = NP * NT * HD * 16;
+    static constexpr int digits = 3;                          // of a query value
+    static constexpr int stage = 2 * sub * row + 16;          // keys, values, then 2 + 2 scales
+    static constexpr int q = 0;                               // [digits][NT][HD / 32][32 lanes][8]
+    static constexpr int qbytes = digits * NT * HD * 8;
     static constexpr int qscale = q + qbytes;                 // [8 NT] floats
     static constexpr int ring = (qscale + 8 * NT * 4 + 15) & ~15;
     static constexpr int state = HD + 4;                      // a row's accumulator, then m, r, l
@@ -115,11 +127,12 @@ struct DecSmem {
 template <int HD, int NT, int NP>
 __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a) {
     using L = DecSmem<HD, NT, NP>;
-    constexpr int NR = 8 * NT, KB = HD / 32;
+    constexpr int NR = 8 * NT, KB = HD / 32, SUB = L::sub, NB = SUB / 16, UNIT = kDecWarps * SUB, PL = L::digits;
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ long long wsum[kDecWarps], found[2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int V = a.requests * a.tiles;  // (request, row tile) pairs
+    pdl_trigger();  // (kv8_combine_kernel's CTAs may come and wait: all of this grid's are resident)
 
     // ---- this CTA's run of units ----
     auto block_scan = [&](long long x, long long& before) {  // exclusive sum over threads, and the total
@@ -141,32 +154,30 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
         }
         return total;
     };
-    long long total = 0;
+    // (request, row tile) pairs by the thread; one look at the lengths is enough for up
+    // to as many pairs as threads
+    auto units_of = [&](int v) { return v < V ? (long long)kv8_units(a, v) * a.kv_heads : 0; };
+    long long total = 0, mine = 0, before = 0;
     for (int v0 = 0; v0 < V; v0 += kDecThreads) {
-        long long before;
-        const int v = v0 + tid;
-        const long long n = v < V ? (long long)kv8_units(a, v) * a.kv_heads : 0;
-        const long long sum = block_scan(n, before);
-        if (blockIdx.x == 0 && v < V) a.prefix[v] = total + before;
+        mine = units_of(v0 + tid);
+        const long long sum = block_scan(mine, before);
+        if (blockIdx.x == 0 && v0 + tid < V) a.prefix[v0 + tid] = total + before;
         total += sum;
     }
     if (blockIdx.x == 0 && tid == 0) a.prefix[V] = total;
     const long long share = (total + gridDim.x - 1) / gridDim.x;
     const long long begin = min(total, share * (long long)blockIdx.x), end = min(total, begin + share);
     if (begin >= end) return;
-    {
-        long long run = 0;
-        for (int v0 = 0; v0 < V; v0 += kDecThreads) {
-            long long before;
-            const int v = v0 + tid;
-        const long long n = v < V ? (long long)kv8_units(a, v) * a.kv_heads : 0;
-            const long long sum = block_scan(n, before);
-            if (n && run + before <= begin && begin < run + before + n) found[0] = v, found[1] = run + before;
-            run += sum;
-            if (run > begin) break;
+    for (long long v0 = 0, run = 0; v0 < V && run <= begin; v0 += kDecThreads) {
+        long long sum = total;
+        if (V > kDecThreads) {
+            mine = units_of(int(v0) + tid);
+            sum = block_scan(mine, before);
         }
-        __syncthreads();
+        if (run + before <= begin && begin < run + before + mine) found[0] = v0 + tid, found[1] = run + before;
+        run += sum;
     }
+    __syncthreads();
     int v = int(found[0]);
     long long base = found[1], u = begin;  // base: the first unit of pair v
 
@@ -186,15 +197,15 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
         const int s0 = a.starts[req], nq = a.starts[req + 1] - s0, len = kv8_len(a, req);
         const int row0 = tile * NR, rows = min(NR, nq * a.group - row0);
         const int keys = kv8_keys(a, nq, len, tile);
-        const int k0 = unit0 * kDecUnit, k1 = min(keys, (unit0 + units) * kDecUnit);
+        const int k0 = unit0 * UNIT, k1 = min(keys, (unit0 + units) * UNIT);
         u += units;
         __syncthreads();  // the ring and the queries of the piece before are done with
 
-        // ---- tokens k0 .. k1 - 1, 32 at a time in turn among the warps ----
-        const int steps = max(0, (k1 - k0 - kDecSub * warp + kDecUnit - 1) / kDecUnit);
+        // ---- tokens k0 .. k1 - 1, SUB at a time in turn among the warps ----
+        const int steps = max(0, (k1 - k0 - SUB * warp + UNIT - 1) / UNIT);
         const int32_t* trow = a.table + size_t(req) * a.width;
-        auto page_of = [&](int j) {  // lanes 0, 1: the pages of step j's two blocks of 16 tokens
-            const int tok = k0 + kDecSub * (warp + kDecWarps * j) + 16 * (lane & 1);
+        auto page_of = [&](int j) {  // lanes 0, 1: the pages of step j's blocks of 16 tokens
+            const int tok = k0 + SUB * (warp + kDecWarps * j) + 16 * (lane & (NB - 1));
             int p = 0;
             if (j < steps && tok < k1) {
                 p = __ldg(trow + (tok >> a.shift));
@@ -209,8 +220,8 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
             if (j < steps) {
                 uint8_t* st = ring + (j % kDecStages) * L::stage;
 #pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    const int tok = k0 + kDecSub * (warp + kDecWarps * j) + 16 * b;
+                for (int b = 0; b < NB; b++) {
+                    const int tok = k0 + SUB * (warp + kDecWarps * j) + 16 * b;
                     const int p = __shfl_sync(0xffffffffu, mine, b);
                     if (tok >= k1 || p < 0) continue;
                     const size_t at = size_t(p) * a.kv_heads + head;
@@ -219,10 +230,10 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
                     for (int i = 0; i < HD / 32; i++) {
                         const int c = lane + 32 * i, r = c / (HD / 16), o = c % (HD / 16);
                         cp_async16(st + L::at(16 * b + r, o), a.k_codes + from + 16 * c);
-                        cp_async16(st + kDecSub * L::row + L::at(16 * b + r, o), a.v_codes + from + 16 * c);
+                        cp_async16(st + SUB * L::row + L::at(16 * b + r, o), a.v_codes + from + 16 * c);
                     }
-                    if (lane == 0) cp_async4(st + 2 * kDecSub * L::row + 4 * b, a.k_scales + at);
-                    if (lane == 1) cp_async4(st + 2 * kDecSub * L::row + 8 + 4 * b, a.v_scales + at);
+                    if (lane == 0) cp_async4(st + 2 * SUB * L::row + 4 * b, a.k_scales + at);
+                    if (lane == 1) cp_async4(st + 2 * SUB * L::row + 8 + 4 * b, a.v_scales + at);
                 }
             }
             cp_async_commit();
@@ -235,7 +246,7 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
             ahead = next;
         }
 
-        // ---- the queries, split into fp16 parts in the order of the codes' bytes ----
+        // ---- the queries in fixed point, as B operands ----
         for (int r = warp; r < NR; r += kDecWarps) {
             float x[HD / 32];
             uint32_t big = 0;
@@ -246,25 +257,29 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
                 big = max(big, __float_as_uint(x[i]) & 0x7fffffffu);
             }
             big = __reduce_max_sync(0xffffffffu, big);
-            // to 2^10 .. 2^11; as it is where nothing or infinity stands there
-            const int up = big >= 0x00800000u && big < 0x7f800000u ? min(137 - int(big >> 23), 126) : 0;
+            // the largest to 2^21 .. 2^22 (2^13 .. 2^14), or as far up as a power of two reaches
+            const int up = min((PL == 3 ? 21 : 13) + 127 - int(big >> 23), 126);
             const float mul = pow2i(up);
-            if (lane == 0) qscale[r] = a.scale_log2 * pow2i(-up);
-            __half* dst = reinterpret_cast<__half*>(sm + L::q);
+            if (lane == 0) qscale[r] = big < 0x7f800000u ? a.scale_log2 * pow2i(-up) : __int_as_float(0x7fffffff);
+            int8_t* dst = reinterpret_cast<int8_t*>(sm + L::q) + (r >> 3) * HD * 8;
 #pragma unroll
             for (int i = 0; i < HD / 32; i++) {
-                const int d = lane + 32 * i, blk = d >> 4, tt = (d >> 2) & 3;
-                const float y = __fmul_rn(x[i], mul);
-                const __half hi = __float2half_rn(y);
-                const int at = (((r >> 3) * (HD / 16) + blk) * 32 + (r & 7) * 4 + tt) * 4 + (d & 3);
-                dst[at] = hi;
-                if (NP == 2) dst[NT * (HD / 16) * 128 + at] = __float2half_rn(__fsub_rn(y, __half2float(hi)));
+                // dimension 32 i + lane: half, then group t of four within it
+                int v = __float2int_rn(__fmul_rn(x[i], mul));
+                const int at = (i * 32 + (r & 7) * 4 + ((lane >> 2) & 3)) * 8 + ((lane >> 4) << 2) + (lane & 3);
+#pragma unroll
+                for (int p = 0; p < PL; p++) {
+                    const int8_t digit = int8_t(v);
+                    dst[p * NT * HD * 8 + at] = digit;
+                    v = (v - digit) >> 8;
+                }
             }
         }
         __syncthreads();
 
         float o[HD / 16][NT][4], m_run[NT][2], r_run[NT][2], l_run[NT][2], qs[NT][2];
         int limit[NT][2];  // keys that the lane's columns see
+        const int clear = min(k1, len - nq + row0 / a.group + 1);  // every row sees the keys before it
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -284,86 +299,100 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
             cp_async_wait<kDecStages - 1>();
             __syncwarp();
             const uint8_t* st = ring + (j % kDecStages) * L::stage;
-            const uint32_t kb = saddr(st), vb = kb + kDecSub * L::row;
-            const float* scales = reinterpret_cast<const float*>(st + 2 * kDecSub * L::row);
-            const int tok0 = k0 + kDecSub * (warp + kDecWarps * j);
-            const bool two = tok0 + 16 < k1;  // the second block holds tokens
-            float s[2][NT][4];
+            const uint32_t kb = saddr(st), vb = kb + SUB * L::row;
+            const float* scales = reinterpret_cast<const float*>(st + 2 * SUB * L::row);
+            const int tok0 = k0 + SUB * (warp + kDecWarps * j);
+            float s[NB][NT][4];
+            {
+                int sum[PL][NB][NT][4];
 #pragma unroll
-            for (int b = 0; b < 2; b++)
+                for (int p = 0; p < PL; p++)
 #pragma unroll
-                for (int n = 0; n < NT; n++) s[b][n][0] = s[b][n][1] = s[b][n][2] = s[b][n][3] = 0.f;
+                    for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int d = 0; d < KB; d++) {
-                uint2 q[NP][NT][2];
+                        for (int n = 0; n < NT; n++) sum[p][b][n][0] = sum[p][b][n][1] = sum[p][b][n][2] = sum[p][b][n][3] = 0;
 #pragma unroll
-                for (int p = 0; p < NP; p++)
+                for (int d = 0; d < KB; d++) {
+                    uint2 q[PL][NT];
 #pragma unroll
-                    for (int n = 0; n < NT; n++)
+                    for (int p = 0; p < PL; p++)
 #pragma unroll
-                        for (int e = 0; e < 2; e++)
-                            q[p][n][e] = *reinterpret_cast<const uint2*>(
-                                sm + L::q + (((p * NT + n) * (HD / 16) + 2 * d + e) * 32 + lane) * 8);
+                        for (int n = 0; n < NT; n++)
+                            q[p][n] = *reinterpret_cast<const uint2*>(sm + L::q + (((p * NT + n) * KB + d) * 32 + lane) * 8);
 #pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    if (b && !two) break;
-                    uint32_t x[4];
-                    ldsm4(x, kb + b * 16 * L::row + L::at(lrow, lchunk + 2 * d));
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const uint32_t lo = x[2 * e] ^ 0x80808080u, hi = x[2 * e + 1] ^ 0x80808080u;
-                        const uint32_t a0 = codes2<0x4140>(lo), a1 = codes2<0x4140>(hi), a2 = codes2<0x4342>(lo),
-                                       a3 = codes2<0x4342>(hi);
+                    for (int b = 0; b < NB; b++) {
+                        uint32_t x[4];
+                        ldsm4(x, kb + b * 16 * L::row + L::at(lrow, lchunk + 2 * d));
 #pragma unroll
                         for (int n = 0; n < NT; n++)
 #pragma unroll
-                            for (int p = NP - 1; p >= 0; p--) mma_f16(s[b][n], a0, a1, a2, a3, q[p][n][e].x, q[p][n][e].y);
+                            for (int p = 0; p < PL; p++) mma_s8(sum[p][b][n], x, q[p][n].x, q[p][n].y);
                     }
+                }
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    const float ks = scales[b];
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            float f = float(sum[0][b][n][e] + (sum[1][b][n][e] << 8));
+                            if (PL == 3) f = fmaf(float(sum[PL - 1][b][n][e]), 65536.f, f);
+                            s[b][n][e] = f * (ks * qs[n][e & 1]);
+                        }
                 }
             }
             // ---- softmax: s[b][n][0, 1] token 16 b + g, columns 2t, 2t + 1; [2, 3] token + 8 ----
-            uint32_t w[2][NT][NP][2];  // weights as B operands
-            const float ve[2] = {exponent_of(scales[2]), two ? exponent_of(scales[3]) : -INFINITY};
-            const float ks[2] = {scales[0], two ? scales[1] : 0.f};
+            if (tok0 + SUB > clear) {  // some key of the step is hidden from some query, or past the end
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (tok0 + 16 * b + g + 8 * (e >> 1) >= min(limit[n][e & 1], k1)) s[b][n][e] = -INFINITY;
+            }
+            uint32_t w[NB][NT][NP][2];  // weights as B operands
+            float ve[NB];
+#pragma unroll
+            for (int b = 0; b < NB; b++) ve[b] = tok0 + 16 * b < k1 ? exponent_of(scales[2 + b]) : -INFINITY;
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                float top[2][2];
+                float top[NB][2];
 #pragma unroll
-                for (int b = 0; b < 2; b++)
+                for (int b = 0; b < NB; b++)
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        const int tok = tok0 + 16 * b + g;
-                        const float f = ks[b] * qs[n][c];
-                        s[b][n][c] = tok < limit[n][c] && tok < k1 ? s[b][n][c] * f : -INFINITY;
-                        s[b][n][c + 2] = tok + 8 < limit[n][c] && tok + 8 < k1 ? s[b][n][c + 2] * f : -INFINITY;
-                        top[b][c] = fmaxf(s[b][n][c], s[b][n][c + 2]);
-                    }
+                    for (int c = 0; c < 2; c++) top[b][c] = fmaxf(s[b][n][c], s[b][n][c + 2]);
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1)
 #pragma unroll
-                    for (int b = 0; b < 2; b++)
+                    for (int b = 0; b < NB; b++)
 #pragma unroll
                         for (int c = 0; c < 2; c++) top[b][c] = fmaxf(top[b][c], __shfl_xor_sync(0xffffffffu, top[b][c], x));
                 float down[2];
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    const float t0 = ceilf(top[0][c]), t1 = ceilf(top[1][c]);
-                    const float m = fmaxf(m_run[n][c], fmaxf(t0, t1));
-                    const float r = fmaxf(r_run[n][c], fmaxf(t0 + ve[0], t1 + ve[1]));
+                    float m = m_run[n][c], r = r_run[n][c];
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        const float t0 = ceilf(top[b][c]);
+                        m = fmaxf(m, t0);
+                        r = fmaxf(r, t0 + ve[b]);
+                    }
                     l_run[n][c] *= step_down(m_run[n][c], m);
                     down[c] = step_down(r_run[n][c], r);
                     m_run[n][c] = m;
                     r_run[n][c] = r;
                     const float m0 = m == -INFINITY ? 0.f : m;
 #pragma unroll
-                    for (int b = 0; b < 2; b++) {
+                    for (int b = 0; b < NB; b++) {
                         // 2^(m + f - r), at least 0 where the page's values are all zero
                         const float f = ve[b] != ve[b] ? ve[b]
                                         : ve[b] == -INFINITY || r == -INFINITY ? 0.f
                                         : pow2i(int(fminf(fmaxf(m0 + ve[b] - r, -126.f), 126.f)));
 #pragma unroll
                         for (int e = c; e < 4; e += 2) {
-                            const float p = exp2f(s[b][n][e] - m0);
+                            const float p = exp2_fast(s[b][n][e] - m0);
                             l_run[n][c] += p;
                             // (a masked key adds nothing even to a page of NaN)
                             s[b][n][e] = s[b][n][e] == -INFINITY ? 0.f : p * f;
@@ -380,7 +409,7 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
                     }
                 }
 #pragma unroll
-                for (int b = 0; b < 2; b++)
+                for (int b = 0; b < NB; b++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const uint32_t hi = half2_bits(s[b][n][2 * e], s[b][n][2 * e + 1]);
@@ -393,8 +422,8 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
             }
             // ---- values ----
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
-                if (b && !two) break;
+            for (int b = 0; b < NB; b++) {
+                if (tok0 + 16 * b >= k1) break;
 #pragma unroll
                 for (int d = 0; d < KB; d++) {
                     uint32_t x[4];
@@ -472,60 +501,75 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
 
 // Adds the parts of every (row tile, kv head) that the runs cut, in the order of
 // the runs: the part of run c is its second where the pair begins in it after
-// another (or after its own first piece), else its first.
-template <int NR>
-__global__ void __launch_bounds__(128) kv8_combine_kernel(const Kv8Args a, int grid, int hd) {
+// another, else its first.  One CTA of head_dim threads for each row.
+constexpr int kJoin = 64;  // parts whose factors are held at a time
+
+__global__ void __launch_bounds__(256) kv8_combine_kernel(const Kv8Args a, int grid, int hd) {
+    __shared__ float mul[kJoin], worst[2][8];
     pdl_wait();
-    const int v = blockIdx.x, head = blockIdx.y, V = a.requests * a.tiles;
+    const int v = blockIdx.x, head = blockIdx.y, r = blockIdx.z, V = a.requests * a.tiles, NR = a.tile_rows;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, W = hd + 4;
     const long long p0 = a.prefix[v], p1 = a.prefix[v + 1], total = a.prefix[V];
     const int nu = int((p1 - p0) / a.kv_heads);
     if (nu == 0) return;
     const long long share = (total + grid - 1) / grid, u0 = p0 + (long long)head * nu, u1 = u0 + nu;
     const int c0 = int(u0 / share), c1 = int((u1 - 1) / share);
     if (c0 == c1) return;  // one run held all of it and wrote the result
-    const int req = v / a.tiles, s0 = a.starts[req], nq = a.starts[req + 1] - s0, row0 = (v % a.tiles) * NR;
-    const int rows = min(NR, nq * a.group - row0), W = hd + 4;
-    auto part = [&](int c) {
-        const int second = u0 > share * c ? 1 : 0;
-        return a.parts + size_t(2 * c + second) * NR * W;
-    };
-    for (int e = threadIdx.x; e < rows * hd; e += 128) {
-        const int r = e / hd, d = e % hd;
-        float m = -INFINITY, ref = -INFINITY, sum = 0.f, acc = 0.f;
-        for (int c = c0; c <= c1; c++) {
-            const float* p = part(c) + r * W;
-            m = fmaxf(m, p[hd]);
-            ref = fmaxf(ref, p[hd + 1]);
-        }
-        for (int c = c0; c <= c1; c++) {
-            const float* p = part(c) + r * W;
-            sum = fmaf(p[hd + 2], step_down(p[hd], m), sum);
-            acc = fmaf(p[d], step_down(p[hd + 1], ref), acc);
-        }
-        const int qr = row0 + r, qi = qr / a.group, qh = head * a.group + qr % a.group;
-        kv8_store(a, int64_t(s0 + qi) * a.o_token + qh * a.o_head + d, kv8_finish(acc, ref, sum, m));
+    const int req = v / a.tiles, s0 = a.starts[req], nq = a.starts[req + 1] - s0, row = (v % a.tiles) * NR + r;
+    if (row >= nq * a.group) return;
+    auto part = [&](int c) { return a.parts + (size_t(2 * c + (u0 > share * c ? 1 : 0)) * NR + r) * W; };
+    float m = -INFINITY, ref = -INFINITY;
+    for (int c = c0 + tid; c <= c1; c += hd) {
+        m = fmaxf(m, part(c)[hd]);
+        ref = fmaxf(ref, part(c)[hd + 1]);
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
+    }
+    if (lane == 0) worst[0][warp] = m, worst[1][warp] = ref;
+    __syncthreads();
+    for (int w = 0; w < hd / 32; w++) {
+        m = fmaxf(m, worst[0][w]);
+        ref = fmaxf(ref, worst[1][w]);
+    }
+    float sum = 0.f, acc = 0.f;
+    for (int b = c0; b <= c1; b += kJoin) {
+        const int n = min(kJoin, c1 + 1 - b);
+        __syncthreads();
+        for (int c = tid; c < n; c += hd) mul[c] = step_down(part(b + c)[hd + 1], ref);
+        __syncthreads();
+#pragma unroll 4
+        for (int c = 0; c < n; c++) {
+            const float* p = part(b + c);
+            sum = fmaf(p[hd + 2], step_down(p[hd], m), sum);
+            acc = fmaf(p[tid], mul[c], acc);
+        }
+    }
+    const int qi = row / a.group, qh = head * a.group + row % a.group;
+    kv8_store(a, int64_t(s0 + qi) * a.o_token + qh * a.o_head + tid, kv8_finish(acc, ref, sum, m));
 }
 
 template <int HD, int NT, int NP>
 void launch_decode(const Kv8Args& a, int grid, cudaStream_t st) {
     constexpr int smem = DecSmem<HD, NT, NP>::total;
     static_assert(smem <= 227 * 1024, "a CTA's shared memory");
-    static_assert(DecSmem<HD, NT, NP>::per_sm() == (HD <= 128 ? 2 : 1), "plan_of's grid");
+    static_assert(NT == 2 || kDecPerSm * (smem + 1024) <= 228 * 1024, "the grid is made for this many CTAs on an SM");
     static unsigned long long done = 0;
     allow_smem(kv8_decode_kernel<HD, NT, NP>, smem, done);
     kv8_decode_kernel<HD, NT, NP><<<grid, kDecThreads, smem, st>>>(a);
     CUDA_OK(cudaGetLastError());
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(a.requests * a.tiles), unsigned(a.kv_heads));
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3(unsigned(a.requests * a.tiles), unsigned(a.kv_heads), unsigned(std::min(a.tile_rows, a.most * a.group)));
+    cfg.blockDim = dim3(HD);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    CUDA_OK(cudaLaunchKernelEx(&cfg, kv8_combine_kernel<8 * NT>, a, grid, HD));
+    CUDA_OK(cudaLaunchKernelEx(&cfg, kv8_combine_kernel, a, grid, HD));
 }
 
 template <int HD>
@@ -549,8 +593,8 @@ Plan plan_of(const spm_kv8* c, int heads, int requests, int most, int width) {
     p.tiles = int((rows + 8 * p.nt - 1) / (8 * p.nt));
     const int64_t pairs = int64_t(requests) * p.tiles;
     if (pairs > INT32_MAX) fail(SPM_E_ARG, "too many requests and queries for one call");
-    const int per_sm = c->head_dim <= 128 ? 2 : 1;  // DecSmem's per_sm
-    const int64_t units = (int64_t(width) * c->page_tokens + kDecUnit - 1) / kDecUnit;
+    const int per_sm = kDecPerSm, unit = kDecWarps * kv8_sub(c->head_dim);
+    const int64_t units = (int64_t(width) * c->page_tokens + unit - 1) / unit;
     if (units * pairs > INT64_MAX / 65536) fail(SPM_E_ARG, "too many requests and queries for one call");
     p.grid = int(std::max<int64_t>(1, std::min<int64_t>(int64_t(per_sm) * sms, std::max<int64_t>(units, 1) * pairs * c->kv_heads)));
     p.prefix_bytes = (uint64_t(pairs + 1) * 8 + 15) & ~uint64_t(15);
@@ -606,6 +650,7 @@ spm_status spm_kv8_attention(const spm_kv8* c, uint32_t dtype, const void* q, in
         a.q = q, a.q_token = q_token, a.q_head = q_head, a.dtype = dtype, a.rows = rows;
         a.starts = starts, a.lens = lens, a.requests = requests, a.most = most;
         a.table = table, a.width = table_width, a.tile_rows = 8 * p.nt, a.tiles = p.tiles;
+        a.unit = kDecWarps * kv8_sub(c->head_dim);
         a.scale_log2 = float(double(scale) * 1.4426950408889634);
         a.out = out, a.o_token = out_token, a.o_head = out_head;
         a.prefix = static_cast<long long*>(workspace);

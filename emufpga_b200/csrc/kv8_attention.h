@@ -4,10 +4,11 @@
 
 namespace spm {
 
-constexpr int kDecWarps = 4;                   // of a CTA
-constexpr int kDecSub = 32;                    // tokens of a warp's step
-constexpr int kDecUnit = kDecWarps * kDecSub;  // tokens of a unit
-constexpr int kDecStages = 3;
+constexpr int kDecWarps = 4;   // of a CTA
+constexpr int kDecStages = 2;
+constexpr int kDecPerSm = 3;   // CTAs per SM that the grid is made for
+// Tokens of a warp's step.
+constexpr int kv8_sub(int head_dim) { return head_dim <= 128 ? 32 : 16; }
 
 struct Kv8Args {
     const int8_t *k_codes, *v_codes;
@@ -21,6 +22,7 @@ struct Kv8Args {
     int32_t requests, most;
     const int32_t* table;
     int32_t width, tile_rows, tiles;           // a tile: tile_rows (query, head of the group) rows
+    int32_t unit;                              // tokens
     float scale_log2;
     void* out;
     int64_t o_token, o_head;
@@ -44,7 +46,7 @@ __device__ __forceinline__ int kv8_keys(const Kv8Args& a, int nq, int len, int t
     return max(0, len - nq + last);
 }
 
-// Units of 128 keys of pair v = (request, row tile), one at least where the tile
+// Units of keys of pair v = (request, row tile), one at least where the tile
 // has rows; 0 for requests whose rows are not what the call says.
 __device__ __forceinline__ int kv8_units(const Kv8Args& a, int v) {
     const int req = v / a.tiles, tile = v % a.tiles;
@@ -54,7 +56,7 @@ __device__ __forceinline__ int kv8_units(const Kv8Args& a, int v) {
         return 0;
     }
     if ((long long)tile * a.tile_rows >= (long long)(e - s) * a.group) return 0;
-    return max(1, (kv8_keys(a, e - s, kv8_len(a, req), tile) + kDecUnit - 1) / kDecUnit);
+    return max(1, (kv8_keys(a, e - s, kv8_len(a, req), tile) + a.unit - 1) / a.unit);
 }
 
 __device__ __forceinline__ float kv8_load(const Kv8Args& a, int64_t i) {
