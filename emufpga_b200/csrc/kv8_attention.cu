@@ -69,36 +69,10 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint
         : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float exp2_fast(float x) {  // to 2^-22
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// Bytes of x (already + 128) picked by SEL, as two fp16 codes.
-template <uint32_t SEL>
-__device__ __forceinline__ uint32_t codes2(uint32_t x) {
-    const uint32_t u = __byte_perm(x, 0x64646464u, SEL);
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
 __device__ __forceinline__ float2 half2_floats(uint32_t b) { return __half22float2(*reinterpret_cast<const __half2*>(&b)); }
 __device__ __forceinline__ void cp_async4(void* dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(saddr(dst)), "l"(src) : "memory");
 }
-// 2^(to - from) for integer-valued references; 0 where there was none yet.
-__device__ __forceinline__ float step_down(float from, float to) {
-    return from == -INFINITY ? 0.f : pow2i(int(fmaxf(from - to, -126.f)));
-}
-
-// The exponent of a scale (a power of two); -inf for 0, NaN for NaN.
-__device__ __forceinline__ float exponent_of(float s) {
-    return s > 0.f ? float((__float_as_int(s) >> 23) - 127) : s == 0.f ? -INFINITY : __int_as_float(0x7fffffff);
-}
-
 template <int HD, int NT, int NP>
 struct DecSmem {
     static constexpr int sub = kv8_sub(HD);
@@ -355,7 +329,7 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
             uint32_t w[NB][NT][NP][2];  // weights as B operands
             float ve[NB];
 #pragma unroll
-            for (int b = 0; b < NB; b++) ve[b] = tok0 + 16 * b < k1 ? exponent_of(scales[2 + b]) : -INFINITY;
+            for (int b = 0; b < NB; b++) ve[b] = tok0 + 16 * b < k1 ? kv8_exponent(scales[2 + b]) : -INFINITY;
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 float top[NB][2];
@@ -379,8 +353,8 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
                         m = fmaxf(m, t0);
                         r = fmaxf(r, t0 + ve[b]);
                     }
-                    l_run[n][c] *= step_down(m_run[n][c], m);
-                    down[c] = step_down(r_run[n][c], r);
+                    l_run[n][c] *= kv8_step(m_run[n][c], m);
+                    down[c] = kv8_step(r_run[n][c], r);
                     m_run[n][c] = m;
                     r_run[n][c] = r;
                     const float m0 = m == -INFINITY ? 0.f : m;
@@ -392,7 +366,7 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
                                         : pow2i(int(fminf(fmaxf(m0 + ve[b] - r, -126.f), 126.f)));
 #pragma unroll
                         for (int e = c; e < 4; e += 2) {
-                            const float p = exp2_fast(s[b][n][e] - m0);
+                            const float p = kv8_exp2(s[b][n][e] - m0);
                             l_run[n][c] += p;
                             // (a masked key adds nothing even to a page of NaN)
                             s[b][n][e] = s[b][n][e] == -INFINITY ? 0.f : p * f;
@@ -412,11 +386,11 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
                 for (int b = 0; b < NB; b++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const uint32_t hi = half2_bits(s[b][n][2 * e], s[b][n][2 * e + 1]);
+                        const uint32_t hi = kv8_half2(s[b][n][2 * e], s[b][n][2 * e + 1]);
                         w[b][n][0][e] = transposed(hi);
                         if (NP == 2) {
                             const float2 h = half2_floats(hi);
-                            w[b][n][NP - 1][e] = transposed(half2_bits(s[b][n][2 * e] - h.x, s[b][n][2 * e + 1] - h.y));
+                            w[b][n][NP - 1][e] = transposed(kv8_half2(s[b][n][2 * e] - h.x, s[b][n][2 * e + 1] - h.y));
                         }
                     }
             }
@@ -431,8 +405,8 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const uint32_t lo = x[2 * e] ^ 0x80808080u, hi = x[2 * e + 1] ^ 0x80808080u;
-                        const uint32_t a0 = codes2<0x4240>(lo), a1 = codes2<0x4341>(lo), a2 = codes2<0x4240>(hi),
-                                       a3 = codes2<0x4341>(hi);
+                        const uint32_t a0 = kv8_codes2<0x4240>(lo), a1 = kv8_codes2<0x4341>(lo), a2 = kv8_codes2<0x4240>(hi),
+                                       a3 = kv8_codes2<0x4341>(hi);
 #pragma unroll
                         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -481,8 +455,8 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
 #pragma unroll
             for (int x = 0; x < kDecWarps; x++) {
                 const float* sx = st + x * NR * L::state;
-                sum = fmaf(sx[HD + 2], step_down(sx[HD], m), sum);
-                acc = fmaf(sx[d], step_down(sx[HD + 1], ref), acc);
+                sum = fmaf(sx[HD + 2], kv8_step(sx[HD], m), sum);
+                acc = fmaf(sx[d], kv8_step(sx[HD + 1], ref), acc);
             }
             if (whole) {
                 const int qr = row0 + r, qi = qr / a.group, qh = head * a.group + qr % a.group;
@@ -538,12 +512,12 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const Kv8Args a, int g
     for (int b = c0; b <= c1; b += kJoin) {
         const int n = min(kJoin, c1 + 1 - b);
         __syncthreads();
-        for (int c = tid; c < n; c += hd) mul[c] = step_down(part(b + c)[hd + 1], ref);
+        for (int c = tid; c < n; c += hd) mul[c] = kv8_step(part(b + c)[hd + 1], ref);
         __syncthreads();
 #pragma unroll 4
         for (int c = 0; c < n; c++) {
             const float* p = part(b + c);
-            sum = fmaf(p[hd + 2], step_down(p[hd], m), sum);
+            sum = fmaf(p[hd + 2], kv8_step(p[hd], m), sum);
             acc = fmaf(p[tid], mul[c], acc);
         }
     }
@@ -580,6 +554,7 @@ void launch_dim(const Kv8Args& a, int nt, bool two, int grid, cudaStream_t st) {
 
 // How a call is cut, from what the host knows of it.
 struct Plan {
+    bool prompt;  // kv8_prompt.cu's kernel
     int nt, tiles, grid;
     uint64_t prefix_bytes, parts_bytes;
 };
@@ -591,6 +566,16 @@ Plan plan_of(const spm_kv8* c, int heads, int requests, int most, int width) {
     const int64_t rows = int64_t(std::max(most, 1)) * group;
     p.nt = rows <= 8 ? 1 : 2;
     p.tiles = int((rows + 8 * p.nt - 1) / (8 * p.nt));
+    const int64_t small = int64_t(requests) * c->kv_heads * p.tiles;
+    const int64_t large = int64_t(requests) * c->kv_heads * ((rows + kv8_prompt_rows - 1) / kv8_prompt_rows);
+    p.prompt = rows > 16 && small >= 96 * ((large + sms - 1) / sms);
+    if (p.prompt) {
+        p.tiles = int((rows + kv8_prompt_rows - 1) / kv8_prompt_rows);
+        if (requests > 65535 || p.tiles > INT32_MAX / kv8_prompt_rows) fail(SPM_E_ARG, "too many requests and queries for one call");
+        p.grid = 0;
+        p.prefix_bytes = p.parts_bytes = 0;
+        return p;
+    }
     const int64_t pairs = int64_t(requests) * p.tiles;
     if (pairs > INT32_MAX) fail(SPM_E_ARG, "too many requests and queries for one call");
     const int per_sm = kDecPerSm, unit = kDecWarps * kv8_sub(c->head_dim);
@@ -638,7 +623,7 @@ spm_status spm_kv8_attention(const spm_kv8* c, uint32_t dtype, const void* q, in
         if (requests == 0 || rows == 0 || most == 0) return;
         if (!q || !out || !starts || !lens || (table_width && !table)) fail(SPM_E_ARG, "null argument");
         const Plan p = plan_of(c, heads, requests, most, table_width);
-        if (!workspace || workspace_bytes < p.prefix_bytes + p.parts_bytes)
+        if ((p.prefix_bytes && !workspace) || workspace_bytes < p.prefix_bytes + p.parts_bytes)
             fail(SPM_E_ARG, "the workspace is smaller than spm_kv8_attention_workspace says");
         if (reinterpret_cast<uintptr_t>(workspace) & 15) fail(SPM_E_ARG, "the workspace must be 16-byte aligned");
         DeviceScope scope(c->device);
@@ -649,14 +634,20 @@ spm_status spm_kv8_attention(const spm_kv8* c, uint32_t dtype, const void* q, in
         a.kv_heads = c->kv_heads, a.group = heads / c->kv_heads;
         a.q = q, a.q_token = q_token, a.q_head = q_head, a.dtype = dtype, a.rows = rows;
         a.starts = starts, a.lens = lens, a.requests = requests, a.most = most;
-        a.table = table, a.width = table_width, a.tile_rows = 8 * p.nt, a.tiles = p.tiles;
+        a.table = table, a.width = table_width, a.tile_rows = p.prompt ? kv8_prompt_rows : 8 * p.nt, a.tiles = p.tiles;
         a.unit = kDecWarps * kv8_sub(c->head_dim);
         a.scale_log2 = float(double(scale) * 1.4426950408889634);
         a.out = out, a.o_token = out_token, a.o_head = out_head;
         a.prefix = static_cast<long long*>(workspace);
         a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.prefix_bytes);
         a.status = c->status;
+        const int64_t size = dtype == SPM_F32 ? 4 : 2;
+        a.o_vec = !((reinterpret_cast<uintptr_t>(out) | uintptr_t(out_token * size) | uintptr_t(out_head * size)) & 15);
         const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+        if (p.prompt) {
+            launch_kv8_prompt(a, c->head_dim, st);
+            return;
+        }
         const bool two = dtype == SPM_F32;
         switch (c->head_dim) {
             case 64: launch_dim<64>(a, p.nt, two, p.grid, st); break;

@@ -10,6 +10,8 @@ constexpr int kDecPerSm = 3;   // CTAs per SM that the grid is made for
 // Tokens of a warp's step.
 constexpr int kv8_sub(int head_dim) { return head_dim <= 128 ? 32 : 16; }
 
+constexpr int kv8_prompt_rows = 128;  // rows of a prompt kernel's tile
+
 struct Kv8Args {
     const int8_t *k_codes, *v_codes;
     const float *k_scales, *v_scales;
@@ -26,10 +28,14 @@ struct Kv8Args {
     float scale_log2;
     void* out;
     int64_t o_token, o_head;
+    bool o_vec;                                // out and its strides are multiples of 16 bytes
     long long* prefix;                         // [requests * tiles + 1] units before a pair
     float* parts;                              // [CTA][2][tile_rows][head_dim + 4]
     int32_t* status;
 };
+
+// The kernel of many queries (kv8_prompt.cu): a.tile_rows = kv8_prompt_rows, a.tiles to match.
+void launch_kv8_prompt(const Kv8Args& a, int head_dim, cudaStream_t st);
 
 namespace dev {
 
@@ -68,6 +74,62 @@ __device__ __forceinline__ void kv8_store(const Kv8Args& a, int64_t i, float y) 
     if (a.dtype == SPM_F32) static_cast<float*>(a.out)[i] = y;
     else if (a.dtype == SPM_F16) static_cast<__half*>(a.out)[i] = __float2half_rn(y);
     else static_cast<__nv_bfloat16*>(a.out)[i] = __float2bfloat16_rn(y);
+}
+
+// Sixteen values of a row, in 16-byte pieces where out's strides allow them.
+__device__ __forceinline__ void kv8_store16(const Kv8Args& a, int64_t i, const float (&v)[16]) {
+    if (a.dtype == SPM_F32) {
+        float* o = static_cast<float*>(a.out) + i;
+        if (a.o_vec) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) reinterpret_cast<float4*>(o)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            return;
+        }
+    } else if (a.o_vec) {
+        __align__(16) uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if (a.dtype == SPM_F16) {
+                const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+                w[j] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+                w[j] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+        uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + i);
+        o[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        o[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; j++) kv8_store(a, i + j, v[j]);
+}
+
+// Bytes of x (codes + 128) picked by SEL, as two fp16 codes.
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t kv8_codes2(uint32_t x) {
+    const uint32_t u = __byte_perm(x, 0x64646464u, SEL);
+    const __half bias = __ushort_as_half(0x6480);  // 1152
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), __halves2half2(bias, bias));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t kv8_half2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float kv8_exp2(float x) {  // to 2^-22
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 2^(from - to) for integer-valued references, from <= to; 0 where there was none yet.
+__device__ __forceinline__ float kv8_step(float from, float to) {
+    return from == -INFINITY ? 0.f : pow2i(int(fmaxf(from - to, -126.f)));
+}
+// The exponent of a scale (a power of two); -inf for 0, NaN for NaN.
+__device__ __forceinline__ float kv8_exponent(float s) {
+    return s > 0.f ? float((__float_as_int(s) >> 23) - 127) : s == 0.f ? -INFINITY : __int_as_float(0x7fffffff);
 }
 
 // acc 2^ref / (sum 2^m); 0 for a row that saw nothing.

@@ -24,7 +24,8 @@ from ._lib import BF16, F16, F32, Kv8, SpmError, call
 DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 STATUS = {11: "a length is negative or past its table", 12: "more pages wanted than free",
           13: "more tokens than the slot map holds", 14: "more pages back than the pool has",
-          15: "a page or slot is not in the pool", 16: "a request's rows are not what the call says"}
+          15: "a page or slot is not in the pool", 16: "a request's rows are not what the call says",
+          17: "a device wait gave up"}
 
 
 _I32 = torch.int32
@@ -67,7 +68,7 @@ def check(status: torch.Tensor) -> None:
     code = int(status.item())
     if code:
         status.zero_()
-        raise SpmError(-9 if code in (12, 13) else -1, STATUS.get(code, f"code {code}"))
+        raise SpmError(-9 if code in (12, 13) else -8 if code == 17 else -1, STATUS.get(code, f"code {code}"))
 
 
 class Plan(NamedTuple):

@@ -445,8 +445,10 @@ enum {
     SPM_PAGE_TOKENS = 13,  /* more tokens than the slot map holds             */
     SPM_PAGE_STACK = 14,   /* more pages back than the pool has               */
     SPM_PAGE_ID = 15,      /* a page or slot that is not in the pool          */
-    SPM_PAGE_QUERIES = 16  /* a request with more queries than `most`, or
+    SPM_PAGE_QUERIES = 16, /* a request with more queries than `most`, or
                               starts that do not ascend within the rows       */
+    SPM_PAGE_WAIT = 17     /* a bounded device wait gave up: the outputs are
+                              not to be used                                  */
 };
 
 /* Block table, slot map and free stack of one tick, from the requests'

@@ -305,6 +305,22 @@ def test_attention_of_several_tokens(dtype, page, heads, kv_heads, dim, news, le
     assert not got[starts[-1]:].any()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("page,heads,kv_heads,news,lens", [
+    (16, 16, 8, [200], [777]), (64, 24, 8, [129, 0, 77], [129, 40, 1100]), (256, 12, 12, [300], [300]),
+    (32, 64, 4, [33, 40], [64, 1500]), (128, 16, 16, [1, 250, 3], [129, 380, 3])])
+def test_attention_of_many_tokens(dtype, dim, page, heads, kv_heads, news, lens):
+    rng = np.random.default_rng(page + dim)
+    table, pages = tables(rng, lens, page)
+    c = pool(pages, page, kv_heads, dim, seed=dim)
+    starts = np.concatenate([[0], np.cumsum(news)]).tolist()
+    q = torch.randn(starts[-1], heads, dim, device="cuda", generator=gen(page)).to(TYPES[dtype])
+    out = torch.full_like(q, 7.0)
+    check_attention(c, q, starts, lens, table, max(news), out=out)
+    check_attention(c, q, starts, lens, table, max(news), scale=-0.05)
+
+
 def test_attention_with_more_queries_than_keys_leaves_the_first_empty():
     table, pages = tables(np.random.default_rng(0), [3, 40], 16)
     c = pool(pages, 16, 2, 64)
