@@ -567,11 +567,12 @@ Plan plan_of(const spm_kv8* c, int heads, int requests, int most, int width) {
     p.nt = rows <= 8 ? 1 : 2;
     p.tiles = int((rows + 8 * p.nt - 1) / (8 * p.nt));
     const int64_t small = int64_t(requests) * c->kv_heads * p.tiles;
-    const int64_t large = int64_t(requests) * c->kv_heads * ((rows + kv8_prompt_rows - 1) / kv8_prompt_rows);
+    const int tall = kv8_prompt_rows(c->head_dim);
+    const int64_t large = int64_t(requests) * c->kv_heads * ((rows + tall - 1) / tall);
     p.prompt = rows > 16 && small >= 96 * ((large + sms - 1) / sms);
     if (p.prompt) {
-        p.tiles = int((rows + kv8_prompt_rows - 1) / kv8_prompt_rows);
-        if (requests > 65535 || p.tiles > INT32_MAX / kv8_prompt_rows) fail(SPM_E_ARG, "too many requests and queries for one call");
+        p.tiles = int((rows + tall - 1) / tall);
+        if (requests > 65535 || p.tiles > INT32_MAX / tall) fail(SPM_E_ARG, "too many requests and queries for one call");
         p.grid = 0;
         p.prefix_bytes = p.parts_bytes = 0;
         return p;
@@ -634,7 +635,7 @@ spm_status spm_kv8_attention(const spm_kv8* c, uint32_t dtype, const void* q, in
         a.kv_heads = c->kv_heads, a.group = heads / c->kv_heads;
         a.q = q, a.q_token = q_token, a.q_head = q_head, a.dtype = dtype, a.rows = rows;
         a.starts = starts, a.lens = lens, a.requests = requests, a.most = most;
-        a.table = table, a.width = table_width, a.tile_rows = p.prompt ? kv8_prompt_rows : 8 * p.nt, a.tiles = p.tiles;
+        a.table = table, a.width = table_width, a.tile_rows = p.prompt ? kv8_prompt_rows(c->head_dim) : 8 * p.nt, a.tiles = p.tiles;
         a.unit = kDecWarps * kv8_sub(c->head_dim);
         a.scale_log2 = float(double(scale) * 1.4426950408889634);
         a.out = out, a.o_token = out_token, a.o_head = out_head;

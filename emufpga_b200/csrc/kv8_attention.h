@@ -10,7 +10,8 @@ constexpr int kDecPerSm = 3;   // CTAs per SM that the grid is made for
 // Tokens of a warp's step.
 constexpr int kv8_sub(int head_dim) { return head_dim <= 128 ? 32 : 16; }
 
-constexpr int kv8_prompt_rows = 128;  // rows of a prompt kernel's tile
+// Rows of a tile of the kernel of many queries.
+constexpr int kv8_prompt_rows(int head_dim) { return head_dim <= 128 ? 256 : 128; }
 
 struct Kv8Args {
     const int8_t *k_codes, *v_codes;
@@ -34,7 +35,7 @@ struct Kv8Args {
     int32_t* status;
 };
 
-// The kernel of many queries (kv8_prompt.cu): a.tile_rows = kv8_prompt_rows, a.tiles to match.
+// The kernel of many queries (kv8_prompt.cu): a.tile_rows = kv8_prompt_rows(head_dim), a.tiles to match.
 void launch_kv8_prompt(const Kv8Args& a, int head_dim, cudaStream_t st);
 
 namespace dev {

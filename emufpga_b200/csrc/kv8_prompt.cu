@@ -2,25 +2,27 @@
 // 5th-generation tensor cores (the other half of spm_kv8_attention; the formulas
 // and the scaling by powers of two are kv8_attention.cu's).
 //
-// A CTA owns 128 rows (query x head of the group) of a request and kv head and
-// walks the keys in tiles of TN, once:
-//   producers (8 warps)  codes from global memory to fp16 (exact) in shared
+// A CTA owns G groups of 128 rows (query x head of the group) of a request and kv
+// head and walks the keys in tiles of TN, once:
+//   producers (4 warps)  codes from global memory to fp16 (exact) in shared
 //                        memory: a token's row of 64 dimensions is 128 bytes in the
 //                        128-byte swizzled layout, which is K-major for the keys
 //                        (S = Q K^T) and MN-major for the values (O = P V), so both
 //                        are written alike and nothing is transposed
-//   MMA (1 thread)       S(j + 1) = Q K(j + 1)^T into the other half of two TMEM
-//                        buffers while the softmax of S(j) runs, then O += P(j) V(j)
-//                        with P from TMEM
-//   softmax (4 warps)    a thread owns a row: S from TMEM, scale, mask, the running
-//                        references, weights in fp16 back to TMEM
+//   MMA (1 thread)       per group: O += P(j) V(j) with P from TMEM, then
+//                        S(j + 1) = Q K(j + 1)^T over the P just read
+//   softmax (4 warps a group)  a thread owns a row: S from TMEM, scale, mask, the
+//                        running references, weights in fp16 back to where S stood
+// With two groups the products of one run under the softmax of the other, and both
+// share the conversion of the codes.  (head_dim over 128 leaves TMEM and shared
+// memory for one.)
 // The references move only where a row's maximum passes them by more than 2^8, so
 // that the accumulator is hardly ever read back to be rescaled: weights are then at
 // most 2^8, which fp16 holds as exactly as those below 1.
 // f32 queries and weights are two fp16 parts (22 bits), twice the products.
 //
-// What bounds it is the softmax's instructions (16384 exponentials of a 128 x 128
-// tile take 1024 cycles of the special function unit alone, its products 1024).
+// What bounds it is the softmax: the 16384 exponentials of a 128 x 128 tile take
+// 1024 cycles of the special function unit, as long as its products.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -33,29 +35,33 @@ namespace spm {
 namespace {
 using namespace dev;
 
-constexpr int kRows = kv8_prompt_rows;                 // of a tile: the MMA's M
-constexpr int kSoftWarps = 4, kFillWarps = 8, kPromptThreads = 32 * (kSoftWarps + kFillWarps + 1);
-constexpr int kFillThreads = 32 * kFillWarps;
+constexpr int kRows = 128;                             // of a group: the MMA's M
+constexpr int kFillWarps = 4, kFillThreads = 32 * kFillWarps;
 constexpr float kSlack = 8.f;                          // in powers of two
 
 template <int HD, int NP>
 struct PromptShape {
+    static constexpr int G = kv8_prompt_rows(HD) / kRows;
+    static constexpr int threads = 32 * (4 * G + kFillWarps + 1);
     static constexpr int TN = HD <= 128 ? 128 : 64;    // keys of a tile
     static constexpr int atoms = (HD + 63) / 64;       // 64 dimensions, 128 bytes
-    static constexpr int qpart = atoms * kRows * 128;  // bytes of a part of Q
+    static constexpr int qgroup = atoms * kRows * 128; // bytes of a group's part of Q
+    static constexpr int qbytes = G * NP * qgroup;
     static constexpr int tile = atoms * TN * 128;      // bytes of a tile of K or V
-    static constexpr int stages = NP * qpart + 4 * tile + 4096 <= 227 * 1024 ? 2 : 1;
+    static constexpr int stages = qbytes + 4 * tile + 4096 <= 227 * 1024 ? 2 : 1;
     // (at least half of an SM's: a second CTA would wait for the first one's TMEM)
-    static constexpr int need = NP * qpart + 2 * stages * tile + 1024, smem = need > 120 * 1024 ? need : 120 * 1024;
-    static constexpr int s_col = 0, o_col = 2 * TN, p_col = o_col + HD;  // TMEM columns
-    static_assert(p_col + NP * TN / 2 <= 512, "TMEM");
+    static constexpr int need = qbytes + 2 * stages * tile + 1024, smem = need > 120 * 1024 ? need : 120 * 1024;
+    // TMEM columns: S of a group, which its P replaces (16 columns of S, 16 keys, hold
+    // the 8 columns of their high parts, then of their low ones), and O
+    static constexpr int s_col = 0, o_col = G * TN;
+    static_assert(o_col + G * HD <= 512, "TMEM");
 };
 
 struct PromptSync {
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready, o_done, drained;
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_done[2], drained;
     uint32_t tmem;
     volatile int gave_up;
-    float qscale[kRows];
+    float qscale[2 * kRows];
     // scales of K and exponents of V's for a tile's blocks of 16 keys; tile j's are
     // overwritten with j + 4, for which P(j) V(j) has to be done
     float ks[4][8], ve[4][8];
@@ -85,7 +91,64 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const float (&v)[16]) {
         "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
         : "memory");
 }
+template <int N>
+__device__ __forceinline__ void tmem_st(uint32_t at, const uint32_t (&r)[N]) {
+    static_assert(N == 8 || N == 16, "the forms below");
+    if constexpr (N == 8) {
+        tmem_st8(at, r);
+    } else {
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+        tmem_st16(at, v);
+    }
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Thirty-two columns of this warp's lanes, without waiting for them.
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at));
+}
+// Waits for this thread's loads from TMEM; the registers of `r` are good after it.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i++) asm volatile("" : "+r"(r[i]));
+}
+
+// Two f32 at a time.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ float2 floats_of(uint64_t p) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+    return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 
 // The descriptor of an MN-major tile in the 128-byte swizzled layout: 8 rows (k) of
 // 64 values (n) to an atom; `next` bytes from 64 values to the next 64, 1024 from 8
@@ -96,12 +159,12 @@ __device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t at, uint32_t next) {
 }
 
 template <int HD, int NP>
-__global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8Args a) {
+__global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_kernel(const Kv8Args a) {
     using S = PromptShape<HD, NP>;
-    constexpr int TN = S::TN, ST = S::stages;
+    constexpr int TN = S::TN, ST = S::stages, G = S::G, kSoftWarps = 4 * G;
     extern __shared__ __align__(1024) uint8_t raw[];
     __shared__ PromptSync y;
-    const uint32_t qs = (saddr(raw) + 1023u) & ~1023u, ks = qs + NP * S::qpart, vs = ks + ST * S::tile;
+    const uint32_t qs = (saddr(raw) + 1023u) & ~1023u, ks = qs + S::qbytes, vs = ks + ST * S::tile;
     uint8_t* const base = raw + (qs - saddr(raw));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // the last rows see the most keys: they go first
@@ -111,7 +174,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         if (tid == 0) flag(a.status, SPM_PAGE_QUERIES);
         return;
     }
-    const int nq = e0 - s0, len = kv8_len(a, req), row0 = tile * kRows, rows = min(kRows, nq * a.group - row0);
+    const int nq = e0 - s0, len = kv8_len(a, req), row0 = tile * G * kRows, rows = min(G * kRows, nq * a.group - row0);
+    const int groups = (rows + kRows - 1) / kRows;  // that have rows
     if (rows <= 0) return;
     const int keys = kv8_keys(a, nq, len, tile), tiles = (keys + TN - 1) / TN;
     if (tid == 0) {
@@ -121,9 +185,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
             mbar_init(&y.v_full[i], kFillThreads);
             mbar_init(&y.v_empty[i], 1);
             mbar_init(&y.s_full[i], 1);
+            mbar_init(&y.p_ready[i], kRows);
+            mbar_init(&y.o_done[i], 1);
         }
-        mbar_init(&y.p_ready, 32 * kSoftWarps);
-        mbar_init(&y.o_done, 1);
         mbar_init(&y.drained, 1);
         y.gave_up = 0;
         mbar_fence_init();
@@ -134,7 +198,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     } else {
         // ---- Q: rows scaled to 2^10 by a power of two, in fp16 parts ----
-        for (int r = warp; r < kRows; r += kSoftWarps + kFillWarps) {
+        for (int r = warp; r < groups * kRows; r += kSoftWarps + kFillWarps) {
             float x[HD / 32];
             uint32_t big = 0;
             const int qr = row0 + r, qi = qr / a.group, qh = head * a.group + qr % a.group;
@@ -153,9 +217,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                 const int d = lane + 32 * i;
                 const float v = big < 0x7f800000u ? __fmul_rn(x[i], mul) : 0.f;
                 const __half hi = __float2half_rn(v);
-                const uint32_t at = uint32_t(d >> 6) * (kRows * 128) + sw128_offset(r, (d & 63) >> 3) + 2 * (d & 7);
+                const uint32_t at = uint32_t(r / kRows) * (NP * S::qgroup) + uint32_t(d >> 6) * (kRows * 128) +
+                                    sw128_offset(r % kRows, (d & 63) >> 3) + 2 * (d & 7);
                 *reinterpret_cast<__half*>(base + at) = hi;
-                if (NP == 2) *reinterpret_cast<__half*>(base + S::qpart + at) = __float2half_rn(__fsub_rn(v, __half2float(hi)));
+                if (NP == 2) *reinterpret_cast<__half*>(base + S::qgroup + at) = __float2half_rn(__fsub_rn(v, __half2float(hi)));
             }
         }
     }
@@ -173,32 +238,40 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
     };
 
     if (warp >= kSoftWarps && warp < kMmaWarp) {
-        // ---- producers: the codes of tile j, converted while those of j + 1 load ----
+        // ---- producers: codes of tile j converted while those of j + 1 and the page
+        // numbers of j + 2 are on their way ----
         constexpr int SEG = HD / 16, N = TN * SEG / kFillThreads;  // 16-byte pieces of a token, and of a thread
         static_assert(TN * SEG % kFillThreads == 0, "whole pieces");
         const int t = tid - 32 * kSoftWarps;
         const int32_t* trow = a.table + size_t(req) * a.width;
-        auto page_of = [&](int tok) {
-            int p = tok < keys ? __ldg(trow + (tok >> a.shift)) : -1;
+        uint4 k[N], v[N];
+        int page[N];
+        auto find = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int tok = j * TN + (t + i * kFillThreads) / SEG;
+                page[i] = tok < keys ? __ldg(trow + (tok >> a.shift)) : -1;
+            }
+        };
+        // -1 for none, and for a page that is not in the pool
+        auto known = [&](int p, int tok) {
             if (tok < keys && uint32_t(p) >= uint32_t(a.pages)) {
                 flag(a.status, SPM_PAGE_ID);
-                p = a.pages ? 0 : -1;
+                return -1;
             }
             return p;
         };
-        uint4 c[N];
-        auto load = [&](const int8_t* codes, int j) {
+        auto load = [&](const int8_t* codes, int j, uint4 (&c)[N]) {
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int e = t + i * kFillThreads, r = e / SEG, o = e % SEG, tok = j * TN + r;
-                const int p = page_of(tok);
+                const int e = t + i * kFillThreads, r = e / SEG, o = e % SEG, tok = j * TN + r, p = known(page[i], tok);
                 c[i] = make_uint4(0, 0, 0, 0);
                 if (p >= 0)
                     c[i] = __ldg(reinterpret_cast<const uint4*>(
                         codes + ((size_t(p) * a.kv_heads + head) * a.page + (tok & (a.page - 1))) * HD + 16 * o));
             }
         };
-        auto store = [&](uint8_t* to) {
+        auto store = [&](uint8_t* to, const uint4 (&c)[N]) {
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const int e = t + i * kFillThreads, r = e / SEG, o = e % SEG;
@@ -215,165 +288,216 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Kv8
                 *reinterpret_cast<uint4*>(atom + sw128_offset(r, 2 * (o & 3) + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
             }
         };
-        if (tiles) load(a.k_codes, 0);
+        // the scales of tile j's blocks, a thread to a block; likewise a tile ahead
+        float kscale = 0.f, vscale = 0.f;
+        auto scales = [&](int j) {
+            const int tok = j * TN + 16 * t;
+            kscale = vscale = 0.f;
+            if (t >= TN / 16 || tok >= keys) return;
+            const int p = known(__ldg(trow + (tok >> a.shift)), tok);
+            if (p < 0) return;
+            kscale = __ldg(a.k_scales + size_t(p) * a.kv_heads + head);
+            vscale = __ldg(a.v_scales + size_t(p) * a.kv_heads + head);
+        };
+        if (tiles) {
+            find(0);
+            load(a.k_codes, 0, k);
+            load(a.v_codes, 0, v);
+            scales(0);
+            find(1);
+        }
         for (int j = 0; j < tiles; j++) {
             const int st = j % ST;
             const uint32_t again = uint32_t(j / ST - 1) & 1u;
             if (j >= ST && !wait(&y.k_empty[st], again)) break;
-            store(base + NP * S::qpart + st * S::tile);
-            load(a.v_codes, j);
+            store(base + S::qbytes + st * S::tile, k);
             if (t < TN / 16) {
-                const int p = page_of(j * TN + 16 * t);
-                y.ks[j & 3][t] = p >= 0 ? __ldg(a.k_scales + size_t(p) * a.kv_heads + head) : 0.f;
-                y.ve[j & 3][t] = p >= 0 ? kv8_exponent(__ldg(a.v_scales + size_t(p) * a.kv_heads + head)) : -INFINITY;
+                y.ks[j & 3][t] = kscale;
+                y.ve[j & 3][t] = kv8_exponent(vscale);
             }
             fence_proxy_async();
             mbar_arrive(&y.k_full[st]);
+            load(a.k_codes, j + 1, k);
+            scales(j + 1);
             if (j >= ST && !wait(&y.v_empty[st], again)) break;
-            store(base + NP * S::qpart + (ST + st) * S::tile);
-            if (j + 1 < tiles) load(a.k_codes, j + 1);
+            store(base + S::qbytes + (ST + st) * S::tile, v);
             fence_proxy_async();
             mbar_arrive(&y.v_full[st]);
+            load(a.v_codes, j + 1, v);
+            find(j + 2);
         }
     } else if (warp == kMmaWarp) {
         if (lane == 0) {
             constexpr uint32_t f32_out = 1u << 4, m = uint32_t(kRows >> 4) << 24;
             constexpr uint32_t id_s = f32_out | m | uint32_t(TN >> 3) << 17;
             constexpr uint32_t id_o = f32_out | m | uint32_t(HD >> 3) << 17 | 1u << 16;  // V is MN-major
-            auto scores = [&](int j) {
-                if (!wait(&y.k_full[j % ST], uint32_t(j / ST) & 1u)) return false;
-                tc_fence_after();
-                const uint32_t k = ks + uint32_t(j % ST) * S::tile, d = tmem + S::s_col + uint32_t(j & 1) * TN;
+            auto scores = [&](int g, int j) {
+                const uint32_t k = ks + uint32_t(j % ST) * S::tile, q = qs + uint32_t(g * NP) * S::qgroup;
 #pragma unroll
                 for (int p = NP - 1; p >= 0; p--)
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; kk++)
-                        umma_f16(d, sw128_desc(qs + uint32_t(p) * S::qpart + (kk >> 2) * (kRows * 128) + 32u * (kk & 3)),
+                        umma_f16(tmem + S::s_col + g * TN,
+                                 sw128_desc(q + uint32_t(p) * S::qgroup + (kk >> 2) * (kRows * 128) + 32u * (kk & 3)),
                                  sw128_desc(k + (kk >> 2) * (TN * 128) + 32u * (kk & 3)), id_s, p != NP - 1 || kk != 0);
-                umma_commit(&y.k_empty[j % ST]);
-                umma_commit(&y.s_full[j & 1]);
-                return true;
+                if (g == groups - 1) umma_commit(&y.k_empty[j % ST]);
+                umma_commit(&y.s_full[g]);
             };
-            bool ok = tiles == 0 || scores(0);
-            for (int j = 0; ok && j < tiles; j++) {
-                // (S(j + 1) takes the buffer of S(j - 1), which the softmax had read when P(j - 1) was ready)
-                if (j + 1 < tiles && !scores(j + 1)) break;
-                if (!wait(&y.v_full[j % ST], uint32_t(j / ST) & 1u)) break;
-                if (!wait(&y.p_ready, uint32_t(j) & 1u)) break;
+            bool ok = true;
+            if (tiles) {
+                ok = wait(&y.k_full[0], 0);
                 tc_fence_after();
-                const uint32_t v = vs + uint32_t(j % ST) * S::tile;
-#pragma unroll
-                for (int p = NP - 1; p >= 0; p--)
-#pragma unroll
-                    for (int kk = 0; kk < TN / 16; kk++)
-                        umma_f16_ts(tmem + S::o_col, tmem + S::p_col + uint32_t(p) * (TN / 2) + 8u * kk,
-                                    sw128_mn_desc(v + 2048u * kk, TN * 128), id_o, j != 0 || p != NP - 1 || kk != 0);
-                umma_commit(&y.v_empty[j % ST]);
-                umma_commit(&y.o_done);
+                for (int g = 0; ok && g < groups; g++) scores(g, 0);
             }
+            for (int j = 0; ok && j < tiles; j++)
+                for (int g = 0; g < groups; g++) {
+                    if (g == 0) ok = wait(&y.v_full[j % ST], uint32_t(j / ST) & 1u);
+                    ok = ok && wait(&y.p_ready[g], uint32_t(j) & 1u);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t v = vs + uint32_t(j % ST) * S::tile;
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; p--)
+#pragma unroll
+                        for (int kk = 0; kk < TN / 16; kk++)
+                            umma_f16_ts(tmem + S::o_col + g * HD, tmem + S::s_col + g * TN + 16u * kk + 8u * p,
+                                        sw128_mn_desc(v + 2048u * kk, TN * 128), id_o, j != 0 || p != NP - 1 || kk != 0);
+                    if (g == groups - 1) umma_commit(&y.v_empty[j % ST]);
+                    if (j + 1 < tiles) {
+                        // over the P that the products above read: they run in order
+                        if (g == 0) ok = wait(&y.k_full[(j + 1) % ST], uint32_t((j + 1) / ST) & 1u);
+                        if (!ok) break;
+                        tc_fence_after();
+                        scores(g, j + 1);
+                    } else {
+                        umma_commit(&y.o_done[g]);
+                    }
+                }
             umma_commit(&y.drained);  // TMEM is given back when every product has ended
             mbar_wait(&y.drained, 0);
         }
         __syncwarp();
     } else {
-        // ---- softmax: thread = row = TMEM lane ----
-        const int r = tid;
-        const uint32_t lanes = uint32_t(32 * warp) << 16;
+        // ---- softmax: thread = row = TMEM lane of its group ----
+        const int g = warp >> 2, r = tid;
+        const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
+        const uint32_t s = tmem + lanes + S::s_col + uint32_t(g) * TN, o = tmem + lanes + S::o_col + uint32_t(g) * HD;
         const float qscale = y.qscale[r];
         const int limit = r < rows ? len - nq + (row0 + r) / a.group + 1 : 0;  // keys that the row sees
         float m = -INFINITY, ref = -INFINITY, sum = 0.f;
         bool ok = true;
-        for (int j = 0; j < tiles; j++) {
-            ok = wait(&y.s_full[j & 1], uint32_t(j >> 1) & 1u);
+        const int turns = g < groups ? tiles : 0;
+        for (int j = 0; j < turns; j++) {
+            // (S(j) done means P(j - 1) V(j - 1) done: O may be read and written)
+            ok = wait(&y.s_full[g], uint32_t(j) & 1u);
             if (!__all_sync(0xffffffffu, ok)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
-            const uint32_t s = tmem + lanes + S::s_col + uint32_t(j & 1) * TN;
             const int t0 = j * TN;
             const bool hidden = __any_sync(0xffffffffu, t0 + TN > limit);
+            uint32_t v[2][32];
             // the row's maximum, and the largest exponent that a weighted value can have
             float top = -INFINITY, reach = -INFINITY;
+            tmem_ld32(s, v[0]);
 #pragma unroll
-            for (int b = 0; b < TN / 16; b++) {
-                float v[16], big = -INFINITY;
-                tmem_ld16(s + 16 * b, v);
+            for (int c = 0; c < TN / 32; c++) {
+                tmem_ld_wait(v[c & 1]);
+                if (c + 1 < TN / 32) tmem_ld32(s + 32 * (c + 1), v[(c + 1) & 1]);
 #pragma unroll
-                for (int e = 0; e < 16; e++)
-                    if (!hidden || t0 + 16 * b + e < limit) big = fmaxf(big, v[e]);
-                const float f = qscale * y.ks[j & 3][b];  // not negative, or NaN
-                big = big == -INFINITY ? big : f != f ? 0.f : ceilf(big * f);
-                top = fmaxf(top, big);
-                reach = fmaxf(reach, big + y.ve[j & 3][b]);
+                for (int h = 0; h < 2; h++) {
+                    const int b = 2 * c + h;
+                    float big = -INFINITY;
+                    if (hidden) {
+#pragma unroll
+                        for (int e = 0; e < 16; e++)
+                            if (t0 + 16 * b + e < limit) big = fmaxf(big, __uint_as_float(v[c & 1][16 * h + e]));
+                    } else {
+                        float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (int e = 0; e < 16; e++) x[e & 3] = fmaxf(x[e & 3], __uint_as_float(v[c & 1][16 * h + e]));
+                        big = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                    }
+                    const float f = qscale * y.ks[j & 3][b];  // not negative, or NaN
+                    big = big == -INFINITY ? big : f != f ? 0.f : ceilf(big * f);
+                    top = fmaxf(top, big);
+                    reach = fmaxf(reach, big + y.ve[j & 3][b]);
+                }
             }
             const float m_new = top > m + kSlack || m == -INFINITY ? top : m;
             const float r_new = reach > ref + kSlack || ref == -INFINITY ? reach : ref;
             sum *= kv8_step(m, m_new);
-            const float down = kv8_step(ref, r_new);
+            const float down = r_new != ref ? kv8_step(ref, r_new) : 1.f;
             m = m_new;
-            // P and O are the last product's until it is done
-            if (j) {
-                ok = wait(&y.o_done, uint32_t(j - 1) & 1u);
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                if (__any_sync(0xffffffffu, r_new != ref)) {
-#pragma unroll 1
-                    for (int d = 0; d < HD; d += 16) {
-                        float v[16];
-                        tmem_ld16(tmem + lanes + S::o_col + d, v);
-#pragma unroll
-                        for (int e = 0; e < 16; e++) v[e] *= r_new != ref ? down : 1.f;
-                        tmem_st16(tmem + lanes + S::o_col + d, v);
-                    }
-                }
-            }
             ref = r_new;
-            const float m0 = m == -INFINITY ? 0.f : m;
+            if (j && __any_sync(0xffffffffu, down != 1.f)) {
+#pragma unroll 1
+                for (int d = 0; d < HD; d += 16) {
+                    float x[16];
+                    tmem_ld16(o + d, x);
 #pragma unroll
-            for (int b = 0; b < TN / 16; b++) {
-                float v[16];
-                tmem_ld16(s + 16 * b, v);
-                const float f = qscale * y.ks[j & 3][b], ve = y.ve[j & 3][b];
-                const float w = ve != ve ? ve : ve == -INFINITY || ref == -INFINITY ? 0.f
-                                : pow2i(int(fminf(fmaxf(m0 + ve - ref, -126.f), 126.f)));
-                uint32_t hi[8], lo[8];
-#pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    float p[2];
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const bool seen = !hidden || t0 + 16 * b + e + h < limit;
-                        const float x = kv8_exp2(fmaf(v[e + h], f, -m0));
-                        sum += seen ? x : 0.f;
-                        p[h] = seen ? x * w : 0.f;
-                    }
-                    hi[e / 2] = kv8_half2(p[0], p[1]);
-                    if (NP == 2) {
-                        const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&hi[e / 2]));
-                        lo[e / 2] = kv8_half2(p[0] - q.x, p[1] - q.y);
-                    }
+                    for (int e = 0; e < 16; e++) x[e] *= down;
+                    tmem_st16(o + d, x);
                 }
-                tmem_st8(tmem + lanes + S::p_col + 8 * b, hi);
-                if (NP == 2) tmem_st8(tmem + lanes + S::p_col + TN / 2 + 8 * b, lo);
             }
+            const float m0 = m == -INFINITY ? 0.f : m;
+            const uint64_t minus = pair_of(-m0, -m0);
+            uint64_t sums[2] = {0, 0};
+            tmem_ld32(s, v[0]);
+#pragma unroll
+            for (int c = 0; c < TN / 32; c++) {
+                tmem_ld_wait(v[c & 1]);
+                if (c + 1 < TN / 32) tmem_ld32(s + 32 * (c + 1), v[(c + 1) & 1]);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int b = 2 * c + h;
+                    const float f = qscale * y.ks[j & 3][b], ve = y.ve[j & 3][b];
+                    const float w = ve != ve ? ve : ve == -INFINITY || ref == -INFINITY ? 0.f
+                                    : pow2i(int(fminf(fmaxf(m0 + ve - ref, -126.f), 126.f)));
+                    const uint64_t ff = pair_of(f, f), ww = pair_of(w, w);
+                    uint32_t out[8 * NP];
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float2 x = floats_of(fma2(
+                            pair_of(__uint_as_float(v[c & 1][16 * h + e]), __uint_as_float(v[c & 1][16 * h + e + 1])), ff, minus));
+                        uint64_t p = pair_of(kv8_exp2(x.x), kv8_exp2(x.y));
+                        if (hidden) {
+                            // (a masked key adds nothing even to a page of NaN)
+                            const bool s0 = t0 + 16 * b + e < limit, s1 = t0 + 16 * b + e + 1 < limit;
+                            const float2 q = floats_of(p), z = floats_of(mul2(p, ww));
+                            sums[h] = add2(sums[h], pair_of(s0 ? q.x : 0.f, s1 ? q.y : 0.f));
+                            p = pair_of(s0 ? z.x : 0.f, s1 ? z.y : 0.f);
+                        } else {
+                            sums[h] = add2(sums[h], p);
+                            p = mul2(p, ww);
+                        }
+                        const float2 z = floats_of(p);
+                        out[e / 2] = kv8_half2(z.x, z.y);
+                        if (NP == 2) {
+                            const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&out[e / 2]));
+                            out[8 * (NP - 1) + e / 2] = kv8_half2(z.x - q.x, z.y - q.y);
+                        }
+                    }
+                    tmem_st<8 * NP>(s + 16 * b, out);
+                }
+            }
+            const float2 s2 = floats_of(add2(sums[0], sums[1]));
+            sum += s2.x + s2.y;
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(&y.p_ready);
+            mbar_arrive(&y.p_ready[g]);
         }
-        if (ok && tiles) ok = wait(&y.o_done, uint32_t(tiles - 1) & 1u);
+        if (ok && turns) ok = wait(&y.o_done[g], 0);
         tc_fence_after();
-        if (__all_sync(0xffffffffu, ok)) {
+        if (__all_sync(0xffffffffu, ok) && g < groups) {
             const int qr = row0 + r, qi = qr / a.group, qh = head * a.group + qr % a.group;
             const int64_t at = int64_t(s0 + qi) * a.o_token + qh * a.o_head;
 #pragma unroll 1
             for (int d = 0; d < HD; d += 16) {
                 float v[16];
                 if (tiles) {
-                    tmem_ld16(tmem + lanes + S::o_col + d, v);
+                    tmem_ld16(o + d, v);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 16; e++) v[e] = 0.f;
@@ -401,7 +525,7 @@ void launch(const Kv8Args& a, cudaStream_t st) {
     static unsigned long long done = 0;
     allow_smem(kv8_prompt_kernel<HD, NP>, smem, done);
     const dim3 grid(unsigned(a.tiles), unsigned(a.kv_heads), unsigned(a.requests));
-    kv8_prompt_kernel<HD, NP><<<grid, kPromptThreads, smem, st>>>(a);
+    kv8_prompt_kernel<HD, NP><<<grid, PromptShape<HD, NP>::threads, smem, st>>>(a);
     CUDA_OK(cudaGetLastError());
 }
 
