@@ -26,6 +26,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kv8.h"
 #include "kv8_attention.h"
@@ -157,6 +158,9 @@ __device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t at, uint32_t next) {
     return uint64_t((at & 0x3FFFFu) >> 4) | (uint64_t(next >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
            (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
+
+typedef std::true_type Yes;
+typedef std::false_type No;
 
 template <int HD, int NP>
 __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_kernel(const Kv8Args a) {
@@ -397,34 +401,42 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
             tc_fence_after();
             const int t0 = j * TN;
             const bool hidden = __any_sync(0xffffffffu, t0 + TN > limit);
+            // f(columns 32 c .. of S, c), the next columns on their way meanwhile
             uint32_t v[2][32];
+            auto columns = [&](auto&& f) {
+                tmem_ld32(s, v[0]);
+#pragma unroll 1
+                for (int c = 0; c < TN / 32; c += 2) {
+                    tmem_ld_wait(v[0]);
+                    tmem_ld32(s + 32 * (c + 1), v[1]);
+                    f(v[0], c);
+                    tmem_ld_wait(v[1]);
+                    if (c + 2 < TN / 32) tmem_ld32(s + 32 * (c + 2), v[0]);
+                    f(v[1], c + 1);
+                }
+            };
             // the row's maximum, and the largest exponent that a weighted value can have
             float top = -INFINITY, reach = -INFINITY;
-            tmem_ld32(s, v[0]);
+            auto maxima = [&](auto masked) {
+                columns([&](const uint32_t (&v)[32], int c) {
 #pragma unroll
-            for (int c = 0; c < TN / 32; c++) {
-                tmem_ld_wait(v[c & 1]);
-                if (c + 1 < TN / 32) tmem_ld32(s + 32 * (c + 1), v[(c + 1) & 1]);
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int b = 2 * c + h;
-                    float big = -INFINITY;
-                    if (hidden) {
-#pragma unroll
-                        for (int e = 0; e < 16; e++)
-                            if (t0 + 16 * b + e < limit) big = fmaxf(big, __uint_as_float(v[c & 1][16 * h + e]));
-                    } else {
+                    for (int h = 0; h < 2; h++) {
+                        const int b = 2 * c + h;
                         float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int e = 0; e < 16; e++) x[e & 3] = fmaxf(x[e & 3], __uint_as_float(v[c & 1][16 * h + e]));
-                        big = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                        for (int e = 0; e < 16; e++) {
+                            const float y = __uint_as_float(v[16 * h + e]);
+                            x[e & 3] = fmaxf(x[e & 3], masked && t0 + 16 * b + e >= limit ? -INFINITY : y);
+                        }
+                        float big = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                        const float f = qscale * y.ks[j & 3][b];  // not negative, or NaN
+                        big = big == -INFINITY ? big : f != f ? 0.f : ceilf(big * f);
+                        top = fmaxf(top, big);
+                        reach = fmaxf(reach, big + y.ve[j & 3][b]);
                     }
-                    const float f = qscale * y.ks[j & 3][b];  // not negative, or NaN
-                    big = big == -INFINITY ? big : f != f ? 0.f : ceilf(big * f);
-                    top = fmaxf(top, big);
-                    reach = fmaxf(reach, big + y.ve[j & 3][b]);
-                }
-            }
+                });
+            };
+            hidden ? maxima(Yes()) : maxima(No());
             const float m_new = top > m + kSlack || m == -INFINITY ? top : m;
             const float r_new = reach > ref + kSlack || ref == -INFINITY ? reach : ref;
             sum *= kv8_step(m, m_new);
@@ -444,44 +456,43 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
             const float m0 = m == -INFINITY ? 0.f : m;
             const uint64_t minus = pair_of(-m0, -m0);
             uint64_t sums[2] = {0, 0};
-            tmem_ld32(s, v[0]);
+            auto weights = [&](auto masked) {
+                columns([&](const uint32_t (&v)[32], int c) {
 #pragma unroll
-            for (int c = 0; c < TN / 32; c++) {
-                tmem_ld_wait(v[c & 1]);
-                if (c + 1 < TN / 32) tmem_ld32(s + 32 * (c + 1), v[(c + 1) & 1]);
+                    for (int h = 0; h < 2; h++) {
+                        const int b = 2 * c + h;
+                        const float f = qscale * y.ks[j & 3][b], ve = y.ve[j & 3][b];
+                        const float w = ve != ve ? ve : ve == -INFINITY || ref == -INFINITY ? 0.f
+                                        : pow2i(int(fminf(fmaxf(m0 + ve - ref, -126.f), 126.f)));
+                        const uint64_t ff = pair_of(f, f), ww = pair_of(w, w);
+                        uint32_t out[8 * NP];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int b = 2 * c + h;
-                    const float f = qscale * y.ks[j & 3][b], ve = y.ve[j & 3][b];
-                    const float w = ve != ve ? ve : ve == -INFINITY || ref == -INFINITY ? 0.f
-                                    : pow2i(int(fminf(fmaxf(m0 + ve - ref, -126.f), 126.f)));
-                    const uint64_t ff = pair_of(f, f), ww = pair_of(w, w);
-                    uint32_t out[8 * NP];
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const float2 x = floats_of(fma2(
-                            pair_of(__uint_as_float(v[c & 1][16 * h + e]), __uint_as_float(v[c & 1][16 * h + e + 1])), ff, minus));
-                        uint64_t p = pair_of(kv8_exp2(x.x), kv8_exp2(x.y));
-                        if (hidden) {
-                            // (a masked key adds nothing even to a page of NaN)
-                            const bool s0 = t0 + 16 * b + e < limit, s1 = t0 + 16 * b + e + 1 < limit;
-                            const float2 q = floats_of(p), z = floats_of(mul2(p, ww));
-                            sums[h] = add2(sums[h], pair_of(s0 ? q.x : 0.f, s1 ? q.y : 0.f));
-                            p = pair_of(s0 ? z.x : 0.f, s1 ? z.y : 0.f);
-                        } else {
-                            sums[h] = add2(sums[h], p);
-                            p = mul2(p, ww);
+                        for (int e = 0; e < 16; e += 2) {
+                            const float2 x = floats_of(
+                                fma2(pair_of(__uint_as_float(v[16 * h + e]), __uint_as_float(v[16 * h + e + 1])), ff, minus));
+                            uint64_t p = pair_of(kv8_exp2(x.x), kv8_exp2(x.y));
+                            if (masked) {
+                                // (a masked key adds nothing even to a page of NaN)
+                                const bool s0 = t0 + 16 * b + e < limit, s1 = t0 + 16 * b + e + 1 < limit;
+                                const float2 q = floats_of(p), z = floats_of(mul2(p, ww));
+                                sums[h] = add2(sums[h], pair_of(s0 ? q.x : 0.f, s1 ? q.y : 0.f));
+                                p = pair_of(s0 ? z.x : 0.f, s1 ? z.y : 0.f);
+                            } else {
+                                sums[h] = add2(sums[h], p);
+                                p = mul2(p, ww);
+                            }
+                            const float2 z = floats_of(p);
+                            out[e / 2] = kv8_half2(z.x, z.y);
+                            if (NP == 2) {
+                                const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&out[e / 2]));
+                                out[8 * (NP - 1) + e / 2] = kv8_half2(z.x - q.x, z.y - q.y);
+                            }
                         }
-                        const float2 z = floats_of(p);
-                        out[e / 2] = kv8_half2(z.x, z.y);
-                        if (NP == 2) {
-                            const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&out[e / 2]));
-                            out[8 * (NP - 1) + e / 2] = kv8_half2(z.x - q.x, z.y - q.y);
-                        }
+                        tmem_st<8 * NP>(s + 16 * b, out);
                     }
-                    tmem_st<8 * NP>(s + 16 * b, out);
-                }
-            }
+                });
+            };
+            hidden ? weights(Yes()) : weights(No());
             const float2 s2 = floats_of(add2(sums[0], sums[1]));
             sum += s2.x + s2.y;
             tmem_st_wait();
