@@ -4,7 +4,7 @@
 //
 // A CTA owns G groups of 128 rows (query x head of the group) of a request and kv
 // head and walks the keys in tiles of TN, once:
-//   producers (4 warps)  codes from global memory to fp16 (exact) in shared
+//   producers (8 warps)  codes from global memory to fp16 (exact) in shared
 //                        memory: a token's row of 64 dimensions is 128 bytes in the
 //                        128-byte swizzled layout, which is K-major for the keys
 //                        (S = Q K^T) and MN-major for the values (O = P V), so both
@@ -37,7 +37,7 @@ namespace {
 using namespace dev;
 
 constexpr int kRows = 128;                             // of a group: the MMA's M
-constexpr int kFillWarps = 4, kFillThreads = 32 * kFillWarps;
+constexpr int kFillWarps = 8, kFillThreads = 32 * kFillWarps;
 constexpr float kSlack = 8.f;                          // in powers of two
 
 template <int HD, int NP>
@@ -65,7 +65,8 @@ struct PromptSync {
     float qscale[2 * kRows];
     // scales of K and exponents of V's for a tile's blocks of 16 keys; tile j's are
     // overwritten with j + 4, for which P(j) V(j) has to be done
-    float ks[4][8], ve[4][8];
+    float ks[4][8], ve[4][8], vn[4][8];  // (vn: NaN for a scale that is, else 0)
+    int vi[4][8];                        // ve, -10000 for a scale of 0
 };
 
 __device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
@@ -317,7 +318,10 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
             store(base + S::qbytes + st * S::tile, k);
             if (t < TN / 16) {
                 y.ks[j & 3][t] = kscale;
-                y.ve[j & 3][t] = kv8_exponent(vscale);
+                const float e = kv8_exponent(vscale);
+                y.ve[j & 3][t] = e;
+                y.vi[j & 3][t] = vscale > 0.f ? int(e) : -10000;
+                y.vn[j & 3][t] = e != e ? e : 0.f;
             }
             fence_proxy_async();
             mbar_arrive(&y.k_full[st]);
@@ -401,18 +405,14 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
             tc_fence_after();
             const int t0 = j * TN;
             const bool hidden = __any_sync(0xffffffffu, t0 + TN > limit);
-            // f(columns 32 c .. of S, c), the next columns on their way meanwhile
-            uint32_t v[2][32];
+            // f(columns 32 c .. of S, c)
             auto columns = [&](auto&& f) {
-                tmem_ld32(s, v[0]);
 #pragma unroll 1
-                for (int c = 0; c < TN / 32; c += 2) {
-                    tmem_ld_wait(v[0]);
-                    tmem_ld32(s + 32 * (c + 1), v[1]);
-                    f(v[0], c);
-                    tmem_ld_wait(v[1]);
-                    if (c + 2 < TN / 32) tmem_ld32(s + 32 * (c + 2), v[0]);
-                    f(v[1], c + 1);
+                for (int c = 0; c < TN / 32; c++) {
+                    uint32_t v[32];
+                    tmem_ld32(s + 32 * c, v);
+                    tmem_ld_wait(v);
+                    f(v, c);
                 }
             };
             // the row's maximum, and the largest exponent that a weighted value can have
@@ -455,15 +455,16 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
             }
             const float m0 = m == -INFINITY ? 0.f : m;
             const uint64_t minus = pair_of(-m0, -m0);
+            const int lift = ref == -INFINITY ? -20000 : int(fminf(fmaxf(m0 - ref, -5000.f), 5000.f));
             uint64_t sums[2] = {0, 0};
             auto weights = [&](auto masked) {
                 columns([&](const uint32_t (&v)[32], int c) {
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         const int b = 2 * c + h;
-                        const float f = qscale * y.ks[j & 3][b], ve = y.ve[j & 3][b];
-                        const float w = ve != ve ? ve : ve == -INFINITY || ref == -INFINITY ? 0.f
-                                        : pow2i(int(fminf(fmaxf(m0 + ve - ref, -126.f), 126.f)));
+                        // 2^(m + ve - ref); 2^-126, 0 in fp16, for a page of zeros; NaN for one of NaN
+                        const float f = qscale * y.ks[j & 3][b];
+                        const float w = pow2i(min(lift + y.vi[j & 3][b], 126)) + y.vn[j & 3][b];
                         const uint64_t ff = pair_of(f, f), ww = pair_of(w, w);
                         uint32_t out[8 * NP];
 #pragma unroll
