@@ -202,30 +202,39 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&y.tmem)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     } else {
-        // ---- Q: rows scaled to 2^10 by a power of two, in fp16 parts ----
-        for (int r = warp; r < groups * kRows; r += kSoftWarps + kFillWarps) {
-            float x[HD / 32];
-            uint32_t big = 0;
-            const int qr = row0 + r, qi = qr / a.group, qh = head * a.group + qr % a.group;
+        // ---- Q: rows scaled to 2^10 by a power of two, in fp16 parts; four rows' loads together ----
+        constexpr int AT_ONCE = 4, STEP = kSoftWarps + kFillWarps;
+        for (int r0 = warp; r0 < groups * kRows; r0 += AT_ONCE * STEP) {
+            float x[AT_ONCE][HD / 32];
 #pragma unroll
-            for (int i = 0; i < HD / 32; i++) {
-                x[i] = r < rows ? kv8_load(a, int64_t(s0 + qi) * a.q_token + qh * a.q_head + lane + 32 * i) : 0.f;
-                big = max(big, __float_as_uint(x[i]) & 0x7fffffffu);
+            for (int u = 0; u < AT_ONCE; u++) {
+                const int r = r0 + u * STEP, qr = row0 + r, qi = qr / a.group, qh = head * a.group + qr % a.group;
+#pragma unroll
+                for (int i = 0; i < HD / 32; i++)
+                    x[u][i] = r < rows ? kv8_load(a, int64_t(s0 + qi) * a.q_token + qh * a.q_head + lane + 32 * i) : 0.f;
             }
-            big = __reduce_max_sync(0xffffffffu, big);
-            const int up = min(137 - int(big >> 23), 126);
-            // (a negative scale is the queries' sign: the largest sum is then the largest score)
-            const float mul = a.scale_log2 < 0.f ? -pow2i(up) : pow2i(up);
-            if (lane == 0) y.qscale[r] = big < 0x7f800000u ? fabsf(a.scale_log2) * pow2i(-up) : __int_as_float(0x7fffffff);
 #pragma unroll
-            for (int i = 0; i < HD / 32; i++) {
-                const int d = lane + 32 * i;
-                const float v = big < 0x7f800000u ? __fmul_rn(x[i], mul) : 0.f;
-                const __half hi = __float2half_rn(v);
-                const uint32_t at = uint32_t(r / kRows) * (NP * S::qgroup) + uint32_t(d >> 6) * (kRows * 128) +
-                                    sw128_offset(r % kRows, (d & 63) >> 3) + 2 * (d & 7);
-                *reinterpret_cast<__half*>(base + at) = hi;
-                if (NP == 2) *reinterpret_cast<__half*>(base + S::qgroup + at) = __float2half_rn(__fsub_rn(v, __half2float(hi)));
+            for (int u = 0; u < AT_ONCE; u++) {
+                const int r = r0 + u * STEP;
+                if (r >= groups * kRows) break;
+                uint32_t big = 0;
+#pragma unroll
+                for (int i = 0; i < HD / 32; i++) big = max(big, __float_as_uint(x[u][i]) & 0x7fffffffu);
+                big = __reduce_max_sync(0xffffffffu, big);
+                const int up = min(137 - int(big >> 23), 126);
+                // (a negative scale is the queries' sign: the largest sum is then the largest score)
+                const float mul = a.scale_log2 < 0.f ? -pow2i(up) : pow2i(up);
+                if (lane == 0) y.qscale[r] = big < 0x7f800000u ? fabsf(a.scale_log2) * pow2i(-up) : __int_as_float(0x7fffffff);
+#pragma unroll
+                for (int i = 0; i < HD / 32; i++) {
+                    const int d = lane + 32 * i;
+                    const float v = big < 0x7f800000u ? __fmul_rn(x[u][i], mul) : 0.f;
+                    const __half hi = __float2half_rn(v);
+                    const uint32_t at = uint32_t(r / kRows) * (NP * S::qgroup) + uint32_t(d >> 6) * (kRows * 128) +
+                                        sw128_offset(r % kRows, (d & 63) >> 3) + 2 * (d & 7);
+                    *reinterpret_cast<__half*>(base + at) = hi;
+                    if (NP == 2) *reinterpret_cast<__half*>(base + S::qgroup + at) = __float2half_rn(__fsub_rn(v, __half2float(hi)));
+                }
             }
         }
     }
@@ -405,7 +414,8 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
             tc_fence_after();
             const int t0 = j * TN;
             const bool hidden = __any_sync(0xffffffffu, t0 + TN > limit);
-            // f(columns 32 c .. of S, c)
+            // f(columns 32 c .. of S, c).  (Fetching the next columns meanwhile costs 32
+            // registers more than 17 warps leave a thread, and more in spills than it saves.)
             auto columns = [&](auto&& f) {
 #pragma unroll 1
                 for (int c = 0; c < TN / 32; c++) {
