@@ -88,6 +88,11 @@ class SweepInfo(C.Structure):
                 ("device_bytes", C.c_uint64), ("copies", C.c_uint64), ("bytes_copied", C.c_uint64)]
 
 
+class SamplingSpec(C.Structure):
+    """spm_sampling (spmgpu.h)."""
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float)]
+
+
 class Kv8(C.Structure):
     """spm_kv8 (spmgpu.h)."""
     _fields_ = [("device", C.c_int32), ("pages", C.c_int32), ("page_tokens", C.c_int32), ("kv_heads", C.c_int32),
@@ -130,6 +135,10 @@ PROTOTYPES = {
     "spm_weights_gemv": (C.c_int32, [_P, _P, C.c_int32, _P, _P]),
     "spm_weights_dequant": (C.c_int32, [_P, C.c_uint64, C.c_uint64, _FP]),
     "spm_session_create": (C.c_int32, [_P, C.c_int32, C.c_int32, C.POINTER(_P)]),
+    "spm_session_create_paged": (C.c_int32, [_P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(_P)]),
+    "spm_session_free_pages": (C.c_int32, [_P, _I32P]),
+    "spm_decode_step_sampled": (C.c_int32, [_P, _U32P, C.c_int32, C.POINTER(SamplingSpec), C.POINTER(C.c_float), _FP,
+                                            _U32P, _U32P]),
     "spm_session_destroy": (C.c_int32, [_P]),
     "spm_client_reset": (C.c_int32, [_P, C.c_int32]),
     "spm_client_len": (C.c_int32, [_P, C.c_int32, _I32P]),

@@ -89,6 +89,25 @@ struct spm_session {
     float *act = nullptr, *logits = nullptr;
     float2* rope = nullptr;
     int32_t* pos = nullptr;
+    // Paged sessions (spm_session_create_paged): every layer's 8-bit pages, one table
+    // and free stack for all of them, and the tick's plan.  The host keeps the number
+    // of free pages itself: it knows every length.
+    struct Paged {
+        int page = 0, pages = 0, width = 0, free = 0;
+        int8_t *k_codes = nullptr, *v_codes = nullptr;
+        float *k_scales = nullptr, *v_scales = nullptr;
+        int32_t *table = nullptr, *stack = nullptr, *count = nullptr;
+        int32_t *ones = nullptr, *fresh = nullptr, *ended = nullptr;  // [max_clients]: 1; a prompt's tokens; 0 but in a reset
+        int32_t *starts = nullptr, *lens = nullptr, *positions = nullptr, *slots = nullptr;
+        uint8_t* work = nullptr;
+        uint64_t work_bytes = 0;
+        int need(int len) const { return (len + page - 1) / page; }
+    } pg;
+    bool paged() const { return pg.page != 0; }
+    // sampled steps: settings and numbers by client, then the tokens drawn
+    float *samp_temperature = nullptr, *samp_p = nullptr, *samp_min = nullptr, *samp_u = nullptr;
+    int32_t *samp_k = nullptr, *samp_token = nullptr;
+    int32_t* h_samp = nullptr;
     uint32_t *tokens = nullptr, *argmax = nullptr;
     uint32_t *h_tokens = nullptr, *h_argmax = nullptr;
     float* sumsq = nullptr;            // two [kMaxParts][8] partial sum-of-squares buffers
@@ -166,6 +185,7 @@ struct spm_session {
         if (h_tokens) cudaFreeHost(h_tokens);
         if (h_argmax) cudaFreeHost(h_argmax);
         if (h_status) cudaFreeHost(h_status);
+        if (h_samp) cudaFreeHost(h_samp);
         if (stream) cudaStreamDestroy(stream);
     }
     template <class T>
@@ -755,6 +775,51 @@ int run_gemv(const spm_model* m, GemvLaunch L, uint32_t dtype, cudaStream_t st, 
 // The RMSNorms are fused into the GEMV that consumes them: the residual-add
 // epilogues (and the embedding) write per-CTA sums of squares, which the next
 // GEMV reduces in a fixed order before normalising its activations on load.
+// An entry point of this library called from another: its message stands.
+void inner(spm_status st) {
+    if (st != SPM_OK) fail(st, spm::last_error());
+}
+
+// Layer l's pages of a paged session.
+spm_kv8 paged_layer(const spm_session* s, int l) {
+    const spm_model_cfg& c = s->m->cfg;
+    const auto& g = s->pg;
+    const size_t scales = size_t(l) * g.pages * c.kv_heads, codes = scales * g.page * c.head_dim;
+    return spm_kv8{s->m->device, g.pages, g.page, int32_t(c.kv_heads), int32_t(c.head_dim), 0, g.k_codes + codes,
+                   g.v_codes + codes, g.k_scales + scales, g.v_scales + scales, s->status};
+}
+
+// The plan of rows [row, row + n) of the table: cached tokens in s->pos, `fresh` more.
+void paged_plan(spm_session* s, int row, int n, const int32_t* fresh, const int32_t* ended, int tokens) {
+    auto& g = s->pg;
+    inner(spm_page_plan(s->m->device, s->pos + row, fresh, ended, n, g.page, g.table + size_t(row) * g.width, g.width,
+                        g.stack, g.pages, g.count, g.count, tokens, g.starts, g.lens, g.positions, g.slots, s->status,
+                        s->stream));
+}
+
+// A layer's attention over T planned rows of q, k, v (rows of the table from `row`
+// on): QK-norm and RoPE in place, the rows into their pages, attention into out.
+void paged_attention(spm_session* s, int l, const LayerIdx& L, int row, int requests, int most, int T, float* q, float* k,
+                     const float* v, float* out) {
+    spm_model* m = s->m;
+    const spm_model_cfg& c = m->cfg;
+    auto& g = s->pg;
+    QkArgs a{};
+    a.q = q; a.k = k; a.v = v; a.k_out = k; a.pos = g.positions; a.rope = s->rope;
+    a.q_norm = L.q_norm >= 0 ? m->gains + L.q_norm : nullptr;
+    a.k_norm = L.k_norm >= 0 ? m->gains + L.k_norm : nullptr;
+    a.layer = l; a.layers = int(c.layers); a.context = s->context;
+    a.heads = int(c.heads); a.kv_heads = int(c.kv_heads); a.head_dim = int(c.head_dim); a.family = int(c.family);
+    a.eps = c.eps;
+    CUDA_OK(launch_qk_rope_append(a, T, s->stream));
+    const spm_kv8 cache = paged_layer(s, l);
+    const int64_t hd = c.head_dim, kvw = hd * c.kv_heads, qw = hd * c.heads;
+    inner(spm_kv8_append(&cache, SPM_F32, k, kvw, hd, v, kvw, hd, T, g.slots, s->stream));
+    inner(spm_kv8_attention(&cache, SPM_F32, q, qw, hd, int32_t(c.heads), T, g.starts, g.lens, requests, most,
+                            g.table + size_t(row) * g.width, g.width, 1.0f / std::sqrt(float(hd)), out, qw, hd, g.work,
+                            g.work_bytes, s->stream));
+}
+
 void enqueue_step(spm_session* s, int n) {
     spm_model* m = s->m;
     const spm_model_cfg& c = m->cfg;
@@ -794,6 +859,11 @@ void enqueue_step(spm_session* s, int n) {
                              part[0], st, false, f0));
         return 0;
     });
+    if (s->paged())
+        timed(SPM_KERNEL_OTHER, -1, -1, 0, [&] {
+            paged_plan(s, 0, n, s->pg.ones, nullptr, n);
+            return 0;
+        });
     int parts = nl;
     auto norm_in = [&](GemvLaunch& g, int64_t gain, int which) {
         g.gain = m->gains + gain;
@@ -822,7 +892,8 @@ void enqueue_step(spm_session* s, int n) {
         P.heads = int(c.heads); P.kv_heads = int(c.kv_heads); P.head_dim = int(c.head_dim);
         P.family = int(c.family); P.eps = c.eps; P.status = s->status;
         timed(SPM_KERNEL_ATTENTION, int(l), -1, 0, [&] {
-            CUDA_OK(launch_attention(P, nl, st, pdl));
+            if (s->paged()) paged_attention(s, int(l), L, 0, n, 1, n, s->q, s->k, s->v, s->attn);
+            else CUDA_OK(launch_attention(P, nl, st, pdl));
             return 0;
         });
         GemvLaunch go = gemv_base(m, L.o, s->attn, nl);
@@ -990,6 +1061,8 @@ void check_status(spm_session* s) {
         *s->h_status = 0;
         cudaMemsetAsync(s->status, 0, sizeof(int32_t), s->stream);
         cudaStreamSynchronize(s->stream);
+        if (code >= SPM_PAGE_LENGTH && code < SPM_PAGE_WAIT)
+            fail(SPM_E_CUDA, "the paged cache's tables are not consistent (code " + std::to_string(code) + ")");
         fail(SPM_E_TIMEOUT, "a device wait gave up (code " + std::to_string(code) + ")");
     }
 }
@@ -1032,6 +1105,12 @@ void step(spm_session* s, int n) {
     if (n % s->m->world) fail(SPM_E_ARG, "expert parallel: the client count must be a multiple of the ranks");
     for (int i = 0; i < n; i++)
         if (s->lens[i] >= s->context) fail(SPM_E_CONTEXT, "context " + std::to_string(s->context) + " exhausted");
+    int take = 0;  // pages
+    if (s->paged()) {
+        for (int i = 0; i < n; i++) take += s->pg.need(s->lens[i] + 1) - s->pg.need(s->lens[i]);
+        if (take > s->pg.free)
+            fail(SPM_E_CONTEXT, "the step needs " + std::to_string(take) + " pages, " + std::to_string(s->pg.free) + " are free");
+    }
     if (s->graphs && !s->prof) {
         auto it = s->exec.find(n);
         if (it == s->exec.end()) {
@@ -1066,6 +1145,7 @@ void step(spm_session* s, int n) {
         if (s->prof) collect_profile(s);
     }
     for (int i = 0; i < n; i++) s->lens[i]++;
+    s->pg.free -= take;
 }
 
 // ---- prompts on the tensor cores ----
@@ -1138,6 +1218,19 @@ void prefill_chunk(spm_session* s, int client, const uint32_t* tokens, int T, in
     const int d = int(c.hidden);
     std::vector<int32_t> qpos(T);
     for (int t = 0; t < T; t++) qpos[t] = pos0 + t;
+    if (s->paged()) {
+        const int32_t at[2] = {pos0, T};
+        CUDA_OK(cudaMemcpyAsync(s->pos + client, at, sizeof(int32_t), cudaMemcpyHostToDevice, st));
+        CUDA_OK(cudaMemcpyAsync(s->pg.fresh, at + 1, sizeof(int32_t), cudaMemcpyHostToDevice, st));
+        paged_plan(s, client, 1, s->pg.fresh, nullptr, T);
+        const spm_kv8 cache = paged_layer(s, 0);
+        uint64_t need = 0;
+        inner(spm_kv8_attention_workspace(&cache, int32_t(c.heads), 1, T, s->pg.width, &need));
+        if (need > s->pg.work_bytes) {  // (steps keep the first one: their graphs hold it)
+            s->pg.work = s->alloc<uint8_t>(need);
+            s->pg.work_bytes = need;
+        }
+    }
     CUDA_OK(cudaMemcpyAsync(P.tokens, tokens, size_t(T) * sizeof(uint32_t), cudaMemcpyHostToDevice, st));
     CUDA_OK(cudaMemcpyAsync(P.qpos, qpos.data(), size_t(T) * sizeof(int32_t), cudaMemcpyHostToDevice, st));
     const StreamDesc& E = m->streams[m->embed];
@@ -1150,22 +1243,26 @@ void prefill_chunk(spm_session* s, int client, const uint32_t* tokens, int T, in
         gemm_rows(s, L.q, P.xn, nullptr, T, P.q, EPI_STORE);
         gemm_rows(s, L.k, P.xn, nullptr, T, P.k, EPI_STORE);
         gemm_rows(s, L.v, P.xn, nullptr, T, P.v, EPI_STORE);
-        QkArgs q{};
-        q.q = P.q; q.k = P.k; q.v = P.v; q.kcache = s->kc; q.vcache = s->vc; q.rope = s->rope;
-        q.kplanes = s->kp; q.vplanes = s->vp;
-        q.q_norm = L.q_norm >= 0 ? m->gains + L.q_norm : nullptr;
-        q.k_norm = L.k_norm >= 0 ? m->gains + L.k_norm : nullptr;
-        q.client = client; q.layer = int(l); q.layers = int(c.layers); q.context = s->context; q.pos0 = pos0;
-        q.heads = int(c.heads); q.kv_heads = int(c.kv_heads); q.head_dim = int(c.head_dim); q.family = int(c.family);
-        q.eps = c.eps;
-        CUDA_OK(launch_qk_rope_append(q, T, st));
-        AttnParams A{};
-        A.q = P.q; A.out = P.attn; A.kcache = s->kc; A.vcache = s->vc; A.rope = s->rope;
-        A.layer = int(l); A.layers = int(c.layers); A.context = s->context;
-        A.heads = int(c.heads); A.kv_heads = int(c.kv_heads); A.head_dim = int(c.head_dim);
-        A.family = int(c.family); A.eps = c.eps; A.status = s->status;
-        A.qpos = P.qpos; A.cache_client = client;
-        CUDA_OK(launch_attention_queries(A, T, st));
+        if (s->paged()) {
+            paged_attention(s, int(l), L, client, 1, T, T, P.q, P.k, P.v, P.attn);
+        } else {
+            QkArgs q{};
+            q.q = P.q; q.k = P.k; q.v = P.v; q.kcache = s->kc; q.vcache = s->vc; q.rope = s->rope;
+            q.kplanes = s->kp; q.vplanes = s->vp;
+            q.q_norm = L.q_norm >= 0 ? m->gains + L.q_norm : nullptr;
+            q.k_norm = L.k_norm >= 0 ? m->gains + L.k_norm : nullptr;
+            q.client = client; q.layer = int(l); q.layers = int(c.layers); q.context = s->context; q.pos0 = pos0;
+            q.heads = int(c.heads); q.kv_heads = int(c.kv_heads); q.head_dim = int(c.head_dim); q.family = int(c.family);
+            q.eps = c.eps;
+            CUDA_OK(launch_qk_rope_append(q, T, st));
+            AttnParams A{};
+            A.q = P.q; A.out = P.attn; A.kcache = s->kc; A.vcache = s->vc; A.rope = s->rope;
+            A.layer = int(l); A.layers = int(c.layers); A.context = s->context;
+            A.heads = int(c.heads); A.kv_heads = int(c.kv_heads); A.head_dim = int(c.head_dim);
+            A.family = int(c.family); A.eps = c.eps; A.status = s->status;
+            A.qpos = P.qpos; A.cache_client = client;
+            CUDA_OK(launch_attention_queries(A, T, st));
+        }
         gemm_rows(s, L.o, P.attn, nullptr, T, P.x, EPI_ADD);
         CUDA_OK(launch_norm_rows(P.x, m->gains + L.ffn_norm, c.eps, d, T, P.xn, st));
         if (!is_moe(c)) {
@@ -1531,98 +1628,177 @@ spm_status spm_weights_dequant(const spm_weights* w, uint64_t row0, uint64_t row
     });
 }
 
-spm_status spm_session_create(spm_model* m, int32_t max_clients, int32_t max_context, spm_session** out) {
-    return guarded([&] {
-        if (max_clients < 1 || max_context < 1) fail(SPM_E_ARG, "clients and context must be positive");
-        CUDA_OK(cudaSetDevice(m->device));
-        std::unique_ptr<spm_session> s(new spm_session());
-        s->m = m;
-        s->max_clients = max_clients;
-        s->context = max_context;
-        const spm_model_cfg& c = m->cfg;
-        const size_t n = size_t(max_clients), d = c.hidden, qw = size_t(c.heads) * c.head_dim;
-        const size_t kvw = size_t(c.kv_heads) * c.head_dim;
-        const size_t ff = std::max<size_t>(c.intermediate, c.expert_ff);
-        CUDA_OK(cudaStreamCreateWithFlags(&s->stream, cudaStreamNonBlocking));
+}  // extern "C"
+
+namespace {
+
+// `page` tokens to each of `pages` pages: a paged session; 0: fp32 rows by client.
+void create_session(spm_model* m, int32_t max_clients, int32_t max_context, int32_t page, int32_t pages, spm_session** out) {
+    if (max_clients < 1 || max_context < 1) fail(SPM_E_ARG, "clients and context must be positive");
+    CUDA_OK(cudaSetDevice(m->device));
+    std::unique_ptr<spm_session> s(new spm_session());
+    s->m = m;
+    s->max_clients = max_clients;
+    s->context = max_context;
+    const spm_model_cfg& c = m->cfg;
+    const size_t n = size_t(max_clients), d = c.hidden, qw = size_t(c.heads) * c.head_dim;
+    const size_t kvw = size_t(c.kv_heads) * c.head_dim;
+    const size_t ff = std::max<size_t>(c.intermediate, c.expert_ff);
+    CUDA_OK(cudaStreamCreateWithFlags(&s->stream, cudaStreamNonBlocking));
+    if (page) {
+        if (m->world > 1) fail(SPM_E_ARG, "paged sessions run on single-GPU models");
+        auto& g = s->pg;
+        g.page = page;
+        g.pages = g.free = pages;
+        const spm_kv8 shape = paged_layer(s.get(), 0);
+        uint64_t bytes = 0;
+        // (checks head_dim, page_tokens and the counts as every spm_kv8 call does; the memory comes below)
+        spm_kv8 probe = shape;
+        probe.k_codes = probe.v_codes = reinterpret_cast<int8_t*>(16);
+        probe.k_scales = probe.v_scales = reinterpret_cast<float*>(16);
+        g.width = (max_context - 1) / std::max(page, 1) + 1;
+        inner(spm_kv8_attention_workspace(&probe, int32_t(c.heads), 1, 1, g.width, &bytes));
+        if (pages < 1) fail(SPM_E_ARG, "a paged session needs pages");
+        const size_t scales = size_t(c.layers) * pages * c.kv_heads, codes = scales * page * c.head_dim;
+        g.k_codes = s->alloc<int8_t>(codes);
+        g.v_codes = s->alloc<int8_t>(codes);
+        g.k_scales = s->alloc<float>(scales);
+        g.v_scales = s->alloc<float>(scales);
+        g.table = s->alloc<int32_t>(n * g.width);
+        g.stack = s->alloc<int32_t>(pages);
+        g.count = s->alloc<int32_t>(1);
+        g.ones = s->alloc<int32_t>(n);
+        g.fresh = s->alloc<int32_t>(1);
+        g.ended = s->alloc<int32_t>(1);
+        const size_t rows = std::max<size_t>(n, kPrefillRows);
+        g.starts = s->alloc<int32_t>(n + 1);
+        g.lens = s->alloc<int32_t>(n);
+        g.positions = s->alloc<int32_t>(rows);
+        g.slots = s->alloc<int32_t>(rows);
+        for (int b = 1; b <= std::min<int>(max_clients, kMaxBatch); b++) {
+            inner(spm_kv8_attention_workspace(&probe, int32_t(c.heads), b, 1, g.width, &bytes));
+            g.work_bytes = std::max(g.work_bytes, bytes);
+        }
+        g.work = s->alloc<uint8_t>(g.work_bytes);
+        std::vector<int32_t> ids(std::max<size_t>(pages, n), 1);
+        CUDA_OK(cudaMemcpy(g.ones, ids.data(), n * sizeof(int32_t), cudaMemcpyHostToDevice));
+        for (int p = 0; p < pages; p++) ids[p] = pages - 1 - p;
+        CUDA_OK(cudaMemcpy(g.stack, ids.data(), size_t(pages) * sizeof(int32_t), cudaMemcpyHostToDevice));
+        CUDA_OK(cudaMemcpy(g.count, &pages, sizeof(int32_t), cudaMemcpyHostToDevice));
+    } else {
         s->kc = s->alloc<float>(n * c.layers * size_t(max_context) * kvw);
         s->vc = s->alloc<float>(n * c.layers * size_t(max_context) * kvw);
-        {
-            const uint32_t grp = c.heads / c.kv_heads;
-            if (grp >= 4 && grp <= 8 && (c.head_dim == 64 || c.head_dim == 128)) {
-                s->kp = s->alloc<uint16_t>(3 * n * c.layers * size_t(max_context) * kvw);
-                s->vp = s->alloc<uint16_t>(3 * n * c.layers * size_t(max_context) * kvw);
-            }
+    }
+    if (!page) {
+        const uint32_t grp = c.heads / c.kv_heads;
+        if (grp >= 4 && grp <= 8 && (c.head_dim == 64 || c.head_dim == 128)) {
+            s->kp = s->alloc<uint16_t>(3 * n * c.layers * size_t(max_context) * kvw);
+            s->vp = s->alloc<uint16_t>(3 * n * c.layers * size_t(max_context) * kvw);
         }
-        s->normed = s->alloc<float>(n * d);
-        s->q = s->alloc<float>(n * qw);
-        s->k = s->alloc<float>(n * kvw);
-        s->v = s->alloc<float>(n * kvw);
-        s->attn = s->alloc<float>(n * qw);
-        s->act = s->alloc<float>(n * ff);
-        s->logits = s->alloc<float>(n * c.vocab);
-        s->pos = s->alloc<int32_t>(n);
-        s->tokens = s->alloc<uint32_t>(n);
-        s->status = s->alloc<int32_t>(1);
-        const size_t chunks = (size_t(max_context) + kAttnMinChunk - 1) / kAttnMinChunk;
-        const size_t group = c.heads / c.kv_heads;
-        // the attention kernel splits a score over 8 / group warps, four values at a time
-        if (group > 8 || group * c.head_dim > 1024 || c.head_dim > 256 || c.head_dim % (4 * (8 / group)))
-            fail(SPM_E_ARG, "attention supports at most 8 query heads and 1024 query values per kv head, "
-                            "head_dim up to 256 and a multiple of 4 * (8 / group)");
-        s->attn_scratch = s->alloc<float>(n * c.kv_heads * chunks * group * (c.head_dim + 2));
-        s->attn_counters = s->alloc<int32_t>(n * c.kv_heads);
-        if (is_moe(c)) {
-            if (c.experts > uint32_t(kMoeMaxExperts) || c.experts_used > uint32_t(kMoeMaxUsed))
-                fail(SPM_E_ARG, "at most 256 experts and 8 routed per token");
-            if (c.expert_ff % kTileRows || c.hidden % kTileRows) fail(SPM_E_ARG, "expert rows must be whole tiles");
-            s->moe_max_active = int(std::min<size_t>(c.experts, std::min<size_t>(n, kMoeMaxClients) * c.experts_used));
-            s->moe_logits = s->alloc<float>(n * c.experts);
-            s->route_counter = s->alloc<uint32_t>(1);
-            s->plans = s->alloc<MoePlan>(c.layers);
-            s->moe_act = s->alloc<float>(size_t(s->moe_max_active) * kMoeMaxClients * c.expert_ff);
-            s->moe_out = s->alloc<float>(size_t(s->moe_max_active) * kMoeMaxClients * c.hidden);
-            if (m->world > 1) {
-                s->ep_xbytes = (size_t(s->moe_max_active) * kMoeMaxClients * c.hidden * sizeof(float) + 255) & ~size_t(255);
-                // after the exchange: flags [2][64] + [64], greedy picks,
-                // states, sums of squares (every rank writes into them)
-                s->dp_off = 512 + 2 * s->ep_xbytes;
-                const size_t pick_off = 1024, states_off = pick_off + ((n * sizeof(uint32_t) + 255) & ~size_t(255));
-                s->dp_states_bytes = (n * d * sizeof(float) + 255) & ~size_t(255);
-                const size_t sumsq_off = states_off + s->dp_states_bytes;
-                const size_t dp_bytes = sumsq_off + 2 * size_t(kMaxParts) * 8 * sizeof(float);
-                s->ep_region = s->alloc<uint8_t>(s->dp_off + dp_bytes);
-                uint8_t* dp = s->ep_region + s->dp_off;
-                s->dp_flags = reinterpret_cast<uint32_t*>(dp);
-                s->argmax = reinterpret_cast<uint32_t*>(dp + pick_off);
-                s->states = reinterpret_cast<float*>(dp + states_off);
-                s->sumsq = reinterpret_cast<float*>(dp + sumsq_off);
-                s->ep_done = s->alloc<uint32_t>(1);
-                s->ep_done2 = s->alloc<uint32_t>(1);
-                s->ep_peer_y = s->alloc<float*>(2 * size_t(m->world));
-                s->ep_peer_flag = s->alloc<uint32_t*>(2 * size_t(m->world));
-                s->dp_peer_states = s->alloc<float*>(m->world);
-                s->dp_peer_sumsq = s->alloc<float*>(m->world);
-                s->dp_peer_flag = s->alloc<uint32_t*>(2 * size_t(m->world));
-                s->dp_peer_argmax = s->alloc<uint32_t*>(m->world);
-                s->dp_peer_gflag = s->alloc<uint32_t*>(m->world);
-            }
+    }
+    s->normed = s->alloc<float>(n * d);
+    s->q = s->alloc<float>(n * qw);
+    s->k = s->alloc<float>(n * kvw);
+    s->v = s->alloc<float>(n * kvw);
+    s->attn = s->alloc<float>(n * qw);
+    s->act = s->alloc<float>(n * ff);
+    s->logits = s->alloc<float>(n * c.vocab);
+    s->pos = s->alloc<int32_t>(n);
+    s->tokens = s->alloc<uint32_t>(n);
+    s->status = s->alloc<int32_t>(1);
+    const size_t chunks = (size_t(max_context) + kAttnMinChunk - 1) / kAttnMinChunk;
+    const size_t group = c.heads / c.kv_heads;
+    // the attention kernel splits a score over 8 / group warps, four values at a time
+    if (group > 8 || group * c.head_dim > 1024 || c.head_dim > 256 || c.head_dim % (4 * (8 / group)))
+        fail(SPM_E_ARG, "attention supports at most 8 query heads and 1024 query values per kv head, "
+                        "head_dim up to 256 and a multiple of 4 * (8 / group)");
+    s->attn_scratch = s->alloc<float>(n * c.kv_heads * chunks * group * (c.head_dim + 2));
+    s->attn_counters = s->alloc<int32_t>(n * c.kv_heads);
+    if (is_moe(c)) {
+        if (c.experts > uint32_t(kMoeMaxExperts) || c.experts_used > uint32_t(kMoeMaxUsed))
+            fail(SPM_E_ARG, "at most 256 experts and 8 routed per token");
+        if (c.expert_ff % kTileRows || c.hidden % kTileRows) fail(SPM_E_ARG, "expert rows must be whole tiles");
+        s->moe_max_active = int(std::min<size_t>(c.experts, std::min<size_t>(n, kMoeMaxClients) * c.experts_used));
+        s->moe_logits = s->alloc<float>(n * c.experts);
+        s->route_counter = s->alloc<uint32_t>(1);
+        s->plans = s->alloc<MoePlan>(c.layers);
+        s->moe_act = s->alloc<float>(size_t(s->moe_max_active) * kMoeMaxClients * c.expert_ff);
+        s->moe_out = s->alloc<float>(size_t(s->moe_max_active) * kMoeMaxClients * c.hidden);
+        if (m->world > 1) {
+            s->ep_xbytes = (size_t(s->moe_max_active) * kMoeMaxClients * c.hidden * sizeof(float) + 255) & ~size_t(255);
+            // after the exchange: flags [2][64] + [64], greedy picks,
+            // states, sums of squares (every rank writes into them)
+            s->dp_off = 512 + 2 * s->ep_xbytes;
+            const size_t pick_off = 1024, states_off = pick_off + ((n * sizeof(uint32_t) + 255) & ~size_t(255));
+            s->dp_states_bytes = (n * d * sizeof(float) + 255) & ~size_t(255);
+            const size_t sumsq_off = states_off + s->dp_states_bytes;
+            const size_t dp_bytes = sumsq_off + 2 * size_t(kMaxParts) * 8 * sizeof(float);
+            s->ep_region = s->alloc<uint8_t>(s->dp_off + dp_bytes);
+            uint8_t* dp = s->ep_region + s->dp_off;
+            s->dp_flags = reinterpret_cast<uint32_t*>(dp);
+            s->argmax = reinterpret_cast<uint32_t*>(dp + pick_off);
+            s->states = reinterpret_cast<float*>(dp + states_off);
+            s->sumsq = reinterpret_cast<float*>(dp + sumsq_off);
+            s->ep_done = s->alloc<uint32_t>(1);
+            s->ep_done2 = s->alloc<uint32_t>(1);
+            s->ep_peer_y = s->alloc<float*>(2 * size_t(m->world));
+            s->ep_peer_flag = s->alloc<uint32_t*>(2 * size_t(m->world));
+            s->dp_peer_states = s->alloc<float*>(m->world);
+            s->dp_peer_sumsq = s->alloc<float*>(m->world);
+            s->dp_peer_flag = s->alloc<uint32_t*>(2 * size_t(m->world));
+            s->dp_peer_argmax = s->alloc<uint32_t*>(m->world);
+            s->dp_peer_gflag = s->alloc<uint32_t*>(m->world);
         }
-        if (!s->states) {
-            s->states = s->alloc<float>(n * d);
-            s->argmax = s->alloc<uint32_t>(n);
-            s->sumsq = s->alloc<float>(2 * size_t(kMaxParts) * 8);
-        }
-        s->step = s->alloc<uint32_t>(1);
-        auto table = rope_table(c, max_context);
-        s->rope = s->alloc<float2>(table.size());
-        CUDA_OK(cudaMemcpy(s->rope, table.data(), table.size() * sizeof(float2), cudaMemcpyHostToDevice));
-        CUDA_OK(cudaMallocHost(&s->h_tokens, n * sizeof(uint32_t)));
-        CUDA_OK(cudaMallocHost(&s->h_argmax, n * sizeof(uint32_t)));
-        CUDA_OK(cudaMallocHost(&s->h_status, sizeof(int32_t)));
-        s->lens.assign(n, 0);
-        *out = s.release();
+    }
+    if (!s->states) {
+        s->states = s->alloc<float>(n * d);
+        s->argmax = s->alloc<uint32_t>(n);
+        s->sumsq = s->alloc<float>(2 * size_t(kMaxParts) * 8);
+    }
+    s->step = s->alloc<uint32_t>(1);
+    auto table = rope_table(c, max_context);
+    s->rope = s->alloc<float2>(table.size());
+    CUDA_OK(cudaMemcpy(s->rope, table.data(), table.size() * sizeof(float2), cudaMemcpyHostToDevice));
+    CUDA_OK(cudaMallocHost(&s->h_tokens, n * sizeof(uint32_t)));
+    CUDA_OK(cudaMallocHost(&s->h_argmax, n * sizeof(uint32_t)));
+    CUDA_OK(cudaMallocHost(&s->h_status, sizeof(int32_t)));
+    CUDA_OK(cudaMallocHost(&s->h_samp, 6 * n * sizeof(int32_t)));
+    int32_t* samp = s->alloc<int32_t>(6 * n);
+    s->samp_temperature = reinterpret_cast<float*>(samp);
+    s->samp_k = samp + n;
+    s->samp_p = reinterpret_cast<float*>(samp + 2 * n);
+    s->samp_min = reinterpret_cast<float*>(samp + 3 * n);
+    s->samp_u = reinterpret_cast<float*>(samp + 4 * n);
+    s->samp_token = samp + 5 * n;
+    s->lens.assign(n, 0);
+    *out = s.release();
+}
+
+}  // namespace
+
+extern "C" {
+
+spm_status spm_session_create(spm_model* m, int32_t max_clients, int32_t max_context, spm_session** out) {
+    return guarded([&] { create_session(m, max_clients, max_context, 0, 0, out); });
+}
+
+spm_status spm_session_create_paged(spm_model* m, int32_t max_clients, int32_t max_context, int32_t page_tokens,
+                                    int32_t pages, spm_session** out) {
+    return guarded([&] {
+        if (!m || !out) fail(SPM_E_ARG, "null argument");
+        if (page_tokens < 1) fail(SPM_E_ARG, "page_tokens is 16, 32, 64, 128 or 256");
+        create_session(m, max_clients, max_context, page_tokens, pages, out);
     });
 }
+
+spm_status spm_session_free_pages(const spm_session* s, int32_t* pages) {
+    return guarded([&] {
+        if (!s || !pages) fail(SPM_E_ARG, "null argument");
+        if (!s->paged()) fail(SPM_E_ARG, "the session is not paged");
+        *pages = s->pg.free;
+    });
+}
+
 
 spm_status spm_session_destroy(spm_session* s) {
     return guarded([&] {
@@ -1636,6 +1812,14 @@ spm_status spm_client_reset(spm_session* s, int32_t client) {
         if (client < 0 || client >= s->max_clients) fail(SPM_E_ARG, "client index out of range");
         CUDA_OK(cudaSetDevice(s->m->device));
         CUDA_OK(cudaMemsetAsync(s->pos + client, 0, sizeof(int32_t), s->stream));
+        if (s->paged() && s->lens[client]) {
+            // the client's pages go back to the stack
+            const int32_t len = s->lens[client];
+            CUDA_OK(cudaMemcpyAsync(s->pg.ended, &len, sizeof(int32_t), cudaMemcpyHostToDevice, s->stream));
+            CUDA_OK(cudaMemsetAsync(s->pg.fresh, 0, sizeof(int32_t), s->stream));
+            paged_plan(s, client, 1, s->pg.fresh, s->pg.ended, 0);
+            s->pg.free += s->pg.need(len);
+        }
         CUDA_OK(cudaStreamSynchronize(s->stream));
         s->lens[client] = 0;
     });
@@ -1686,6 +1870,49 @@ spm_status spm_decode_step_device(spm_session* s, const uint32_t* tokens_dev, in
     });
 }
 
+spm_status spm_decode_step_sampled(spm_session* s, const uint32_t* tokens, int32_t n, const spm_sampling* how,
+                                   const float* u, float* logits_host, uint32_t* argmax_host, uint32_t* next_host) {
+    return guarded([&] {
+        if (!s || !tokens || !how || !u || !next_host) fail(SPM_E_ARG, "null argument");
+        if (s->m->world > 1) fail(SPM_E_ARG, "sampled steps run on single-GPU models");
+        if (n < 1 || n > s->max_clients) fail(SPM_E_ARG, "client count out of range");
+        const spm_model_cfg& c = s->m->cfg;
+        for (int i = 0; i < n; i++) {
+            if (tokens[i] >= c.vocab) fail(SPM_E_ARG, "token id out of range");
+            if (!(how[i].temperature >= 0.f)) fail(SPM_E_ARG, "a temperature is 0 or more");
+            if (!(u[i] >= 0.f && u[i] < 1.f)) fail(SPM_E_ARG, "a uniform number lies in [0, 1)");
+        }
+        CUDA_OK(cudaSetDevice(s->m->device));
+        const size_t m = size_t(s->max_clients);
+        float* f = reinterpret_cast<float*>(s->h_samp);
+        for (int i = 0; i < n; i++) {
+            f[i] = how[i].temperature;
+            s->h_samp[m + i] = how[i].top_k;
+            f[2 * m + i] = how[i].top_p;
+            f[3 * m + i] = how[i].min_p;
+            f[4 * m + i] = u[i];
+        }
+        std::memcpy(s->h_tokens, tokens, size_t(n) * sizeof(uint32_t));
+        CUDA_OK(cudaMemcpyAsync(s->tokens, s->h_tokens, size_t(n) * sizeof(uint32_t), cudaMemcpyHostToDevice, s->stream));
+        CUDA_OK(cudaMemcpyAsync(s->samp_temperature, s->h_samp, 5 * m * sizeof(int32_t), cudaMemcpyHostToDevice, s->stream));
+        step(s, n);
+        inner(spm_sample(s->m->device, SPM_F32, s->logits, c.vocab, n, int32_t(c.vocab), s->samp_temperature, s->samp_k,
+                         s->samp_p, s->samp_min, s->samp_u, s->samp_token, nullptr, nullptr, s->stream));
+        CUDA_OK(cudaMemcpyAsync(s->h_samp + 5 * m, s->samp_token, size_t(n) * sizeof(int32_t), cudaMemcpyDeviceToHost, s->stream));
+        CUDA_OK(cudaMemcpyAsync(s->h_argmax, s->argmax, size_t(n) * sizeof(uint32_t), cudaMemcpyDeviceToHost, s->stream));
+        if (logits_host)
+            CUDA_OK(cudaMemcpyAsync(logits_host, s->logits, size_t(n) * c.vocab * sizeof(float), cudaMemcpyDeviceToHost, s->stream));
+        CUDA_OK(cudaMemcpyAsync(s->h_status, s->status, sizeof(int32_t), cudaMemcpyDeviceToHost, s->stream));
+        CUDA_OK(cudaStreamSynchronize(s->stream));
+        check_status(s);
+        if (argmax_host) std::memcpy(argmax_host, s->h_argmax, size_t(n) * sizeof(uint32_t));
+        for (int i = 0; i < n; i++) {
+            if (s->h_samp[5 * m + i] < 0) fail(SPM_E_ARG, "client " + std::to_string(i) + " has no finite logit");
+            next_host[i] = uint32_t(s->h_samp[5 * m + i]);
+        }
+    });
+}
+
 spm_status spm_prefill(spm_session* s, int32_t client, const uint32_t* tokens, int32_t len) {
     return guarded([&] {
         spm_model* m = s->m;
@@ -1696,6 +1923,13 @@ spm_status spm_prefill(spm_session* s, int32_t client, const uint32_t* tokens, i
             if (tokens[t] >= m->cfg.vocab) fail(SPM_E_ARG, "token id out of range");
         if (int64_t(s->lens[client]) + len > s->context)
             fail(SPM_E_CONTEXT, "context " + std::to_string(s->context) + " exhausted");
+        int take = 0;
+        if (s->paged()) {
+            take = s->pg.need(s->lens[client] + len) - s->pg.need(s->lens[client]);
+            if (take > s->pg.free)
+                fail(SPM_E_CONTEXT, "the prompt needs " + std::to_string(take) + " pages, " + std::to_string(s->pg.free) +
+                                        " are free");
+        }
         if (m->streams[m->embed].pk.cols % 64) fail(SPM_E_ARG, "prefill needs hidden a multiple of 64");
         CUDA_OK(cudaSetDevice(m->device));
         prefill_buffers(s);
@@ -1704,6 +1938,7 @@ spm_status spm_prefill(spm_session* s, int32_t client, const uint32_t* tokens, i
             prefill_chunk(s, client, tokens + t0, T, s->lens[client]);
             s->lens[client] += T;
         }
+        s->pg.free -= take;
         const int32_t pos = s->lens[client];
         CUDA_OK(cudaMemcpyAsync(s->pos + client, &pos, sizeof(int32_t), cudaMemcpyHostToDevice, s->stream));
         CUDA_OK(cudaMemcpyAsync(s->h_status, s->status, sizeof(int32_t), cudaMemcpyDeviceToHost, s->stream));

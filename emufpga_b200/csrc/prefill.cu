@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(256) qk_rope_append_kernel(const QkArgs a) {
         }
         __syncthreads();
     }
-    const int pos = a.pos0 + t, half = hd / 2;
+    const int pos = a.pos ? a.pos[t] : a.pos0 + t, half = hd / 2;
     const float2* rt = a.rope + size_t(pos) * half;
     for (int e = threadIdx.x; e < (a.heads + a.kv_heads) * half; e += blockDim.x) {
         const int h = e / half, j = e % half;
@@ -130,6 +130,10 @@ __global__ void __launch_bounds__(256) qk_rope_append_kernel(const QkArgs a) {
     __syncthreads();
     float* qo = a.q + size_t(t) * qw;
     for (int c = threadIdx.x; c < qw; c += blockDim.x) qo[c] = q[c];
+    if (!a.kcache) {
+        for (int c = threadIdx.x; c < kvw; c += blockDim.x) a.k_out[size_t(t) * kvw + c] = k[c];
+        return;
+    }
     const size_t row = ((size_t(a.client) * a.layers + a.layer) * a.context + pos) * kvw;
     for (int c = threadIdx.x; c < kvw; c += blockDim.x) {
         const float vv = a.v[size_t(t) * kvw + c];

@@ -18,7 +18,11 @@ cudaError_t launch_norm_rows(const float* x, const float* gain, float eps, int w
 struct QkArgs {
     float* q;                      // [T][heads * head_dim], normed and rotated in place
     const float *k, *v;            // [T][kv_heads * head_dim]
-    float *kcache, *vcache;        // [client][layer][context][kv_width]
+    float *kcache, *vcache;        // [client][layer][context][kv_width], or nullptr: no append
+    // Without a cache (a paged session's): row t stands at pos[t], and its key goes to
+    // k_out (which may be k).
+    const int32_t* pos;
+    float* k_out;
     uint16_t *kplanes, *vplanes;   // the rows as three bf16 parts (AttnParams), or nullptr
     const float2* rope;            // [context][head_dim / 2]
     const float *q_norm, *k_norm;  // QK-norm gains or nullptr (LLAMA)
@@ -26,7 +30,7 @@ struct QkArgs {
     int32_t heads, kv_heads, head_dim, family;
     float eps;
 };
-// Row t at position pos0 + t: QK-norm, RoPE, and the KV cache append.
+// Row t at position pos0 + t (or pos[t]): QK-norm, RoPE, and the KV cache append (or k_out).
 cudaError_t launch_qk_rope_append(const QkArgs& a, int T, cudaStream_t stream);
 
 // Routing of T rows: sel/prob [T][K] in route order, norm [T] (sum of the

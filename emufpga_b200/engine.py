@@ -264,10 +264,17 @@ class Weights:
 class Session:
     """N clients sharing one weight sweep per step (spm-batch Client + Scratch)."""
 
-    def __init__(self, model: Model, max_clients: int, context: int, graphs: bool = True):
+    def __init__(self, model: Model, max_clients: int, context: int, graphs: bool = True,
+                 paged: tuple[int, int] | None = None):
+        """`paged=(pages, page_tokens)`: keys and values in that many pages of
+        the 8-bit cache, shared by the clients (spm_session_create_paged)."""
         h = C.c_void_p()
-        call("spm_session_create", model._h, max_clients, context, C.byref(h))
+        if paged is None:
+            call("spm_session_create", model._h, max_clients, context, C.byref(h))
+        else:
+            call("spm_session_create_paged", model._h, max_clients, context, paged[1], paged[0], C.byref(h))
         self._h, self.model, self.max_clients, self.context = h, model, max_clients, context
+        self.page_tokens = None if paged is None else paged[1]
         if not graphs:
             call("spm_session_set_graphs", h, 0)
 
@@ -300,6 +307,31 @@ class Session:
         call("spm_decode_step", self._h, tok, n,
              logits.ctypes.data_as(C.POINTER(C.c_float)) if want_logits else None, arg)
         return list(arg), logits
+
+    def decode_step_sampled(self, tokens: Sequence[int], how: Sequence, u: Sequence[float], want_logits: bool = False):
+        """decode_step with a drawn token per client too: `how` holds each
+        client's Sampling (None: greedy), `u` its uniform number in [0, 1).
+        Returns (next ids, argmax ids, logits or None); a greedy client's next
+        id is its argmax."""
+        n = len(tokens)
+        if len(how) != n or len(u) != n:
+            raise SpmError(-1, "one Sampling and one number per client")
+        tok = (C.c_uint32 * n)(*tokens)
+        arg, nxt = (C.c_uint32 * n)(), (C.c_uint32 * n)()
+        spec = (_lib.SamplingSpec * n)(*((0.0, 0, 1.0, 0.0) if w is None else (w.temperature, w.top_k, w.top_p, w.min_p)
+                                         for w in how))
+        vocab = self.model.shape.vocab if self.model.shape else None
+        logits = np.empty((n, vocab), dtype=np.float32) if want_logits else None
+        call("spm_decode_step_sampled", self._h, tok, n, spec, (C.c_float * n)(*u),
+             logits.ctypes.data_as(C.POINTER(C.c_float)) if want_logits else None, arg, nxt)
+        return [a if w is None else t for a, t, w in zip(arg, nxt, how)], list(arg), logits
+
+    @property
+    def free_pages(self) -> int:
+        """Free pages of a paged session."""
+        v = C.c_int32()
+        call("spm_session_free_pages", self._h, C.byref(v))
+        return v.value
 
     def set_wait_limit(self, nanoseconds: int) -> None:
         """How long device waits on other ranks spin before the step reports SPM_E_TIMEOUT."""
@@ -379,24 +411,36 @@ class Session:
 
 
 def serve(model: Model, prompts: Sequence[Sequence[int]], steps: int, max_ticks: int | None = None,
-          want_logits: bool = False):
+          want_logits: bool = False, sampling=None, paged: tuple[int, int] | None = None):
     """The lockstep loop of spm-batch/examples/serve-demo.rs:45-91.
 
     Every tick runs one decode step for all clients; a client feeds its next
     prompt token until its prompt is exhausted, then feeds back its greedy
-    pick.  Returns (produced tokens per client, logits of the last tick)."""
+    pick.  Returns (produced tokens per client, logits of the last tick).
+
+    `sampling` (a sampling.Sampling for each client, None for a greedy one)
+    draws the tokens fed back instead, client i's from its own seed's numbers,
+    one for each token it produces.  `paged`: as for Session."""
     longest = max(len(p) for p in prompts)
     context = longest + steps + 1
     total = longest + steps - 1
     if max_ticks is not None:
         total = min(total, max_ticks)
-    sess = Session(model, len(prompts), context)
+    if sampling is not None and len(sampling) != len(prompts):
+        raise ValueError("one Sampling (or None) per prompt")
+    sess = Session(model, len(prompts), context, paged=paged)
     try:
         tokens = [p[0] for p in prompts]
         produced: list[list[int]] = [[] for _ in prompts]
         logits = None
+        numbers = [None if w is None else w.numbers() for w in sampling or ()]
         for tick in range(total):
-            best, logits = sess.decode_step(tokens, want_logits=want_logits)
+            if sampling is None:
+                best, logits = sess.decode_step(tokens, want_logits=want_logits)
+            else:
+                u = [float(g.random(dtype=np.float32)) if g is not None and tick + 1 >= len(p) else 0.0
+                     for g, p in zip(numbers, prompts)]
+                best, _, logits = sess.decode_step_sampled(tokens, sampling, u, want_logits=want_logits)
             for i, p in enumerate(prompts):
                 if tick + 1 < len(p):
                     tokens[i] = p[tick + 1]

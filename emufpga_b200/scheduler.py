@@ -30,6 +30,7 @@ class Request:
     prompt: Sequence[int]
     max_new: int
     arrival: int = 0  # first step at which the request may start
+    sampling: object = None  # a sampling.Sampling; None: greedy
 
 
 class DecodeSession(Protocol):
@@ -44,6 +45,9 @@ class DecodeSession(Protocol):
 
     def decode_step(self, tokens: Sequence[int], want_logits: bool = False): ...
 
+    # only with a sampled request: (next ids, argmax ids, logits)
+    def decode_step_sampled(self, tokens: Sequence[int], how: Sequence, u: Sequence[float], want_logits: bool = False): ...
+
     # only with prefill=True: run tokens for `client` at its next positions
     def prefill(self, client: int, tokens: Sequence[int]) -> None: ...
 
@@ -54,7 +58,9 @@ def serve_continuous(session: DecodeSession, requests: Sequence[Request], filler
 
     Requests start in arrival order (ties in list order) as slots free up.
     With prefill, a starting request's prompt but its last token is run at
-    once by session.prefill.  Raises ValueError when a request cannot fit the
+    once by session.prefill.  A request with `sampling` feeds back tokens drawn
+    with it, from its own seed's numbers, one for each token it produces, so
+    that its tokens do not depend on what else is served.  Raises ValueError when a request cannot fit the
     session's context."""
     for r in requests:
         if not r.prompt or r.max_new < 1:
@@ -64,6 +70,7 @@ def serve_continuous(session: DecodeSession, requests: Sequence[Request], filler
     waiting = sorted(range(len(requests)), key=lambda i: (requests[i].arrival, i))
     out: list[list[int]] = [[] for _ in requests]
     active: dict[int, list[int]] = {}  # slot -> [request, local step, next token]
+    numbers = [None if r.sampling is None else r.sampling.numbers() for r in requests]
     step = 0
     while waiting or active:
         for s in range(session.max_clients):
@@ -86,7 +93,15 @@ def serve_continuous(session: DecodeSession, requests: Sequence[Request], filler
         for s in range(n):
             if s not in active and session.length(s) + 1 >= session.context:
                 session.reset(s)
-        best, _ = session.decode_step([active[s][2] if s in active else filler for s in range(n)])
+        feed = [active[s][2] if s in active else filler for s in range(n)]
+        how = [requests[active[s][0]].sampling if s in active else None for s in range(n)]
+        if any(w is not None for w in how):
+            # a number for every client that produces a token in this step
+            u = [float(numbers[active[s][0]].random(dtype="float32"))
+                 if how[s] is not None and active[s][1] + 1 >= len(requests[active[s][0]].prompt) else 0.0 for s in range(n)]
+            best, _, _ = session.decode_step_sampled(feed, how, u)
+        else:
+            best, _ = session.decode_step(feed)
         for s in list(active):
             st = active[s]
             r, k = st[0], st[1]

@@ -30,6 +30,8 @@
  *                         .spm files streamed from host memory through a device ring
  *   spm_page_plan, spm_kv8_*  no counterpart: spm-kv/src/cache.rs:49-58 and
  *                         attend.rs:37-94 hold f32 rows of one client
+ *   spm_session_create_paged, spm_decode_step_sampled  no counterpart: the two
+ *                         above under a session
  *   spm_sample            no counterpart: the reference picks greedily
  *                         (spm-batch/examples/serve-demo.rs:74-79)
  */
@@ -183,6 +185,19 @@ spm_status spm_weights_dequant(const spm_weights* w, uint64_t row0, uint64_t row
 /* ---- sessions: N clients, one weight sweep per step ---- */
 spm_status spm_session_create(spm_model* m, int32_t max_clients, int32_t max_context,
                               spm_session** out);
+/* A session whose keys and values lie in the paged 8-bit cache of spm_kv8 (one
+ * byte a value where spm_session_create holds four, or ten with the tensor cores'
+ * planes): `pages` pages of page_tokens tokens for all clients together, each client
+ * taking the pages its length needs, up to max_context tokens; a step or prompt
+ * that finds too few free pages is SPM_E_CONTEXT and changes nothing, and
+ * spm_client_reset gives a client's pages back.  Steps and prompts run
+ * spm_page_plan, spm_kv8_append and spm_kv8_attention; every other call is as for
+ * spm_session_create's sessions, and tokens may differ from theirs by the rounding
+ * of keys and values to 8 bits.  One GPU; head_dim as spm_kv8 takes it. */
+spm_status spm_session_create_paged(spm_model* m, int32_t max_clients, int32_t max_context, int32_t page_tokens,
+                                    int32_t pages, spm_session** out);
+/* Free pages of a paged session. */
+spm_status spm_session_free_pages(const spm_session* s, int32_t* pages);
 spm_status spm_session_destroy(spm_session* s);
 /* Empty client `client`'s KV cache (position 0). */
 spm_status spm_client_reset(spm_session* s, int32_t client);
@@ -197,6 +212,18 @@ spm_status spm_decode_step(spm_session* s, const uint32_t* tokens, int32_t n, fl
 spm_status spm_decode_step_device(spm_session* s, const uint32_t* tokens_dev, int32_t n,
                                   float* logits_dev, uint32_t* argmax_dev);
 spm_status spm_session_sync(spm_session* s);
+/* spm_decode_step with a drawn token for each client as well (spm_sample on the
+ * step's logits): client i's settings how[i] and uniform number u[i] in [0, 1) give
+ * next_host[i].  argmax_host (may be NULL) receives the greedy picks of the same
+ * step.  One GPU. */
+typedef struct spm_sampling {
+    float temperature;   /* 0: the largest logit, the first by index */
+    int32_t top_k;       /* 0: off */
+    float top_p;         /* 1: off */
+    float min_p;         /* 0: off */
+} spm_sampling;
+spm_status spm_decode_step_sampled(spm_session* s, const uint32_t* tokens, int32_t n, const spm_sampling* how,
+                                   const float* u, float* logits_host, uint32_t* argmax_host, uint32_t* next_host);
 /* Run a prompt through the model for `client`: its next `len` positions take
  * tokens[0..len), their keys and values are appended to the client's cache,
  * and the client's length grows by `len`.  The layers' products over all the

@@ -86,3 +86,49 @@ def test_prefill_of_joining_requests_changes_no_token():
     # every prompt longer than one token went through prefill, all but its last token
     assert sorted(n for _, n in fast.prefills) == sorted(len(r.prompt) - 1 for r in reqs if len(r.prompt) > 1)
     assert len(fast.steps) < len(plain.steps)
+
+
+class SampledSession:
+    """A fake whose sampled step returns a token made of what it was given."""
+
+    max_clients, context = 2, 64
+
+    def __init__(self):
+        self.lens, self.calls = [0, 0], []
+
+    def reset(self, client):
+        self.lens[client] = 0
+
+    def length(self, client):
+        return self.lens[client]
+
+    def decode_step(self, tokens, want_logits=False):
+        self.calls.append(("greedy", list(tokens)))
+        for i in range(len(tokens)):
+            self.lens[i] += 1
+        return [t + 1 for t in tokens], None
+
+    def decode_step_sampled(self, tokens, how, u, want_logits=False):
+        self.calls.append(("sampled", list(tokens), list(how), list(u)))
+        for i in range(len(tokens)):
+            self.lens[i] += 1
+        return [t + 1 if w is None else int(1000 * x) for t, w, x in zip(tokens, how, u)], None, None
+
+
+def test_sampled_requests_draw_their_own_numbers():
+    from emufpga_b200.sampling import Sampling
+
+    how = [Sampling(seed=5), Sampling(seed=6)]
+
+    def want(w, n):
+        g = w.numbers()
+        return [int(1000 * float(g.random(dtype="float32"))) for _ in range(n)]
+
+    s = SampledSession()
+    got = serve_continuous(s, [Request([1, 2, 3], 4, sampling=how[0]), Request([7], 2), Request([9, 9], 3, sampling=how[1])])
+    assert got == [want(how[0], 4), [8, 9], want(how[1], 3)]
+    # a greedy client's place in a sampled step has no settings, and a prompt's steps draw no number
+    first = next(c for c in s.calls if c[0] == "sampled")
+    assert first[2][1] is None and first[3] == [0.0, 0.0]
+    s = SampledSession()
+    assert serve_continuous(s, [Request([1], 2)]) == [[2, 3]] and all(c[0] == "greedy" for c in s.calls)
