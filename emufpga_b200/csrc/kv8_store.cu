@@ -95,23 +95,41 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_append_kernel(const StoreAr
     const int64_t stride = a.token[kv];
     int8_t* codes = a.codes[kv];
     float* scales = a.scales[kv];
-    for (int i = warp; i < n; i += kStoreWarps) {
-        const int l = lead[i], s = slot[i];
-        if (l < 0 || uint32_t(s) >= limit) {
-            if (l >= 0 && s != -1 && lane == 0) flag(a.status, SPM_PAGE_ID);
-            continue;
-        }
-        const T* row = x + (w0 + i) * stride;
-        uint32_t m = 0;
-        for (int c = 4 * lane; c < D; c += 128) {
-            float v[4];
-            load4(row + c, a.vec, v);
+    // f(run, slot, column, sixteen values) for the CTA's rows, D / 16 threads to a row;
+    // two turns' loads overlap
+    const int lanes = D / 16, turns = kStoreThreads / lanes;  // (rows at a time; spare threads idle)
+    const int mine = tid / lanes, col = 16 * (tid - mine * lanes);
+    auto rows = [&](auto&& f) {
+        for (int i0 = mine; i0 < n && mine < turns; i0 += 2 * turns) {
+            float v[2][16];
 #pragma unroll
-            for (int j = 0; j < 4; j++) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+            for (int u = 0; u < 2; u++) {
+                const int i = i0 + u * turns;
+                if (i >= n) break;
+                const T* row = x + (w0 + i) * stride + col;
+#pragma unroll
+                for (int c = 0; c < 16; c += 4) load4(row + c, a.vec, reinterpret_cast<float (&)[4]>(v[u][c]));
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int i = i0 + u * turns;
+                if (i >= n) break;
+                const int l = lead[i], s = slot[i];
+                if (l < 0) continue;
+                if (uint32_t(s) >= limit) {
+                    if (s != -1) flag(a.status, SPM_PAGE_ID);
+                    continue;
+                }
+                f(l, s, v[u]);
+            }
         }
-        m = __reduce_max_sync(0xffffffffu, m);
-        if (lane == 0) atomicMax(&amax[l], m);
-    }
+    };
+    rows([&](int l, int, const float (&v)[16]) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 16; j++) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+        if (m > amax[l]) atomicMax(&amax[l], m);  // (a stale look only costs the atomic)
+    });
     __syncthreads();
     if (tid < win) {
         inv[tid] = ratio[tid] = 0.f;
@@ -129,34 +147,39 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_append_kernel(const StoreAr
             inv[tid] = sc > 0.f ? __fdiv_rn(1.f, sc) : 0.f;
         }
     }
-    __syncthreads();
-    // rows that were there, where the scale has grown
-    for (int l = 0; l < win; l++) {
-        const float q = ratio[l];
-        if (q == 0.f) continue;
-        const int s = slot[l], rows = s & (P - 1);
-        uint32_t* w = reinterpret_cast<uint32_t*>(codes + ((size_t(s >> a.shift) * a.kv_heads + h) * P) * D);
-        for (int i = tid; i < rows * D / 4; i += kStoreThreads) {
-            const uint32_t c = w[i];
-            uint32_t o = 0;
+    // rows that were there, where the scale has grown (seldom)
+    if (__syncthreads_or(tid < win && ratio[tid] != 0.f)) {
+        for (int l = 0; l < win; l++) {
+            const float q = ratio[l];
+            if (q == 0.f) continue;
+            const int s = slot[l], rows = s & (P - 1);
+            uint32_t* w = reinterpret_cast<uint32_t*>(codes + ((size_t(s >> a.shift) * a.kv_heads + h) * P) * D);
+            for (int i = tid; i < rows * D / 4; i += kStoreThreads) {
+                const uint32_t c = w[i];
+                uint32_t o = 0;
 #pragma unroll
-            for (int j = 0; j < 4; j++) o |= code_of(float(int8_t(c >> (8 * j))), q) << (8 * j);
-            w[i] = o;
+                for (int j = 0; j < 4; j++) o |= code_of(float(int8_t(c >> (8 * j))), q) << (8 * j);
+                w[i] = o;
+            }
         }
     }
-    for (int i = warp; i < n; i += kStoreWarps) {
-        const int l = lead[i], s = slot[i];
-        if (l < 0 || uint32_t(s) >= limit) continue;
-        const T* row = x + (w0 + i) * stride;
+    // (the values again: from L1 as a rule)
+    rows([&](int l, int s, const float (&v)[16]) {
         const float q = inv[l];
-        uint32_t* o = reinterpret_cast<uint32_t*>(
-            codes + ((size_t(s >> a.shift) * a.kv_heads + h) * P + (s & (P - 1))) * D);
-        for (int c = 4 * lane; c < D; c += 128) {
-            float v[4];
-            load4(row + c, a.vec, v);
-            o[c >> 2] = code_of(v[0], q) | code_of(v[1], q) << 8 | code_of(v[2], q) << 16 | code_of(v[3], q) << 24;
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            // x / scale is exact, at most 127: adding 1.5 * 2^23 rounds it, half to even, to
+            // an integer in the low byte; 0 where the scale is 0 or NaN
+            uint32_t b[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) b[e] = __float_as_uint(__fmaf_rn(v[j + e], q, 12582912.f));
+            const uint32_t lo = __byte_perm(b[0], b[1], 0x0040), hi = __byte_perm(b[2], b[3], 0x0040);
+            w[j >> 2] = q == 0.f ? 0 : __byte_perm(lo, hi, 0x5410);
         }
-    }
+        *reinterpret_cast<uint4*>(codes + ((size_t(s >> a.shift) * a.kv_heads + h) * P + (s & (P - 1))) * D + col) =
+            make_uint4(w[0], w[1], w[2], w[3]);
+    });
 }
 
 struct ValueArgs {
@@ -164,37 +187,64 @@ struct ValueArgs {
     const float* scales[2];
     void* out[2];
     const int32_t* ids;
-    int32_t n, pages, kv_heads, words;  // words: 16-code pieces of a (page, head)
+    int32_t n, pages, kv_heads, block;  // block: codes of a (page, head)
     int32_t* status;
 };
 
-// 16 codes to a thread: 16 bytes in, 32 or 64 out.
+// Sixteen bytes out for each thread and turn (4 or 8 codes in), so that a warp
+// writes whole lines; four turns' loads overlap.
+constexpr int kValueTurns = 4;
+
 template <class T>
 __global__ void __launch_bounds__(256) kv8_values_kernel(const ValueArgs a) {
-    const int kv = blockIdx.y;
+    constexpr int V = 16 / sizeof(T);
+    const int kv = blockIdx.y, per = a.block / V;  // pieces of a (page, head)
     T* out = static_cast<T*>(a.out[kv]);
     if (!out) return;
-    const size_t total = size_t(a.n) * a.kv_heads * a.words;
-    for (size_t i = size_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += size_t(gridDim.x) * 256) {
-        const size_t ph = i / a.words, w = i % a.words;
-        const int p = int(ph / a.kv_heads), h = int(ph % a.kv_heads);
-        const int id = a.ids ? a.ids[p] : p;
-        uint4 c = make_uint4(0, 0, 0, 0);
-        float s = 0.f;
-        if (uint32_t(id) < uint32_t(a.pages)) {
-            const size_t at = size_t(id) * a.kv_heads + h;
-            c = __ldg(reinterpret_cast<const uint4*>(a.codes[kv]) + at * a.words + w);
-            s = __ldg(a.scales[kv] + at);
-        } else if (w == 0) {
-            flag(a.status, SPM_PAGE_ID);
+    // this CTA's pieces: one long division for all of them
+    const size_t base = size_t(blockIdx.x) * 256 * kValueTurns, ph0 = base / per, total = size_t(a.n) * a.kv_heads * per;
+    const uint32_t off = uint32_t(base - ph0 * per) + threadIdx.x;
+    uint32_t c[kValueTurns][V / 4];
+    float s[kValueTurns];
+#pragma unroll
+    for (int u = 0; u < kValueTurns; u++) {
+        s[u] = 0.f;
+#pragma unroll
+        for (int j = 0; j < V / 4; j++) c[u][j] = 0;
+        if (base + threadIdx.x + 256 * u >= total) continue;
+        const uint32_t o = off + 256 * u, skip = o / uint32_t(per), e = (o - skip * per) * V;
+        const size_t ph = ph0 + skip;
+        size_t at = ph;
+        if (a.ids) {
+            const int p = int(ph / a.kv_heads), id = a.ids[p];
+            if (uint32_t(id) >= uint32_t(a.pages)) {
+                if (e == 0) flag(a.status, SPM_PAGE_ID);
+                continue;
+            }
+            at = size_t(id) * a.kv_heads + (ph - size_t(p) * a.kv_heads);
         }
-        const uint32_t q[4] = {c.x, c.y, c.z, c.w};
-        __align__(16) T v[16];
+        s[u] = __ldg(a.scales[kv] + at);
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(a.codes[kv] + at * a.block + e);
 #pragma unroll
-        for (int j = 0; j < 16; j++) v[j] = from_f32<T>(__fmul_rn(float(int8_t(q[j >> 2] >> (8 * (j & 3)))), s));
-        uint4* o = reinterpret_cast<uint4*>(out + 16 * i);
+        for (int j = 0; j < V / 4; j++) c[u][j] = __ldg(from + j);
+    }
 #pragma unroll
-        for (int j = 0; j < int(sizeof(T)); j++) o[j] = reinterpret_cast<const uint4*>(v)[j];
+    for (int u = 0; u < kValueTurns; u++) {
+        const size_t i = base + threadIdx.x + 256 * u;
+        if (i >= total) break;
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const float y = __fmul_rn(float(int8_t(c[u][j >> 2] >> (8 * (j & 3)))), s[u]);
+            if constexpr (sizeof(T) == 4) {
+                w[j] = __float_as_uint(y);
+            } else {
+                const T t = from_f32<T>(y);
+                const uint32_t b = *reinterpret_cast<const uint16_t*>(&t);
+                w[j >> 1] = j & 1 ? w[j >> 1] | b << 16 : b;
+            }
+        }
+        __stcs(reinterpret_cast<uint4*>(out) + i, make_uint4(w[0], w[1], w[2], w[3]));
     }
 }
 
@@ -255,10 +305,13 @@ spm_status spm_kv8_values(const spm_kv8* c, uint32_t dtype, const int32_t* page_
         a.scales[0] = c->k_scales, a.scales[1] = c->v_scales;
         a.out[0] = k_out, a.out[1] = v_out;
         a.ids = page_ids, a.n = n, a.pages = c->pages, a.kv_heads = c->kv_heads;
-        a.words = c->page_tokens * c->head_dim / 16;
+        a.block = c->page_tokens * c->head_dim;
         a.status = c->status;
-        const size_t total = size_t(n) * c->kv_heads * a.words;
-        const dim3 grid(unsigned(std::min<size_t>((total + 255) / 256, size_t(device_sms()) * 8)), 2);
+        if (!page_ids && n > c->pages) fail(SPM_E_ARG, "the pool has fewer pages");
+        const size_t per = size_t(256) * kValueTurns * (dtype == SPM_F32 ? 4 : 8);
+        const size_t ctas = (size_t(n) * c->kv_heads * a.block + per - 1) / per;
+        if (ctas > INT32_MAX) fail(SPM_E_ARG, "too many pages for one call");
+        const dim3 grid(unsigned(ctas), 2);
         const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
         if (dtype == SPM_F32) kv8_values_kernel<float><<<grid, 256, 0, st>>>(a);
         else if (dtype == SPM_F16) kv8_values_kernel<__half><<<grid, 256, 0, st>>>(a);

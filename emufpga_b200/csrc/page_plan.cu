@@ -132,35 +132,76 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanArgs 
         if (rank == 0) a.starts[R] = int32_t(ts);
     }
     __syncthreads();
-    // pages of ended requests onto the stack, a warp to a row
-    for (int r = rank * kPlanWarps + warp; r < R; r += ranks * kPlanWarps)
-        for (int j = lane; j < E[r + 1] - E[r]; j += 32) a.free_pages[count + E[r] + j] = a.table[size_t(r) * a.width + j];
+    // The row of item t in exclusive sums X: X[row] <= t < X[row + 1].
+    auto row_of = [&](const int32_t* X, int t) {
+        int lo = 0, hi = R;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (X[mid] <= t) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    };
+    // Four items to a thread at a time: their searches and then their loads overlap.
+    constexpr int U = 4;
+    const int step = ranks * kPlanThreads, me = rank * kPlanThreads + tid;
+    // pages of ended requests onto the stack
+    for (int t0 = me; t0 < te; t0 += U * step) {
+        int page[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int t = t0 + u * step;
+            if (t >= te) continue;
+            const int r = row_of(E, t);
+            page[u] = a.table[size_t(r) * a.width + (t - E[r])];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (t0 + u * step < te) a.free_pages[count + t0 + u * step] = page[u];
+    }
     __threadfence();
     cl.sync();  // the whole stack stands, and the rows' old entries have been read
     if (rank == 0 && tid == 0) *a.left = int32_t(count + te - tf);
-    for (int r = rank * kPlanWarps + warp; r < R; r += ranks * kPlanWarps) {
-        const int old = int((uint32_t(C[r]) + P - 1) >> a.shift);
-        for (int j = lane; j < F[r + 1] - F[r]; j += 32)
-            a.table[size_t(r) * a.width + old + j] = __ldcg(a.free_pages + (count + te - 1 - F[r] - j));
+    for (int t0 = me; t0 < tf; t0 += U * step) {
+        int page[U];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (t0 + u * step < tf) page[u] = __ldcg(a.free_pages + (count + te - 1 - (t0 + u * step)));
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int t = t0 + u * step;
+            if (t >= tf) continue;
+            const int r = row_of(F, t), old = int((uint32_t(C[r]) + P - 1) >> a.shift);
+            a.table[size_t(r) * a.width + old + (t - F[r])] = page[u];
+        }
     }
     __threadfence();
     cl.sync();  // the table stands
-    for (int t = rank * kPlanThreads + tid; t < a.tokens; t += ranks * kPlanThreads) {
-        int pos = -1, slot = -1;
-        if (t < ts) {
-            int lo = 0, hi = R;  // S[lo] <= t < S[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (S[mid] <= t) lo = mid;
-                else hi = mid;
-            }
-            pos = C[lo] + t - S[lo];
-            const int page = __ldcg(a.table + size_t(lo) * a.width + (pos >> a.shift));
-            if (uint32_t(page) < uint32_t(a.pages)) slot = page * P + (pos & (P - 1));
-            else flag(a.status, SPM_PAGE_ID);
+    // four tokens in a row to a thread: one search finds the first one's request
+    for (int t0 = U * me; t0 < a.tokens; t0 += U * step) {
+        int pos[U], page[U];
+        int r = t0 < ts ? row_of(S, t0) : 0;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int t = t0 + u;
+            pos[u] = -1;
+            if (t >= ts) continue;
+            while (S[r + 1] <= t) r++;
+            pos[u] = C[r] + t - S[r];
+            page[u] = __ldcg(a.table + size_t(r) * a.width + (pos[u] >> a.shift));
         }
-        a.positions[t] = pos;
-        a.slots[t] = slot;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int t = t0 + u;
+            if (t >= a.tokens) break;
+            int slot = -1;
+            if (pos[u] >= 0) {
+                if (uint32_t(page[u]) < uint32_t(a.pages)) slot = page[u] * P + (pos[u] & (P - 1));
+                else flag(a.status, SPM_PAGE_ID);
+            }
+            a.positions[t] = pos[u];
+            a.slots[t] = slot;
+        }
     }
 }
 
