@@ -91,10 +91,10 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_append_kernel(const StoreAr
     __syncthreads();
     const int n = own;
     const uint32_t limit = uint32_t(a.pages) * uint32_t(P);
-    const T* x = static_cast<const T*>(a.x[kv]) + h * a.head[kv];
-    const int64_t stride = a.token[kv];
-    int8_t* codes = a.codes[kv];
-    float* scales = a.scales[kv];
+    const T* x = static_cast<const T*>(kv ? a.x[1] : a.x[0]) + h * (kv ? a.head[1] : a.head[0]);
+    const int64_t stride = kv ? a.token[1] : a.token[0];
+    int8_t* codes = kv ? a.codes[1] : a.codes[0];
+    float* scales = kv ? a.scales[1] : a.scales[0];
     // f(run, slot, column, sixteen values) for the CTA's rows, D / 16 threads to a row;
     // two turns' loads overlap
     const int lanes = D / 16, turns = kStoreThreads / lanes;  // (rows at a time; spare threads idle)
@@ -198,8 +198,12 @@ constexpr int kValueTurns = 4;
 template <class T>
 __global__ void __launch_bounds__(256) kv8_values_kernel(const ValueArgs a) {
     constexpr int V = 16 / sizeof(T);
-    const int kv = blockIdx.y, per = a.block / V;  // pieces of a (page, head)
-    T* out = static_cast<T*>(a.out[kv]);
+    // (keys or values by a select: an array in the arguments indexed by the block goes to local memory)
+    const int per = a.block / V;  // pieces of a (page, head)
+    const bool keys = blockIdx.y == 0;
+    const int8_t* const codes = keys ? a.codes[0] : a.codes[1];
+    const float* const scales = keys ? a.scales[0] : a.scales[1];
+    T* out = static_cast<T*>(keys ? a.out[0] : a.out[1]);
     if (!out) return;
     // this CTA's pieces: one long division for all of them
     const size_t base = size_t(blockIdx.x) * 256 * kValueTurns, ph0 = base / per, total = size_t(a.n) * a.kv_heads * per;
@@ -208,30 +212,25 @@ __global__ void __launch_bounds__(256) kv8_values_kernel(const ValueArgs a) {
     float s[kValueTurns];
 #pragma unroll
     for (int u = 0; u < kValueTurns; u++) {
-        s[u] = 0.f;
-#pragma unroll
-        for (int j = 0; j < V / 4; j++) c[u][j] = 0;
-        if (base + threadIdx.x + 256 * u >= total) continue;
+        const bool some = base + threadIdx.x + 256 * u < total;
         const uint32_t o = off + 256 * u, skip = o / uint32_t(per), e = (o - skip * per) * V;
         const size_t ph = ph0 + skip;
         size_t at = ph;
-        if (a.ids) {
+        bool known = some;
+        if (a.ids && some) {
             const int p = int(ph / a.kv_heads), id = a.ids[p];
-            if (uint32_t(id) >= uint32_t(a.pages)) {
-                if (e == 0) flag(a.status, SPM_PAGE_ID);
-                continue;
-            }
+            known = uint32_t(id) < uint32_t(a.pages);
+            if (!known && e == 0) flag(a.status, SPM_PAGE_ID);
             at = size_t(id) * a.kv_heads + (ph - size_t(p) * a.kv_heads);
         }
-        s[u] = __ldg(a.scales[kv] + at);
-        const uint32_t* from = reinterpret_cast<const uint32_t*>(a.codes[kv] + at * a.block + e);
+        s[u] = known ? __ldg(scales + at) : 0.f;
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(codes + at * a.block + e);
 #pragma unroll
-        for (int j = 0; j < V / 4; j++) c[u][j] = __ldg(from + j);
+        for (int j = 0; j < V / 4; j++) c[u][j] = known ? __ldg(from + j) : 0;
     }
 #pragma unroll
     for (int u = 0; u < kValueTurns; u++) {
         const size_t i = base + threadIdx.x + 256 * u;
-        if (i >= total) break;
         uint32_t w[4];
 #pragma unroll
         for (int j = 0; j < V; j++) {
@@ -244,7 +243,7 @@ __global__ void __launch_bounds__(256) kv8_values_kernel(const ValueArgs a) {
                 w[j >> 1] = j & 1 ? w[j >> 1] | b << 16 : b;
             }
         }
-        __stcs(reinterpret_cast<uint4*>(out) + i, make_uint4(w[0], w[1], w[2], w[3]));
+        if (i < total) __stcs(reinterpret_cast<uint4*>(out) + i, make_uint4(w[0], w[1], w[2], w[3]));
     }
 }
 
