@@ -36,6 +36,45 @@ struct StoreArgs {
     bool vec;                 // four elements at a time: strides and bases allow it
 };
 
+// Sixteen consecutive elements of a row, in their own type.
+template <class T>
+struct Sixteen {
+    static constexpr int W = 4 * sizeof(T);
+    uint32_t w[W];
+    __device__ __forceinline__ void load(const T* p, bool vec) {
+        if (vec) {  // (8 bytes for each four elements)
+#pragma unroll
+            for (int i = 0; i < W; i += sizeof(T)) {
+                if constexpr (sizeof(T) == 4) {
+                    const uint4 q = *reinterpret_cast<const uint4*>(p + i);
+                    w[i] = q.x, w[i + 1] = q.y, w[i + 2] = q.z, w[i + 3] = q.w;
+                } else {
+                    const uint2 q = *reinterpret_cast<const uint2*>(p + 2 * i);
+                    w[i] = q.x, w[i + 1] = q.y;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; i++) {
+                if constexpr (sizeof(T) == 4) {
+                    w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+                } else {
+                    const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + 2 * i;
+                    w[i] = h[0] | uint32_t(h[1]) << 16;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ float at(int j) const {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(w[j]);
+        } else {
+            const uint16_t h = uint16_t(j & 1 ? w[j >> 1] >> 16 : w[j >> 1]);
+            return to_f32(*reinterpret_cast<const T*>(&h));
+        }
+    }
+};
+
 __device__ __forceinline__ uint32_t code_of(float x, float inv) {
     // rounds half to even; NaN (a value or scale that is not finite) is 0
     return uint32_t(min(max(__float2int_rn(__fmul_rn(x, inv)), -127), 127)) & 0xffu;
@@ -51,20 +90,31 @@ __device__ __forceinline__ float scale_of(uint32_t amax) {
     return pow2i(x - 6 + ((amax & 0x7fffffu) > 0x7e0000u ? 1 : 0));
 }
 
-// Grid (window of tokens, kv head, keys or values).  A run is the tokens of
+// A CTA for each window of tokens, kv head, keys or values.  A run is the tokens of
 // one page that follow one another in the call; a CTA takes the runs that begin
 // in its window, whose last may reach up to a page beyond it.
 template <class T>
-__global__ void __launch_bounds__(kStoreThreads) kv8_append_kernel(const StoreArgs a) {
+__global__ void __launch_bounds__(kStoreThreads, 4) kv8_append_kernel(const StoreArgs a) {
     __shared__ int32_t slot[kStoreWindow + 256];
     __shared__ int16_t lead[kStoreWindow + 256];   // the first token of a token's run, within the window
     __shared__ uint32_t amax[kStoreWindow];
     __shared__ float inv[kStoreWindow], ratio[kStoreWindow];
     __shared__ int own;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int w0 = blockIdx.x * a.window, h = blockIdx.y, kv = blockIdx.z;
+    // keys and values of all heads side by side: their rows lie together in memory
+    const int kv = blockIdx.x & 1, h = int(blockIdx.x >> 1) % a.kv_heads, w0 = int(blockIdx.x >> 1) / a.kv_heads * a.window;
     const int P = a.page, D = a.dim;
     const int win = min(a.window, a.tokens - w0), span = min(a.tokens - w0, win + P - 1);
+    // D / 16 threads to a row, sixteen values each (spare threads idle).  The first rows'
+    // values are on their way before anything else is known, and stay in registers.
+    const T* x = static_cast<const T*>(kv ? a.x[1] : a.x[0]) + h * (kv ? a.head[1] : a.head[0]);
+    const int64_t stride = kv ? a.token[1] : a.token[0];
+    const int lanes = D / 16, turns = kStoreThreads / lanes;
+    const int mine = tid / lanes, col = 16 * (tid - mine * lanes);
+    Sixteen<T> held[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+        if (mine < turns && mine + u * turns < span) held[u].load(x + (w0 + mine + u * turns) * stride + col, a.vec);
     for (int i = tid; i < span; i += kStoreThreads) slot[i] = a.slots[w0 + i];
     if (tid < win) amax[tid] = 0;
     __syncthreads();
@@ -91,43 +141,32 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_append_kernel(const StoreAr
     __syncthreads();
     const int n = own;
     const uint32_t limit = uint32_t(a.pages) * uint32_t(P);
-    const T* x = static_cast<const T*>(kv ? a.x[1] : a.x[0]) + h * (kv ? a.head[1] : a.head[0]);
-    const int64_t stride = kv ? a.token[1] : a.token[0];
     int8_t* codes = kv ? a.codes[1] : a.codes[0];
     float* scales = kv ? a.scales[1] : a.scales[0];
-    // f(run, slot, column, sixteen values) for the CTA's rows, D / 16 threads to a row;
-    // two turns' loads overlap
-    const int lanes = D / 16, turns = kStoreThreads / lanes;  // (rows at a time; spare threads idle)
-    const int mine = tid / lanes, col = 16 * (tid - mine * lanes);
+    // f(run, slot, sixteen values) for this thread's pieces of the CTA's rows
     auto rows = [&](auto&& f) {
-        for (int i0 = mine; i0 < n && mine < turns; i0 += 2 * turns) {
-            float v[2][16];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int i = i0 + u * turns;
-                if (i >= n) break;
-                const T* row = x + (w0 + i) * stride + col;
-#pragma unroll
-                for (int c = 0; c < 16; c += 4) load4(row + c, a.vec, reinterpret_cast<float (&)[4]>(v[u][c]));
+        for (int u = 0, i = mine; i < n && mine < turns; u++, i += turns) {
+            const int l = lead[i], s = slot[i];
+            if (l < 0) continue;
+            if (uint32_t(s) >= limit) {
+                if (s != -1) flag(a.status, SPM_PAGE_ID);
+                continue;
             }
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int i = i0 + u * turns;
-                if (i >= n) break;
-                const int l = lead[i], s = slot[i];
-                if (l < 0) continue;
-                if (uint32_t(s) >= limit) {
-                    if (s != -1) flag(a.status, SPM_PAGE_ID);
-                    continue;
-                }
-                f(l, s, v[u]);
+            if (u == 0) {
+                f(l, s, held[0]);
+            } else if (u == 1) {
+                f(l, s, held[1]);
+            } else {  // (a run that goes on behind the window; head_dim over 128)
+                Sixteen<T> more;
+                more.load(x + (w0 + i) * stride + col, a.vec);
+                f(l, s, more);
             }
         }
     };
-    rows([&](int l, int, const float (&v)[16]) {
+    rows([&](int l, int, const Sixteen<T>& v) {
         uint32_t m = 0;
 #pragma unroll
-        for (int j = 0; j < 16; j++) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+        for (int j = 0; j < 16; j++) m = max(m, __float_as_uint(v.at(j)) & 0x7fffffffu);
         if (m > amax[l]) atomicMax(&amax[l], m);  // (a stale look only costs the atomic)
     });
     __syncthreads();
@@ -163,8 +202,7 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_append_kernel(const StoreAr
             }
         }
     }
-    // (the values again: from L1 as a rule)
-    rows([&](int l, int s, const float (&v)[16]) {
+    rows([&](int l, int s, const Sixteen<T>& v) {
         const float q = inv[l];
         uint32_t w[4];
 #pragma unroll
@@ -173,7 +211,7 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_append_kernel(const StoreAr
             // an integer in the low byte; 0 where the scale is 0 or NaN
             uint32_t b[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) b[e] = __float_as_uint(__fmaf_rn(v[j + e], q, 12582912.f));
+            for (int e = 0; e < 4; e++) b[e] = __float_as_uint(__fmaf_rn(v.at(j + e), q, 12582912.f));
             const uint32_t lo = __byte_perm(b[0], b[1], 0x0040), hi = __byte_perm(b[2], b[3], 0x0040);
             w[j >> 2] = q == 0.f ? 0 : __byte_perm(lo, hi, 0x5410);
         }
@@ -259,7 +297,6 @@ spm_status spm_kv8_append(const spm_kv8* c, uint32_t dtype, const void* k, int64
         kv8_check(c);
         kv8_check_type(dtype);
         if (tokens < 0) fail(SPM_E_ARG, "negative token count");
-        if (c->kv_heads > 65535) fail(SPM_E_ARG, "too many kv heads");
         if (tokens == 0) return;
         if (!k || !v || !slots) fail(SPM_E_ARG, "null keys, values or slots");
         DeviceScope scope(c->device);
@@ -280,11 +317,12 @@ spm_status spm_kv8_append(const spm_kv8* c, uint32_t dtype, const void* k, int64
         a.window = kStoreWindow;
         while (a.window > kStoreWarps && int64_t((tokens + a.window - 1) / a.window) * c->kv_heads * 2 < 2 * device_sms())
             a.window /= 2;
-        const dim3 grid(unsigned((tokens + a.window - 1) / a.window), unsigned(c->kv_heads), 2);
+        const int64_t grid = int64_t((tokens + a.window - 1) / a.window) * c->kv_heads * 2;
+        if (grid > INT32_MAX) fail(SPM_E_ARG, "too many tokens for one call");
         const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
-        if (dtype == SPM_F32) kv8_append_kernel<float><<<grid, kStoreThreads, 0, st>>>(a);
-        else if (dtype == SPM_F16) kv8_append_kernel<__half><<<grid, kStoreThreads, 0, st>>>(a);
-        else kv8_append_kernel<__nv_bfloat16><<<grid, kStoreThreads, 0, st>>>(a);
+        if (dtype == SPM_F32) kv8_append_kernel<float><<<unsigned(grid), kStoreThreads, 0, st>>>(a);
+        else if (dtype == SPM_F16) kv8_append_kernel<__half><<<unsigned(grid), kStoreThreads, 0, st>>>(a);
+        else kv8_append_kernel<__nv_bfloat16><<<unsigned(grid), kStoreThreads, 0, st>>>(a);
         CUDA_OK(cudaGetLastError());
     });
 }
