@@ -86,4 +86,14 @@ void allow_smem(K kernel, size_t bytes, unsigned long long& done) {
     if (d < 64) done |= 1ull << d;
 }
 
+// Likewise for clusters of more than eight CTAs.
+template <class K>
+void allow_wide_clusters(K kernel, unsigned long long& done) {
+    int d = 0;
+    CUDA_OK(cudaGetDevice(&d));
+    if (d < 64 && (done >> d & 1)) return;
+    CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    if (d < 64) done |= 1ull << d;
+}
+
 }  // namespace spm

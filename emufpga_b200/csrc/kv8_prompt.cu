@@ -9,13 +9,16 @@
 //                        128-byte swizzled layout, which is K-major for the keys
 //                        (S = Q K^T) and MN-major for the values (O = P V), so both
 //                        are written alike and nothing is transposed
-//   MMA (1 thread)       per group: O += P(j) V(j) with P from TMEM, then
-//                        S(j + 1) = Q K(j + 1)^T over the P just read
+//   MMA (1 thread)       per group: O += P(j) V(j) with P from TMEM, then, once that
+//                        is done (products of other accumulators do not order each
+//                        other), the next S = Q K^T over the P just read
 //   softmax (4 warps a group)  a thread owns a row: S from TMEM, scale, mask, the
 //                        running references, weights in fp16 back to where S stood
 // With two groups the products of one run under the softmax of the other, and both
-// share the conversion of the codes.  (head_dim over 128 leaves TMEM and shared
-// memory for one.)
+// share the conversion of the codes.  head_dim over 128 leaves TMEM and shared memory
+// for one group, which has two buffers of S instead.  (Two buffers of 64 keys for
+// two groups too: 176 us where one of 128 takes 135, 1024 queries over 4096 keys; a
+// product of 64 columns takes the tensor cores as long as one of 128.)
 // The references move only where a row's maximum passes them by more than 2^8, so
 // that the accumulator is hardly ever read back to be rescaled: weights are then at
 // most 2^8, which fp16 holds as exactly as those below 1.
@@ -45,28 +48,31 @@ struct PromptShape {
     static constexpr int G = kv8_prompt_rows(HD) / kRows;
     static constexpr int threads = 32 * (4 * G + kFillWarps + 1);
     static constexpr int TN = HD <= 128 ? 128 : 64;    // keys of a tile
+    static constexpr int BUF = G == 1 ? 2 : 1;         // buffers of S
     static constexpr int atoms = (HD + 63) / 64;       // 64 dimensions, 128 bytes
     static constexpr int qgroup = atoms * kRows * 128; // bytes of a group's part of Q
     static constexpr int qbytes = G * NP * qgroup;
     static constexpr int tile = atoms * TN * 128;      // bytes of a tile of K or V
-    static constexpr int stages = qbytes + 4 * tile + 4096 <= 227 * 1024 ? 2 : 1;
+    static constexpr int room = (227 * 1024 - 8192 - qbytes) / (2 * tile), stages = room > 4 ? 4 : room;
+    static_assert(stages >= 1, "a tile of K and one of V");
     // (at least half of an SM's: a second CTA would wait for the first one's TMEM)
     static constexpr int need = qbytes + 2 * stages * tile + 1024, smem = need > 120 * 1024 ? need : 120 * 1024;
-    // TMEM columns: S of a group, which its P replaces (16 columns of S, 16 keys, hold
-    // the 8 columns of their high parts, then of their low ones), and O
-    static constexpr int s_col = 0, o_col = G * TN;
+    // TMEM columns: the buffers of S of each group, which its P replaces (16 columns
+    // of S, 16 keys, hold the 8 columns of their high parts, then of their low ones),
+    // and O
+    static constexpr int s_col = 0, o_col = BUF * G * TN;
     static_assert(o_col + G * HD <= 512, "TMEM");
 };
 
 struct PromptSync {
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_done[2], drained;
+    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2][2], p_ready[2][2], o_done[2], o_last[2], drained;
     uint32_t tmem;
     volatile int gave_up;
     float qscale[2 * kRows];
     // scales of K and exponents of V's for a tile's blocks of 16 keys; tile j's are
-    // overwritten with j + 4, for which P(j) V(j) has to be done
-    float ks[4][8], ve[4][8], vn[4][8];  // (vn: NaN for a scale that is, else 0)
-    int vi[4][8];                        // ve, -10000 for a scale of 0
+    // overwritten with j + 8's, for which P(j) V(j) has to be done (four stages)
+    float ks[8][8], ve[8][8], vn[8][8];  // (vn: NaN for a scale that is, else 0)
+    int vi[8][8];                        // ve, -10000 for a scale of 0
 };
 
 __device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
@@ -166,7 +172,7 @@ typedef std::false_type No;
 template <int HD, int NP>
 __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_kernel(const Kv8Args a) {
     using S = PromptShape<HD, NP>;
-    constexpr int TN = S::TN, ST = S::stages, G = S::G, kSoftWarps = 4 * G;
+    constexpr int TN = S::TN, ST = S::stages, G = S::G, BUF = S::BUF, kSoftWarps = 4 * G;
     extern __shared__ __align__(1024) uint8_t raw[];
     __shared__ PromptSync y;
     const uint32_t qs = (saddr(raw) + 1023u) & ~1023u, ks = qs + S::qbytes, vs = ks + ST * S::tile;
@@ -184,14 +190,19 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
     if (rows <= 0) return;
     const int keys = kv8_keys(a, nq, len, tile), tiles = (keys + TN - 1) / TN;
     if (tid == 0) {
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < 4; i++) {
             mbar_init(&y.k_full[i], kFillThreads);
             mbar_init(&y.k_empty[i], 1);
             mbar_init(&y.v_full[i], kFillThreads);
             mbar_init(&y.v_empty[i], 1);
-            mbar_init(&y.s_full[i], 1);
-            mbar_init(&y.p_ready[i], kRows);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&y.s_full[0][i], 1);
+            mbar_init(&y.s_full[1][i], 1);
+            mbar_init(&y.p_ready[0][i], kRows);
+            mbar_init(&y.p_ready[1][i], kRows);
             mbar_init(&y.o_done[i], 1);
+            mbar_init(&y.o_last[i], 1);
         }
         mbar_init(&y.drained, 1);
         y.gave_up = 0;
@@ -254,8 +265,9 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
     if (warp >= kSoftWarps && warp < kMmaWarp) {
         // ---- producers: codes of tile j converted while those of j + 1 and the page
         // numbers of j + 2 are on their way ----
-        constexpr int SEG = HD / 16, N = TN * SEG / kFillThreads;  // 16-byte pieces of a token, and of a thread
-        static_assert(TN * SEG % kFillThreads == 0, "whole pieces");
+        // 16-byte pieces of a token, and of a thread (head_dim 96: the last ones of half the threads)
+        constexpr int SEG = HD / 16, PIECES = TN * SEG, N = (PIECES + kFillThreads - 1) / kFillThreads;
+        constexpr bool ragged = PIECES % kFillThreads != 0;
         const int t = tid - 32 * kSoftWarps;
         const int32_t* trow = a.table + size_t(req) * a.width;
         uint4 k[N], v[N];
@@ -264,7 +276,7 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const int tok = j * TN + (t + i * kFillThreads) / SEG;
-                page[i] = tok < keys ? __ldg(trow + (tok >> a.shift)) : -1;
+                page[i] = tok < keys && (!ragged || t + i * kFillThreads < PIECES) ? __ldg(trow + (tok >> a.shift)) : -1;
             }
         };
         // -1 for none, and for a page that is not in the pool
@@ -278,7 +290,7 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
         auto load = [&](const int8_t* codes, int j, uint4 (&c)[N]) {
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int e = t + i * kFillThreads, r = e / SEG, o = e % SEG, tok = j * TN + r, p = known(page[i], tok);
+                const int e = t + i * kFillThreads, r = e / SEG, o = e % SEG, tok = j * TN + r, p = ragged && e >= PIECES ? -1 : known(page[i], tok);
                 c[i] = make_uint4(0, 0, 0, 0);
                 if (p >= 0)
                     c[i] = __ldg(reinterpret_cast<const uint4*>(
@@ -289,6 +301,7 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const int e = t + i * kFillThreads, r = e / SEG, o = e % SEG;
+                if (ragged && e >= PIECES) break;
                 uint32_t h[8];
                 const uint32_t w[4] = {c[i].x ^ 0x80808080u, c[i].y ^ 0x80808080u, c[i].z ^ 0x80808080u, c[i].w ^ 0x80808080u};
 #pragma unroll
@@ -326,11 +339,11 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
             if (j >= ST && !wait(&y.k_empty[st], again)) break;
             store(base + S::qbytes + st * S::tile, k);
             if (t < TN / 16) {
-                y.ks[j & 3][t] = kscale;
+                y.ks[j & 7][t] = kscale;
                 const float e = kv8_exponent(vscale);
-                y.ve[j & 3][t] = e;
-                y.vi[j & 3][t] = vscale > 0.f ? int(e) : -10000;
-                y.vn[j & 3][t] = e != e ? e : 0.f;
+                y.ve[j & 7][t] = e;
+                y.vi[j & 7][t] = vscale > 0.f ? int(e) : -10000;
+                y.vn[j & 7][t] = e != e ? e : 0.f;
             }
             fence_proxy_async();
             mbar_arrive(&y.k_full[st]);
@@ -354,22 +367,27 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
                 for (int p = NP - 1; p >= 0; p--)
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; kk++)
-                        umma_f16(tmem + S::s_col + g * TN,
+                        umma_f16(tmem + S::s_col + (BUF * g + j % BUF) * TN,
                                  sw128_desc(q + uint32_t(p) * S::qgroup + (kk >> 2) * (kRows * 128) + 32u * (kk & 3)),
                                  sw128_desc(k + (kk >> 2) * (TN * 128) + 32u * (kk & 3)), id_s, p != NP - 1 || kk != 0);
                 if (g == groups - 1) umma_commit(&y.k_empty[j % ST]);
-                umma_commit(&y.s_full[g]);
+                umma_commit(&y.s_full[g][j % BUF]);
+            };
+            auto keys_in = [&](int j) {
+                const bool in = wait(&y.k_full[j % ST], uint32_t(j / ST) & 1u);
+                tc_fence_after();
+                return in;
             };
             bool ok = true;
-            if (tiles) {
-                ok = wait(&y.k_full[0], 0);
-                tc_fence_after();
-                for (int g = 0; ok && g < groups; g++) scores(g, 0);
+            for (int j = 0; ok && j < min(BUF, tiles); j++) {
+                ok = keys_in(j);
+                for (int g = 0; ok && g < groups; g++) scores(g, j);
             }
             for (int j = 0; ok && j < tiles; j++)
                 for (int g = 0; g < groups; g++) {
                     if (g == 0) ok = wait(&y.v_full[j % ST], uint32_t(j / ST) & 1u);
-                    ok = ok && wait(&y.p_ready[g], uint32_t(j) & 1u);
+                    // (a barrier for each buffer: the softmax may be a tile further already)
+                    ok = ok && wait(&y.p_ready[g][j % BUF], uint32_t(j / BUF) & 1u);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t v = vs + uint32_t(j % ST) * S::tile;
@@ -377,17 +395,17 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
                     for (int p = NP - 1; p >= 0; p--)
 #pragma unroll
                         for (int kk = 0; kk < TN / 16; kk++)
-                            umma_f16_ts(tmem + S::o_col + g * HD, tmem + S::s_col + g * TN + 16u * kk + 8u * p,
+                            umma_f16_ts(tmem + S::o_col + g * HD, tmem + S::s_col + (BUF * g + j % BUF) * TN + 16u * kk + 8u * p,
                                         sw128_mn_desc(v + 2048u * kk, TN * 128), id_o, j != 0 || p != NP - 1 || kk != 0);
                     if (g == groups - 1) umma_commit(&y.v_empty[j % ST]);
-                    if (j + 1 < tiles) {
-                        // over the P that the products above read: they run in order
-                        if (g == 0) ok = wait(&y.k_full[(j + 1) % ST], uint32_t((j + 1) / ST) & 1u);
+                    umma_commit(&y.o_done[g]);
+                    if (j + 1 == tiles) umma_commit(&y.o_last[g]);
+                    if (j + BUF < tiles) {
+                        if (g == 0) ok = keys_in(j + BUF);
+                        ok = ok && wait(&y.o_done[g], uint32_t(j) & 1u);
                         if (!ok) break;
                         tc_fence_after();
-                        scores(g, j + 1);
-                    } else {
-                        umma_commit(&y.o_done[g]);
+                        scores(g, j + BUF);
                     }
                 }
             umma_commit(&y.drained);  // TMEM is given back when every product has ended
@@ -398,19 +416,20 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
         // ---- softmax: thread = row = TMEM lane of its group ----
         const int g = warp >> 2, r = tid;
         const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
-        const uint32_t s = tmem + lanes + S::s_col + uint32_t(g) * TN, o = tmem + lanes + S::o_col + uint32_t(g) * HD;
+        const uint32_t s0col = tmem + lanes + S::s_col + uint32_t(BUF * g) * TN, o = tmem + lanes + S::o_col + uint32_t(g) * HD;
         const float qscale = y.qscale[r];
         const int limit = r < rows ? len - nq + (row0 + r) / a.group + 1 : 0;  // keys that the row sees
-        float m = -INFINITY, ref = -INFINITY, sum = 0.f;
+        float m = -INFINITY, ref = -INFINITY, sum = 0.f, m0 = 0.f;  // m0: m, 0 for none yet
+        int lift = -20000;                                        // m0 - ref
         bool ok = true;
         const int turns = g < groups ? tiles : 0;
         for (int j = 0; j < turns; j++) {
-            // (S(j) done means P(j - 1) V(j - 1) done: O may be read and written)
-            ok = wait(&y.s_full[g], uint32_t(j) & 1u);
+            ok = wait(&y.s_full[g][j % BUF], uint32_t(j / BUF) & 1u);
             if (!__all_sync(0xffffffffu, ok)) {
                 ok = false;
                 break;
             }
+            const uint32_t s = s0col + uint32_t(j % BUF) * TN;
             tc_fence_after();
             const int t0 = j * TN;
             const bool hidden = __any_sync(0xffffffffu, t0 + TN > limit);
@@ -439,33 +458,46 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
                             x[e & 3] = fmaxf(x[e & 3], masked && t0 + 16 * b + e >= limit ? -INFINITY : y);
                         }
                         float big = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                        const float f = qscale * y.ks[j & 3][b];  // not negative, or NaN
+                        const float f = qscale * y.ks[j & 7][b];  // not negative, or NaN
                         big = big == -INFINITY ? big : f != f ? 0.f : ceilf(big * f);
                         top = fmaxf(top, big);
-                        reach = fmaxf(reach, big + y.ve[j & 3][b]);
+                        reach = fmaxf(reach, big + y.ve[j & 7][b]);
                     }
                 });
             };
             hidden ? maxima(Yes()) : maxima(No());
-            const float m_new = top > m + kSlack || m == -INFINITY ? top : m;
-            const float r_new = reach > ref + kSlack || ref == -INFINITY ? reach : ref;
-            sum *= kv8_step(m, m_new);
-            const float down = r_new != ref ? kv8_step(ref, r_new) : 1.f;
-            m = m_new;
-            ref = r_new;
-            if (j && __any_sync(0xffffffffu, down != 1.f)) {
+            // the references move seldom (see above), a warp's rows together
+            const bool moves = top > m + kSlack || reach > ref + kSlack || (m == -INFINITY && top > m) ||
+                               (ref == -INFINITY && reach > ref);
+            if (__any_sync(0xffffffffu, moves)) {
+                const float m_new = top > m + kSlack || m == -INFINITY ? top : m;
+                const float r_new = reach > ref + kSlack || ref == -INFINITY ? reach : ref;
+                sum *= kv8_step(m, m_new);
+                const float down = r_new != ref ? kv8_step(ref, r_new) : 1.f;
+                m = m_new;
+                ref = r_new;
+                m0 = m == -INFINITY ? 0.f : m;
+                lift = ref == -INFINITY ? -20000 : int(fminf(fmaxf(m0 - ref, -5000.f), 5000.f));
+                if (j) {
+                    // O is the products' until P(j - 1) V(j - 1) is done (the one before
+                    // is, S(j) waited for it: the parity is that of one phase alone)
+                    ok = wait(&y.o_done[g], uint32_t(j - 1) & 1u);
+                    if (!__all_sync(0xffffffffu, ok)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
 #pragma unroll 1
-                for (int d = 0; d < HD; d += 16) {
-                    float x[16];
-                    tmem_ld16(o + d, x);
+                    for (int d = 0; d < HD; d += 16) {
+                        float x[16];
+                        tmem_ld16(o + d, x);
 #pragma unroll
-                    for (int e = 0; e < 16; e++) x[e] *= down;
-                    tmem_st16(o + d, x);
+                        for (int e = 0; e < 16; e++) x[e] *= down;
+                        tmem_st16(o + d, x);
+                    }
                 }
             }
-            const float m0 = m == -INFINITY ? 0.f : m;
             const uint64_t minus = pair_of(-m0, -m0);
-            const int lift = ref == -INFINITY ? -20000 : int(fminf(fmaxf(m0 - ref, -5000.f), 5000.f));
             uint64_t sums[2] = {0, 0};
             auto weights = [&](auto masked) {
                 columns([&](const uint32_t (&v)[32], int c) {
@@ -473,8 +505,8 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
                     for (int h = 0; h < 2; h++) {
                         const int b = 2 * c + h;
                         // 2^(m + ve - ref); 2^-126, 0 in fp16, for a page of zeros; NaN for one of NaN
-                        const float f = qscale * y.ks[j & 3][b];
-                        const float w = pow2i(min(lift + y.vi[j & 3][b], 126)) + y.vn[j & 3][b];
+                        const float f = qscale * y.ks[j & 7][b];
+                        const float w = pow2i(min(lift + y.vi[j & 7][b], 126)) + y.vn[j & 7][b];
                         const uint64_t ff = pair_of(f, f), ww = pair_of(w, w);
                         uint32_t out[8 * NP];
 #pragma unroll
@@ -508,9 +540,10 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
             sum += s2.x + s2.y;
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(&y.p_ready[g]);
+            mbar_arrive(&y.p_ready[g][j % BUF]);
         }
-        if (ok && turns) ok = wait(&y.o_done[g], 0);
+        // (a barrier of its own: o_done may be two phases behind here, and its parity says nothing)
+        if (ok && turns) ok = wait(&y.o_last[g], 0);
         tc_fence_after();
         if (__all_sync(0xffffffffu, ok) && g < groups) {
             const int qr = row0 + r, qi = qr / a.group, qh = head * a.group + qr % a.group;

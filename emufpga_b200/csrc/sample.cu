@@ -34,7 +34,7 @@ using namespace dev;
 namespace cg = cooperative_groups;
 
 constexpr int kBins = 1024;
-constexpr int kSampleClusters = 8;        // CTAs of a row, at most
+constexpr int kSampleClusters = 16;       // CTAs of a row, at most (8: the portable ones, see launch_type)
 constexpr int kList = 2048;               // tokens that are sorted, at most
 constexpr int kSampleSlice = 160 * 1024;  // bytes of a slice that shared memory holds
 constexpr int kTable = 128;               // of the exponential
@@ -317,6 +317,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
         cl.map_shared_rank(s.top, tid)[rank] = top;
     }
     cl.sync();
+#pragma unroll 8
     for (int c = 0; c < C; c++) top = fmaxf(top, s.top[c]);
     if (top == -INFINITY) {  // the same for the whole cluster
         if (rank == 0 && tid == 0) {
@@ -387,14 +388,25 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
         }
         cl.sync();
     };
-    // the cluster's lists, whole, in this CTA's `sorted`; their length
+    // the lengths of the cluster's lists together, which may be past what they hold
+    auto listed = [&]() {
+        const int m = lane < C ? int(*cl.map_shared_rank(&s.listed, lane)) : 0;
+        return int(__reduce_add_sync(0xffffffffu, uint32_t(m)));
+    };
+    // the lists, whole, in this CTA's `sorted`, its warps sharing out the CTAs; their length
     auto collect = [&]() {
-        int len = 0;
-        for (int c = 0; c < C; c++) {
-            const int m = int(*cl.map_shared_rank(&s.listed, c));
+        const int m = lane < C ? int(*cl.map_shared_rank(&s.listed, lane)) : 0;
+        int to = m;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, to, o);
+            if (lane >= o) to += y;
+        }
+        const int len = __shfl_sync(0xffffffffu, to, 31), share = max(1, W / C);
+        for (int c = warp % C; c < C; c += W) {
+            const int at = __shfl_sync(0xffffffffu, to - m, c), n = __shfl_sync(0xffffffffu, m, c);
             const u64* from = cl.map_shared_rank(s.list, c);
-            for (int i = tid; i < m; i += NT) s.sorted[len + i] = from[i];
-            len += m;
+            for (int i = warp / C * 32 + lane; i < n; i += 32 * share) s.sorted[at + i] = from[i];
         }
         __syncthreads();
         return len;
@@ -523,8 +535,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
             __syncthreads();  // (the list lies over the totals)
             list(inside);
             cl.sync();
-            m = 0;
-            for (int c = 0; c < C; c++) m += int(*cl.map_shared_rank(&s.listed, c));
+            m = listed();
             if (m <= (sub < 0 ? kSoon : kList) || sub >= 0) break;
             cl.sync();  // the lists' lengths have been read
             if (tid == 0) s.listed = 0;
@@ -663,58 +674,49 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
         cl.map_shared_rank(s.seg_ties, lane)[to] = tied;
     }
     cl.sync();
-    // four segments to a lane of the first warp; ties go to the first by index
-    constexpr int PER = kSampleClusters * W / 32;
+    // a few segments to each lane of the first warp; ties go to the first by index
     if (warp == 0) {
-        u64 t[PER], m[PER], c = 0, tsum = 0;
+        const int segs = C * W, w0 = lane * (kSampleClusters * W / 32), w1 = min(segs, w0 + kSampleClusters * W / 32);
+        auto inclusive = [&](u64 v) {
 #pragma unroll
-        for (int j = 0; j < PER; j++) {
-            const int w = lane * PER + j;
-            t[j] = w < C * W ? s.seg_ties[w] : 0;
-            tsum += t[j];
+            for (int o = 1; o < 32; o <<= 1) {
+                const u64 y = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += y;
+            }
+            return v;
+        };
+        u64 t = 0;
+        for (int w = w0; w < w1; w++) t += s.seg_ties[w];
+        const u64 ties0 = inclusive(t) - t;
+        auto taken = [&](u64 before, int w) { return before >= ties ? 0 : min(u64(s.seg_ties[w]), ties - before); };
+        u64 m = 0, c = 0, tb = ties0;
+        for (int w = w0; w < w1; w++) {
+            const u64 k = taken(tb, w);
+            m += k * tie_mass + s.seg_mass[w];
+            c += k + s.seg_count[w];
+            tb += s.seg_ties[w];
         }
-        u64 tb = tsum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const u64 y = __shfl_up_sync(0xffffffffu, tb, o);
-            if (lane >= o) tb += y;
-        }
-        tb -= tsum;
-        u64 msum = 0, before[PER];
-#pragma unroll
-        for (int j = 0; j < PER; j++) {
-            const int w = lane * PER + j;
-            const u64 taken = tb >= ties ? 0 : min(t[j], ties - tb);
-            before[j] = tb;
-            tb += t[j];
-            m[j] = taken * tie_mass + (w < C * W ? s.seg_mass[w] : 0);
-            c += taken + (w < C * W ? s.seg_count[w] : 0);
-            msum += m[j];
-        }
-        u64 mb = msum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const u64 y = __shfl_up_sync(0xffffffffu, mb, o);
-            if (lane >= o) mb += y;
-        }
+        u64 mb = inclusive(m);
         const u64 total = __shfl_sync(0xffffffffu, mb, 31);
-        mb -= msum;
+        mb -= m;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
         const float u = a.u[row];
         // the first token with cumulated mass > target
         u64 target = u > 0.f ? __double2ull_rd(fmin(double(u), 1.0) * double(total)) : 0;
         target = min(target, total - 1);
-#pragma unroll
-        for (int j = 0; j < PER; j++) {
-            if (mb <= target && target < mb + m[j]) {
-                s.pick_seg = lane * PER + j;
+        tb = ties0;
+        for (int w = w0; w < w1 && mb <= target; w++) {
+            const u64 here = taken(tb, w) * tie_mass + s.seg_mass[w];
+            if (target < mb + here) {
+                s.pick_seg = w;
                 s.pick_before = target - mb;  // still to pass inside the segment
-                s.pick_ties = before[j];
+                s.pick_ties = tb;
                 s.pick_total = total;
                 s.pick_count = c;
             }
-            mb += m[j];
+            mb += here;
+            tb += s.seg_ties[w];
         }
     }
     __syncthreads();
@@ -741,7 +743,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
 template <class T, int NT>
 void launch_sample(const SampleArgs& a, int rows, int ctas, size_t smem, cudaStream_t st) {
     static unsigned long long done = 0;
+    static unsigned long long wide = 0;
     allow_smem(sample_kernel<T, NT>, sizeof(Shared) + kSampleSlice, done);
+    if (ctas > 8) allow_wide_clusters(sample_kernel<T, NT>, wide);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(rows) * unsigned(ctas));
     cfg.blockDim = dim3(NT);
@@ -757,10 +761,19 @@ void launch_sample(const SampleArgs& a, int rows, int ctas, size_t smem, cudaStr
 }
 
 template <class T>
-void launch_type(const SampleArgs& a, int rows, int ctas, size_t smem, cudaStream_t st) {
-    // While every CTA has an SM to itself, 1024 threads shorten its passes; beyond
-    // that two CTAs of 512 to an SM hide each other's barriers.
-    if (int64_t(rows) * ctas <= device_sms()) launch_sample<T, 1024>(a, rows, ctas, smem, st);
+void launch_type(SampleArgs a, int rows, cudaStream_t st) {
+    // A CTA for every 2048 logits, up to 16 (more than 8 is not portable, but fits a
+    // B200's groups of SMs) while every CTA has an SM to itself, else up to 8; then 1024
+    // threads shorten its passes, and beyond one CTA an SM two of 512 hide each other's
+    // barriers.
+    const int sms = device_sms();
+    int ctas = 1;
+    while (ctas < kSampleClusters && a.vocab > 2048 * ctas && (ctas < 8 || int64_t(rows) * 2 * ctas <= sms)) ctas *= 2;
+    const int per = 4 * 32;  // four for each warp, of 32 at most
+    a.slice = ((a.vocab + ctas - 1) / ctas + per - 1) / per * per;
+    const size_t bytes = size_t(a.slice) * sizeof(T);
+    const size_t smem = sizeof(Shared) + (bytes <= size_t(kSampleSlice) ? bytes : 0);
+    if (int64_t(rows) * ctas <= sms) launch_sample<T, 1024>(a, rows, ctas, smem, st);
     else launch_sample<T, 512>(a, rows, ctas, smem, st);
 }
 
@@ -782,16 +795,9 @@ spm_status spm_sample(int device, uint32_t dtype, const void* logits, int64_t ro
         if (!logits || !u || !token) fail(SPM_E_ARG, "null logits, u or token");
         DeviceScope scope(device);
         SampleArgs a{logits, row_stride, vocab, 0, temperature, top_k, top_p, min_p, u, token, kept, prob};
-        // a CTA for every 2048 logits, eight at most
-        int ctas = 1;
-        while (ctas < kSampleClusters && vocab > 2048 * ctas) ctas *= 2;
-        const int per = 4 * 32;  // four for each warp, of 32 at most
-        a.slice = ((vocab + ctas - 1) / ctas + per - 1) / per * per;
-        const size_t bytes = size_t(a.slice) * (dtype == SPM_F32 ? 4 : 2);
-        const size_t smem = sizeof(Shared) + (bytes <= size_t(kSampleSlice) ? bytes : 0);
         const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
-        if (dtype == SPM_F32) launch_type<float>(a, rows, ctas, smem, st);
-        else if (dtype == SPM_F16) launch_type<__half>(a, rows, ctas, smem, st);
-        else launch_type<__nv_bfloat16>(a, rows, ctas, smem, st);
+        if (dtype == SPM_F32) launch_type<float>(a, rows, st);
+        else if (dtype == SPM_F16) launch_type<__half>(a, rows, st);
+        else launch_type<__nv_bfloat16>(a, rows, st);
     });
 }
