@@ -569,7 +569,11 @@ Plan plan_of(const spm_kv8* c, int heads, int requests, int most, int width) {
     const int64_t small = int64_t(requests) * c->kv_heads * p.tiles;
     const int tall = kv8_prompt_rows(c->head_dim);
     const int64_t large = int64_t(requests) * c->kv_heads * ((rows + tall - 1) / tall);
-    p.prompt = rows > 16 && small >= 96 * ((large + sms - 1) / sms);
+    // A row tile of 16 costs this kernel as much as one of 128 or 256 costs the kernel of
+    // many queries, but shares its keys out over all SMs: 256 such tiles for each wave of
+    // the other's CTAs is where they meet (256 tiles, 1024 to 8000 keys: 137 against 144
+    // us, 90 against 86; 336: 70 against 47; 640: 168 against 56; 128: 88 against 143).
+    p.prompt = rows > 16 && small > 256 * ((large + sms - 1) / sms);
     if (p.prompt) {
         p.tiles = int((rows + tall - 1) / tall);
         if (requests > 65535 || p.tiles > INT32_MAX / tall) fail(SPM_E_ARG, "too many requests and queries for one call");

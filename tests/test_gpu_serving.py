@@ -308,8 +308,8 @@ def test_attention_of_several_tokens(dtype, page, heads, kv_heads, dim, news, le
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim", [64, 96, 128, 192, 256])
 @pytest.mark.parametrize("page,heads,kv_heads,news,lens", [
-    (16, 16, 8, [200], [777]), (64, 24, 8, [129, 0, 77], [129, 40, 1100]), (256, 12, 12, [300], [300]),
-    (32, 64, 4, [33, 40], [64, 1500]), (128, 16, 16, [1, 250, 3], [129, 380, 3])])
+    (16, 32, 16, [200], [777]), (64, 36, 12, [129, 0, 77], [129, 40, 1100]), (256, 24, 24, [300], [300]),
+    (32, 64, 4, [33, 40], [64, 1500]), (128, 32, 32, [1, 250, 3], [129, 380, 3])])
 def test_attention_of_many_tokens(dtype, dim, page, heads, kv_heads, news, lens):
     rng = np.random.default_rng(page + dim)
     table, pages = tables(rng, lens, page)
@@ -330,11 +330,12 @@ def test_attention_with_more_queries_than_keys_leaves_the_first_empty():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("most", [1, 30])
-def test_attention_where_pages_differ_widely(dtype, most):
+@pytest.mark.parametrize("most,kv_heads", [(1, 2), (30, 2), (30, 40)])  # the last: the kernel of many queries
+def test_attention_where_pages_differ_widely(dtype, most, kv_heads):
     # scales from 2^-60 to 2^60, pages of zeros, and a page of NaN that no query sees
     table, pages = tables(np.random.default_rng(1), [300, 200], 16)
-    c = pool(pages, 16, 2, 128)
+    c = pool(pages, 16, kv_heads, 128)
+    heads = 2 * kv_heads
     g = gen(7)
     c.v_scales.copy_(2.0 ** torch.randint(-60, 61, c.v_scales.shape, device="cuda", generator=g))
     c.k_scales.copy_(2.0 ** torch.randint(-9, -3, c.k_scales.shape, device="cuda", generator=g))
@@ -342,7 +343,7 @@ def test_attention_where_pages_differ_widely(dtype, most):
         p = table[row, 4].item()
         c.k_codes[p], c.v_codes[p], c.k_scales[p], c.v_scales[p] = 0, 0, 0, 0
     starts, lens = [0, most, 2 * most], [300, 200]
-    q = torch.randn(2 * most, 4, 128, device="cuda", generator=g).to(TYPES[dtype])
+    q = torch.randn(2 * most, heads, 128, device="cuda", generator=g).to(TYPES[dtype])
     want, _ = ref.attention(q, starts, lens, table, (c.k_codes, c.v_codes), (c.k_scales, c.v_scales), 0.02)
     got = c.attention(q, ints(starts), ints(lens), table, most, scale=0.02)
     # outputs near 2^60 times a weight: an fp16 type overflows to infinity
@@ -355,27 +356,27 @@ def test_attention_where_pages_differ_widely(dtype, most):
     # a small page alone, with a huge one masked behind it, keeps its own precision
     c.v_scales[table[0, 0]] = 2.0 ** -60
     c.v_scales[table[0, 1]] = 2.0 ** 60
-    one = torch.randn(1, 4, 128, device="cuda", generator=g).to(TYPES[dtype])
+    one = torch.randn(1, heads, 128, device="cuda", generator=g).to(TYPES[dtype])
     check_attention(c, one, [0, 1], [16], table[:1].contiguous(), 1)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("most", [1, 40])
-def test_attention_masks_what_is_not_finite(dtype, most):
+@pytest.mark.parametrize("most,kv_heads", [(1, 2), (40, 2), (40, 40)])
+def test_attention_masks_what_is_not_finite(dtype, most, kv_heads):
     # the page behind the last token is NaN, and so are the codes' scales of pages no table names
     lens = [40, 64]
     table, pages = tables(np.random.default_rng(2), lens, 16, spare=2)
-    c = pool(pages, 16, 2, 64)
+    c = pool(pages, 16, kv_heads, 64)
     unused = [p for p in range(pages) if p not in table.flatten().tolist()]
     c.k_scales[unused[0]] = c.v_scales[unused[0]] = math.nan
     table[0, 3] = unused[0]
-    q = torch.randn(2 * most, 4, 64, device="cuda", generator=gen(8)).to(TYPES[dtype])
+    q = torch.randn(2 * most, 2 * kv_heads, 64, device="cuda", generator=gen(8)).to(TYPES[dtype])
     got = check_attention(c, q, [0, most, 2 * most], lens, table, most)
     assert not got.isnan().any()
     # and a NaN page that queries do see makes theirs NaN, and no earlier query's
     if most > 1:
         p = table[1, 3].item()
-        c.k_scales[p, 0] = c.v_scales[p, 1] = math.nan
+        c.k_scales[p, 0::2] = c.v_scales[p, 1::2] = math.nan
         got = c.attention(q, ints([0, most, 2 * most]), ints(lens), table, most)
         seen = torch.arange(24, 64) >= 48
         assert torch.equal(got[most:].isnan().all(2).all(1).cpu(), seen) and not got[:most].isnan().any()
@@ -393,12 +394,12 @@ def test_attention_strides_scale_and_rows_behind_the_last():
     assert got is out and (out[7:] == 7.0).all()
 
 
-@pytest.mark.parametrize("most", [1, 64])
-def test_attention_marks_lengths_pages_and_rows_that_are_wrong(most):
+@pytest.mark.parametrize("most,kv_heads", [(1, 2), (64, 2), (64, 40)])
+def test_attention_marks_lengths_pages_and_rows_that_are_wrong(most, kv_heads):
     lens = [100, 50]
     table, pages = tables(np.random.default_rng(4), lens, 16, spare=0)
-    c = pool(pages, 16, 2, 64)
-    q = torch.randn(2 * most, 4, 64, device="cuda", generator=gen(10))
+    c = pool(pages, 16, kv_heads, 64)
+    q = torch.randn(2 * most, 2 * kv_heads, 64, device="cuda", generator=gen(10))
     s = [0, most, 2 * most]
 
     def code(starts, lens, table):
@@ -443,15 +444,16 @@ def test_attention_over_a_cache_past_32_bits(dtype):
     assert torch.equal(x[0], small.values()[0][0])
 
 
-@pytest.mark.parametrize("most", [1, 200])
-def test_attention_repeats_bit_for_bit_and_does_not_depend_on_the_batch(most):
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("most,dim", [(1, 128), (20, 128), (200, 64), (200, 128), (200, 256)])
+def test_attention_repeats_bit_for_bit(dtype, most, dim):
     lens = [5000, 300, 1200, 4000]
     table, pages = tables(np.random.default_rng(5), lens, 64)
-    c = pool(pages, 64, 2, 128)
-    q = torch.randn(4 * most, 16, 128, device="cuda", generator=gen(12))
+    c = pool(pages, 64, 2, dim)
+    q = torch.randn(4 * most, 16, dim, device="cuda", generator=gen(12)).to(TYPES[dtype])
     s = ints([most * i for i in range(5)])
     first = c.attention(q, s, ints(lens), table, most)
-    for _ in range(3):
+    for _ in range(30):
         assert torch.equal(c.attention(q, s, ints(lens), table, most), first)
 
 
