@@ -185,7 +185,7 @@ PROTOTYPES = {
     "spm_kv8_attention_workspace": (C.c_int32, [C.POINTER(Kv8), C.c_int32, C.c_int32, C.c_int32, C.c_int32, _U64P]),
     "spm_kv8_attention": (C.c_int32, [C.POINTER(Kv8), C.c_uint32, _P, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _P,
                                       _P, C.c_int32, C.c_int32, _P, C.c_int32, C.c_float, _P, C.c_int64, C.c_int64,
-                                      _P, C.c_uint64, _P]),
+                                      C.c_int32, _P, C.c_uint64, _P]),
     "spm_sample": (C.c_int32, [C.c_int, C.c_uint32, _P, C.c_int64, C.c_int32, C.c_int32, _P, _P, _P, _P, _P, _P, _P,
                                _P, _P]),
 }

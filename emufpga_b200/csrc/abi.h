@@ -4,6 +4,7 @@
 #pragma once
 #include <cuda_runtime_api.h>
 
+#include <atomic>
 #include <exception>
 #include <new>
 #include <string>
@@ -65,7 +66,7 @@ struct DeviceScope {
 
 // The multiprocessors of the current device (asked for once per device).
 inline int device_sms() {
-    static int sms[64] = {};
+    static std::atomic<int> sms[64] = {};
     int d = 0;
     CUDA_OK(cudaGetDevice(&d));
     if (d < 64 && sms[d]) return sms[d];
@@ -78,7 +79,7 @@ inline int device_sms() {
 // Raises a kernel's dynamic shared memory limit on the current device, once
 // per device (`done` is the kernel's own bit per device).
 template <class K>
-void allow_smem(K kernel, size_t bytes, unsigned long long& done) {
+void allow_smem(K kernel, size_t bytes, std::atomic<unsigned long long>& done) {
     int d = 0;
     CUDA_OK(cudaGetDevice(&d));
     if (d < 64 && (done >> d & 1)) return;
@@ -88,7 +89,7 @@ void allow_smem(K kernel, size_t bytes, unsigned long long& done) {
 
 // Likewise for clusters of more than eight CTAs.
 template <class K>
-void allow_wide_clusters(K kernel, unsigned long long& done) {
+void allow_wide_clusters(K kernel, std::atomic<unsigned long long>& done) {
     int d = 0;
     CUDA_OK(cudaGetDevice(&d));
     if (d < 64 && (done >> d & 1)) return;

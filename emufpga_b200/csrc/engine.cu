@@ -816,8 +816,8 @@ void paged_attention(spm_session* s, int l, const LayerIdx& L, int row, int requ
     const int64_t hd = c.head_dim, kvw = hd * c.kv_heads, qw = hd * c.heads;
     inner(spm_kv8_append(&cache, SPM_F32, k, kvw, hd, v, kvw, hd, T, g.slots, s->stream));
     inner(spm_kv8_attention(&cache, SPM_F32, q, qw, hd, int32_t(c.heads), T, g.starts, g.lens, requests, most,
-                            g.table + size_t(row) * g.width, g.width, 1.0f / std::sqrt(float(hd)), out, qw, hd, g.work,
-                            g.work_bytes, s->stream));
+                            g.table + size_t(row) * g.width, g.width, 1.0f / std::sqrt(float(hd)), out, qw, hd, 0,
+                            g.work, g.work_bytes, s->stream));
 }
 
 void enqueue_step(spm_session* s, int n) {

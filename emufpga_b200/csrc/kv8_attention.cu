@@ -106,6 +106,7 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
     __shared__ long long wsum[kDecWarps], found[2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int V = a.requests * a.tiles;  // (request, row tile) pairs
+    kv8_clear<HD>(a, blockIdx.x, gridDim.x);
     pdl_trigger();  // (kv8_combine_kernel's CTAs may come and wait: all of this grid's are resident)
 
     // ---- this CTA's run of units ----
@@ -530,10 +531,11 @@ void launch_decode(const Kv8Args& a, int grid, cudaStream_t st) {
     constexpr int smem = DecSmem<HD, NT, NP>::total;
     static_assert(smem <= 227 * 1024, "a CTA's shared memory");
     static_assert(NT == 2 || kDecPerSm * (smem + 1024) <= 228 * 1024, "the grid is made for this many CTAs on an SM");
-    static unsigned long long done = 0;
+    static std::atomic<unsigned long long> done{0};
     allow_smem(kv8_decode_kernel<HD, NT, NP>, smem, done);
     kv8_decode_kernel<HD, NT, NP><<<grid, kDecThreads, smem, st>>>(a);
     CUDA_OK(cudaGetLastError());
+    if (a.requests == 0 || a.most == 0) return;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(a.requests * a.tiles), unsigned(a.kv_heads), unsigned(std::min(a.tile_rows, a.most * a.group)));
     cfg.blockDim = dim3(HD);
@@ -573,10 +575,10 @@ Plan plan_of(const spm_kv8* c, int heads, int requests, int most, int width) {
     // many queries, but shares its keys out over all SMs: 256 such tiles for each wave of
     // the other's CTAs is where they meet (256 tiles, 1024 to 8000 keys: 137 against 144
     // us, 90 against 86; 336: 70 against 47; 640: 168 against 56; 128: 88 against 143).
-    p.prompt = rows > 16 && small > 256 * ((large + sms - 1) / sms);
+    // (More requests than a grid has in z stay here.)
+    p.prompt = rows > 16 && requests <= 65535 && small > 256 * ((large + sms - 1) / sms);
     if (p.prompt) {
         p.tiles = int((rows + tall - 1) / tall);
-        if (requests > 65535 || p.tiles > INT32_MAX / tall) fail(SPM_E_ARG, "too many requests and queries for one call");
         p.grid = 0;
         p.prefix_bytes = p.parts_bytes = 0;
         return p;
@@ -594,10 +596,10 @@ Plan plan_of(const spm_kv8* c, int heads, int requests, int most, int width) {
 
 void check_attention(const spm_kv8* c, int32_t heads, int32_t requests, int32_t most, int32_t width) {
     kv8_check(c);
-    if (heads < 1 || heads % c->kv_heads) fail(SPM_E_ARG, "heads must be a multiple of kv_heads");
+    if (heads < 1 || heads % c->kv_heads || heads > INT32_MAX / 256) fail(SPM_E_ARG, "heads must be a multiple of kv_heads");
     if (requests < 0 || most < 0 || width < 0) fail(SPM_E_ARG, "negative size");
     if (int64_t(width) * c->page_tokens > INT32_MAX) fail(SPM_E_ARG, "positions are 32-bit: table_width * page_tokens must fit");
-    if (int64_t(most) * (heads / c->kv_heads) > INT32_MAX) fail(SPM_E_ARG, "too many queries");
+    if (int64_t(most) * (heads / c->kv_heads) > INT32_MAX - 1024) fail(SPM_E_ARG, "too many queries");
     if (c->kv_heads > 65535) fail(SPM_E_ARG, "too many kv heads");
 }
 
@@ -619,14 +621,14 @@ spm_status spm_kv8_attention_workspace(const spm_kv8* c, int32_t heads, int32_t 
 spm_status spm_kv8_attention(const spm_kv8* c, uint32_t dtype, const void* q, int64_t q_token, int64_t q_head,
                              int32_t heads, int32_t rows, const int32_t* starts, const int32_t* lens,
                              int32_t requests, int32_t most, const int32_t* table, int32_t table_width, float scale,
-                             void* out, int64_t out_token, int64_t out_head, void* workspace,
-                             uint64_t workspace_bytes, void* cuda_stream) {
+                             void* out, int64_t out_token, int64_t out_head, int32_t clear_rest,
+                             void* workspace, uint64_t workspace_bytes, void* cuda_stream) {
     return guarded([&] {
         check_attention(c, heads, requests, most, table_width);
         kv8_check_type(dtype);
         if (rows < 0) fail(SPM_E_ARG, "negative row count");
-        if (requests == 0 || rows == 0 || most == 0) return;
-        if (!q || !out || !starts || !lens || (table_width && !table)) fail(SPM_E_ARG, "null argument");
+        if (rows == 0 || ((requests == 0 || most == 0) && !clear_rest)) return;
+        if (!q || !out || !starts || (requests && !lens) || (requests && table_width && !table)) fail(SPM_E_ARG, "null argument");
         const Plan p = plan_of(c, heads, requests, most, table_width);
         if ((p.prefix_bytes && !workspace) || workspace_bytes < p.prefix_bytes + p.parts_bytes)
             fail(SPM_E_ARG, "the workspace is smaller than spm_kv8_attention_workspace says");
@@ -646,6 +648,7 @@ spm_status spm_kv8_attention(const spm_kv8* c, uint32_t dtype, const void* q, in
         a.prefix = static_cast<long long*>(workspace);
         a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.prefix_bytes);
         a.status = c->status;
+        a.clear = clear_rest != 0;
         const int64_t size = dtype == SPM_F32 ? 4 : 2;
         a.o_vec = !((reinterpret_cast<uintptr_t>(out) | uintptr_t(out_token * size) | uintptr_t(out_head * size)) & 15);
         const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);

@@ -29,6 +29,7 @@ struct Kv8Args {
     float scale_log2;
     void* out;
     int64_t o_token, o_head;
+    bool clear;                                // rows of out that no request has become zero
     bool o_vec;                                // out and its strides are multiples of 16 bytes
     long long* prefix;                         // [requests * tiles + 1] units before a pair
     float* parts;                              // [CTA][2][tile_rows][head_dim + 4]
@@ -75,6 +76,18 @@ __device__ __forceinline__ void kv8_store(const Kv8Args& a, int64_t i, float y) 
     if (a.dtype == SPM_F32) static_cast<float*>(a.out)[i] = y;
     else if (a.dtype == SPM_F16) static_cast<__half*>(a.out)[i] = __float2half_rn(y);
     else static_cast<__nv_bfloat16*>(a.out)[i] = __float2bfloat16_rn(y);
+}
+
+// Rows of out that no request has, shared out among the grid's `ctas` CTAs.
+template <int HD>
+__device__ __forceinline__ void kv8_clear(const Kv8Args& a, long long cta, long long ctas) {
+    if (!a.clear) return;
+    const int before = min(max(a.starts[0], 0), a.rows), from = min(max(a.starts[a.requests], before), a.rows);
+    const int heads = a.kv_heads * a.group, rest = before + a.rows - from;
+    for (long long e = cta * blockDim.x + threadIdx.x; e < (long long)rest * heads * HD; e += ctas * blockDim.x) {
+        const int row = int(e / (heads * HD)), d = int(e % (heads * HD));
+        kv8_store(a, int64_t(row < before ? row : from + row - before) * a.o_token + d / HD * a.o_head + d % HD, 0.f);
+    }
 }
 
 // Sixteen values of a row, in 16-byte pieces where out's strides allow them.

@@ -178,6 +178,8 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
     const uint32_t qs = (saddr(raw) + 1023u) & ~1023u, ks = qs + S::qbytes, vs = ks + ST * S::tile;
     uint8_t* const base = raw + (qs - saddr(raw));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    kv8_clear<HD>(a, (blockIdx.z * (long long)gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x,
+                  (long long)gridDim.x * gridDim.y * gridDim.z);
     // the last rows see the most keys: they go first
     const int tile = int(gridDim.x) - 1 - int(blockIdx.x), head = blockIdx.y, req = blockIdx.z;
     const int s0 = a.starts[req], e0 = a.starts[req + 1];
@@ -577,7 +579,7 @@ template <int HD, int NP>
 void launch(const Kv8Args& a, cudaStream_t st) {
     constexpr int smem = PromptShape<HD, NP>::smem;
     static_assert(smem + int(sizeof(PromptSync)) <= 227 * 1024, "a CTA's shared memory");
-    static unsigned long long done = 0;
+    static std::atomic<unsigned long long> done{0};
     allow_smem(kv8_prompt_kernel<HD, NP>, smem, done);
     const dim3 grid(unsigned(a.tiles), unsigned(a.kv_heads), unsigned(a.requests));
     kv8_prompt_kernel<HD, NP><<<grid, PromptShape<HD, NP>::threads, smem, st>>>(a);

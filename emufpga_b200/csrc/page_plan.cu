@@ -230,7 +230,7 @@ spm_status spm_page_plan(int device, const int32_t* cached, const int32_t* fresh
         PlanArgs a{cached, fresh, ended, requests, page_tokens, __builtin_ctz(unsigned(page_tokens)), table, table_width,
                    free_pages, pages, free_count, free_left, tokens, starts, lens, positions, slots, status};
         const size_t smem = size_t(4 * requests + 3) * sizeof(int32_t);
-        static unsigned long long done = 0;
+        static std::atomic<unsigned long long> done{0};
         allow_smem(page_plan_kernel, size_t(4 * kPlanRequests + 3) * sizeof(int32_t), done);
         // one CTA up to a few rows and tokens for each of its threads, else a cluster of eight
         const unsigned ctas = requests <= 64 && tokens <= 4 * kPlanThreads ? 1 : 8;

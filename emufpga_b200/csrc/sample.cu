@@ -742,8 +742,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
 
 template <class T, int NT>
 void launch_sample(const SampleArgs& a, int rows, int ctas, size_t smem, cudaStream_t st) {
-    static unsigned long long done = 0;
-    static unsigned long long wide = 0;
+    static std::atomic<unsigned long long> done{0}, wide{0};
     allow_smem(sample_kernel<T, NT>, sizeof(Shared) + kSampleSlice, done);
     if (ctas > 8) allow_wide_clusters(sample_kernel<T, NT>, wide);
     cudaLaunchConfig_t cfg = {};

@@ -212,8 +212,8 @@ class Cache:
 
         Request r's rows starts[r] .. starts[r + 1] (at most ``most``) stand at
         the last of its lens[r] positions, whose pages are table[r].  ``scale``
-        defaults to head_dim ** -0.5.  Rows behind starts[-1] of ``out`` are left
-        as they were (zeros where ``out`` is not given)."""
+        defaults to head_dim ** -0.5.  Rows of ``out`` that no request has are left
+        as they were (zeros where ``out`` is not given); ``out`` may be ``q``."""
         qp, dt = self._rows(q, "q"), _dtype(q, "q")
         T, H, _ = q.shape
         if table.dim() != 2:
@@ -224,16 +224,16 @@ class Cache:
         raw, scratch = _on(self._index, stream)
         need = self._bytes(H, R, most, width)
         with scratch:
-            if out is None:
-                # rows that no request has are zero; a decode tick without padding has none
-                out = (torch.empty if T == R and most == 1 else torch.zeros)(q.shape, dtype=q.dtype, device=self.device)
+            clear = out is None
+            if clear:
+                out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
             elif out.shape != q.shape or out.dtype is not q.dtype:
                 raise SpmError(-1, "out must have q's shape and type")
             work = torch.empty(need, dtype=torch.uint8, device=self.device)
         op = self._rows(out, "out")
         call("spm_kv8_attention", self._ref, dt, qp, q.stride(0), q.stride(1), H, T, *args,
-             head_scale(self.head_dim) if scale is None else scale, op, out.stride(0), out.stride(1), work.data_ptr(),
-             need, raw)
+             head_scale(self.head_dim) if scale is None else scale, op, out.stride(0), out.stride(1), clear,
+             work.data_ptr(), need, raw)
         return out
 
     def check(self) -> None:

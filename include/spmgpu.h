@@ -532,16 +532,17 @@ spm_status spm_kv8_values(const spm_kv8* cache, uint32_t dtype, const int32_t* p
  * none: 0), standing at its last positions: row i of n sees the keys up to position
  * lens[r] - n + i, the cache holding lens[r] tokens in the pages of table row r.
  * heads is a multiple of kv_heads, head h reads kv head h / (heads / kv_heads).
- * A row that sees no key is zero; rows behind starts[requests] are left as they
- * were.  `workspace` is scratch of spm_kv8_attention_workspace bytes (for the same
+ * A row that sees no key is zero; rows that no request has (before starts[0], from
+ * starts[requests] on) are left as they were, or zero where clear_rest is not 0.  out
+ * may be q.  `workspace` is scratch of spm_kv8_attention_workspace bytes (for the same
  * arguments; 16-byte aligned), not shared by calls that may overlap. */
 spm_status spm_kv8_attention_workspace(const spm_kv8* cache, int32_t heads, int32_t requests, int32_t most,
                                        int32_t table_width, uint64_t* bytes);
 spm_status spm_kv8_attention(const spm_kv8* cache, uint32_t dtype, const void* q, int64_t q_token, int64_t q_head,
                              int32_t heads, int32_t rows, const int32_t* starts, const int32_t* lens,
                              int32_t requests, int32_t most, const int32_t* table, int32_t table_width, float scale,
-                             void* out, int64_t out_token, int64_t out_head, void* workspace,
-                             uint64_t workspace_bytes, void* cuda_stream);
+                             void* out, int64_t out_token, int64_t out_head, int32_t clear_rest,
+                             void* workspace, uint64_t workspace_bytes, void* cuda_stream);
 
 /* A pick per row of logits[rows][vocab] (row_stride elements apart).  Tokens in
  * the order (logit descending, index ascending), weights exp((logit - max) /

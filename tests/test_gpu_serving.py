@@ -394,6 +394,46 @@ def test_attention_strides_scale_and_rows_behind_the_last():
     assert got is out and (out[7:] == 7.0).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("news,rows,most,kv_heads", [
+    ([1, 1, 0, 1], 4, 1, 2), ([1, 0, 0, 1], 9, 1, 2), ([0, 0], 3, 1, 2), ([], 5, 1, 2), ([0], 5, 0, 2),
+    ([30, 0, 20], 60, 30, 2), ([30, 0, 20], 60, 30, 40)])
+@pytest.mark.parametrize("before", [0, 2])
+def test_attention_rows_of_no_request(dtype, news, rows, most, kv_heads, before):
+    lens = [40 + 30 * i for i in range(len(news))]
+    table, pages = tables(np.random.default_rng(6), lens or [1], 16)
+    table = table[:len(lens)]
+    c = pool(pages, 16, kv_heads, 64)
+    q = torch.randn(before + rows, 2 * kv_heads, 64, device="cuda", generator=gen(20)).to(TYPES[dtype])
+    starts = np.concatenate([[before], before + np.cumsum(news, dtype=np.int64)]).tolist()
+    rest = torch.ones(before + rows, dtype=torch.bool, device="cuda")
+    rest[before:starts[-1]] = False
+    torch.full((4,) + q.shape, math.nan, dtype=q.dtype, device="cuda")  # what fresh memory may hold
+    got = check_attention(c, q, starts, lens, table, most)
+    assert (got[rest] == 0).all()
+    out = torch.full_like(q, 7.0)
+    c.attention(q, ints(starts), ints(lens), table, most, out=out)
+    assert (out[rest] == 7).all() and torch.equal(out[~rest], got[~rest])
+    same = q.clone()
+    assert c.attention(same, ints(starts), ints(lens), table, most, out=same) is same  # in place
+    assert torch.equal(same[~rest], got[~rest]) and torch.equal(same[rest], q[rest])
+
+
+def test_attention_of_more_requests_than_a_grid_is_deep():
+    R, lens = 65600, [20, 33]
+    table, pages = tables(np.random.default_rng(7), lens, 16)
+    c = pool(pages, 16, 1, 64)
+    q = torch.randn(40, 4, 64, device="cuda", generator=gen(21))
+    wide = torch.full((R, table.shape[1]), -1, dtype=torch.int32, device="cuda")
+    wide[0], wide[-1] = table[0], table[1]
+    starts, all_lens = np.full(R + 1, 20), np.zeros(R, dtype=np.int64)
+    starts[0], starts[-1], all_lens[0], all_lens[-1] = 0, 40, 20, 33
+    got = c.attention(q, ints(starts), ints(all_lens), wide, 20)
+    c.check()
+    want, tol = ref.attention(q, [0, 20, 40], lens, table, (c.k_codes, c.v_codes), (c.k_scales, c.v_scales), 0.125)
+    assert ((got.double() - want).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("most,kv_heads", [(1, 2), (64, 2), (64, 40)])
 def test_attention_marks_lengths_pages_and_rows_that_are_wrong(most, kv_heads):
     lens = [100, 50]

@@ -59,9 +59,9 @@ def test_append_and_values_refused():
 
 
 def attend(c=None, dtype=_lib.F32, q=A, heads=4, rows=2, starts=A, lens=A, requests=2, most=1, table=A, width=3, out=A,
-           work=A, size=1 << 40, code="SPM_E_ARG"):
+           work=A, size=1 << 40, clear=0, code="SPM_E_ARG"):
     refused("spm_kv8_attention", c or cache(), dtype, q, 256, 64, heads, rows, starts, lens, requests, most, table, width,
-            0.125, out, 256, 64, work, size, None, code=code)
+            0.125, out, 256, 64, clear, work, size, None, code=code)
 
 
 def test_attention_refused():
@@ -77,11 +77,15 @@ def test_attention_refused():
     attend(size=16)
     attend(work=A + 8)
     attend(requests=1 << 20, most=1 << 20)
+    attend(most=(1 << 30) - 1)
+    attend(heads=1 << 30, most=1)
+    for name in ("q", "starts", "out", "work"):
+        attend(requests=0, clear=1, **{name: None})
     n = C.c_uint64()
     call("spm_kv8_attention_workspace", cache(), 4, 2, 1, 3, C.byref(n))
     attend(size=n.value - 1)
-    call("spm_kv8_attention", cache(), _lib.F32, None, 256, 64, 4, 0, None, None, 0, 1, None, 3, 0.125, None, 256, 64, None,
-         0, None)  # no requests: nothing to do
+    call("spm_kv8_attention", cache(), _lib.F32, None, 256, 64, 4, 0, None, None, 0, 1, None, 3, 0.125, None, 256, 64, 0,
+         None, 0, None)  # no requests: nothing to do
 
 
 def planned(requests=2, page=16, width=4, pages=8, tokens=8, code="SPM_E_ARG", **kw):
