@@ -104,8 +104,8 @@ struct Row {
         const double t = p * table[n & (kTable - 1)];  // in [1, 2) or a rounding beside it
         // t 2^(n >> 7), at most 2^44, added to 2^52: its integer is the mantissa
         const double w = __hiloint2double(__double2hiint(t) + ((n & ~(kTable - 1)) << 13), __double2loint(t)) + 4503599627370496.0;
-        // (2^-46 down the weight is 0, and its exponent above soon past a double's)
-        const u64 m = x > -INFINITY && distance(x) * bins < 46.f * 22.2f ? __double_as_longlong(w) & 0xfffffffffffffull : 0;
+        // (under 2^-46 the weight is 0, and the exponent above soon past a double's; NaN is not above either)
+        const u64 m = s > -2.0 * kTable ? __double_as_longlong(w) & 0xfffffffffffffull : 0;
         return x == INFINITY ? 1ull << 44 : m;
     }
     __device__ __forceinline__ float distance(float x) const { return fminf(ftop - x, 3.402823466e38f); }
@@ -705,6 +705,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
         // the first token with cumulated mass > target
         u64 target = u > 0.f ? __double2ull_rd(fmin(double(u), 1.0) * double(total)) : 0;
         target = min(target, total - 1);
+        if (lane == 0) s.pick_seg = segs;
+        __syncwarp();
         tb = ties0;
         for (int w = w0; w < w1 && mb <= target; w++) {
             const u64 here = taken(tb, w) * tie_mass + s.seg_mass[w];

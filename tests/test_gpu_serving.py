@@ -561,6 +561,19 @@ def test_sample_rows_that_are_special():
     assert got.token[0] == -1 and got.token[1] == -1 and got.token[7] == 0 and got.token[10] == 0
 
 
+def test_sample_at_the_smallest_temperatures():
+    # gaps a little and far over the temperature, normal and subnormal
+    t = [2.0 ** -100, 2.0 ** -110, 2.0 ** -126, 2.0 ** -140, 2.0 ** -149, 2.0 ** -60]
+    x = torch.zeros(6, 300, device="cuda")
+    for i, v in enumerate(t):
+        x[i, 10:40] = torch.arange(30, device="cuda").double().mul(v).float()
+        x[i, 50] = 25 * v
+        x[i, 60] = -2.0 ** -90
+    rng = np.random.default_rng(8)
+    for k, p in [(0, 1.0), (0, 0.9), (20, 0.9), (45, 1.0)]:
+        check_sample(x, t, [k] * 6, [p] * 6, [0.0] * 6, rng.random(6))
+
+
 def test_sample_settings_at_their_edges():
     n = 9
     x = torch.randn(1, 3001, device="cuda", generator=gen(4)).repeat(n, 1)
