@@ -33,6 +33,7 @@ namespace {
 using namespace dev;
 namespace cg = cooperative_groups;
 
+constexpr int kSampleThreads = 512;       // of a CTA
 constexpr int kBins = 1024;
 constexpr int kSampleClusters = 16;       // CTAs of a row, at most (8: the portable ones, see launch_type)
 constexpr int kList = 2048;               // tokens that are sorted, at most
@@ -64,9 +65,9 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 struct alignas(16) Shared {
     union {
         struct {
-            uint32_t low[kBins], mid[kBins], high[kBins];  // this CTA's: counts in low, or masses in 16 + 16 + the rest
-            u64 total[kBins];                              // the cluster's
-            u64 part[kBins];                      // sums of a share of the bins over some of the CTAs
+            uint32_t low[kBins], high[kBins];  // this CTA's: counts in low, or masses in two words
+            u64 total[kBins];                  // the cluster's
+            u64 part[kBins];                   // sums of a share of the bins over some of the CTAs
         };
         struct {
             u64 list[kList];    // this CTA's border tokens: key, then the index's complement
@@ -75,8 +76,8 @@ struct alignas(16) Shared {
     };
     double table[kTable];                 // 2^(j / kTable)
     u64 scan[32];
-    u64 need_out, seg_mass[kSampleClusters * 32];
-    uint32_t seg_count[kSampleClusters * 32], seg_ties[kSampleClusters * 32];
+    u64 need_out, seg_mass[kSampleClusters * kSampleThreads / 32];
+    uint32_t seg_count[kSampleClusters * kSampleThreads / 32], seg_ties[kSampleClusters * kSampleThreads / 32];
     float top[kSampleClusters];           // each CTA's largest logit
     uint32_t listed;                      // length of this CTA's list
     int bin_out;
@@ -123,7 +124,6 @@ struct Row {
 };
 
 // Inclusive sum over the block's threads on top of `base`; base becomes the total.
-template <int NT>
 __device__ __forceinline__ u64 block_sums(Shared& s, u64 w, u64& base) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -134,7 +134,7 @@ __device__ __forceinline__ u64 block_sums(Shared& s, u64 w, u64& base) {
     __syncthreads();
     if (lane == 31) s.scan[warp] = w;
     __syncthreads();
-    u64 t = lane < NT / 32 ? s.scan[lane] : 0;  // a sum for each warp
+    u64 t = lane < kSampleThreads / 32 ? s.scan[lane] : 0;  // a sum for each warp
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const u64 y = __shfl_up_sync(0xffffffffu, t, o);
@@ -149,9 +149,9 @@ __device__ __forceinline__ u64 block_sums(Shared& s, u64 w, u64& base) {
 // From the cluster's totals, bins in the order FIRST (ascending or descending):
 // the bin in which the running sum reaches `need` (>= 1), and what is needed
 // inside it; -1 where the sum stays below.
-template <int NT, bool DOWN>
+template <bool DOWN>
 __device__ void select_bin(Shared& s, u64 need, int& bin, u64& left, u64& all) {
-    constexpr int PER = kBins / NT;
+    constexpr int PER = kBins / kSampleThreads;
     static_assert(PER >= 1, "a bin for each thread");
     const int tid = threadIdx.x;
     auto at = [&](int i) { return s.total[DOWN ? kBins - 1 - i : i]; };
@@ -159,7 +159,7 @@ __device__ void select_bin(Shared& s, u64 need, int& bin, u64& left, u64& all) {
 #pragma unroll
     for (int j = 0; j < PER; j++) mine += at(tid * PER + j);
     all = 0;
-    u64 before = block_sums<NT>(s, mine, all) - mine;
+    u64 before = block_sums(s, mine, all) - mine;
     if (tid == 0) s.bin_out = -1;
     __syncthreads();
     if (need == 0) return;  // the sum alone is asked for
@@ -182,9 +182,8 @@ __device__ void select_bin(Shared& s, u64 need, int& bin, u64& left, u64& all) {
 // Descending bitonic sort of n <= kList entries, padded with 0: E neighbours to a
 // thread, exchanges among them in registers, up to 32 E apart between lanes, and
 // the rest through shared memory.
-template <int NT>
 __device__ void sort_descending(u64* v, int n) {
-    constexpr int E = kList / NT;
+    constexpr int E = kList / kSampleThreads;
     const int tid = threadIdx.x, i = E * tid;
     int size = 32 * E;
     while (size < n) size *= 2;
@@ -232,9 +231,9 @@ __device__ void sort_descending(u64* v, int n) {
     __syncthreads();
 }
 
-template <class T, int NT>
-__global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs a) {
-    constexpr int W = NT / 32;
+template <class T>
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleArgs a) {
+    constexpr int W = kSampleThreads / 32;
     extern __shared__ __align__(16) uint8_t raw[];
     Shared& s = *reinterpret_cast<Shared*>(raw);
     T* held = reinterpret_cast<T*>(raw + sizeof(Shared));
@@ -256,7 +255,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     };
     // f(four logits, the first's place) over the slice, by whole warps; -inf behind the end
     auto quads = [&](auto&& f) {
-        for (int i0 = 128 * warp; i0 < n; i0 += 4 * NT) {
+        for (int i0 = 128 * warp; i0 < n; i0 += 4 * kSampleThreads) {
             float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             if (i0 + 4 * lane < n) four(i0 + 4 * lane, v);
             f(v, i0 + 4 * lane);
@@ -264,7 +263,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     };
     // f(logit, its place in the slice) for the candidates of this thread
     auto each = [&](auto&& f) {
-        for (int i = 4 * tid; i < n; i += 4 * NT) {
+        for (int i = 4 * tid; i < n; i += 4 * kSampleThreads) {
             float v[4];
             four(i, v);
 #pragma unroll
@@ -288,7 +287,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
         const int whole = (n - head) / V;
         const uint4* wide = reinterpret_cast<const uint4*>(from + head);
 #pragma unroll 4
-        for (int i = tid; i < whole; i += NT) {
+        for (int i = tid; i < whole; i += kSampleThreads) {
             const uint4 q = __ldcs(wide + i);
             const T* e = reinterpret_cast<const T*>(&q);
             if (holds && head == 0) reinterpret_cast<uint4*>(held)[i] = q;
@@ -303,7 +302,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
         if (holds && tid < 4 && n + tid < a.slice) held[n + tid] = from_f32<T>(-INFINITY);  // the last four's places
     }
     if (tid < kTable) s.table[tid] = exp2(double(tid) / kTable);
-    for (int b = tid; b < kBins; b += NT) s.low[b] = s.mid[b] = s.high[b] = 0;
+    for (int b = tid; b < kBins; b += kSampleThreads) s.low[b] = s.high[b] = 0;
     if (tid == 0) s.listed = 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -348,26 +347,28 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     auto keeps = [&](float v) { return !floored || r.below(v) * r.inv <= reach; };
 
     auto clear = [&]() {
-        for (int b = tid; b < kBins; b += NT) s.low[b] = s.mid[b] = s.high[b] = 0;
+        for (int b = tid; b < kBins; b += kSampleThreads) s.low[b] = s.high[b] = 0;
         __syncthreads();
     };
-    auto add_mass = [&](int b, u64 w) {
-        if (w & 0xffffu) atomicAdd(&s.low[b], uint32_t(w & 0xffffu));
-        if (w >> 16 & 0xffffu) atomicAdd(&s.mid[b], uint32_t(w >> 16 & 0xffffu));
-        if (w >> 32) atomicAdd(&s.high[b], uint32_t(w >> 32));
+    // A 64-bit sum of two 32-bit atomics, the second one for a carry or a weight from
+    // 2^-12 on: few.
+    auto add_low = [&](int b, u64 w) { return uint32_t(w) ? atomicAdd(&s.low[b], uint32_t(w)) : 0u; };
+    auto add_high = [&](int b, u64 w, uint32_t old) {
+        const uint32_t up = uint32_t(w >> 32) + (old + uint32_t(w) < old);
+        if (up) atomicAdd(&s.high[b], up);
     };
+    auto add_mass = [&](int b, u64 w) { add_high(b, w, add_low(b, w)); };
     // the CTAs' histograms added into every CTA's total
     auto gather = [&](bool mass) {
         cl.sync();
-        const int share = kBins / C, parts = max(1, min(4, NT / share)), each = (C + parts - 1) / parts;
-        for (int e = tid; e < share * parts; e += NT) {
+        const int share = kBins / C, parts = max(1, min(4, kSampleThreads / share)), each = (C + parts - 1) / parts;
+        for (int e = tid; e < share * parts; e += kSampleThreads) {
             const int b = rank * share + e % share, q = e / share;
             u64 sum = 0;
 #pragma unroll 2
             for (int c = q * each; c < min(C, (q + 1) * each); c++) {
                 sum += cl.map_shared_rank(s.low, c)[b];
-                if (mass)
-                    sum += (u64(cl.map_shared_rank(s.mid, c)[b]) << 16) + (u64(cl.map_shared_rank(s.high, c)[b]) << 32);
+                if (mass) sum += u64(cl.map_shared_rank(s.high, c)[b]) << 32;
             }
             if (parts == 1) {
                 for (int c = 0; c < C; c++) cl.map_shared_rank(s.total, c)[b] = sum;
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
         }
         if (parts > 1) {
             __syncthreads();
-            for (int e = tid; e < share * parts; e += NT) {
+            for (int e = tid; e < share * parts; e += kSampleThreads) {
                 const int i = e % share, q = e / share;
                 u64 sum = 0;
                 for (int g = 0; g < parts; g++) sum += s.part[g * share + i];
@@ -446,7 +447,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
         gather(false);
         int bin = 0;
         u64 left = 0, all = 0;
-        select_bin<NT, false>(s, u64(k), bin, left, all);
+        select_bin<false>(s, u64(k), bin, left, all);
         if (bin >= 0) {
             const u64 upto = k - left + s.total[bin];  // tokens of this bin and those before
             __syncthreads();                           // (the list lies over the totals)
@@ -457,21 +458,21 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
                 int len = rank == 0 ? collect() : 0;
                 cl.sync();  // the others' lists have been read
                 if (rank) return;
-                sort_descending<NT>(s.sorted, len);
+                sort_descending(s.sorted, len);
                 len = min(len, k);
                 // masses of the k first, and their running sum (over the list, which is done with)
                 u64* mass = s.list;
                 u64 total = 0;
-                for (int c0 = 0; c0 < len; c0 += NT) {
+                for (int c0 = 0; c0 < len; c0 += kSampleThreads) {
                     const int i = c0 + tid;
-                    const u64 w = block_sums<NT>(s, i < len ? r.mass(value_of(uint32_t(s.sorted[i] >> 32))) : 0, total);
+                    const u64 w = block_sums(s, i < len ? r.mass(value_of(uint32_t(s.sorted[i] >> 32))) : 0, total);
                     if (i < len) mass[i] = w;
                 }
                 if (tid == 0) s.listed = 0;
                 __syncthreads();
                 const double want = ceil(double(p) * double(total));
                 const u64 need = !nucleus ? total : want < 1.0 ? 1 : min(total, __double2ull_rn(want));
-                for (int i = tid; i < len; i += NT)
+                for (int i = tid; i < len; i += kSampleThreads)
                     if (((i == 0 || mass[i - 1] < need) || !nucleus) && keeps(value_of(uint32_t(s.sorted[i] >> 32))))
                         atomicAdd(&s.listed, 1u);  // a prefix: its length is its count
                 __syncthreads();
@@ -482,13 +483,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
                 target = min(target, total - 1);
                 __syncthreads();
                 // by index: complement first, descending
-                for (int i = tid; i < kept; i += NT) s.sorted[i] = s.sorted[i] << 32 | s.sorted[i] >> 32;
+                for (int i = tid; i < kept; i += kSampleThreads) s.sorted[i] = s.sorted[i] << 32 | s.sorted[i] >> 32;
                 __syncthreads();
-                sort_descending<NT>(s.sorted, kept);
+                sort_descending(s.sorted, kept);
                 u64 run = 0;
-                for (int c0 = 0; c0 < kept; c0 += NT) {
+                for (int c0 = 0; c0 < kept; c0 += kSampleThreads) {
                     const int i = c0 + tid;
-                    const u64 own = i < kept ? r.mass(value_of(uint32_t(s.sorted[i]))) : 0, w = block_sums<NT>(s, own, run);
+                    const u64 own = i < kept ? r.mass(value_of(uint32_t(s.sorted[i]))) : 0, w = block_sums(s, own, run);
                     if (i < kept && w - own <= target && target < w) {
                         a.token[row] = int32_t(0xffffffffu - uint32_t(s.sorted[i] >> 32));
                         if (a.kept) a.kept[row] = kept;
@@ -511,11 +512,17 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
             u64 m[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) m[j] = r.mass(v[j]);
+            uint32_t old[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                if (m[j] >= small) add_mass(r.bin(v[j]), m[j]);
-                else rest += m[j];
+                if (m[j] < small) {
+                    rest += m[j];
+                    m[j] = 0;
+                }
+                old[j] = add_low(r.bin(v[j]), m[j]);
             }
+#pragma unroll
+            for (int j = 0; j < 4; j++) add_high(r.bin(v[j]), m[j], old[j]);
         });
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
@@ -523,10 +530,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
         gather(true);
         int bin = 0, sub = -1, m = 0;
         u64 need = 0, left = 0, sum = 0;
-        select_bin<NT, false>(s, 0, bin, left, sum);
+        select_bin<false>(s, 0, bin, left, sum);
         const double want = ceil(double(p) * double(sum));
         need = want < 1.0 ? 1 : min(sum, __double2ull_rn(want));
-        select_bin<NT, false>(s, need, bin, left, sum);
+        select_bin<false>(s, need, bin, left, sum);
         auto inside = [&](float v) { return r.in_bin(v, bin) && (sub < 0 || r.part(v, bin) == sub); };
         // what lies in the border's bin; in its part of the bin where that is too much
         // to sort soon
@@ -544,18 +551,18 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
                 if (r.in_bin(v, bin)) add_mass(r.part(v, bin), r.mass(v));
             });
             gather(true);
-            select_bin<NT, false>(s, left, sub, left, sum);
+            select_bin<false>(s, left, sub, left, sum);
         }
         if (m <= kList) {
             collect();
             cl.sync();  // every list has been read
-            sort_descending<NT>(s.sorted, m);
+            sort_descending(s.sorted, m);
             // the first whose running sum reaches what is needed inside the bin
             u64 run = 0;
             if (tid == 0) s.bin_out = m - 1;
-            for (int c0 = 0; c0 < m; c0 += NT) {
+            for (int c0 = 0; c0 < m; c0 += kSampleThreads) {
                 const int i = c0 + tid;
-                const u64 own = i < m ? r.mass(value_of(uint32_t(s.sorted[i] >> 32))) : 0, w = block_sums<NT>(s, own, run);
+                const u64 own = i < m ? r.mass(value_of(uint32_t(s.sorted[i] >> 32))) : 0, w = block_sums(s, own, run);
                 if (i < m && w - own < left && left <= w) s.bin_out = i;
             }
             __syncthreads();
@@ -564,7 +571,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
             // its rank among the tokens that equal it (they lie side by side)
             if (tid == 0) s.listed = 0;
             __syncthreads();
-            for (int i = tid; i <= last; i += NT)
+            for (int i = tid; i <= last; i += kSampleThreads)
                 if (uint32_t(s.sorted[i] >> 32) == thr) atomicAdd(&s.listed, 1u);
             __syncthreads();
             ties = s.listed;
@@ -588,7 +595,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
             });
             gather(false);
             int bin;
-            select_bin<NT, true>(s, need, bin, need, all);
+            select_bin<true>(s, need, bin, need, all);
             prefix |= uint32_t(bin) << shift[level];
         }
         thr = prefix;
@@ -610,11 +617,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
                 add_mass(thr >> shift[level] & digits[level], r.mass(value_of(thr)) * ties);
             gather(true);
             if (level == 0) {
-                select_bin<NT, true>(s, 0, bin, need, all);
+                select_bin<true>(s, 0, bin, need, all);
                 const double want = ceil(double(p) * double(all));
                 need = want < 1.0 ? 1 : min(all, __double2ull_rn(want));
             }
-            select_bin<NT, true>(s, need, bin, need, all);
+            select_bin<true>(s, need, bin, need, all);
             prefix |= uint32_t(bin) << shift[level];
         }
         const u64 w = r.mass(value_of(prefix)), m = (need + w - 1) / w;
@@ -726,13 +733,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     const int from = min(n, s.pick_seg % W * seg), to = min(n, from + seg);
     u64 run = 0, seen = s.pick_ties;
     const u64 target = s.pick_before;
-    for (int c0 = from; c0 < to; c0 += NT) {
+    for (int c0 = from; c0 < to; c0 += kSampleThreads) {
         const int i = c0 + tid;
         const float v = i < to ? to_f32(holds ? held[i] : x[i0 + i]) : 0.f;
         const bool tie = i < to && v == cut && cut > -INFINITY;
-        const u64 rank_of = block_sums<NT>(s, tie, seen);  // this one counted
+        const u64 rank_of = block_sums(s, tie, seen);  // this one counted
         const u64 own = tie ? (rank_of <= ties ? tie_mass : 0) : i < to && v > cut ? r.mass(v) : 0;
-        const u64 w = block_sums<NT>(s, own, run);
+        const u64 w = block_sums(s, own, run);
         if (w - own <= target && target < w) {
             a.token[row] = i0 + i;
             if (a.kept) a.kept[row] = int32_t(s.pick_count);
@@ -742,14 +749,14 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     }
 }
 
-template <class T, int NT>
+template <class T>
 void launch_sample(const SampleArgs& a, int rows, int ctas, size_t smem, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0}, wide{0};
-    allow_smem(sample_kernel<T, NT>, sizeof(Shared) + kSampleSlice, done);
-    if (ctas > 8) allow_wide_clusters(sample_kernel<T, NT>, wide);
+    allow_smem(sample_kernel<T>, sizeof(Shared) + kSampleSlice, done);
+    if (ctas > 8) allow_wide_clusters(sample_kernel<T>, wide);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(rows) * unsigned(ctas));
-    cfg.blockDim = dim3(NT);
+    cfg.blockDim = dim3(kSampleThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -758,24 +765,25 @@ void launch_sample(const SampleArgs& a, int rows, int ctas, size_t smem, cudaStr
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    CUDA_OK(cudaLaunchKernelEx(&cfg, sample_kernel<T, NT>, a));
+    CUDA_OK(cudaLaunchKernelEx(&cfg, sample_kernel<T>, a));
 }
 
 template <class T>
 void launch_type(SampleArgs a, int rows, cudaStream_t st) {
-    // A CTA for every 2048 logits, up to 16 (more than 8 is not portable, but fits a
-    // B200's groups of SMs) while every CTA has an SM to itself, else up to 8; then 1024
-    // threads shorten its passes, and beyond one CTA an SM two of 512 hide each other's
-    // barriers.
+    // A CTA for every 2048 logits, up to 8; 16 (not portable, but a B200's groups of SMs
+    // hold them) from 65537 logits on while that leaves an SM to each CTA: 8 rows of
+    // 151936 take 38 us so where clusters of 8 take 44, of 49152 30 and 25, 16 rows 66 and
+    // 48.  (1024 threads instead of 512, one CTA an SM: 32 us instead of 35 for top-p on
+    // one row, 66 instead of 38 on eight.)
     const int sms = device_sms();
     int ctas = 1;
-    while (ctas < kSampleClusters && a.vocab > 2048 * ctas && (ctas < 8 || int64_t(rows) * 2 * ctas <= sms)) ctas *= 2;
+    while (ctas < 8 && a.vocab > 2048 * ctas) ctas *= 2;
+    if (a.vocab > 65536 && int64_t(rows) * kSampleClusters <= sms) ctas = kSampleClusters;
     const int per = 4 * 32;  // four for each warp, of 32 at most
     a.slice = ((a.vocab + ctas - 1) / ctas + per - 1) / per * per;
     const size_t bytes = size_t(a.slice) * sizeof(T);
     const size_t smem = sizeof(Shared) + (bytes <= size_t(kSampleSlice) ? bytes : 0);
-    if (int64_t(rows) * ctas <= sms) launch_sample<T, 1024>(a, rows, ctas, smem, st);
-    else launch_sample<T, 512>(a, rows, ctas, smem, st);
+    launch_sample<T>(a, rows, ctas, smem, st);
 }
 
 }  // namespace
