@@ -9,8 +9,11 @@
 // (half + quarter + ...) away from its values, and a code is the same whatever
 // order sums run in.  It costs less than one of the eight bits.
 //
-// Bound: bytes (rows in, one byte a value out) for prompts; launch latency for
-// a decode tick.
+// Bound: bytes (rows in, one byte a value out) for prompts, and each CTA's chain of
+// slots, rows, scales and codes; launch latency for a decode tick.  Keys and values
+// of 8 x 128 in f32: 8 tokens 5 us, 1024 tokens 8 us (1.3 TB/s), 19 400 bf16 tokens of
+// 4 x 128 in 37 prompts 27 us (60 MB, 2.2 TB/s).  Reading their pages back as bf16
+// takes 18 us (100 MB, 5.6 TB/s).
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -10,7 +10,8 @@
 //
 // What bounds it is latency: a few kilobytes and three dependent phases (push,
 // pop, slots), so it is ONE launch of one cluster whose CTAs each form the sums
-// in their own shared memory and then share out rows and tokens.
+// in their own shared memory and then share out rows and tokens.  8 requests of a
+// decode tick take 6 us (one CTA), 1024 with 96 prompts and 50 000 tokens 15 us (eight).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
