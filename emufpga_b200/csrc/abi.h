@@ -49,10 +49,14 @@ struct DeviceBuf {
 struct DeviceScope {
     int before = -1;
     explicit DeviceScope(int device) {
-        int n = 0;
-        if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
-            cudaGetLastError();
-            fail(SPM_E_NO_DEVICE, "no CUDA device is visible");
+        static std::atomic<int> devices{0};
+        int n = devices;
+        if (n == 0) {
+            if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
+                cudaGetLastError();
+                fail(SPM_E_NO_DEVICE, "no CUDA device is visible");
+            }
+            devices = n;
         }
         if (device < 0 || device >= n) fail(SPM_E_ARG, "device index out of range");
         CUDA_OK(cudaGetDevice(&before));

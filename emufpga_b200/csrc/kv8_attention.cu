@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const Kv8Args a, int g
 }
 
 template <int HD, int NT, int NP>
-void launch_decode(const Kv8Args& a, int grid, cudaStream_t st) {
+void launch_decode(const Kv8Args& a, int grid, bool join, cudaStream_t st) {
     constexpr int smem = DecSmem<HD, NT, NP>::total;
     static_assert(smem <= 227 * 1024, "a CTA's shared memory");
     static_assert(NT == 2 || kDecPerSm * (smem + 1024) <= 228 * 1024, "the grid is made for this many CTAs on an SM");
@@ -538,7 +538,7 @@ void launch_decode(const Kv8Args& a, int grid, cudaStream_t st) {
     allow_smem(kv8_decode_kernel<HD, NT, NP>, smem, done);
     kv8_decode_kernel<HD, NT, NP><<<grid, kDecThreads, smem, st>>>(a);
     CUDA_OK(cudaGetLastError());
-    if (a.requests == 0 || a.most == 0) return;
+    if (!join) return;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(a.requests * a.tiles), unsigned(a.kv_heads), unsigned(std::min(a.tile_rows, a.most * a.group)));
     cfg.blockDim = dim3(HD);
@@ -552,14 +552,15 @@ void launch_decode(const Kv8Args& a, int grid, cudaStream_t st) {
 }
 
 template <int HD>
-void launch_dim(const Kv8Args& a, int nt, bool two, int grid, cudaStream_t st) {
-    if (nt == 1) two ? launch_decode<HD, 1, 2>(a, grid, st) : launch_decode<HD, 1, 1>(a, grid, st);
-    else two ? launch_decode<HD, 2, 2>(a, grid, st) : launch_decode<HD, 2, 1>(a, grid, st);
+void launch_dim(const Kv8Args& a, int nt, bool two, int grid, bool join, cudaStream_t st) {
+    if (nt == 1) two ? launch_decode<HD, 1, 2>(a, grid, join, st) : launch_decode<HD, 1, 1>(a, grid, join, st);
+    else two ? launch_decode<HD, 2, 2>(a, grid, join, st) : launch_decode<HD, 2, 1>(a, grid, join, st);
 }
 
 // How a call is cut, from what the host knows of it.
 struct Plan {
     bool prompt;  // kv8_prompt.cu's kernel
+    bool join;    // a (row tile, kv head) may be cut: kv8_combine_kernel has parts to add
     int nt, tiles, grid;
     uint64_t prefix_bytes, parts_bytes;
 };
@@ -583,6 +584,7 @@ Plan plan_of(const spm_kv8* c, int heads, int requests, int most, int width) {
     if (p.prompt) {
         p.tiles = int((rows + tall - 1) / tall);
         p.grid = 0;
+        p.join = false;
         p.prefix_bytes = p.parts_bytes = 0;
         return p;
     }
@@ -592,8 +594,9 @@ Plan plan_of(const spm_kv8* c, int heads, int requests, int most, int width) {
     const int64_t units = (int64_t(width) * c->page_tokens + unit - 1) / unit;
     if (units * pairs > INT64_MAX / 65536) fail(SPM_E_ARG, "too many requests and queries for one call");
     p.grid = int(std::max<int64_t>(1, std::min<int64_t>(int64_t(per_sm) * sms, std::max<int64_t>(units, 1) * pairs * c->kv_heads)));
+    p.join = units > 1 && pairs > 0 && most > 0;  // (a table of one unit: every run holds whole ones)
     p.prefix_bytes = (uint64_t(pairs + 1) * 8 + 15) & ~uint64_t(15);
-    p.parts_bytes = uint64_t(p.grid) * 2 * 8 * p.nt * (c->head_dim + 4) * 4;
+    p.parts_bytes = !p.join ? 0 : uint64_t(p.grid) * 2 * 8 * p.nt * (c->head_dim + 4) * 4;
     return p;
 }
 
@@ -661,11 +664,11 @@ spm_status spm_kv8_attention(const spm_kv8* c, uint32_t dtype, const void* q, in
         }
         const bool two = dtype == SPM_F32;
         switch (c->head_dim) {
-            case 64: launch_dim<64>(a, p.nt, two, p.grid, st); break;
-            case 96: launch_dim<96>(a, p.nt, two, p.grid, st); break;
-            case 128: launch_dim<128>(a, p.nt, two, p.grid, st); break;
-            case 192: launch_dim<192>(a, p.nt, two, p.grid, st); break;
-            default: launch_dim<256>(a, p.nt, two, p.grid, st); break;
+            case 64: launch_dim<64>(a, p.nt, two, p.grid, p.join, st); break;
+            case 96: launch_dim<96>(a, p.nt, two, p.grid, p.join, st); break;
+            case 128: launch_dim<128>(a, p.nt, two, p.grid, p.join, st); break;
+            case 192: launch_dim<192>(a, p.nt, two, p.grid, p.join, st); break;
+            default: launch_dim<256>(a, p.nt, two, p.grid, p.join, st); break;
         }
     });
 }

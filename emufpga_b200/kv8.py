@@ -29,6 +29,7 @@ STATUS = {11: "a length is negative or past its table", 12: "more pages wanted t
 
 
 _I32 = torch.int32
+_HERE = contextlib.nullcontext()
 # the current stream's handle (torch.cuda.current_stream builds an object around it, 2 us)
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
@@ -59,7 +60,7 @@ def _cuda(t: torch.Tensor, what: str) -> int:
 def _on(index: int, stream):
     """The raw stream to launch on, and a context in which scratch is allocated for it."""
     if stream is None:
-        return _raw_stream(index), contextlib.nullcontext()
+        return _raw_stream(index), _HERE
     return stream.cuda_stream, torch.cuda.stream(stream)
 
 
@@ -103,7 +104,7 @@ def plan(cached, new, table, free, count, page_tokens: int, tokens: int, ended=N
     raw, scratch = _on(index, stream)
     with scratch:
         maps = table.new_empty(2 * R + 1 + 2 * tokens)
-    starts, lens, positions, slots = maps.split((R + 1, R, tokens, tokens))
+    starts, lens, positions, slots = maps.split_with_sizes((R + 1, R, tokens, tokens))
     at = maps.data_ptr()
     call("spm_page_plan", *args, at, at + 4 * (R + 1), at + 4 * (2 * R + 1), at + 4 * (2 * R + 1 + tokens), word, raw)
     return Plan(starts, lens, positions, slots)
@@ -170,6 +171,8 @@ class Cache:
         key = (heads, requests, most, width)
         n = self._work.get(key)
         if n is None:
+            if len(self._work) >= 1024:  # (lengths of a long life)
+                self._work.clear()
             v = C.c_uint64()
             call("spm_kv8_attention_workspace", self._ref, heads, requests, most, width, C.byref(v))
             n = self._work[key] = v.value
@@ -226,11 +229,11 @@ class Cache:
         with scratch:
             clear = out is None
             if clear:
-                out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+                out = q.new_empty(q.shape)
             elif out.shape != q.shape or out.dtype is not q.dtype:
                 raise SpmError(-1, "out must have q's shape and type")
-            work = torch.empty(need, dtype=torch.uint8, device=self.device)
-        op = self._rows(out, "out")
+            work = table.new_empty(need // 4)
+        op = out.data_ptr() if clear else self._rows(out, "out")
         call("spm_kv8_attention", self._ref, dt, qp, q.stride(0), q.stride(1), H, T, *args,
              head_scale(self.head_dim) if scale is None else scale, op, out.stride(0), out.stride(1), clear,
              work.data_ptr(), need, raw)

@@ -65,7 +65,7 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, stre
     dt = _dtype(logits, "logits")
     raw, scratch = _on(index, stream)
     with scratch:
-        token, kept, prob = (u.new_empty(n, dtype=t) for t in (torch.int32, torch.int32, torch.float32))
+        token, kept, prob = u.new_empty(n, dtype=torch.int32), u.new_empty(n, dtype=torch.int32), u.new_empty(n)
     call("spm_sample", index, dt, logits.data_ptr(), logits.stride(0), n, vocab, *args, token.data_ptr(), kept.data_ptr(),
          prob.data_ptr(), raw)
     return Picks(token, kept, prob)
