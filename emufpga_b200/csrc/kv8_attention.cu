@@ -23,9 +23,9 @@
 //   of bytes: the even and odd dimensions of a 16-byte column become rows g and g + 8.
 //
 // What bounds it is the cache's bytes (64 requests of 1000 to 16384 keys, 8 kv heads of
-// 128: 1.16 GB in 212 us, 5.4 TB/s, and 9 us to join the parts), nearly as much the
+// 128: 1.16 GB in 215 us, 5.4 TB/s, and 8 us to join the parts), nearly as much the
 // issue of its products; for a few requests the latency of one unit (8 requests of 1200
-// keys: 12 and 8 us).  Each warp streams its own 32 tokens (16 where
+// keys: 9.5 and 5 us).  Each warp streams its own 32 tokens (16 where
 // head_dim is over 128) at a time through a ring in shared memory (16-byte asynchronous copies, no barrier
 // among warps).  Work is cut into units of four such steps of a (row tile, kv head),
 // and every CTA takes an equal run of the units of all requests, so that ragged
@@ -43,6 +43,9 @@ namespace {
 using namespace dev;
 
 constexpr int kDecThreads = 32 * kDecWarps;
+
+// Units of a CTA's run.
+__device__ __forceinline__ int kv8_share(int total, int ctas) { return (total + ctas - 1) / ctas; }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&a)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -106,25 +109,25 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
     using L = DecSmem<HD, NT, NP>;
     constexpr int NR = 8 * NT, KB = HD / 32, SUB = L::sub, NB = SUB / 16, UNIT = kDecWarps * SUB, PL = L::digits;
     extern __shared__ __align__(128) uint8_t sm[];
-    __shared__ long long wsum[kDecWarps], found[2];
+    __shared__ int wsum[kDecWarps], found[2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int V = a.requests * a.tiles;  // (request, row tile) pairs
     kv8_clear<HD>(a, blockIdx.x, gridDim.x);
     pdl_trigger();  // (kv8_combine_kernel's CTAs may come and wait: all of this grid's are resident)
 
     // ---- this CTA's run of units ----
-    auto block_scan = [&](long long x, long long& before) {  // exclusive sum over threads, and the total
-        long long v = x;
+    auto block_scan = [&](int x, int& before) {  // exclusive sum over threads, and the total
+        int v = x;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long n = __shfl_up_sync(0xffffffffu, v, o);
+            const int n = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += n;
         }
         __syncthreads();
         if (lane == 31) wsum[warp] = v;
         __syncthreads();
         before = v - x;
-        long long total = 0;
+        int total = 0;
 #pragma unroll
         for (int w = 0; w < kDecWarps; w++) {
             if (w < warp) before += wsum[w];
@@ -134,45 +137,44 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
     };
     // (request, row tile) pairs by the thread; one look at the lengths is enough for up
     // to as many pairs as threads
-    auto units_of = [&](int v) { return v < V ? (long long)kv8_units(a, v) * a.kv_heads : 0; };
-    long long total = 0, mine = 0, before = 0;
+    auto units_of = [&](int v) { return v < V ? kv8_units(a, v) * a.kv_heads : 0; };
+    int total = 0, mine = 0, before = 0;
     for (int v0 = 0; v0 < V; v0 += kDecThreads) {
         mine = units_of(v0 + tid);
-        const long long sum = block_scan(mine, before);
+        const int sum = block_scan(mine, before);
         if (blockIdx.x == 0 && v0 + tid < V) a.prefix[v0 + tid] = total + before;
         total += sum;
     }
     if (blockIdx.x == 0 && tid == 0) a.prefix[V] = total;
-    const long long share = (total + gridDim.x - 1) / gridDim.x;
-    const long long begin = min(total, share * (long long)blockIdx.x), end = min(total, begin + share);
+    const int share = kv8_share(total, gridDim.x);
+    const int begin = min(total, share * int(blockIdx.x)), end = min(total, begin + share);
     if (begin >= end) return;
-    for (long long v0 = 0, run = 0; v0 < V && run <= begin; v0 += kDecThreads) {
-        long long sum = total;
+    for (int v0 = 0, run = 0; v0 < V && run <= begin; v0 += kDecThreads) {
+        int sum = total;
         if (V > kDecThreads) {
-            mine = units_of(int(v0) + tid);
+            mine = units_of(v0 + tid);
             sum = block_scan(mine, before);
         }
         if (run + before <= begin && begin < run + before + mine) found[0] = v0 + tid, found[1] = run + before;
         run += sum;
     }
     __syncthreads();
-    int v = int(found[0]);
-    long long base = found[1], u = begin;  // base: the first unit of pair v
+    int v = found[0], base = found[1], u = begin;  // base: the first unit of pair v
 
     const int lrow = (lane & 7) + 8 * ((lane >> 3) & 1), lchunk = lane >> 4;  // this lane's ldmatrix row
     uint8_t* ring = sm + L::ring + warp * kDecStages * L::stage;
     float* qscale = reinterpret_cast<float*>(sm + L::qscale);
     for (int piece = 0; u < end; piece++) {
         int nu = kv8_units(a, v);
-        while (u >= base + (long long)nu * a.kv_heads) {
-            base += (long long)nu * a.kv_heads;
+        while (u >= base + nu * a.kv_heads) {
+            base += nu * a.kv_heads;
             v++;
             nu = kv8_units(a, v);
         }
         const int req = v / a.tiles, tile = v % a.tiles;
-        const int head = int((u - base) / nu), unit0 = int((u - base) % nu);
-        const int units = int(min((long long)(nu - unit0), end - u));
-        const int s0 = a.starts[req], nq = a.starts[req + 1] - s0, len = kv8_len(a, req);
+        const int head = (u - base) / nu, unit0 = (u - base) - head * nu;
+        const int units = min(nu - unit0, end - u);
+        const int s0 = a.starts[req], nq = a.starts[req + 1] - s0, len = kv8_len(a, a.lens[req]);
         const int row0 = tile * NR, rows = min(NR, nq * a.group - row0);
         const int keys = kv8_keys(a, nq, len, tile);
         const int k0 = unit0 * UNIT, k1 = min(keys, (unit0 + units) * UNIT);
@@ -216,6 +218,16 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
             }
             cp_async_commit();
         };
+        // this warp's queries, on their way with the first page numbers
+        constexpr int QR = NR / kDecWarps;
+        float x[QR][HD / 32];
+#pragma unroll
+        for (int y = 0; y < QR; y++) {
+            const int r = warp + kDecWarps * y, qr = row0 + r, qi = qr / a.group, qh = head * a.group + qr % a.group;
+#pragma unroll
+            for (int i = 0; i < HD / 32; i++)
+                x[y][i] = r < rows ? kv8_load(a, int64_t(s0 + qi) * a.q_token + qh * a.q_head + lane + 32 * i) : 0.f;
+        }
         int ahead = page_of(0);
 #pragma unroll
         for (int j = 0; j < kDecStages - 1; j++) {
@@ -225,15 +237,12 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
         }
 
         // ---- the queries in fixed point, as B operands ----
-        for (int r = warp; r < NR; r += kDecWarps) {
-            float x[HD / 32];
-            uint32_t big = 0;
-            const int qr = row0 + r, qi = qr / a.group, qh = head * a.group + qr % a.group;
 #pragma unroll
-            for (int i = 0; i < HD / 32; i++) {
-                x[i] = r < rows ? kv8_load(a, int64_t(s0 + qi) * a.q_token + qh * a.q_head + lane + 32 * i) : 0.f;
-                big = max(big, __float_as_uint(x[i]) & 0x7fffffffu);
-            }
+        for (int y = 0; y < QR; y++) {
+            const int r = warp + kDecWarps * y;
+            uint32_t big = 0;
+#pragma unroll
+            for (int i = 0; i < HD / 32; i++) big = max(big, __float_as_uint(x[y][i]) & 0x7fffffffu);
             big = __reduce_max_sync(0xffffffffu, big);
             // the largest to 2^21 .. 2^22 (2^13 .. 2^14), or as far up as a power of two reaches
             const int up = min((PL == 3 ? 21 : 13) + 127 - int(big >> 23), 126);
@@ -243,7 +252,7 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
 #pragma unroll
             for (int i = 0; i < HD / 32; i++) {
                 // dimension 32 i + lane: half, then group t of four within it
-                int v = __float2int_rn(__fmul_rn(x[i], mul));
+                int v = __float2int_rn(__fmul_rn(x[y][i], mul));
                 const int at = (i * 32 + (r & 7) * 4 + ((lane >> 2) & 3)) * 8 + ((lane >> 4) << 2) + (lane & 3);
 #pragma unroll
                 for (int p = 0; p < PL; p++) {
@@ -446,8 +455,8 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
         const bool whole = units == nu;
         // the run's first piece may be a pair's tail or middle, its last one a pair's head
         float* part = a.parts + size_t(2 * blockIdx.x + (piece ? 1 : 0)) * NR * (HD + 4);
-        for (int e = tid; e < rows * HD; e += kDecThreads) {
-            const int r = e / HD, d = e % HD;
+        for (int e = tid; e < rows * (HD / 4); e += kDecThreads) {
+            const int r = e / (HD / 4), d = e % (HD / 4) * 4;
             const float* st = reinterpret_cast<const float*>(sm + L::ring) + r * L::state;
             float m = -INFINITY, ref = -INFINITY;
 #pragma unroll
@@ -455,23 +464,24 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
                 m = fmaxf(m, st[x * NR * L::state + HD]);
                 ref = fmaxf(ref, st[x * NR * L::state + HD + 1]);
             }
-            float sum = 0.f, acc = 0.f;
+            float sum = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int x = 0; x < kDecWarps; x++) {
                 const float* sx = st + x * NR * L::state;
                 sum = fmaf(sx[HD + 2], kv8_step(sx[HD], m), sum);
-                acc = fmaf(sx[d], kv8_step(sx[HD + 1], ref), acc);
+                const float down = kv8_step(sx[HD + 1], ref);
+                const float4 y = *reinterpret_cast<const float4*>(sx + d);
+                acc = make_float4(fmaf(y.x, down, acc.x), fmaf(y.y, down, acc.y), fmaf(y.z, down, acc.z), fmaf(y.w, down, acc.w));
             }
             if (whole) {
                 const int qr = row0 + r, qi = qr / a.group, qh = head * a.group + qr % a.group;
-                kv8_store(a, int64_t(s0 + qi) * a.o_token + qh * a.o_head + d, kv8_finish(acc, ref, sum, m));
+                kv8_store4(a, int64_t(s0 + qi) * a.o_token + qh * a.o_head + d,
+                           make_float4(kv8_finish(acc.x, ref, sum, m), kv8_finish(acc.y, ref, sum, m),
+                                       kv8_finish(acc.z, ref, sum, m), kv8_finish(acc.w, ref, sum, m)));
             } else {
-                part[r * (HD + 4) + d] = acc;
-                if (d == 0) {
-                    part[r * (HD + 4) + HD] = m;
-                    part[r * (HD + 4) + HD + 1] = ref;
-                    part[r * (HD + 4) + HD + 2] = sum;
-                }
+                *reinterpret_cast<float4*>(part + r * (HD + 4) + d) = acc;
+                if (d == 0) *reinterpret_cast<float4*>(part + r * (HD + 4) + HD) = make_float4(m, ref, sum, 0.f);
             }
         }
     }
@@ -479,52 +489,59 @@ __global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a
 
 // Adds the parts of every (row tile, kv head) that the runs cut, in the order of
 // the runs: the part of run c is its second where the pair begins in it after
-// another, else its first.  One CTA of head_dim threads for each row.
-constexpr int kJoin = 64;  // parts whose factors are held at a time
-
+// another, else its first.  One CTA of head_dim threads for each row; every warp
+// forms the parts' factors for itself, a part to a lane, so that nothing waits but
+// for the parts themselves.
 __global__ void __launch_bounds__(256) kv8_combine_kernel(const Kv8Args a, int grid, int hd) {
-    __shared__ float mul[kJoin], worst[2][8];
-    pdl_wait();
     const int v = blockIdx.x, head = blockIdx.y, r = blockIdx.z, V = a.requests * a.tiles, NR = a.tile_rows;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, W = hd + 4;
-    const long long p0 = a.prefix[v], p1 = a.prefix[v + 1], total = a.prefix[V];
-    const int nu = int((p1 - p0) / a.kv_heads);
-    if (nu == 0) return;
-    const long long share = (total + grid - 1) / grid, u0 = p0 + (long long)head * nu, u1 = u0 + nu;
-    const int c0 = int(u0 / share), c1 = int((u1 - 1) / share);
+    const int tid = threadIdx.x, lane = tid & 31, W = hd + 4;
+    const int req = v / a.tiles, row = (v - req * a.tiles) * NR + r, s0 = a.starts[req], nq = a.starts[req + 1] - s0;
+    pdl_wait();
+    const int p0 = a.prefix[v], p1 = a.prefix[v + 1], total = a.prefix[V];
+    const int nu = (p1 - p0) / a.kv_heads;
+    if (nu == 0 || row >= nq * a.group) return;
+    const int share = kv8_share(total, grid), u0 = p0 + head * nu, u1 = u0 + nu;
+    const int c0 = u0 / share, c1 = (u1 - 1) / share;
     if (c0 == c1) return;  // one run held all of it and wrote the result
-    const int req = v / a.tiles, s0 = a.starts[req], nq = a.starts[req + 1] - s0, row = (v % a.tiles) * NR + r;
-    if (row >= nq * a.group) return;
     auto part = [&](int c) { return a.parts + (size_t(2 * c + (u0 > share * c ? 1 : 0)) * NR + r) * W; };
-    float m = -INFINITY, ref = -INFINITY;
-    for (int c = c0 + tid; c <= c1; c += hd) {
-        m = fmaxf(m, part(c)[hd]);
-        ref = fmaxf(ref, part(c)[hd + 1]);
+    // (m, reference, sum) of a part
+    auto state = [&](int c) { return c <= c1 ? *reinterpret_cast<const float4*>(part(c) + hd) : make_float4(-INFINITY, -INFINITY, 0.f, 0.f); };
+    constexpr int U = 8;  // parts on their way at a time
+    float x[U];
+    auto fetch = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < U; i++) x[i] = c + i <= c1 ? part(c + i)[tid] : 0.f;
+    };
+    const float4 first = state(c0 + lane);
+    fetch(c0);
+    float m = first.x, ref = first.y;
+    for (int c = c0 + 32; c <= c1; c += 32) {
+        const float4 s = state(c + lane);
+        m = fmaxf(m, s.x);
+        ref = fmaxf(ref, s.y);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
     }
-    if (lane == 0) worst[0][warp] = m, worst[1][warp] = ref;
-    __syncthreads();
-    for (int w = 0; w < hd / 32; w++) {
-        m = fmaxf(m, worst[0][w]);
-        ref = fmaxf(ref, worst[1][w]);
-    }
     float sum = 0.f, acc = 0.f;
-    for (int b = c0; b <= c1; b += kJoin) {
-        const int n = min(kJoin, c1 + 1 - b);
-        __syncthreads();
-        for (int c = tid; c < n; c += hd) mul[c] = kv8_step(part(b + c)[hd + 1], ref);
-        __syncthreads();
-#pragma unroll 4
-        for (int c = 0; c < n; c++) {
-            const float* p = part(b + c);
-            sum = fmaf(p[hd + 2], kv8_step(p[hd], m), sum);
-            acc = fmaf(p[tid], mul[c], acc);
+    for (int b = c0; b <= c1; b += 32) {
+        const float4 s = b == c0 ? first : state(b + lane);
+        sum = fmaf(s.z, kv8_step(s.x, m), sum);
+        const float mul = kv8_step(s.y, ref);
+        const int n = min(32, c1 + 1 - b);
+        for (int c = 0; c < n; c += U) {
+            float y[U];
+#pragma unroll
+            for (int i = 0; i < U; i++) y[i] = x[i];
+            fetch(b + c + U);
+#pragma unroll
+            for (int i = 0; i < U; i++) acc = fmaf(y[i], __shfl_sync(0xffffffffu, mul, c + i), acc);
         }
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const int qi = row / a.group, qh = head * a.group + row % a.group;
     kv8_store(a, int64_t(s0 + qi) * a.o_token + qh * a.o_head + tid, kv8_finish(acc, ref, sum, m));
 }
@@ -592,10 +609,11 @@ Plan plan_of(const spm_kv8* c, int heads, int requests, int most, int width) {
     if (pairs > INT32_MAX) fail(SPM_E_ARG, "too many requests and queries for one call");
     const int per_sm = kDecPerSm, unit = kDecWarps * kv8_sub(c->head_dim);
     const int64_t units = (int64_t(width) * c->page_tokens + unit - 1) / unit;
-    if (units * pairs > INT64_MAX / 65536) fail(SPM_E_ARG, "too many requests and queries for one call");
+    if (std::max<int64_t>(units, 1) * c->kv_heads > (INT32_MAX - 65536) / std::max<int64_t>(pairs, 1))  // (counted in 32 bits)
+        fail(SPM_E_ARG, "too many requests, queries and tokens for one call");
     p.grid = int(std::max<int64_t>(1, std::min<int64_t>(int64_t(per_sm) * sms, std::max<int64_t>(units, 1) * pairs * c->kv_heads)));
     p.join = units > 1 && pairs > 0 && most > 0;  // (a table of one unit: every run holds whole ones)
-    p.prefix_bytes = (uint64_t(pairs + 1) * 8 + 15) & ~uint64_t(15);
+    p.prefix_bytes = (uint64_t(pairs + 1) * 4 + 15) & ~uint64_t(15);
     p.parts_bytes = !p.join ? 0 : uint64_t(p.grid) * 2 * 8 * p.nt * (c->head_dim + 4) * 4;
     return p;
 }
@@ -651,7 +669,7 @@ spm_status spm_kv8_attention(const spm_kv8* c, uint32_t dtype, const void* q, in
         a.unit = kDecWarps * kv8_sub(c->head_dim);
         a.scale_log2 = float(double(scale) * 1.4426950408889634);
         a.out = out, a.o_token = out_token, a.o_head = out_head;
-        a.prefix = static_cast<long long*>(workspace);
+        a.prefix = static_cast<int32_t*>(workspace);
         a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.prefix_bytes);
         a.status = c->status;
         a.clear = clear_rest != 0;

@@ -31,7 +31,7 @@ struct Kv8Args {
     int64_t o_token, o_head;
     bool clear;                                // rows of out that no request has become zero
     bool o_vec;                                // out and its strides are multiples of 16 bytes
-    long long* prefix;                         // [requests * tiles + 1] units before a pair
+    int32_t* prefix;                           // [requests * tiles + 1] units before a pair
     float* parts;                              // [CTA][2][tile_rows][head_dim + 4]
     int32_t* status;
 };
@@ -42,8 +42,8 @@ void launch_kv8_prompt(const Kv8Args& a, int head_dim, cudaStream_t st);
 namespace dev {
 
 // A request's cached tokens, within its table row.
-__device__ __forceinline__ int kv8_len(const Kv8Args& a, int req) {
-    const int len = a.lens[req], cap = a.width << a.shift;
+__device__ __forceinline__ int kv8_len(const Kv8Args& a, int len) {
+    const int cap = a.width << a.shift;
     if (len < 0 || len > cap) flag(a.status, SPM_PAGE_LENGTH);
     return min(max(len, 0), cap);
 }
@@ -58,13 +58,13 @@ __device__ __forceinline__ int kv8_keys(const Kv8Args& a, int nq, int len, int t
 // has rows; 0 for requests whose rows are not what the call says.
 __device__ __forceinline__ int kv8_units(const Kv8Args& a, int v) {
     const int req = v / a.tiles, tile = v % a.tiles;
-    const int s = a.starts[req], e = a.starts[req + 1];
+    const int s = a.starts[req], e = a.starts[req + 1], len = a.lens[req];  // (loaded together)
     if (s < 0 || e < s || e > a.rows || e - s > a.most) {
         flag(a.status, SPM_PAGE_QUERIES);
         return 0;
     }
     if ((long long)tile * a.tile_rows >= (long long)(e - s) * a.group) return 0;
-    return max(1, (kv8_keys(a, e - s, kv8_len(a, req), tile) + a.unit - 1) / a.unit);
+    return max(1, (kv8_keys(a, e - s, kv8_len(a, len), tile) + a.unit - 1) / a.unit);
 }
 
 __device__ __forceinline__ float kv8_load(const Kv8Args& a, int64_t i) {
@@ -87,6 +87,26 @@ __device__ __forceinline__ void kv8_clear(const Kv8Args& a, long long cta, long 
     for (long long e = cta * blockDim.x + threadIdx.x; e < (long long)rest * heads * HD; e += ctas * blockDim.x) {
         const int row = int(e / (heads * HD)), d = int(e % (heads * HD));
         kv8_store(a, int64_t(row < before ? row : from + row - before) * a.o_token + d / HD * a.o_head + d % HD, 0.f);
+    }
+}
+
+// Four values of a row, in one piece where out's strides allow it.
+__device__ __forceinline__ void kv8_store4(const Kv8Args& a, int64_t i, float4 v) {
+    if (!a.o_vec) {
+        kv8_store(a, i, v.x);
+        kv8_store(a, i + 1, v.y);
+        kv8_store(a, i + 2, v.z);
+        kv8_store(a, i + 3, v.w);
+    } else if (a.dtype == SPM_F32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + i) = v;
+    } else if (a.dtype == SPM_F16) {
+        __half2* o = reinterpret_cast<__half2*>(static_cast<__half*>(a.out) + i);
+        o[0] = __floats2half2_rn(v.x, v.y);
+        o[1] = __floats2half2_rn(v.z, v.w);
+    } else {
+        __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.out) + i);
+        o[0] = __floats2bfloat162_rn(v.x, v.y);
+        o[1] = __floats2bfloat162_rn(v.z, v.w);
     }
 }
 

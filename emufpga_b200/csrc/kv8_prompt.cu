@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
         if (tid == 0) flag(a.status, SPM_PAGE_QUERIES);
         return;
     }
-    const int nq = e0 - s0, len = kv8_len(a, req), row0 = tile * G * kRows, rows = min(G * kRows, nq * a.group - row0);
+    const int nq = e0 - s0, len = kv8_len(a, a.lens[req]), row0 = tile * G * kRows, rows = min(G * kRows, nq * a.group - row0);
     const int groups = (rows + kRows - 1) / kRows;  // that have rows
     if (rows <= 0) return;
     const int keys = kv8_keys(a, nq, len, tile), tiles = (keys + TN - 1) / TN;

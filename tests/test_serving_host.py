@@ -74,7 +74,7 @@ def test_attention_refused():
     attend(requests=-1)
     attend(most=-1)
     attend(width=1 << 28)
-    attend(size=16)
+    attend(size=15)
     attend(work=A + 8)
     attend(requests=1 << 20, most=1 << 20)
     attend(most=(1 << 30) - 1)
