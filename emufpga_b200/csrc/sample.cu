@@ -39,6 +39,7 @@ constexpr int kSampleThreads = 512;       // of a CTA
 constexpr int kBins = 1024;
 constexpr int kSampleClusters = 16;       // CTAs of a row, at most (8: the portable ones, see launch_type)
 constexpr int kList = 2048;               // tokens that are sorted, at most
+constexpr int kOwn = 1024;                // of a CTA's slice
 constexpr int kSampleSlice = 160 * 1024;  // bytes of a slice that shared memory holds
 constexpr int kTable = 128;               // of the exponential
 typedef unsigned long long u64;
@@ -72,13 +73,13 @@ struct alignas(16) Shared {
             u64 part[kBins];                   // sums of a share of the bins over some of the CTAs
         };
         struct {
-            u64 list[kList];    // this CTA's border tokens: key, then the index's complement
+            u64 list[kOwn];     // this CTA's border tokens: key, then the index's complement
             u64 sorted[kList];  // the cluster's
         };
     };
     double table[kTable];                 // 2^(j / kTable)
     u64 scan[32];
-    u64 need_out, seg_mass[kSampleClusters * kSampleThreads / 32];
+    u64 need_out, border, seg_mass[kSampleClusters * kSampleThreads / 32];
     uint32_t seg_count[kSampleClusters * kSampleThreads / 32], seg_ties[kSampleClusters * kSampleThreads / 32];
     float top[kSampleClusters];           // each CTA's largest logit
     uint32_t listed;                      // length of this CTA's list
@@ -391,10 +392,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         }
         cl.sync();
     };
-    // the lengths of the cluster's lists together, which may be past what they hold
+    // the lengths of the cluster's lists together; past kList where one is not whole
     auto listed = [&]() {
         const int m = lane < C ? int(*cl.map_shared_rank(&s.listed, lane)) : 0;
-        return int(__reduce_add_sync(0xffffffffu, uint32_t(m)));
+        const int sum = int(__reduce_add_sync(0xffffffffu, uint32_t(m)));
+        return __any_sync(0xffffffffu, m > kOwn) ? max(sum, kList + 1) : sum;
     };
     // the lists, whole, in this CTA's `sorted`, its warps sharing out the CTAs; their length
     auto collect = [&]() {
@@ -435,7 +437,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
 #pragma unroll
             for (int j = 0; j < 4; j++)
                 if (take >> j & 1) {
-                    if (at < kList) s.list[at] = u64(key_of(v[j])) << 32 | (0xffffffffu - uint32_t(i0 + i + j));
+                    if (at < kOwn) s.list[at] = u64(key_of(v[j])) << 32 | (0xffffffffu - uint32_t(i0 + i + j));
                     at++;
                 }
         });
@@ -453,33 +455,37 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         if (bin >= 0) {
             const u64 upto = k - left + s.total[bin];  // tokens of this bin and those before
             __syncthreads();                           // (the list lies over the totals)
-            if (upto <= u64(kList)) {
-                // all of them sorted: the borders, and the pick among them, in the first CTA
+            bool whole = upto <= u64(kList);
+            if (whole) {
                 list([&](float v) { return r.place(v) < float(bin + 1); });
                 cl.sync();
+                whole = listed() <= kList;
+                if (!whole) cl.sync();  // the lists' lengths have been read
+            }
+            if (whole) {
+                // all of them sorted: the borders, and the pick among them, in the first CTA
                 int len = rank == 0 ? collect() : 0;
                 cl.sync();  // the others' lists have been read
                 if (rank) return;
                 sort_descending(s.sorted, len);
                 len = min(len, k);
-                // masses of the k first, and their running sum (over the list, which is done with)
-                u64* mass = s.list;
+                auto mass_at = [&](int i) { return i < len ? r.mass(value_of(uint32_t(s.sorted[i] >> 32))) : 0; };
                 u64 total = 0;
-                for (int c0 = 0; c0 < len; c0 += kSampleThreads) {
-                    const int i = c0 + tid;
-                    const u64 w = block_sums(s, i < len ? r.mass(value_of(uint32_t(s.sorted[i] >> 32))) : 0, total);
-                    if (i < len) mass[i] = w;
-                }
-                if (tid == 0) s.listed = 0;
-                __syncthreads();
+                for (int c0 = 0; c0 < len; c0 += kSampleThreads) block_sums(s, mass_at(c0 + tid), total);
                 const double want = ceil(double(p) * double(total));
                 const u64 need = !nucleus ? total : want < 1.0 ? 1 : min(total, __double2ull_rn(want));
-                for (int i = tid; i < len; i += kSampleThreads)
-                    if (((i == 0 || mass[i - 1] < need) || !nucleus) && keeps(value_of(uint32_t(s.sorted[i] >> 32))))
-                        atomicAdd(&s.listed, 1u);  // a prefix: its length is its count
+                // a prefix, the first one among it: its length is its count
+                int kept = 0;
+                u64 before = 0;
+                for (int c0 = 0; c0 < len && kept == c0; c0 += kSampleThreads) {
+                    const int i = c0 + tid;
+                    const u64 own = mass_at(i), w = block_sums(s, own, before);
+                    const bool in = i < len && (!nucleus || w - own < need) && keeps(value_of(uint32_t(s.sorted[i] >> 32)));
+                    kept += __syncthreads_count(in);
+                    if (i == kept - 1) s.need_out = w;
+                }
                 __syncthreads();
-                const int kept = max(1, int(s.listed));
-                total = mass[kept - 1];
+                total = s.need_out;
                 const float u = a.u[row];
                 u64 target = u > 0.f ? __double2ull_rd(fmin(double(u), 1.0) * double(total)) : 0;
                 target = min(target, total - 1);
@@ -538,14 +544,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         select_bin<false>(s, need, bin, left, sum);
         auto inside = [&](float v) { return r.in_bin(v, bin) && (sub < 0 || r.part(v, bin) == sub); };
         // what lies in the border's bin; in its part of the bin where that is too much
-        // to sort soon
-        constexpr int kSoon = 512;
         while (true) {
             __syncthreads();  // (the list lies over the totals)
             list(inside);
             cl.sync();
             m = listed();
-            if (m <= (sub < 0 ? kSoon : kList) || sub >= 0) break;
+            if (m <= kList || sub >= 0) break;
             cl.sync();  // the lists' lengths have been read
             if (tid == 0) s.listed = 0;
             clear();
@@ -556,27 +560,32 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
             select_bin<false>(s, left, sub, left, sum);
         }
         if (m <= kList) {
-            collect();
-            cl.sync();  // every list has been read
-            sort_descending(s.sorted, m);
-            // the first whose running sum reaches what is needed inside the bin
-            u64 run = 0;
-            if (tid == 0) s.bin_out = m - 1;
-            for (int c0 = 0; c0 < m; c0 += kSampleThreads) {
-                const int i = c0 + tid;
-                const u64 own = i < m ? r.mass(value_of(uint32_t(s.sorted[i] >> 32))) : 0, w = block_sums(s, own, run);
-                if (i < m && w - own < left && left <= w) s.bin_out = i;
+            // the first CTA sorts and tells the others (their SMs' other rows have the slots)
+            if (rank == 0) {
+                collect();
+                sort_descending(s.sorted, m);
+                // the first whose running sum reaches what is needed inside the bin
+                u64 run = 0;
+                if (tid == 0) s.bin_out = m - 1;
+                for (int c0 = 0; c0 < m; c0 += kSampleThreads) {
+                    const int i = c0 + tid;
+                    const u64 own = i < m ? r.mass(value_of(uint32_t(s.sorted[i] >> 32))) : 0, w = block_sums(s, own, run);
+                    if (i < m && w - own < left && left <= w) s.bin_out = i;
+                }
+                __syncthreads();
+                const int last = max(0, s.bin_out);
+                thr = uint32_t(s.sorted[last] >> 32);
+                // its rank among the tokens that equal it (they lie side by side)
+                if (tid == 0) s.listed = 0;
+                __syncthreads();
+                for (int i = tid; i <= last; i += kSampleThreads)
+                    if (uint32_t(s.sorted[i] >> 32) == thr) atomicAdd(&s.listed, 1u);
+                __syncthreads();
+                if (tid < C) *cl.map_shared_rank(&s.border, tid) = u64(thr) << 32 | s.listed;
             }
-            __syncthreads();
-            const int last = max(0, s.bin_out);
-            thr = uint32_t(s.sorted[last] >> 32);
-            // its rank among the tokens that equal it (they lie side by side)
-            if (tid == 0) s.listed = 0;
-            __syncthreads();
-            for (int i = tid; i <= last; i += kSampleThreads)
-                if (uint32_t(s.sorted[i] >> 32) == thr) atomicAdd(&s.listed, 1u);
-            __syncthreads();
-            ties = s.listed;
+            cl.sync();
+            thr = uint32_t(s.border >> 32);
+            ties = uint32_t(s.border);
         } else {
             cl.sync();  // the lists' lengths have been read
             radix_p = true;
@@ -657,24 +666,34 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     const u64 tie_mass = r.mass(cut);
     u64 mass = 0;
     uint32_t count = 0, tied = 0;
-    for (int i = j0 + 4 * lane; i < j1; i += 128) {
-        float v[4];
-        four(i, v);
-        bool some = false;
+    // what is kept queues up (where the lists were), so that weights are formed 32 at a time
+    float* queue = reinterpret_cast<float*>(s.list) + 64 * warp;
+    int waiting = 0;
+    for (int b = j0; b < j1; b += 128) {
+        const int i = b + 4 * lane;
+        float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (i < j1) four(i, v);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const bool in = i + j < j1;
+            const bool in = i + j < j1, up = in && v[j] > cut;
             tied += in && v[j] == cut;
-            v[j] = in && v[j] > cut ? v[j] : -INFINITY;
-            count += v[j] > -INFINITY;
-            some |= v[j] > -INFINITY;
+            const uint32_t m = __ballot_sync(0xffffffffu, up);
+            if (up) queue[waiting + __popc(m & ((1u << lane) - 1))] = v[j];
+            waiting += __popc(m);
+            count += __popc(m);
+            if (waiting >= 32) {
+                __syncwarp();
+                waiting -= 32;
+                mass += r.mass(queue[waiting + lane]);
+                __syncwarp();
+            }
         }
-        if (some) mass += r.mass(v[0]) + r.mass(v[1]) + r.mass(v[2]) + r.mass(v[3]);
     }
+    __syncwarp();
+    if (lane < waiting) mass += r.mass(queue[lane]);
     if (cut == -INFINITY) tied = 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
-    count = __reduce_add_sync(0xffffffffu, count);
     tied = __reduce_add_sync(0xffffffffu, tied);
     if (lane < C) {
         const int to = rank * W + warp;
@@ -772,19 +791,32 @@ void launch_sample(const SampleArgs& a, int rows, int ctas, size_t smem, cudaStr
 
 template <class T>
 void launch_type(SampleArgs a, int rows, cudaStream_t st) {
-    // A CTA for every 2048 logits, up to 8; 16 (not portable, but a B200's groups of SMs
-    // hold them) from 65537 logits on while that leaves an SM to each CTA: 8 rows of
-    // 151936 take 38 us so where clusters of 8 take 44, of 49152 30 and 25, 16 rows 66 and
-    // 48.  (1024 threads instead of 512, one CTA an SM: 32 us instead of 35 for top-p on
-    // one row, 66 instead of 38 on eight.)
+    // A row's chain of passes and barriers takes as long as 32768 logits of one CTA (20 of
+    // 28 us for one row of 151936 on 16 CTAs), and CTAs beyond two an SM (one, where the
+    // slices are long) come in waves: the number of CTAs with the least waves x (chain +
+    // slice), 2048 logits each at least.  16 (not portable, but a B200's groups of SMs hold
+    // them) from 65537 logits on while that leaves an SM to each: 8 rows of 151936 take 38 us
+    // so where clusters of 8 take 44, of 49152 30 and 25, 16 rows 66 and 48.  (1024 threads
+    // instead of 512, one CTA an SM: 32 us instead of 35 for top-p on one row, 66 instead of
+    // 38 on eight.)
     const int sms = device_sms();
-    int ctas = 1;
-    while (ctas < 8 && a.vocab > 2048 * ctas) ctas *= 2;
-    if (a.vocab > 65536 && int64_t(rows) * kSampleClusters <= sms) ctas = kSampleClusters;
     const int per = 4 * 32;  // four for each warp, of 32 at most
-    a.slice = ((a.vocab + ctas - 1) / ctas + per - 1) / per * per;
-    const size_t bytes = size_t(a.slice) * sizeof(T);
-    const size_t smem = sizeof(Shared) + (bytes <= size_t(kSampleSlice) ? bytes : 0);
+    auto slice_of = [&](int ctas) { return ((a.vocab + ctas - 1) / ctas + per - 1) / per * per; };
+    auto smem_of = [&](int ctas) {
+        const size_t bytes = size_t(slice_of(ctas)) * sizeof(T);
+        return sizeof(Shared) + (bytes <= size_t(kSampleSlice) ? bytes : 0);
+    };
+    int ctas = 1;
+    int64_t least = INT64_MAX;
+    for (int c = 1; c <= 8 && (c == 1 || a.vocab > 1024 * c); c *= 2) {
+        const int64_t at_once = int64_t(sms) * (2 * (smem_of(c) + 1024) <= size_t(228 * 1024) ? 2 : 1);
+        const bool held = size_t(slice_of(c)) * sizeof(T) <= size_t(kSampleSlice);  // else read again at half the rate
+        const int64_t cost = (int64_t(rows) * c + at_once - 1) / at_once * (32768 + (held ? 1 : 2) * int64_t(slice_of(c)));
+        if (cost <= least) least = cost, ctas = c;
+    }
+    if (a.vocab > 65536 && int64_t(rows) * kSampleClusters <= sms) ctas = kSampleClusters;
+    a.slice = slice_of(ctas);
+    const size_t smem = smem_of(ctas);
     launch_sample<T>(a, rows, ctas, smem, st);
 }
 

@@ -561,6 +561,19 @@ def test_sample_rows_that_are_special():
     assert got.token[0] == -1 and got.token[1] == -1 and got.token[7] == 0 and got.token[10] == 0
 
 
+@pytest.mark.parametrize("vocab", [2000, 5000, 70000])
+@pytest.mark.parametrize("spread", [3.0, 1e-3])
+def test_sample_of_long_lists(vocab, spread):
+    # borders with 1000 to 2000 tokens before or beside them, in one CTA's slice or several
+    n = 8
+    x = torch.randn(n, vocab, device="cuda", generator=gen(22)) * spread
+    x[:, 300:] -= torch.tensor([0.0, 0.0, 0.0, 0.0, 30.0, 30.0, 30.0, 30.0], device="cuda")[:, None]
+    x[4:, 300:1700] += 30.0 - spread
+    rng = np.random.default_rng(9)
+    for k, p in [(0, 0.5), (0, 0.97), (1100, 1.0), (1500, 0.8), (1999, 0.99), (600, 0.999)]:
+        check_sample(x, np.linspace(0.5, 1.5, n), [k] * n, [p] * n, np.where(np.arange(n) % 3 == 0, 0.01, 0.0), rng.random(n))
+
+
 def test_sample_at_the_smallest_temperatures():
     # gaps a little and far over the temperature, normal and subnormal
     t = [2.0 ** -100, 2.0 ** -110, 2.0 ** -126, 2.0 ** -140, 2.0 ** -149, 2.0 ** -60]
