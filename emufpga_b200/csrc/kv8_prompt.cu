@@ -19,9 +19,9 @@
 // for one group, which has two buffers of S instead.  (Two buffers of 64 keys for
 // two groups too: 176 us where one of 128 takes 141, 32 heads of 128, 1024 queries over
 // 4096 keys; a product of 64 columns takes the tensor cores as long as one of 128.)
-// The references move only where a row's maximum passes them by more than 2^8, so
+// The references move only where a row's maximum passes them by more than 2^14, so
 // that the accumulator is hardly ever read back to be rescaled: weights are then at
-// most 2^8, which fp16 holds as exactly as those below 1.
+// most 2^14, which fp16 holds as exactly as those below 1.
 // f32 queries and weights are two fp16 parts (22 bits), twice the products.
 //
 // What bounds it is the softmax: the 16384 exponentials of a 128 x 128 tile take
@@ -42,7 +42,7 @@ using namespace dev;
 
 constexpr int kRows = 128;                             // of a group: the MMA's M
 constexpr int kFillWarps = 8, kFillThreads = 32 * kFillWarps;
-constexpr float kSlack = 8.f;                          // in powers of two
+constexpr float kSlack = 14.f;                         // in powers of two
 
 template <int HD, int NP>
 struct PromptShape {
