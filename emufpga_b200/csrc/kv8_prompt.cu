@@ -4,7 +4,7 @@
 //
 // A CTA owns G groups of 128 rows (query x head of the group) of a request and kv
 // head and walks the keys in tiles of TN, once:
-//   producers (8 warps)  codes from global memory to fp16 (exact) in shared
+//   producers            codes from global memory to fp16 (exact) in shared
 //                        memory: a token's row of 64 dimensions is 128 bytes in the
 //                        128-byte swizzled layout, which is K-major for the keys
 //                        (S = Q K^T) and MN-major for the values (O = P V), so both
@@ -12,12 +12,13 @@
 //   MMA (1 thread)       per group: O += P(j) V(j) with P from TMEM, then, once that
 //                        is done (products of other accumulators do not order each
 //                        other), the next S = Q K^T over the P just read
-//   softmax (4 warps a group)  a thread owns a row: S from TMEM, scale, mask, the
-//                        running references, weights in fp16 back to where S stood
+//   softmax (8 warps a group)  two threads own a row, half of a tile's keys each: S
+//                        from TMEM, scale, mask, the running references, weights in
+//                        fp16 back to where S stood
 // With two groups the products of one run under the softmax of the other, and both
 // share the conversion of the codes.  head_dim over 128 leaves TMEM and shared memory
 // for one group, which has two buffers of S instead.  (Two buffers of 64 keys for
-// two groups too: 176 us where one of 128 takes 141, 32 heads of 128, 1024 queries over
+// two groups too: 176 us where one of 128 took 135, 32 heads of 128, 1024 queries over
 // 4096 keys; a product of 64 columns takes the tensor cores as long as one of 128.)
 // The references move only where a row's maximum passes them by more than 2^14, so
 // that the accumulator is hardly ever read back to be rescaled: weights are then at
@@ -26,7 +27,8 @@
 //
 // What bounds it is the softmax: the 16384 exponentials of a 128 x 128 tile take
 // 1024 cycles of the special function unit, as long as its products, and its other
-// instructions as many again: 141 us for the case above is 426 TFLOP/s.
+// instructions as many again: 123 us for the case above, 488 TFLOP/s.  (One thread a
+// row, 128 columns: 136 us; S read once for maximum and weights: 144.)
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -41,13 +43,14 @@ namespace {
 using namespace dev;
 
 constexpr int kRows = 128;                             // of a group: the MMA's M
-constexpr int kFillWarps = 8, kFillThreads = 32 * kFillWarps;
 constexpr float kSlack = 14.f;                         // in powers of two
 
 template <int HD, int NP>
 struct PromptShape {
     static constexpr int G = kv8_prompt_rows(HD) / kRows;
-    static constexpr int threads = 32 * (4 * G + kFillWarps + 1);
+    // converting warps: as many as leave the softmax its registers (80 of 24 warps, 96 of 20)
+    static constexpr int fill = G == 2 ? 7 : 11;
+    static constexpr int threads = 32 * (8 * G + fill + 1);
     static constexpr int TN = HD <= 128 ? 128 : 64;    // keys of a tile
     static constexpr int BUF = G == 1 ? 2 : 1;         // buffers of S
     static constexpr int atoms = (HD + 63) / 64;       // 64 dimensions, 128 bytes
@@ -66,10 +69,11 @@ struct PromptShape {
 };
 
 struct PromptSync {
-    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2][2], p_ready[2][2], o_done[2], o_last[2], drained;
+    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2][2], p_ready[2][2], o_done[2], o_last[2], met[2], drained;
     uint32_t tmem;
     volatile int gave_up;
     float qscale[2 * kRows];
+    float reach[2][2][2 * kRows], state[2][2][2 * kRows];  // of a row's halves (state: m, sum)
     // scales of K and exponents of V's for a tile's blocks of 16 keys; tile j's are
     // overwritten with j + 8's, for which P(j) V(j) has to be done (four stages)
     float ks[8][8], ve[8][8], vn[8][8];  // (vn: NaN for a scale that is, else 0)
@@ -173,7 +177,7 @@ typedef std::false_type No;
 template <int HD, int NP>
 __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_kernel(const Kv8Args a) {
     using S = PromptShape<HD, NP>;
-    constexpr int TN = S::TN, ST = S::stages, G = S::G, BUF = S::BUF, kSoftWarps = 4 * G;
+    constexpr int TN = S::TN, ST = S::stages, G = S::G, BUF = S::BUF, FT = 32 * S::fill, kSoftWarps = 8 * G;
     extern __shared__ __align__(1024) uint8_t raw[];
     __shared__ PromptSync y;
     const uint32_t qs = (saddr(raw) + 1023u) & ~1023u, ks = qs + S::qbytes, vs = ks + ST * S::tile;
@@ -194,16 +198,17 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
     const int keys = kv8_keys(a, nq, len, tile), tiles = (keys + TN - 1) / TN;
     if (tid == 0) {
         for (int i = 0; i < 4; i++) {
-            mbar_init(&y.k_full[i], kFillThreads);
+            mbar_init(&y.k_full[i], FT);
             mbar_init(&y.k_empty[i], 1);
-            mbar_init(&y.v_full[i], kFillThreads);
+            mbar_init(&y.v_full[i], FT);
             mbar_init(&y.v_empty[i], 1);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&y.s_full[0][i], 1);
             mbar_init(&y.s_full[1][i], 1);
-            mbar_init(&y.p_ready[0][i], kRows);
-            mbar_init(&y.p_ready[1][i], kRows);
+            mbar_init(&y.p_ready[0][i], 2 * kRows);
+            mbar_init(&y.p_ready[1][i], 2 * kRows);
+            mbar_init(&y.met[i], 2 * kRows);
             mbar_init(&y.o_done[i], 1);
             mbar_init(&y.o_last[i], 1);
         }
@@ -211,52 +216,14 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
         y.gave_up = 0;
         mbar_fence_init();
     }
-    constexpr int kMmaWarp = kSoftWarps + kFillWarps;
-    if (warp == kMmaWarp) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&y.tmem)), "r"(512));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    } else {
-        // ---- Q: rows scaled to 2^10 by a power of two, in fp16 parts; four rows' loads together ----
-        constexpr int AT_ONCE = 4, STEP = kSoftWarps + kFillWarps;
-        for (int r0 = warp; r0 < groups * kRows; r0 += AT_ONCE * STEP) {
-            float x[AT_ONCE][HD / 32];
-#pragma unroll
-            for (int u = 0; u < AT_ONCE; u++) {
-                const int r = r0 + u * STEP, qr = row0 + r, qi = qr / a.group, qh = head * a.group + qr % a.group;
-#pragma unroll
-                for (int i = 0; i < HD / 32; i++)
-                    x[u][i] = r < rows ? kv8_load(a, int64_t(s0 + qi) * a.q_token + qh * a.q_head + lane + 32 * i) : 0.f;
-            }
-#pragma unroll
-            for (int u = 0; u < AT_ONCE; u++) {
-                const int r = r0 + u * STEP;
-                if (r >= groups * kRows) break;
-                uint32_t big = 0;
-#pragma unroll
-                for (int i = 0; i < HD / 32; i++) big = max(big, __float_as_uint(x[u][i]) & 0x7fffffffu);
-                big = __reduce_max_sync(0xffffffffu, big);
-                const int up = min(137 - int(big >> 23), 126);
-                // (a negative scale is the queries' sign: the largest sum is then the largest score)
-                const float mul = a.scale_log2 < 0.f ? -pow2i(up) : pow2i(up);
-                if (lane == 0) y.qscale[r] = big < 0x7f800000u ? fabsf(a.scale_log2) * pow2i(-up) : __int_as_float(0x7fffffff);
-#pragma unroll
-                for (int i = 0; i < HD / 32; i++) {
-                    const int d = lane + 32 * i;
-                    const float v = big < 0x7f800000u ? __fmul_rn(x[u][i], mul) : 0.f;
-                    const __half hi = __float2half_rn(v);
-                    const uint32_t at = uint32_t(r / kRows) * (NP * S::qgroup) + uint32_t(d >> 6) * (kRows * 128) +
-                                        sw128_offset(r % kRows, (d & 63) >> 3) + 2 * (d & 7);
-                    *reinterpret_cast<__half*>(base + at) = hi;
-                    if (NP == 2) *reinterpret_cast<__half*>(base + S::qgroup + at) = __float2half_rn(__fsub_rn(v, __half2float(hi)));
-                }
-            }
-        }
-    }
-    fence_proxy_async();
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = y.tmem;
+    constexpr int kMmaWarp = kSoftWarps + S::fill;
+    // Each role does what it can before the first products, then all meet.
+    auto together = [&] {
+        fence_proxy_async();
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+    };
     auto wait = [&](uint64_t* bar, uint32_t parity) {  // false once any wait of the CTA has given up
         if (y.gave_up) return false;
         if (mbar_wait(bar, parity)) return true;
@@ -269,8 +236,8 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
         // ---- producers: codes of tile j converted while those of j + 1 and the page
         // numbers of j + 2 are on their way ----
         // 16-byte pieces of a token, and of a thread (head_dim 96: the last ones of half the threads)
-        constexpr int SEG = HD / 16, PIECES = TN * SEG, N = (PIECES + kFillThreads - 1) / kFillThreads;
-        constexpr bool ragged = PIECES % kFillThreads != 0;
+        constexpr int SEG = HD / 16, PIECES = TN * SEG, N = (PIECES + FT - 1) / FT;
+        constexpr bool ragged = PIECES % FT != 0;
         const int t = tid - 32 * kSoftWarps;
         const int32_t* trow = a.table + size_t(req) * a.width;
         uint4 k[N], v[N];
@@ -278,8 +245,8 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
         auto find = [&](int j) {
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int tok = j * TN + (t + i * kFillThreads) / SEG;
-                page[i] = tok < keys && (!ragged || t + i * kFillThreads < PIECES) ? __ldg(trow + (tok >> a.shift)) : -1;
+                const int tok = j * TN + (t + i * FT) / SEG;
+                page[i] = tok < keys && (!ragged || t + i * FT < PIECES) ? __ldg(trow + (tok >> a.shift)) : -1;
             }
         };
         // -1 for none, and for a page that is not in the pool
@@ -293,7 +260,7 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
         auto load = [&](const int8_t* codes, int j, uint4 (&c)[N]) {
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int e = t + i * kFillThreads, r = e / SEG, o = e % SEG, tok = j * TN + r, p = ragged && e >= PIECES ? -1 : known(page[i], tok);
+                const int e = t + i * FT, r = e / SEG, o = e % SEG, tok = j * TN + r, p = ragged && e >= PIECES ? -1 : known(page[i], tok);
                 c[i] = make_uint4(0, 0, 0, 0);
                 if (p >= 0)
                     c[i] = __ldg(reinterpret_cast<const uint4*>(
@@ -303,7 +270,7 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
         auto store = [&](uint8_t* to, const uint4 (&c)[N]) {
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int e = t + i * kFillThreads, r = e / SEG, o = e % SEG;
+                const int e = t + i * FT, r = e / SEG, o = e % SEG;
                 if (ragged && e >= PIECES) break;
                 uint32_t h[8];
                 const uint32_t w[4] = {c[i].x ^ 0x80808080u, c[i].y ^ 0x80808080u, c[i].z ^ 0x80808080u, c[i].w ^ 0x80808080u};
@@ -336,6 +303,7 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
             scales(0);
             find(1);
         }
+        together();
         for (int j = 0; j < tiles; j++) {
             const int st = j % ST;
             const uint32_t again = uint32_t(j / ST - 1) & 1u;
@@ -360,6 +328,10 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
             find(j + 2);
         }
     } else if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&y.tmem)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        together();
+        const uint32_t tmem = y.tmem;
         if (lane == 0) {
             constexpr uint32_t f32_out = 1u << 4, m = uint32_t(kRows >> 4) << 24;
             constexpr uint32_t id_s = f32_out | m | uint32_t(TN >> 3) << 17;
@@ -416,14 +388,52 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
         }
         __syncwarp();
     } else {
-        // ---- softmax: thread = row = TMEM lane of its group ----
-        const int g = warp >> 2, r = tid;
+        // ---- Q: rows scaled to 2^10 by a power of two, in fp16 parts; four rows' loads together, while the first keys and values come ----
+        constexpr int AT_ONCE = 4, STEP = kSoftWarps;
+        for (int r0 = warp; r0 < groups * kRows; r0 += AT_ONCE * STEP) {
+            float x[AT_ONCE][HD / 32];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++) {
+                const int r = r0 + u * STEP, qr = row0 + r, qi = qr / a.group, qh = head * a.group + qr % a.group;
+#pragma unroll
+                for (int i = 0; i < HD / 32; i++)
+                    x[u][i] = r < rows ? kv8_load(a, int64_t(s0 + qi) * a.q_token + qh * a.q_head + lane + 32 * i) : 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++) {
+                const int r = r0 + u * STEP;
+                if (r >= groups * kRows) break;
+                uint32_t big = 0;
+#pragma unroll
+                for (int i = 0; i < HD / 32; i++) big = max(big, __float_as_uint(x[u][i]) & 0x7fffffffu);
+                big = __reduce_max_sync(0xffffffffu, big);
+                const int up = min(137 - int(big >> 23), 126);
+                // (a negative scale is the queries' sign: the largest sum is then the largest score)
+                const float mul = a.scale_log2 < 0.f ? -pow2i(up) : pow2i(up);
+                if (lane == 0) y.qscale[r] = big < 0x7f800000u ? fabsf(a.scale_log2) * pow2i(-up) : __int_as_float(0x7fffffff);
+#pragma unroll
+                for (int i = 0; i < HD / 32; i++) {
+                    const int d = lane + 32 * i;
+                    const float v = big < 0x7f800000u ? __fmul_rn(x[u][i], mul) : 0.f;
+                    const __half hi = __float2half_rn(v);
+                    const uint32_t at = uint32_t(r / kRows) * (NP * S::qgroup) + uint32_t(d >> 6) * (kRows * 128) +
+                                        sw128_offset(r % kRows, (d & 63) >> 3) + 2 * (d & 7);
+                    *reinterpret_cast<__half*>(base + at) = hi;
+                    if (NP == 2) *reinterpret_cast<__half*>(base + S::qgroup + at) = __float2half_rn(__fsub_rn(v, __half2float(hi)));
+                }
+            }
+        }
+        together();
+        const uint32_t tmem = y.tmem;
+        // ---- softmax: two threads to a row, TMEM lane of its group, half of a tile's columns each ----
+        const int g = warp >> 3, half = warp >> 2 & 1, r = g * kRows + 32 * (warp & 3) + lane;
         const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
         const uint32_t s0col = tmem + lanes + S::s_col + uint32_t(BUF * g) * TN, o = tmem + lanes + S::o_col + uint32_t(g) * HD;
+        constexpr int HC = TN / 64;  // of the 32 columns at a time
         const float qscale = y.qscale[r];
         const int limit = r < rows ? len - nq + (row0 + r) / a.group + 1 : 0;  // keys that the row sees
+        // m and the sum are this half's, the accumulator's reference is the row's
         float m = -INFINITY, ref = -INFINITY, sum = 0.f, m0 = 0.f;  // m0: m, 0 for none yet
-        int lift = -20000;                                        // m0 - ref
         bool ok = true;
         const int turns = g < groups ? tiles : 0;
         for (int j = 0; j < turns; j++) {
@@ -437,17 +447,17 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
             const int t0 = j * TN;
             const bool hidden = __any_sync(0xffffffffu, t0 + TN > limit);
             // f(columns 32 c .. of S, c).  (Fetching the next columns meanwhile costs 32
-            // registers more than 17 warps leave a thread, and more in spills than it saves.)
+            // registers more than there are, and more in spills than it saves.)
             auto columns = [&](auto&& f) {
 #pragma unroll 1
-                for (int c = 0; c < TN / 32; c++) {
+                for (int c = HC * half; c < HC * half + HC; c++) {
                     uint32_t v[32];
                     tmem_ld32(s + 32 * c, v);
                     tmem_ld_wait(v);
                     f(v, c);
                 }
             };
-            // the row's maximum, and the largest exponent that a weighted value can have
+            // the half's maximum, and the largest exponent that a weighted value can have
             float top = -INFINITY, reach = -INFINITY;
             auto maxima = [&](auto masked) {
                 columns([&](const uint32_t (&v)[32], int c) {
@@ -469,18 +479,24 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
                 });
             };
             hidden ? maxima(Yes()) : maxima(No());
-            // the references move seldom (see above), a warp's rows together
-            const bool moves = top > m + kSlack || reach > ref + kSlack || (m == -INFINITY && top > m) ||
-                               (ref == -INFINITY && reach > ref);
+            // both halves' (two buffers: who writes the next one has read this one's before)
+            y.reach[j & 1][half][r] = reach;
+            mbar_arrive(&y.met[g]);
+            if (top > m + kSlack || (m == -INFINITY && top > m)) {
+                sum *= kv8_step(m, top);
+                m = m0 = top;
+            }
+            ok = wait(&y.met[g], uint32_t(j) & 1u);
+            if (!__all_sync(0xffffffffu, ok)) {
+                ok = false;
+                break;
+            }
+            reach = fmaxf(reach, y.reach[j & 1][half ^ 1][r]);
+            // the reference moves seldom (see above), a warp's rows together
+            const bool moves = reach > ref + kSlack || (ref == -INFINITY && reach > ref);
             if (__any_sync(0xffffffffu, moves)) {
-                const float m_new = top > m + kSlack || m == -INFINITY ? top : m;
-                const float r_new = reach > ref + kSlack || ref == -INFINITY ? reach : ref;
-                sum *= kv8_step(m, m_new);
-                const float down = r_new != ref ? kv8_step(ref, r_new) : 1.f;
-                m = m_new;
-                ref = r_new;
-                m0 = m == -INFINITY ? 0.f : m;
-                lift = ref == -INFINITY ? -20000 : int(fminf(fmaxf(m0 - ref, -5000.f), 5000.f));
+                const float down = moves ? kv8_step(ref, reach) : 1.f;
+                if (moves) ref = reach;
                 if (j) {
                     // O is the products' until P(j - 1) V(j - 1) is done (the one before
                     // is, S(j) waited for it: the parity is that of one phase alone)
@@ -491,7 +507,7 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
                     }
                     tc_fence_after();
 #pragma unroll 1
-                    for (int d = 0; d < HD; d += 16) {
+                    for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d += 16) {
                         float x[16];
                         tmem_ld16(o + d, x);
 #pragma unroll
@@ -500,6 +516,7 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
                     }
                 }
             }
+            const int lift = ref == -INFINITY ? -20000 : int(fminf(fmaxf(m0 - ref, -5000.f), 5000.f));
             const uint64_t minus = pair_of(-m0, -m0);
             uint64_t sums[2] = {0, 0};
             auto weights = [&](auto masked) {
@@ -546,13 +563,23 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
             mbar_arrive(&y.p_ready[g][j % BUF]);
         }
         // (a barrier of its own: o_done may be two phases behind here, and its parity says nothing)
-        if (ok && turns) ok = wait(&y.o_last[g], 0);
+        if (ok && turns) {
+            y.state[0][half][r] = m;
+            y.state[1][half][r] = sum;
+            mbar_arrive(&y.met[g]);
+            ok = wait(&y.o_last[g], 0) && wait(&y.met[g], uint32_t(turns) & 1u);
+        }
         tc_fence_after();
         if (__all_sync(0xffffffffu, ok) && g < groups) {
+            if (turns) {  // (in the order of the halves for both)
+                const float ma = y.state[0][0][r], mb = y.state[0][1][r];
+                m = fmaxf(ma, mb);
+                sum = y.state[1][0][r] * kv8_step(ma, m) + y.state[1][1][r] * kv8_step(mb, m);
+            }
             const int qr = row0 + r, qi = qr / a.group, qh = head * a.group + qr % a.group;
             const int64_t at = int64_t(s0 + qi) * a.o_token + qh * a.o_head;
 #pragma unroll 1
-            for (int d = 0; d < HD; d += 16) {
+            for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d += 16) {
                 float v[16];
                 if (tiles) {
                     tmem_ld16(o + d, v);
@@ -572,7 +599,7 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
     __syncthreads();
     if (warp == kMmaWarp) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(y.tmem), "r"(512));
     }
 }
 
