@@ -275,6 +275,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         }
     };
     cg::cluster_group::arrival_token started = cl.barrier_arrive();
+    // the row's settings, on their way with its logits
+    const float temp = a.temperature ? a.temperature[row] : 1.f, want_p = a.top_p ? a.top_p[row] : 1.f,
+                want_min = a.min_p ? a.min_p[row] : 0.f, u = a.u[row];
+    const int want_k = a.top_k ? a.top_k[row] : 0;
 
     // ---- the slice into shared memory; the largest logit (NaN is none) ----
     float top = -INFINITY;
@@ -329,7 +333,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         }
         return;
     }
-    const float temp = a.temperature ? a.temperature[row] : 1.f;
     const bool greedy = !(temp > 0.f);
     Row r;
     r.ftop = top;
@@ -338,12 +341,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     r.slope = r.inv * -1.4426950408889634074 * kTable;
     r.bins = r.ftop == INFINITY ? 1e30f : fminf(float(32.0 * r.inv), 1e30f);
     r.table = s.table;
-    int k = greedy ? 0 : a.top_k ? a.top_k[row] : 0;
+    int k = greedy ? 0 : want_k;
     if (k <= 0 || k >= a.vocab) k = 0;
     if (greedy) k = 1;
-    const float p = !greedy && a.top_p ? a.top_p[row] : 1.f;
+    const float p = greedy ? 1.f : want_p;
     const bool nucleus = p < 1.f;
-    const float least = !greedy && a.min_p ? a.min_p[row] : 0.f;
+    const float least = greedy ? 0.f : want_min;
     // weight >= min_p as a distance from the top; off (NaN too) at 0, 1 at most
     const bool floored = least > 0.f;
     const double reach = floored ? -log(fmin(double(least), 1.0)) : 0.0;
@@ -368,7 +371,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         for (int e = tid; e < share * parts; e += kSampleThreads) {
             const int b = rank * share + e % share, q = e / share;
             u64 sum = 0;
-#pragma unroll 2
+#pragma unroll 4
             for (int c = q * each; c < min(C, (q + 1) * each); c++) {
                 sum += cl.map_shared_rank(s.low, c)[b];
                 if (mass) sum += u64(cl.map_shared_rank(s.high, c)[b]) << 32;
@@ -385,7 +388,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
                 const int i = e % share, q = e / share;
                 u64 sum = 0;
                 for (int g = 0; g < parts; g++) sum += s.part[g * share + i];
-#pragma unroll 2
+#pragma unroll 4
                 for (int c = q * each; c < min(C, (q + 1) * each); c++)
                     cl.map_shared_rank(s.total, c)[rank * share + i] = sum;
             }
@@ -486,7 +489,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
                 }
                 __syncthreads();
                 total = s.need_out;
-                const float u = a.u[row];
                 u64 target = u > 0.f ? __double2ull_rd(fmin(double(u), 1.0) * double(total)) : 0;
                 target = min(target, total - 1);
                 __syncthreads();
@@ -729,7 +731,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         mb -= m;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-        const float u = a.u[row];
         // the first token with cumulated mass > target
         u64 target = u > 0.f ? __double2ull_rd(fmin(double(u), 1.0) * double(total)) : 0;
         target = min(target, total - 1);
@@ -754,11 +755,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     const int from = min(n, s.pick_seg % W * seg), to = min(n, from + seg);
     u64 run = 0, seen = s.pick_ties;
     const u64 target = s.pick_before;
+    const bool some = s.seg_ties[s.pick_seg] != 0;
     for (int c0 = from; c0 < to; c0 += kSampleThreads) {
         const int i = c0 + tid;
         const float v = i < to ? to_f32(holds ? held[i] : x[i0 + i]) : 0.f;
         const bool tie = i < to && v == cut && cut > -INFINITY;
-        const u64 rank_of = block_sums(s, tie, seen);  // this one counted
+        const u64 rank_of = some ? block_sums(s, tie, seen) : 0;  // this one counted
         const u64 own = tie ? (rank_of <= ties ? tie_mass : 0) : i < to && v > cut ? r.mass(v) : 0;
         const u64 w = block_sums(s, own, run);
         if (w - own <= target && target < w) {
