@@ -105,7 +105,7 @@ struct DecSmem {
 };
 
 template <int HD, int NT, int NP>
-__global__ void __launch_bounds__(kDecThreads) kv8_decode_kernel(const Kv8Args a) {
+__global__ void __launch_bounds__(kDecThreads, kv8_dec_ctas(HD, NT)) kv8_decode_kernel(const Kv8Args a) {
     using L = DecSmem<HD, NT, NP>;
     constexpr int NR = 8 * NT, KB = HD / 32, SUB = L::sub, NB = SUB / 16, UNIT = kDecWarps * SUB, PL = L::digits;
     extern __shared__ __align__(128) uint8_t sm[];
@@ -550,7 +550,7 @@ template <int HD, int NT, int NP>
 void launch_decode(const Kv8Args& a, int grid, bool join, cudaStream_t st) {
     constexpr int smem = DecSmem<HD, NT, NP>::total;
     static_assert(smem <= 227 * 1024, "a CTA's shared memory");
-    static_assert(NT == 2 || kDecPerSm * (smem + 1024) <= 228 * 1024, "the grid is made for this many CTAs on an SM");
+    static_assert(kv8_dec_ctas(HD, NT) * (smem + 1024) <= 228 * 1024, "the grid is made for this many CTAs on an SM");
     static std::atomic<unsigned long long> done{0};
     allow_smem(kv8_decode_kernel<HD, NT, NP>, smem, done);
     kv8_decode_kernel<HD, NT, NP><<<grid, kDecThreads, smem, st>>>(a);
@@ -607,7 +607,7 @@ Plan plan_of(const spm_kv8* c, int heads, int requests, int most, int width) {
     }
     const int64_t pairs = int64_t(requests) * p.tiles;
     if (pairs > INT32_MAX) fail(SPM_E_ARG, "too many requests and queries for one call");
-    const int per_sm = kDecPerSm, unit = kDecWarps * kv8_sub(c->head_dim);
+    const int per_sm = kv8_dec_ctas(c->head_dim, p.nt), unit = kDecWarps * kv8_sub(c->head_dim);
     const int64_t units = (int64_t(width) * c->page_tokens + unit - 1) / unit;
     if (std::max<int64_t>(units, 1) * c->kv_heads > (INT32_MAX - 65536) / std::max<int64_t>(pairs, 1))  // (counted in 32 bits)
         fail(SPM_E_ARG, "too many requests, queries and tokens for one call");

@@ -6,7 +6,10 @@ namespace spm {
 
 constexpr int kDecWarps = 4;   // of a CTA
 constexpr int kDecStages = 2;
-constexpr int kDecPerSm = 3;   // CTAs per SM that the grid is made for
+// CTAs per SM that the grid is made for: what registers and shared memory hold of row
+// tiles of 8 (nt 1) or 16 (nt 2).  Three where two fit leave a second wave (16 requests
+// of 3 tokens, 32/8 heads of 128, 3000 to 8000 keys: 99 us instead of 75).
+constexpr int kv8_dec_ctas(int head_dim, int nt) { return nt == 2 && head_dim > 64 ? 2 : 3; }
 // Tokens of a warp's step.
 constexpr int kv8_sub(int head_dim) { return head_dim <= 128 ? 32 : 16; }
 
