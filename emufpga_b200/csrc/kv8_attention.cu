@@ -593,11 +593,12 @@ Plan plan_of(const spm_kv8* c, int heads, int requests, int most, int width) {
     const int tall = kv8_prompt_rows(c->head_dim);
     const int64_t large = int64_t(requests) * c->kv_heads * ((rows + tall - 1) / tall);
     // A row tile of 16 costs this kernel as much as one of 128 or 256 costs the kernel of
-    // many queries, but shares its keys out over all SMs: 256 such tiles for each wave of
-    // the other's CTAs is where they meet (256 tiles, 1024 to 8000 keys: 137 against 144
-    // us, 90 against 86; 336: 70 against 47; 640: 168 against 56; 128: 88 against 143).
+    // many queries, but shares its keys out over all SMs: 300 such tiles for each wave of
+    // the other's CTAs is about where they meet (8 kv heads of 128 in bf16, 1024 / 4096 /
+    // 8000 keys: 256 tiles 43 / 95 / 162 us here and 47 / 124 / 221 there, 336 tiles 55 /
+    // 124 / 208 and 47 / 132 / 241, 640 tiles 79 / 209 / 372 and 46 / 124 / 222).
     // (More requests than a grid has in z stay here.)
-    p.prompt = rows > 16 && requests <= 65535 && small > 256 * ((large + sms - 1) / sms);
+    p.prompt = rows > 16 && requests <= 65535 && small > 300 * ((large + sms - 1) / sms);
     if (p.prompt) {
         p.tiles = int((rows + tall - 1) / tall);
         p.grid = 0;

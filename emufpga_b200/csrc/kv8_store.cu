@@ -11,9 +11,9 @@
 //
 // Bound: bytes (rows in, one byte a value out) for prompts, and each CTA's chain of
 // slots, rows, scales and codes; launch latency for a decode tick.  Keys and values
-// of 8 x 128 in f32: 8 tokens 5 us, 1024 tokens 8 us (1.3 TB/s), 19 400 bf16 tokens of
-// 4 x 128 in 37 prompts 27 us (60 MB, 2.2 TB/s).  Reading their pages back as bf16
-// takes 18 us (100 MB, 5.6 TB/s).
+// of 8 x 128 in f32: 8 tokens 3 us, 1024 tokens 7 us (1.5 TB/s), 19 400 bf16 tokens of
+// 4 x 128 in 37 prompts 24 us (60 MB, 2.5 TB/s; one launch after another).  Reading
+// their pages back as f32 takes 16 us (100 MB, 6.2 TB/s).
 #include <cuda_runtime.h>
 
 #include <algorithm>

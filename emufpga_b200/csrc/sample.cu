@@ -20,9 +20,9 @@
 // where top-k does not spare them; for few rows the chain of dependent passes and
 // cluster barriers.  A row is one thread-block cluster whose CTAs keep its
 // slices in shared memory, so the logits are read from HBM once and the
-// histograms are added through distributed shared memory.  One row of 49152 takes 18 to 23
-// us, 8 of 151936 with top-p 38, 128 of 151936 in bf16 95 with top-k (0.4 TB/s) and 227
-// with top-p: about 40 and 200 instructions a logit.
+// histograms are added through distributed shared memory.  One row of 49152 takes 18 to 22
+// us, 8 of 151936 with top-p 38, 128 of 151936 in bf16 75 with top-k (0.5 TB/s) and 160
+// with top-p: about 40 and 170 instructions a logit.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
