@@ -9,8 +9,8 @@
 // order (shared memory atomics included) and the same on every run; a neighbour
 // at a border of top-p or u is told apart at 2^-44 of the largest weight.
 //
-// The row is not sorted.  A histogram over 1024 bins of (max - x) / T, 1/32
-// wide, of counts (top-k) or masses (top-p) shows the bin in which the border
+// The row is not sorted.  A histogram over 1024 bins of (max - x) / T, 1/64
+// wide up to 12 and 5/64 up to 32, of counts (top-k) or masses (top-p) shows the bin in which the border
 // lies; only what lies there (for top-k: there and above) is listed and sorted,
 // a few hundred tokens as a rule.  Where a list would be longer than 2048 (long
 // runs of equal logits, a large top_k) the border is found by radix selection
@@ -90,7 +90,7 @@ struct alignas(16) Shared {
 
 struct Row {
     double top, inv, slope;   // the largest logit, 1 / T, -128 log2(e) / T
-    float ftop, bins;         // 32 / T: bins of a logit's distance from the top
+    float ftop, bins;         // 64 / T: the first bins of a logit's distance from the top
     const double* table;
     __device__ __forceinline__ double below(float x) const { return x == ftop ? 0.0 : top - double(x); }
     __device__ __forceinline__ double weight(float x) const { return x == ftop ? 1.0 : exp(-below(x) * inv); }
@@ -114,7 +114,10 @@ struct Row {
     }
     __device__ __forceinline__ float distance(float x) const { return fminf(ftop - x, 3.402823466e38f); }
     // The bin of a candidate's distance from the top; ascending as x descends.
-    __device__ __forceinline__ float place(float x) const { return fminf(x == INFINITY ? 0.f : distance(x) * bins, float(kBins - 1)); }
+    __device__ __forceinline__ float place(float x) const {
+        const float t = x == INFINITY ? 0.f : distance(x) * bins;
+        return fminf(fminf(t, fmaf(t, 0.2f, 0.8f * 768.f)), float(kBins - 1));  // (768 bins of 1/64, then five times as wide)
+    }
     __device__ __forceinline__ int bin(float x) const { return int(place(x)); }
     __device__ __forceinline__ bool in_bin(float x, int b) const {
         const float p = place(x);
@@ -339,7 +342,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     r.top = double(r.ftop);
     r.inv = greedy ? 1.0 : 1.0 / double(temp);
     r.slope = r.inv * -1.4426950408889634074 * kTable;
-    r.bins = r.ftop == INFINITY ? 1e30f : fminf(float(32.0 * r.inv), 1e30f);
+    r.bins = r.ftop == INFINITY ? 1e30f : fminf(float(64.0 * r.inv), 1e30f);
     r.table = s.table;
     int k = greedy ? 0 : want_k;
     if (k <= 0 || k >= a.vocab) k = 0;
