@@ -21,7 +21,7 @@
 // cluster barriers.  A row is one thread-block cluster whose CTAs keep its
 // slices in shared memory, so the logits are read from HBM once and the
 // histograms are added through distributed shared memory.  One row of 49152 takes 18 to 22
-// us, 8 of 151936 with top-p 38, 128 of 151936 in bf16 75 with top-k (0.5 TB/s) and 160
+// us, 8 of 151936 with top-p 38, 128 of 151936 in bf16 76 with top-k (0.5 TB/s) and 158
 // with top-p: about 40 and 170 instructions a logit.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
