@@ -5,9 +5,9 @@
 // out = sum_j 2^(s_j - m) 2^(f_j) V_j / sum_j 2^(s_j - m), with K_j, V_j the int8
 // codes and 2^(e_j), 2^(f_j) the scales of key j's page.  One pass with running
 // references, all integers, so that every rescaling is a power of two and exact:
-// m = ceil(max s) for the sum, and r = max(ceil(max s in a page's 16 rows) + f)
+// m = ceil(max s) for the sum, and r = max(ceil(max s in a page's 16 rows) + f) - 15
 // for the accumulator, which then holds sum_j 2^(s_j + f_j - r) V_j with every
-// weight at most 1: it fits fp16 whatever the pages' scales are.
+// weight at most 2^15: it fits fp16 whatever the pages' scales are.
 //
 // Products on the tensor cores (mma.sync).  The 16 rows of an mma are cached tokens
 // (or, for the values, head dimensions) and its 8 columns are query rows (tokens x
@@ -18,9 +18,12 @@
 //   bits, would gain 2% of a long decode).  Sums are exact in int32.
 //   Values: fp16 x fp16 (m16n8k16), fp32 sums.  The codes are exact in fp16: byte
 //   permutes make 0x6400 | (code + 128) = 1024 + 128 + code and a subtraction of 1152
-//   the code.  Weights are fp16 (a floating type: a long tail of small ones counts),
-//   high and low part (22 bits) where the result is f32.  ldmatrix transposes pairs
-//   of bytes: the even and odd dimensions of a 16-byte column become rows g and g + 8.
+//   the code.  Weights are fp16: one part, 11 bits for weights down to 2^-29 of the
+//   row's largest (a bit less for each power of two below), where the result is 16
+//   bits; where it is f32 a second part, what is left times 2^11 with the codes times
+//   2^-11 (both exact), makes them 22 bits down to the same 2^-29 and 11 at 2^-40.
+//   ldmatrix transposes pairs of bytes: the even and odd dimensions of a 16-byte
+//   column become rows g and g + 8.
 //
 // What bounds it is the cache's bytes (64 requests of 1000 to 16384 keys, 8 kv heads of
 // 128: 1.16 GB in 215 us, 5.4 TB/s, and 8 us to join the parts), nearly as much the
@@ -364,7 +367,7 @@ __global__ void __launch_bounds__(kDecThreads, kv8_dec_ctas(HD, NT)) kv8_decode_
                     for (int b = 0; b < NB; b++) {
                         const float t0 = ceilf(top[b][c]);
                         m = fmaxf(m, t0);
-                        r = fmaxf(r, t0 + ve[b]);
+                        r = fmaxf(r, t0 + ve[b] - kLift);
                     }
                     l_run[n][c] *= kv8_step(m_run[n][c], m);
                     down[c] = kv8_step(r_run[n][c], r);
@@ -403,7 +406,8 @@ __global__ void __launch_bounds__(kDecThreads, kv8_dec_ctas(HD, NT)) kv8_decode_
                         w[b][n][0][e] = transposed(hi);
                         if (NP == 2) {
                             const float2 h = half2_floats(hi);
-                            w[b][n][NP - 1][e] = transposed(kv8_half2(s[b][n][2 * e] - h.x, s[b][n][2 * e + 1] - h.y));
+                            w[b][n][NP - 1][e] = transposed(
+                                kv8_half2((s[b][n][2 * e] - h.x) * 2048.f, (s[b][n][2 * e + 1] - h.y) * 2048.f));
                         }
                     }
             }
@@ -421,10 +425,12 @@ __global__ void __launch_bounds__(kDecThreads, kv8_dec_ctas(HD, NT)) kv8_decode_
                         const uint32_t a0 = kv8_codes2<0x4240>(lo), a1 = kv8_codes2<0x4341>(lo), a2 = kv8_codes2<0x4240>(hi),
                                        a3 = kv8_codes2<0x4341>(hi);
 #pragma unroll
-                        for (int n = 0; n < NT; n++)
-#pragma unroll
-                            for (int p = NP - 1; p >= 0; p--)
-                                mma_f16(o[2 * d + e][n], a0, a1, a2, a3, w[b][n][p][0], w[b][n][p][1]);
+                        for (int n = 0; n < NT; n++) {
+                            if (NP == 2)
+                                mma_f16(o[2 * d + e][n], kv8_under(a0), kv8_under(a1), kv8_under(a2), kv8_under(a3),
+                                        w[b][n][NP - 1][0], w[b][n][NP - 1][1]);
+                            mma_f16(o[2 * d + e][n], a0, a1, a2, a3, w[b][n][0][0], w[b][n][0][1]);
+                        }
                     }
                 }
             }

@@ -13,6 +13,12 @@ constexpr int kv8_dec_ctas(int head_dim, int nt) { return nt == 2 && head_dim > 
 // Tokens of a warp's step.
 constexpr int kv8_sub(int head_dim) { return head_dim <= 128 ? 32 : 16; }
 
+// Powers of two by which a weight may lie above 1: a row's accumulator has its reference
+// that far under the largest weighted value's.  fp16 holds 2^15 but nothing under 2^-25,
+// and the many small weights beside a large one (a first token that takes nearly all
+// and has no value to speak of) are the result.
+constexpr float kLift = 15.f;
+
 // Rows of a tile of the kernel of many queries.
 constexpr int kv8_prompt_rows(int head_dim) { return head_dim <= 128 ? 256 : 128; }
 
@@ -149,6 +155,12 @@ __device__ __forceinline__ uint32_t kv8_codes2(uint32_t x) {
     const uint32_t u = __byte_perm(x, 0x64646464u, SEL);
     const __half bias = __ushort_as_half(0x6480);  // 1152
     const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), __halves2half2(bias, bias));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Two fp16 codes times 2^-11.
+__device__ __forceinline__ uint32_t kv8_under(uint32_t x) {
+    const __half m = __ushort_as_half(0x1000);  // 2^-11
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&x), __halves2half2(m, m));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t kv8_half2(float lo, float hi) {

@@ -20,14 +20,16 @@
 // for one group, which has two buffers of S instead.  (Two buffers of 64 keys for
 // two groups too: 176 us where one of 128 took 135, 32 heads of 128, 1024 queries over
 // 4096 keys; a product of 64 columns takes the tensor cores as long as one of 128.)
-// The references move only where a row's maximum passes them by more than 2^14, so
-// that the accumulator is hardly ever read back to be rescaled: weights are then at
-// most 2^14, which fp16 holds as exactly as those below 1.
+// The accumulator's reference lies 2^15, what fp16 holds, under the largest weighted value
+// and moves with it, so that weights keep 11 bits down to 2^-29 of the row's largest
+// (and a step of 2^-40 of it in two parts).  A slack of 2^14 instead, which hardly ever
+// reads the accumulator back, took 124.7 us where this takes 130.8, and lost every weight
+// under 2^-25 of the largest.  The sum is f32: its reference has that slack.
 // f32 queries and weights are two fp16 parts (22 bits), twice the products.
 //
 // What bounds it is the softmax: the 16384 exponentials of a 128 x 128 tile take
 // 1024 cycles of the special function unit, as long as its products, and its other
-// instructions as many again: 123 us for the case above, 488 TFLOP/s.  (One thread a
+// instructions as many again: 131 us for the case above, 459 TFLOP/s.  (One thread a
 // row, 128 columns: 136 us; S read once for maximum and weights: 144.)
 #include <cuda_runtime.h>
 
@@ -43,7 +45,7 @@ namespace {
 using namespace dev;
 
 constexpr int kRows = 128;                             // of a group: the MMA's M
-constexpr float kSlack = 14.f;                         // in powers of two
+constexpr float kSlack = 14.f;                         // of the sum's reference, in powers of two
 
 template <int HD, int NP>
 struct PromptShape {
@@ -492,11 +494,12 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
                 break;
             }
             reach = fmaxf(reach, y.reach[j & 1][half ^ 1][r]);
-            // the reference moves seldom (see above), a warp's rows together
-            const bool moves = reach > ref + kSlack || (ref == -INFINITY && reach > ref);
+            // a warp's rows together
+            const bool moves = reach > ref + kLift || (ref == -INFINITY && reach > ref);
             if (__any_sync(0xffffffffu, moves)) {
-                const float down = moves ? kv8_step(ref, reach) : 1.f;
-                if (moves) ref = reach;
+                const float to = reach - kLift;
+                const float down = moves ? kv8_step(ref, to) : 1.f;
+                if (moves) ref = to;
                 if (j) {
                     // O is the products' until P(j - 1) V(j - 1) is done (the one before
                     // is, S(j) waited for it: the parity is that of one phase alone)
