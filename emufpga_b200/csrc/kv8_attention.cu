@@ -18,10 +18,12 @@
 //   bits, would gain 2% of a long decode).  Sums are exact in int32.
 //   Values: fp16 x fp16 (m16n8k16), fp32 sums.  The codes are exact in fp16: byte
 //   permutes make 0x6400 | (code + 128) = 1024 + 128 + code and a subtraction of 1152
-//   the code.  Weights are fp16: one part, 11 bits for weights down to 2^-29 of the
-//   row's largest (a bit less for each power of two below), where the result is 16
-//   bits; where it is f32 a second part, what is left times 2^11 with the codes times
-//   2^-11 (both exact), makes them 22 bits down to the same 2^-29 and 11 at 2^-40.
+//   the code.  Weights are fp16.  For bf16 results one part: 11 bits for weights down
+//   to 2^-29 of the row's largest, a bit less for each power of two below.  f16 results
+//   take a second part for what is left (one alone would add as much as their own
+//   rounding, 1.4 times the error; it takes 5% of a long decode), f32 results hold that
+//   part 2^11 up and give it the codes 2^-11 down (both exact): 22 bits down to the
+//   same 2^-29, 11 at 2^-40.
 //   ldmatrix transposes pairs of bytes: the even and odd dimensions of a 16-byte
 //   column become rows g and g + 8.
 //
@@ -82,7 +84,10 @@ __device__ __forceinline__ float2 half2_floats(uint32_t b) { return __half22floa
 __device__ __forceinline__ void cp_async4(void* dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(saddr(dst)), "l"(src) : "memory");
 }
-template <int HD, int NT, int NP>
+// A weight's fp16 parts: one, two, or two of which the second is held 2^11 up.
+enum class Weights { kOne, kTwo, kTwoApart };
+
+template <int HD, int NT>
 struct DecSmem {
     static constexpr int sub = kv8_sub(HD);
     // a token's codes: the eight rows that an ldmatrix reads lie on distinct banks,
@@ -107,9 +112,12 @@ struct DecSmem {
     static constexpr int total = ring + (ring_bytes > state_bytes ? ring_bytes : state_bytes);
 };
 
-template <int HD, int NT, int NP>
+template <int HD, int NT, Weights WT>
 __global__ void __launch_bounds__(kDecThreads, kv8_dec_ctas(HD, NT)) kv8_decode_kernel(const Kv8Args a) {
-    using L = DecSmem<HD, NT, NP>;
+    using L = DecSmem<HD, NT>;
+    constexpr int NP = WT == Weights::kOne ? 1 : 2;
+    constexpr bool apart = WT == Weights::kTwoApart;
+    constexpr float up = apart ? 2048.f : 1.f;
     constexpr int NR = 8 * NT, KB = HD / 32, SUB = L::sub, NB = SUB / 16, UNIT = kDecWarps * SUB, PL = L::digits;
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ int wsum[kDecWarps], found[2];
@@ -407,7 +415,7 @@ __global__ void __launch_bounds__(kDecThreads, kv8_dec_ctas(HD, NT)) kv8_decode_
                         if (NP == 2) {
                             const float2 h = half2_floats(hi);
                             w[b][n][NP - 1][e] = transposed(
-                                kv8_half2((s[b][n][2 * e] - h.x) * 2048.f, (s[b][n][2 * e + 1] - h.y) * 2048.f));
+                                kv8_half2((s[b][n][2 * e] - h.x) * up, (s[b][n][2 * e + 1] - h.y) * up));
                         }
                     }
             }
@@ -426,9 +434,9 @@ __global__ void __launch_bounds__(kDecThreads, kv8_dec_ctas(HD, NT)) kv8_decode_
                                        a3 = kv8_codes2<0x4341>(hi);
 #pragma unroll
                         for (int n = 0; n < NT; n++) {
-                            if (NP == 2)
-                                mma_f16(o[2 * d + e][n], kv8_under(a0), kv8_under(a1), kv8_under(a2), kv8_under(a3),
-                                        w[b][n][NP - 1][0], w[b][n][NP - 1][1]);
+                            const uint32_t* lo = w[b][n][NP - 1];
+                            if (apart) mma_f16(o[2 * d + e][n], kv8_under(a0), kv8_under(a1), kv8_under(a2), kv8_under(a3), lo[0], lo[1]);
+                            else if (NP == 2) mma_f16(o[2 * d + e][n], a0, a1, a2, a3, lo[0], lo[1]);
                             mma_f16(o[2 * d + e][n], a0, a1, a2, a3, w[b][n][0][0], w[b][n][0][1]);
                         }
                     }
@@ -552,14 +560,14 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const Kv8Args a, int g
     kv8_store(a, int64_t(s0 + qi) * a.o_token + qh * a.o_head + tid, kv8_finish(acc, ref, sum, m));
 }
 
-template <int HD, int NT, int NP>
+template <int HD, int NT, Weights WT>
 void launch_decode(const Kv8Args& a, int grid, bool join, cudaStream_t st) {
-    constexpr int smem = DecSmem<HD, NT, NP>::total;
+    constexpr int smem = DecSmem<HD, NT>::total;
     static_assert(smem <= 227 * 1024, "a CTA's shared memory");
     static_assert(kv8_dec_ctas(HD, NT) * (smem + 1024) <= 228 * 1024, "the grid is made for this many CTAs on an SM");
     static std::atomic<unsigned long long> done{0};
-    allow_smem(kv8_decode_kernel<HD, NT, NP>, smem, done);
-    kv8_decode_kernel<HD, NT, NP><<<grid, kDecThreads, smem, st>>>(a);
+    allow_smem(kv8_decode_kernel<HD, NT, WT>, smem, done);
+    kv8_decode_kernel<HD, NT, WT><<<grid, kDecThreads, smem, st>>>(a);
     CUDA_OK(cudaGetLastError());
     if (!join) return;
     cudaLaunchConfig_t cfg = {};
@@ -574,10 +582,16 @@ void launch_decode(const Kv8Args& a, int grid, bool join, cudaStream_t st) {
     CUDA_OK(cudaLaunchKernelEx(&cfg, kv8_combine_kernel, a, grid, HD));
 }
 
+template <int HD, int NT>
+void launch_type(const Kv8Args& a, int grid, bool join, cudaStream_t st) {
+    if (a.dtype == SPM_F32) launch_decode<HD, NT, Weights::kTwoApart>(a, grid, join, st);
+    else if (a.dtype == SPM_F16) launch_decode<HD, NT, Weights::kTwo>(a, grid, join, st);
+    else launch_decode<HD, NT, Weights::kOne>(a, grid, join, st);
+}
+
 template <int HD>
-void launch_dim(const Kv8Args& a, int nt, bool two, int grid, bool join, cudaStream_t st) {
-    if (nt == 1) two ? launch_decode<HD, 1, 2>(a, grid, join, st) : launch_decode<HD, 1, 1>(a, grid, join, st);
-    else two ? launch_decode<HD, 2, 2>(a, grid, join, st) : launch_decode<HD, 2, 1>(a, grid, join, st);
+void launch_dim(const Kv8Args& a, int nt, int grid, bool join, cudaStream_t st) {
+    nt == 1 ? launch_type<HD, 1>(a, grid, join, st) : launch_type<HD, 2>(a, grid, join, st);
 }
 
 // How a call is cut, from what the host knows of it.
@@ -687,13 +701,12 @@ spm_status spm_kv8_attention(const spm_kv8* c, uint32_t dtype, const void* q, in
             launch_kv8_prompt(a, c->head_dim, st);
             return;
         }
-        const bool two = dtype == SPM_F32;
         switch (c->head_dim) {
-            case 64: launch_dim<64>(a, p.nt, two, p.grid, p.join, st); break;
-            case 96: launch_dim<96>(a, p.nt, two, p.grid, p.join, st); break;
-            case 128: launch_dim<128>(a, p.nt, two, p.grid, p.join, st); break;
-            case 192: launch_dim<192>(a, p.nt, two, p.grid, p.join, st); break;
-            default: launch_dim<256>(a, p.nt, two, p.grid, p.join, st); break;
+            case 64: launch_dim<64>(a, p.nt, p.grid, p.join, st); break;
+            case 96: launch_dim<96>(a, p.nt, p.grid, p.join, st); break;
+            case 128: launch_dim<128>(a, p.nt, p.grid, p.join, st); break;
+            case 192: launch_dim<192>(a, p.nt, p.grid, p.join, st); break;
+            default: launch_dim<256>(a, p.nt, p.grid, p.join, st); break;
         }
     });
 }

@@ -25,7 +25,10 @@
 // (and a step of 2^-40 of it in two parts).  A slack of 2^14 instead, which hardly ever
 // reads the accumulator back, took 124.7 us where this takes 130.8, and lost every weight
 // under 2^-25 of the largest.  The sum is f32: its reference has that slack.
-// f32 queries and weights are two fp16 parts (22 bits), twice the products.
+// f32 queries are two fp16 parts (22 bits), and so are the weights of f32 and f16
+// results: one part, 11 bits, would add as much to an f16 result as its own rounding.
+// For a bf16 result, 8 bits, it is enough.  (1024 queries over 4096 keys, 32/8 heads of
+// 128: f16 140 us, f32 146; heads of 64 f16 126 where one part took 107.)
 //
 // What bounds it is the softmax: the 16384 exponentials of a 128 x 128 tile take
 // 1024 cycles of the special function unit, as long as its products, and its other
@@ -47,7 +50,7 @@ using namespace dev;
 constexpr int kRows = 128;                             // of a group: the MMA's M
 constexpr float kSlack = 14.f;                         // of the sum's reference, in powers of two
 
-template <int HD, int NP>
+template <int HD, int NQ, int NP>
 struct PromptShape {
     static constexpr int G = kv8_prompt_rows(HD) / kRows;
     // converting warps: as many as leave the softmax its registers (80 of 24 warps, 96 of 20)
@@ -57,7 +60,7 @@ struct PromptShape {
     static constexpr int BUF = G == 1 ? 2 : 1;         // buffers of S
     static constexpr int atoms = (HD + 63) / 64;       // 64 dimensions, 128 bytes
     static constexpr int qgroup = atoms * kRows * 128; // bytes of a group's part of Q
-    static constexpr int qbytes = G * NP * qgroup;
+    static constexpr int qbytes = G * NQ * qgroup;
     static constexpr int tile = atoms * TN * 128;      // bytes of a tile of K or V
     static constexpr int room = (227 * 1024 - 8192 - qbytes) / (2 * tile), stages = room > 4 ? 4 : room;
     static_assert(stages >= 1, "a tile of K and one of V");
@@ -176,9 +179,10 @@ __device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t at, uint32_t next) {
 typedef std::true_type Yes;
 typedef std::false_type No;
 
-template <int HD, int NP>
-__global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_kernel(const Kv8Args a) {
-    using S = PromptShape<HD, NP>;
+// NQ, NP: fp16 parts of a query and of a weight.
+template <int HD, int NQ, int NP>
+__global__ void __launch_bounds__(PromptShape<HD, NQ, NP>::threads, 1) kv8_prompt_kernel(const Kv8Args a) {
+    using S = PromptShape<HD, NQ, NP>;
     constexpr int TN = S::TN, ST = S::stages, G = S::G, BUF = S::BUF, FT = 32 * S::fill, kSoftWarps = 8 * G;
     extern __shared__ __align__(1024) uint8_t raw[];
     __shared__ PromptSync y;
@@ -339,14 +343,14 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
             constexpr uint32_t id_s = f32_out | m | uint32_t(TN >> 3) << 17;
             constexpr uint32_t id_o = f32_out | m | uint32_t(HD >> 3) << 17 | 1u << 16;  // V is MN-major
             auto scores = [&](int g, int j) {
-                const uint32_t k = ks + uint32_t(j % ST) * S::tile, q = qs + uint32_t(g * NP) * S::qgroup;
+                const uint32_t k = ks + uint32_t(j % ST) * S::tile, q = qs + uint32_t(g * NQ) * S::qgroup;
 #pragma unroll
-                for (int p = NP - 1; p >= 0; p--)
+                for (int p = NQ - 1; p >= 0; p--)
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; kk++)
                         umma_f16(tmem + S::s_col + (BUF * g + j % BUF) * TN,
                                  sw128_desc(q + uint32_t(p) * S::qgroup + (kk >> 2) * (kRows * 128) + 32u * (kk & 3)),
-                                 sw128_desc(k + (kk >> 2) * (TN * 128) + 32u * (kk & 3)), id_s, p != NP - 1 || kk != 0);
+                                 sw128_desc(k + (kk >> 2) * (TN * 128) + 32u * (kk & 3)), id_s, p != NQ - 1 || kk != 0);
                 if (g == groups - 1) umma_commit(&y.k_empty[j % ST]);
                 umma_commit(&y.s_full[g][j % BUF]);
             };
@@ -418,10 +422,10 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
                     const int d = lane + 32 * i;
                     const float v = big < 0x7f800000u ? __fmul_rn(x[u][i], mul) : 0.f;
                     const __half hi = __float2half_rn(v);
-                    const uint32_t at = uint32_t(r / kRows) * (NP * S::qgroup) + uint32_t(d >> 6) * (kRows * 128) +
+                    const uint32_t at = uint32_t(r / kRows) * (NQ * S::qgroup) + uint32_t(d >> 6) * (kRows * 128) +
                                         sw128_offset(r % kRows, (d & 63) >> 3) + 2 * (d & 7);
                     *reinterpret_cast<__half*>(base + at) = hi;
-                    if (NP == 2) *reinterpret_cast<__half*>(base + S::qgroup + at) = __float2half_rn(__fsub_rn(v, __half2float(hi)));
+                    if (NQ == 2) *reinterpret_cast<__half*>(base + S::qgroup + at) = __float2half_rn(__fsub_rn(v, __half2float(hi)));
                 }
             }
         }
@@ -606,20 +610,23 @@ __global__ void __launch_bounds__(PromptShape<HD, NP>::threads, 1) kv8_prompt_ke
     }
 }
 
-template <int HD, int NP>
+template <int HD, int NQ, int NP>
 void launch(const Kv8Args& a, cudaStream_t st) {
-    constexpr int smem = PromptShape<HD, NP>::smem;
+    constexpr int smem = PromptShape<HD, NQ, NP>::smem;
     static_assert(smem + int(sizeof(PromptSync)) <= 227 * 1024, "a CTA's shared memory");
     static std::atomic<unsigned long long> done{0};
-    allow_smem(kv8_prompt_kernel<HD, NP>, smem, done);
+    allow_smem(kv8_prompt_kernel<HD, NQ, NP>, smem, done);
     const dim3 grid(unsigned(a.tiles), unsigned(a.kv_heads), unsigned(a.requests));
-    kv8_prompt_kernel<HD, NP><<<grid, PromptShape<HD, NP>::threads, smem, st>>>(a);
+    kv8_prompt_kernel<HD, NQ, NP><<<grid, PromptShape<HD, NQ, NP>::threads, smem, st>>>(a);
     CUDA_OK(cudaGetLastError());
 }
 
 template <int HD>
 void launch_parts(const Kv8Args& a, cudaStream_t st) {
-    a.dtype == SPM_F32 ? launch<HD, 2>(a, st) : launch<HD, 1>(a, st);
+    // a 16-bit query is exact in one part (see above for the weights)
+    if (a.dtype == SPM_F32) launch<HD, 2, 2>(a, st);
+    else if (a.dtype == SPM_F16) launch<HD, 1, 2>(a, st);
+    else launch<HD, 1, 1>(a, st);
 }
 
 }  // namespace

@@ -11,8 +11,9 @@ pytestmark = pytest.mark.gpu
 
 
 # -------------------------------------------------------------- attention --
-def softmax_rows(c, q, length, most, scale):
-    """out of the last `most` of `length` positions in 64 bits, pages 0, 1, ... in order."""
+def softmax_rows(c, q, length, most, scale, sizes=False):
+    """out of the last `most` of `length` positions in 64 bits, pages 0, 1, ... in order; with `sizes`
+    the sums of |weight * value| and the largest weight * 127 scales (a page's largest value at most) too."""
     n = -(-length // c.page_tokens)
     k, v = ((codes[:n].double() * scales[:n].double()[..., None, None]).transpose(1, 2).reshape(-1, c.kv_heads, c.head_dim)[:length]
             for codes, scales in ((c.k_codes, c.k_scales), (c.v_codes, c.v_scales)))
@@ -20,7 +21,12 @@ def softmax_rows(c, q, length, most, scale):
     k, v = (t.repeat_interleave(group, 1) for t in (k, v))
     x = torch.einsum("ihd,jhd->hij", q.double(), k) * scale
     hidden = torch.arange(length, device="cuda") > torch.arange(length - most, length, device="cuda")[:, None]
-    return torch.einsum("hij,jhd->ihd", torch.softmax(x.masked_fill(hidden, -math.inf), 2), v)
+    w = torch.softmax(x.masked_fill(hidden, -math.inf), 2)
+    out = torch.einsum("hij,jhd->ihd", w, v)
+    if not sizes:
+        return out
+    most_of = (c.v_scales[:n].double() * 127).repeat_interleave(c.page_tokens, 0)[:length].repeat_interleave(group, 1)
+    return out, torch.einsum("hij,jhd->ihd", w, v.abs()), (w * most_of.t()[:, None]).amax(2).t()[:, :, None]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -60,3 +66,54 @@ def test_attention_keeps_small_weights_beside_a_large_one(dtype, dim, most, head
         bound += 2.0 ** -25 / 2.0 ** (14 - gap * 1.03)
     err = (got.double() - want).abs()
     assert (err <= (bound + HALF[q.dtype]) * want).all(), (err / want).max().item()
+
+
+def weight_error(q, c, length, scale):
+    """How far a weight may be off, relative: its score's sums and products, its power, the sum over keys (serving_cases.attention)."""
+    k = (c.k_codes.double() * c.k_scales.double()[..., None, None]).abs().amax((0, 2))
+    bits = (q.double().abs() * k.repeat_interleave(q.shape[1] // c.kv_heads, 0)).sum(2).max().item() * abs(scale) * 1.4427
+    return 2 * (0.6932 * bits * 2.0 ** -23 * (c.head_dim / 8 + 4) + 2.0 ** -20 + (length / 16 + 8) * 2.0 ** -23)
+
+
+def table_of(c):
+    return torch.arange(c.pages, dtype=torch.int32, device="cuda")[None]
+
+
+@pytest.mark.parametrize("dim", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("most,heads,kv_heads", [(1, 4, 2), (1, 32, 2), (3, 8, 2), (64, 40, 40), (130, 48, 24)])
+def test_f16_attention_is_off_by_its_own_rounding(dim, most, heads, kv_heads):
+    length = 300
+    c = pool(-(-length // 32), 32, kv_heads, dim, seed=dim)
+    q = torch.randn(most, heads, dim, device="cuda", generator=gen(most)).half()
+    scale = float(np.float32(dim ** -0.5))
+    want, size, _ = softmax_rows(c, q, length, most, scale, sizes=True)
+    got = c.attention(q, ints([0, most]), ints([length]), table_of(c), most, scale=scale)
+    c.check()
+    # two parts of a weight: 2^-22 of it; then half a step of the result
+    bound = (weight_error(q, c, length, scale) + 2.0 ** -21) * size + HALF[q.dtype] * want.abs() + 2.0 ** -25
+    assert ((got.double() - want).abs() <= bound).all(), ((got.double() - want).abs() / bound).max().item()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("most,kv_heads", [(1, 2), (30, 2), (30, 40)])  # the last: the kernel of many queries
+@pytest.mark.parametrize("lo,hi", [(-60, 60), (-30, 8), (-24, -10)])
+def test_attention_where_pages_differ_widely_in_every_type(dtype, most, kv_heads, lo, hi):
+    c = pool(13, 16, kv_heads, 128)
+    g = gen(7 + hi)
+    c.v_scales.copy_(2.0 ** torch.randint(lo, hi + 1, c.v_scales.shape, device="cuda", generator=g))
+    c.k_codes[4], c.v_codes[4], c.k_scales[4], c.v_scales[4] = 0, 0, 0, 0
+    q = torch.randn(most, 2 * kv_heads, 128, device="cuda", generator=g).to(TYPES[dtype])
+    for length in (200, 16, 17):  # (the second: every other page is masked)
+        n = min(most, length)
+        scale = float(np.float32(0.02))
+        want, size, large = softmax_rows(c, q[:n], length, n, scale, sizes=True)
+        got = c.attention(q[:n], ints([0, n]), ints([length]), table_of(c), n, scale=scale).double()
+        c.check()
+        # a weight's parts; and fp16's smallest step where the largest weighted scale's is 2^14 at least
+        bound = (weight_error(q, c, length, scale) + (2.0 ** -11 if dtype == "bf16" else 2.0 ** -21)) * size
+        bound = bound + length * 2.0 ** -39 * large + HALF[q.dtype] * want.abs() + (2.0 ** -25 if dtype == "f16" else 0)
+        top = torch.finfo(q.dtype).max * (1 + HALF[q.dtype] / 2)
+        over, under = want.abs() - bound >= top, want.abs() + bound < top
+        assert got[over].isinf().all() and (got[over].sign() == want[over].sign()).all()
+        assert ((got - want).abs() <= bound)[under].all(), ((got - want).abs() / bound)[under].max().item()
+        assert (over | under).any()  # (f16: pages of 2^60 take every output past its range)
