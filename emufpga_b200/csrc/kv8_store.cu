@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kStoreThreads, 4) kv8_append_kernel(const Stor
                 const float was = *p;
                 if (!(was == was)) sc = was;            // NaN stays
                 else if (was > sc) sc = was;
-                else if (was > 0.f && sc > was) ratio[tid] = __fdiv_rn(was, sc);
+                else if (was > 0.f && sc > was) ratio[tid] = fmaxf(__fdiv_rn(was, sc), pow2i(-126));  // (0: none; any code becomes 0)
             }
             *p = sc;
             inv[tid] = sc > 0.f ? __fdiv_rn(1.f, sc) : 0.f;

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_serving import HALF, TYPES, gen, ints, pool
+from test_gpu_serving import HALF, TYPES, check_append, gen, ints, pool
 
 pytestmark = pytest.mark.gpu
 
@@ -117,3 +117,18 @@ def test_attention_where_pages_differ_widely_in_every_type(dtype, most, kv_heads
         assert got[over].isinf().all() and (got[over].sign() == want[over].sign()).all()
         assert ((got - want).abs() <= bound)[under].all(), ((got - want).abs() / bound)[under].max().item()
         assert (over | under).any()  # (f16: pages of 2^60 take every output past its range)
+
+
+# ----------------------------------------------------------------- append --
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("old,new", [(-126, 22), (-126, 23), (-126, 24), (-126, 31), (-126, 120), (-80, 100), (-40, 110), (-30, 119)])
+def test_append_where_the_scale_grows_by_more_than_a_float_holds(dtype, old, new):
+    # rows stored at 2^old under a row at 2^new: from 2^150 on the ratio is none of f32's
+    c = pool(2, 16, 2, 64, fill=False)
+    x = torch.randn(2, 5, 2, 64, device="cuda", generator=gen(1)).clamp(-3, 3)
+    x[:, :4] *= 2.0 ** (old + 5)
+    x[:, 4] *= 2.0 ** (new + 5)
+    x = x.to(TYPES[dtype])
+    check_append(c, x[0, :4], x[1, :4], [16, 17, 18, 19])
+    check_append(c, x[0, 4:], x[1, 4:], [20])
+    assert not c.k_codes[1, :, :4].any() and c.k_codes[1, :, 4].any()
