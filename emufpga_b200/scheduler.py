@@ -18,6 +18,11 @@ at once through the session's `prefill` (the tensor-core prompt path) when
 it takes its slot; it then feeds its last prompt token in the next step and
 decodes from there -- the batched prefill for late joiners that the
 reference's lockstep server lacks (docs/results.md:1189-1191).
+
+A paged session's clients share one pool of pages.  There a request starts only
+when the pool holds its last token's page beside those of all requests in
+flight, a finished request's pages come back at once, and a free slot that
+decodes filler tokens holds one page at most, so that no step runs out of pages.
 """
 from __future__ import annotations
 
@@ -51,6 +56,10 @@ class DecodeSession(Protocol):
     # only with prefill=True: run tokens for `client` at its next positions
     def prefill(self, client: int, tokens: Sequence[int]) -> None: ...
 
+    # only of a paged session (page_tokens neither missing nor None): its pages' length, and how many are free
+    # page_tokens: int
+    # free_pages: int
+
 
 def serve_continuous(session: DecodeSession, requests: Sequence[Request], filler: int = 0,
                      prefill: bool = False) -> list[list[int]]:
@@ -61,12 +70,23 @@ def serve_continuous(session: DecodeSession, requests: Sequence[Request], filler
     once by session.prefill.  A request with `sampling` feeds back tokens drawn
     with it, from its own seed's numbers, one for each token it produces, so
     that its tokens do not depend on what else is served.  Raises ValueError when a request cannot fit the
-    session's context."""
+    session's context, or a paged session's pages (all of which it takes: every client starts empty)."""
     for r in requests:
         if not r.prompt or r.max_new < 1:
             raise ValueError("a request needs a prompt and at least one new token")
         if len(r.prompt) + r.max_new > session.context:
             raise ValueError("a request does not fit the session's context")
+    page = getattr(session, "page_tokens", None)
+    need, pages = [0] * len(requests), 0
+    if page:
+        for s in range(session.max_clients):
+            if session.length(s):
+                session.reset(s)
+        pages = session.free_pages
+        # the last token produced is not fed back
+        need = [-(-(len(r.prompt) + r.max_new - 1) // page) for r in requests]
+        if max(need, default=0) > pages:
+            raise ValueError("a request does not fit the session's pages")
     waiting = sorted(range(len(requests)), key=lambda i: (requests[i].arrival, i))
     out: list[list[int]] = [[] for _ in requests]
     active: dict[int, list[int]] = {}  # slot -> [request, local step, next token]
@@ -78,6 +98,11 @@ def serve_continuous(session: DecodeSession, requests: Sequence[Request], filler
                 break
             if s in active:
                 continue
+            if page:
+                # every slot of a step: its request's pages, or a free slot's one
+                slots = range(max([s, *active]) + 1)
+                if sum(need[waiting[0]] if t == s else need[active[t][0]] if t in active else 1 for t in slots) > pages:
+                    break
             r = waiting.pop(0)
             session.reset(s)
             prompt = requests[r].prompt
@@ -91,7 +116,7 @@ def serve_continuous(session: DecodeSession, requests: Sequence[Request], filler
             continue
         n = max(active) + 1
         for s in range(n):
-            if s not in active and session.length(s) + 1 >= session.context:
+            if s not in active and (session.length(s) + 1 >= session.context or page and session.length(s) >= page):
                 session.reset(s)
         feed = [active[s][2] if s in active else filler for s in range(n)]
         how = [requests[active[s][0]].sampling if s in active else None for s in range(n)]
@@ -114,5 +139,11 @@ def serve_continuous(session: DecodeSession, requests: Sequence[Request], filler
             st[1] = k + 1
             if len(out[r]) >= requests[r].max_new:
                 del active[s]
+                if page:
+                    session.reset(s)
+        if page:
+            for s in range(max(active, default=-1) + 1, n):
+                if session.length(s):
+                    session.reset(s)
         step += 1
     return out

@@ -1,0 +1,30 @@
+"""Requests that come and go over a pool of pages smaller than all clients' contexts."""
+import pytest
+
+import emufpga_b200 as eb
+from emufpga_b200 import configs
+from emufpga_b200.sampling import Sampling
+from emufpga_b200.scheduler import Request, serve_continuous
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+@pytest.mark.parametrize("clients,pages", [(2, 5), (3, 6), (3, 4)])
+def test_requests_share_a_small_pool(prefill, clients, pages):
+    r = configs.TINY["qwen3-q6_k"]
+    m = eb.Model(eb.synth_gguf(r), r.shape)
+    sizes = [(10, 10), (40, 20), (3, 5), (17, 30), (2, 1), (33, 16)]
+    requests = [Request(configs.prompt_tokens(6, i, n, r.shape.vocab), new, arrival=2 * i,
+                        sampling=Sampling(0.9, top_k=30, seed=i) if i % 2 else None) for i, (n, new) in enumerate(sizes)]
+    s = eb.Session(m, clients, 64, paged=(pages, 16))
+    s.decode_step([1] * clients)
+    got = serve_continuous(s, requests, prefill=prefill)
+    assert s.free_pages == pages
+    one = eb.Session(m, 1, 64, paged=(4, 16))
+    assert got == [serve_continuous(one, [q], prefill=prefill)[0] for q in requests]
+    with pytest.raises(ValueError):
+        serve_continuous(eb.Session(m, clients, 64, paged=(2, 16)), requests)
+    for x in (s, one):
+        x.close()
+    m.close()

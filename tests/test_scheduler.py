@@ -132,3 +132,60 @@ def test_sampled_requests_draw_their_own_numbers():
     assert first[2][1] is None and first[3] == [0.0, 0.0]
     s = SampledSession()
     assert serve_continuous(s, [Request([1], 2)]) == [[2, 3]] and all(c[0] == "greedy" for c in s.calls)
+
+
+class PagedToySession(ToySession):
+    """A toy session over one pool of pages: what finds too few free pages raises."""
+
+    def __init__(self, max_clients, context, pages, page_tokens):
+        super().__init__(max_clients, context)
+        self.pages, self.page_tokens, self.least = pages, page_tokens, pages
+
+    def held(self, extra=0):
+        return sum(-(-(len(h) + (i < extra)) // self.page_tokens) for i, h in enumerate(self.hist))
+
+    @property
+    def free_pages(self):
+        return self.pages - self.held()
+
+    def prefill(self, client, tokens):
+        super().prefill(client, tokens)
+        if self.held() > self.pages:
+            raise RuntimeError("pages exhausted")
+
+    def decode_step(self, tokens, want_logits=False):
+        if self.held(len(tokens)) > self.pages:
+            raise RuntimeError("pages exhausted")
+        got = super().decode_step(tokens)
+        self.least = min(self.least, self.free_pages)
+        return got
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+@pytest.mark.parametrize("slots,context,pages,page,sizes", [
+    (2, 64, 5, 16, [(10, 10), (40, 20)]),                            # an idle slot under a long request
+    (2, 250, 16, 16, [(2, 8), (2, 200)]),
+    (3, 64, 4, 16, [(1, 60), (5, 5), (30, 30), (2, 2)]),             # one request takes all pages: one after the other
+    (8, 40, 10, 8, [(i % 7 + 1, 3 * i % 11 + 1) for i in range(30)]),
+    (4, 32, 4, 8, [(3, 25), (1, 1), (1, 30), (8, 8), (9, 8), (16, 1)])])
+def test_a_pool_smaller_than_all_clients_serves_every_request(prefill, slots, context, pages, page, sizes):
+    reqs = [Request([(7 * i + j) % 50 for j in range(n)], new, arrival=i // 3) for i, (n, new) in enumerate(sizes)]
+    sess = PagedToySession(slots, context, pages, page)
+    sess.hist[slots - 1] = [1] * min(context, page + 1)              # what an earlier run left
+    got = serve_continuous(sess, reqs, prefill=prefill)
+    assert got == [alone(r, context) for r in reqs]
+    assert sess.least >= 0 and sess.free_pages == pages              # all pages are back
+
+
+def test_requests_share_a_pool_as_far_as_it_goes():
+    # two requests of two pages each fit four pages together, the third one waits
+    sess = PagedToySession(3, 64, 4, 16)
+    serve_continuous(sess, [Request([1] * 16, 10)] * 3)
+    assert max(sess.steps) == 2 and len(sess.steps) == 2 * 25
+
+
+def test_a_request_that_no_pool_of_pages_holds_is_refused():
+    with pytest.raises(ValueError):
+        serve_continuous(PagedToySession(2, 64, 3, 16), [Request([1], 2), Request([1] * 30, 20)])
+    got = serve_continuous(PagedToySession(2, 64, 3, 16), [Request([1] * 30, 19)])
+    assert len(got[0]) == 19
