@@ -1061,7 +1061,7 @@ void check_status(spm_session* s) {
         *s->h_status = 0;
         cudaMemsetAsync(s->status, 0, sizeof(int32_t), s->stream);
         cudaStreamSynchronize(s->stream);
-        if (code >= SPM_PAGE_LENGTH && code < SPM_PAGE_WAIT)
+        if (code >= SPM_PAGE_LENGTH && code <= SPM_PAGE_SHARED && code != SPM_PAGE_WAIT)
             fail(SPM_E_CUDA, "the paged cache's tables are not consistent (code " + std::to_string(code) + ")");
         fail(SPM_E_TIMEOUT, "a device wait gave up (code " + std::to_string(code) + ")");
     }

@@ -53,7 +53,7 @@ __device__ __forceinline__ long long warp_scan(long long v, int lane) {
 __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanArgs a) {
     extern __shared__ int32_t sm[];
     __shared__ long long part[3][kPlanWarps];
-    __shared__ int bad;
+    __shared__ int bad, shared_pages;
     cg::cluster_group cl = cg::this_cluster();
     const int R = a.requests, P = a.page, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = int(cl.block_rank()), ranks = int(cl.num_blocks());
@@ -61,18 +61,19 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanArgs 
     int32_t* E = S + R + 1;        // pages back before row r
     int32_t* F = E + R + 1;        // pages taken before row r
     int32_t* C = F + R + 1;        // cached
-    if (tid == 0) bad = 0;
+    if (tid == 0) bad = shared_pages = 0;
     __syncthreads();
     const int count = *a.count;
     // a thread's share of the rows, then the exclusive sums over threads
     const int per = (R + kPlanThreads - 1) / kPlanThreads, r0 = min(R, tid * per), r1 = min(R, r0 + per);
     const long long cap = (long long)a.width << a.shift;
     long long s = 0, e = 0, f = 0;
-    bool wrong = false;
+    bool wrong = false, both = false;
     for (int r = r0; r < r1; r++) {
         const long long c = a.cached[r], n = a.fresh[r], d = a.ended ? a.ended[r] : 0;
         C[r] = int32_t(c);
         wrong |= c < 0 || n < 0 || d < 0 || c + n > cap || d > cap;
+        both |= c > 0 && d > 0;  // the row's first pages would lie on the stack and in the row
         S[r] = int32_t(n);
         E[r] = int32_t((d + P - 1) >> a.shift);
         F[r] = int32_t(((c + n + P - 1) >> a.shift) - ((c + P - 1) >> a.shift));
@@ -81,6 +82,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanArgs 
         f += F[r];
     }
     if (wrong) bad = 1;
+    if (both) shared_pages = 1;
     const long long si = warp_scan(s, lane), ei = warp_scan(e, lane), fi = warp_scan(f, lane);
     if (lane == 31) part[0][warp] = si, part[1][warp] = ei, part[2][warp] = fi;
     __syncthreads();
@@ -96,6 +98,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanArgs 
     else if (count < 0 || count + te > a.pages) code = SPM_PAGE_STACK;
     else if (tf > count + te) code = SPM_PAGE_FREE;
     else if (ts > a.tokens) code = SPM_PAGE_TOKENS;
+    else if (shared_pages) code = SPM_PAGE_SHARED;
     if (code) {
         // nothing moves: no CTA of the cluster writes table or stack
         for (int i = rank * kPlanThreads + tid; i < a.tokens; i += ranks * kPlanThreads) a.positions[i] = a.slots[i] = -1;

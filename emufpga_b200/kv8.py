@@ -25,7 +25,7 @@ DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 STATUS = {11: "a length is negative or past its table", 12: "more pages wanted than free",
           13: "more tokens than the slot map holds", 14: "more pages back than the pool has",
           15: "a page or slot is not in the pool", 16: "a request's rows are not what the call says",
-          17: "a device wait gave up"}
+          17: "a device wait gave up", 18: "a row gives back pages that its cached tokens keep"}
 
 
 _I32 = torch.int32
@@ -86,7 +86,7 @@ def plan(cached, new, table, free, count, page_tokens: int, tokens: int, ended=N
 
     Row r of ``table`` (requests x width) holds ``cached[r]`` tokens and takes
     ``new[r]`` more; the pages of ``ended[r]`` tokens of its former request go
-    back first.  ``free`` is the stack of free pages, ``count`` its height (one
+    back first (such a row has no cached tokens).  ``free`` is the stack of free pages, ``count`` its height (one
     int32), ``left`` (default: ``count``) receives the new height.  ``tokens``
     is the length of the slot map, -1 behind the last token."""
     index = _cuda(table, "table")

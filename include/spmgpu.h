@@ -474,8 +474,10 @@ enum {
     SPM_PAGE_ID = 15,      /* a page or slot that is not in the pool          */
     SPM_PAGE_QUERIES = 16, /* a request with more queries than `most`, or
                               starts that do not ascend within the rows       */
-    SPM_PAGE_WAIT = 17     /* a bounded device wait gave up: the outputs are
+    SPM_PAGE_WAIT = 17,    /* a bounded device wait gave up: the outputs are
                               not to be used                                  */
+    SPM_PAGE_SHARED = 18   /* a row gives back pages that its cached tokens
+                              keep                                            */
 };
 
 /* Block table, slot map and free stack of one tick, from the requests'
@@ -489,8 +491,8 @@ enum {
  * tokens in the call, and lens = cached + fresh; per token: its position in its
  * request and its slot, page * page_tokens + offset, -1 behind the last token up
  * to `tokens`.  A row whose request has ended keeps its entries until they are
- * overwritten.  A plan that fails (status: SPM_PAGE_LENGTH, _FREE, _TOKENS,
- * _STACK, in this order) leaves table and stack as they were and returns no
+ * overwritten; one with ended tokens has none cached.  A plan that fails (status: the
+ * first of SPM_PAGE_LENGTH, _STACK, _FREE, _TOKENS, _SHARED) leaves table and stack as they were and returns no
  * tokens: starts and lens 0, positions and slots -1. */
 spm_status spm_page_plan(int device, const int32_t* cached, const int32_t* fresh, const int32_t* ended,
                          int32_t requests, int32_t page_tokens, int32_t* table, int32_t table_width,

@@ -5,9 +5,32 @@ import numpy as np
 import pytest
 import torch
 
+from emufpga_b200 import kv8
+from emufpga_b200._lib import SpmError
 from test_gpu_serving import HALF, TYPES, check_append, gen, ints, pool
 
 pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------- plan --
+@pytest.mark.parametrize("R", [3, 700])
+@pytest.mark.parametrize("cached,new", [(16, 0), (1, 1), (20, 30)])
+def test_plan_refuses_a_row_that_gives_back_what_it_keeps(R, cached, new):
+    cached, new, ended = np.where(np.arange(R) == R - 1, cached, 0), np.where(np.arange(R) == R - 1, new, 1), np.zeros(R, int)
+    ended[R - 1] = 1
+    table = np.full((R, 4), -1)
+    table[R - 1, :2] = 0, 1
+    free = np.concatenate([np.arange(2, 2 * R), np.full(2, -1)])
+    t, f, c, status = ints(table), ints(free), ints([2 * R - 2]), ints([0])
+    got = kv8.plan(ints(cached), ints(new), t, f, c, 16, 800, ended=ints(ended), status=status)
+    assert status.item() == 18
+    with pytest.raises(SpmError):
+        kv8.check(status)
+    assert not got.starts.any() and not got.lens.any() and (got.slots == -1).all() and (got.positions == -1).all()
+    assert t.tolist() == table.tolist() and f.tolist() == free.tolist() and c.item() == 2 * R - 2
+    cached[R - 1] = 0  # the same without tokens kept
+    kv8.plan(ints(cached), ints(new), t, f, c, 16, 800, ended=ints(ended), status=status)
+    kv8.check(status)
 
 
 # -------------------------------------------------------------- attention --
