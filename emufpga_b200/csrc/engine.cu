@@ -1223,13 +1223,6 @@ void prefill_chunk(spm_session* s, int client, const uint32_t* tokens, int T, in
         CUDA_OK(cudaMemcpyAsync(s->pos + client, at, sizeof(int32_t), cudaMemcpyHostToDevice, st));
         CUDA_OK(cudaMemcpyAsync(s->pg.fresh, at + 1, sizeof(int32_t), cudaMemcpyHostToDevice, st));
         paged_plan(s, client, 1, s->pg.fresh, nullptr, T);
-        const spm_kv8 cache = paged_layer(s, 0);
-        uint64_t need = 0;
-        inner(spm_kv8_attention_workspace(&cache, int32_t(c.heads), 1, T, s->pg.width, &need));
-        if (need > s->pg.work_bytes) {  // (steps keep the first one: their graphs hold it)
-            s->pg.work = s->alloc<uint8_t>(need);
-            s->pg.work_bytes = need;
-        }
     }
     CUDA_OK(cudaMemcpyAsync(P.tokens, tokens, size_t(T) * sizeof(uint32_t), cudaMemcpyHostToDevice, st));
     CUDA_OK(cudaMemcpyAsync(P.qpos, qpos.data(), size_t(T) * sizeof(int32_t), cudaMemcpyHostToDevice, st));
@@ -1675,10 +1668,13 @@ void create_session(spm_model* m, int32_t max_clients, int32_t max_context, int3
         g.lens = s->alloc<int32_t>(n);
         g.positions = s->alloc<int32_t>(rows);
         g.slots = s->alloc<int32_t>(rows);
-        for (int b = 1; b <= std::min<int>(max_clients, kMaxBatch); b++) {
-            inner(spm_kv8_attention_workspace(&probe, int32_t(c.heads), b, 1, g.width, &bytes));
+        // scratch for every step and every chunk of a prompt
+        auto room = [&](int requests, int most) {
+            inner(spm_kv8_attention_workspace(&probe, int32_t(c.heads), requests, most, g.width, &bytes));
             g.work_bytes = std::max(g.work_bytes, bytes);
-        }
+        };
+        for (int b = 1; b <= std::min<int>(max_clients, kMaxBatch); b++) room(b, 1);
+        for (int T = 1; T <= std::min<int>(max_context, kPrefillRows); T++) room(1, T);
         g.work = s->alloc<uint8_t>(g.work_bytes);
         std::vector<int32_t> ids(std::max<size_t>(pages, n), 1);
         CUDA_OK(cudaMemcpy(g.ones, ids.data(), n * sizeof(int32_t), cudaMemcpyHostToDevice));
@@ -1923,9 +1919,8 @@ spm_status spm_prefill(spm_session* s, int32_t client, const uint32_t* tokens, i
             if (tokens[t] >= m->cfg.vocab) fail(SPM_E_ARG, "token id out of range");
         if (int64_t(s->lens[client]) + len > s->context)
             fail(SPM_E_CONTEXT, "context " + std::to_string(s->context) + " exhausted");
-        int take = 0;
         if (s->paged()) {
-            take = s->pg.need(s->lens[client] + len) - s->pg.need(s->lens[client]);
+            const int take = s->pg.need(s->lens[client] + len) - s->pg.need(s->lens[client]);
             if (take > s->pg.free)
                 fail(SPM_E_CONTEXT, "the prompt needs " + std::to_string(take) + " pages, " + std::to_string(s->pg.free) +
                                         " are free");
@@ -1936,9 +1931,9 @@ spm_status spm_prefill(spm_session* s, int32_t client, const uint32_t* tokens, i
         for (int32_t t0 = 0; t0 < len; t0 += kPrefillRows) {
             const int T = std::min(kPrefillRows, len - t0);
             prefill_chunk(s, client, tokens + t0, T, s->lens[client]);
+            if (s->paged()) s->pg.free -= s->pg.need(s->lens[client] + T) - s->pg.need(s->lens[client]);
             s->lens[client] += T;
         }
-        s->pg.free -= take;
         const int32_t pos = s->lens[client];
         CUDA_OK(cudaMemcpyAsync(s->pos + client, &pos, sizeof(int32_t), cudaMemcpyHostToDevice, s->stream));
         CUDA_OK(cudaMemcpyAsync(s->h_status, s->status, sizeof(int32_t), cudaMemcpyDeviceToHost, s->stream));

@@ -1,5 +1,6 @@
 """Requests that come and go over a pool of pages smaller than all clients' contexts."""
 import pytest
+import torch
 
 import emufpga_b200 as eb
 from emufpga_b200 import configs
@@ -27,4 +28,21 @@ def test_requests_share_a_small_pool(prefill, clients, pages):
         serve_continuous(eb.Session(m, clients, 64, paged=(2, 16)), requests)
     for x in (s, one):
         x.close()
+    m.close()
+
+
+def test_prompts_take_no_device_memory_of_their_own():
+    # a prompt's scratch is there before its pages are taken: nothing can fail between the two
+    r = configs.TINY["qwen3-q6_k"]
+    m = eb.Model(eb.synth_gguf(r), r.shape)
+    s = eb.Session(m, 2, 8192, paged=(1024, 16))
+    s.prefill(0, [1, 2])             # the layers' buffers
+    s.decode_step([1, 2])
+    before = torch.cuda.mem_get_info()[0]
+    for n in (20, 64, 100, 300, 2500):
+        s.reset(0)
+        s.prefill(0, configs.prompt_tokens(7, 0, n, r.shape.vocab))
+        assert s.length(0) == n and s.free_pages == 1024 - -(-n // 16) - 1
+    assert torch.cuda.mem_get_info()[0] == before
+    s.close()
     m.close()
