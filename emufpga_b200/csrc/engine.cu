@@ -192,8 +192,11 @@ struct spm_session {
     T* alloc(size_t count) {
         void* p = nullptr;
         CUDA_OK(cudaMalloc(&p, std::max<size_t>(count, 1) * sizeof(T)));
-        CUDA_OK(cudaMemset(p, 0, std::max<size_t>(count, 1) * sizeof(T)));
         allocs.push_back(p);
+        // on the session's own stream, which has no order against the default one, and done
+        // before a copy on that one fills the memory
+        CUDA_OK(cudaMemsetAsync(p, 0, std::max<size_t>(count, 1) * sizeof(T), stream));
+        CUDA_OK(cudaStreamSynchronize(stream));
         return static_cast<T*>(p);
     }
 };

@@ -46,3 +46,26 @@ def test_prompts_take_no_device_memory_of_their_own():
     assert torch.cuda.mem_get_info()[0] == before
     s.close()
     m.close()
+
+
+@pytest.mark.parametrize("paged", [None, (40, 16)])
+def test_prompts_do_not_depend_on_the_default_stream(paged):
+    # the first prompt's buffers are cleared in order with what uses them, whatever else the device does
+    r = configs.TINY["qwen3-q6_k"]
+    m = eb.Model(eb.synth_gguf(r), r.shape)
+    prompt = configs.prompt_tokens(8, 0, 200, r.shape.vocab)
+    want = None
+    for busy in (False, True):
+        s = eb.Session(m, 2, 300, paged=paged)
+        if busy:
+            torch.cuda._sleep(200_000_000)  # a tenth of a second of the default stream
+        for _ in range(20):
+            s.reset(0)
+            s.prefill(0, prompt)
+            _, got = s.decode_step([3, 4], want_logits=True)
+            s.reset(1)
+            want = got if want is None else want
+            assert (got == want).all()
+        torch.cuda.synchronize()
+        s.close()
+    m.close()
