@@ -87,6 +87,8 @@ __global__ void __launch_bounds__(256) qk_rope_append_kernel(const QkArgs a) {
     __shared__ float red[33];
     const int t = blockIdx.x, qw = a.heads * a.head_dim, kvw = a.kv_heads * a.head_dim, hd = a.head_dim;
     const bool llama = a.family == SPM_FAMILY_LLAMA;
+    const int pos = a.pos ? a.pos[t] : a.pos0 + t, half = hd / 2;
+    if (pos < 0) return;  // of no request: a plan that failed gives no positions
     float* q = qk;
     float* k = qk + qw;
     const float* qg = a.q + size_t(t) * qw;
@@ -119,7 +121,6 @@ __global__ void __launch_bounds__(256) qk_rope_append_kernel(const QkArgs a) {
         }
         __syncthreads();
     }
-    const int pos = a.pos ? a.pos[t] : a.pos0 + t, half = hd / 2;
     const float2* rt = a.rope + size_t(pos) * half;
     for (int e = threadIdx.x; e < (a.heads + a.kv_heads) * half; e += blockDim.x) {
         const int h = e / half, j = e % half;

@@ -20,7 +20,7 @@ struct QkArgs {
     const float *k, *v;            // [T][kv_heads * head_dim]
     float *kcache, *vcache;        // [client][layer][context][kv_width], or nullptr: no append
     // Without a cache (a paged session's): row t stands at pos[t], and its key goes to
-    // k_out (which may be k).
+    // k_out (which may be k); a row whose pos is negative is left as it is.
     const int32_t* pos;
     float* k_out;
     uint16_t *kplanes, *vplanes;   // the rows as three bf16 parts (AttnParams), or nullptr

@@ -1,9 +1,12 @@
 """Requests that come and go over a pool of pages smaller than all clients' contexts."""
+import ctypes as C
+
 import pytest
 import torch
 
 import emufpga_b200 as eb
-from emufpga_b200 import configs
+from emufpga_b200 import _lib, configs
+from emufpga_b200._lib import LLAMA, QWEN3
 from emufpga_b200.sampling import Sampling
 from emufpga_b200.scheduler import Request, serve_continuous
 
@@ -69,3 +72,35 @@ def test_prompts_do_not_depend_on_the_default_stream(paged):
         torch.cuda.synchronize()
         s.close()
     m.close()
+
+
+class QkArgs(C.Structure):
+    """csrc/prefill.h's."""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "kcache", "vcache", "pos", "k_out", "kplanes", "vplanes", "rope",
+                                          "q_norm", "k_norm")]
+    _fields_ += [(n, C.c_int32) for n in ("client", "layer", "layers", "context", "pos0", "heads", "kv_heads", "head_dim",
+                                          "family")]
+    _fields_ += [("eps", C.c_float)]
+
+
+@pytest.mark.parametrize("family", [LLAMA, QWEN3])
+def test_rows_without_a_position_are_left_as_they_are(family):
+    # a plan that fails on the device gives positions of -1, before the first angle
+    launch = _lib.lib()["_ZN3spm21launch_qk_rope_appendERKNS_6QkArgsEiP11CUstream_st"]
+    launch.argtypes, launch.restype = [C.POINTER(QkArgs), C.c_int, C.c_void_p], C.c_int
+    T, heads, kv_heads, dim, context = 5, 4, 2, 64, 8
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn(T, h * dim, device="cuda", generator=g) for h in (heads, kv_heads, kv_heads))
+    rope = torch.randn(context, dim, device="cuda", generator=g)
+    gains = torch.ones(dim, device="cuda")
+    pos = torch.tensor([3, -1, 0, -1, 7], dtype=torch.int32, device="cuda")
+    had = q.clone(), k.clone()
+    a = QkArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), pos=pos.data_ptr(), k_out=k.data_ptr(), rope=rope.data_ptr(),
+               q_norm=gains.data_ptr(), k_norm=gains.data_ptr(), layers=1, context=context, heads=heads, kv_heads=kv_heads,
+               head_dim=dim, family=family, eps=1e-5)
+    torch.cuda.synchronize()
+    assert launch(C.byref(a), T, None) == 0
+    torch.cuda.synchronize()
+    for now, then in zip((q, k), had):
+        assert torch.equal(now[[1, 3]], then[[1, 3]])
+        assert (now[[0, 2, 4]] != then[[0, 2, 4]]).any(1).all()
