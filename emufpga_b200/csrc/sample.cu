@@ -83,6 +83,7 @@ struct alignas(16) Shared {
     uint32_t seg_count[kSampleClusters * kSampleThreads / 32], seg_ties[kSampleClusters * kSampleThreads / 32];
     float top[kSampleClusters];           // each CTA's largest logit
     uint32_t listed;                      // length of this CTA's list
+    uint32_t equal;                       // tokens on the border up to the last one kept
     int bin_out;
     u64 pick_before, pick_ties, pick_total, pick_count;
     int pick_seg;
@@ -580,13 +581,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
                 __syncthreads();
                 const int last = max(0, s.bin_out);
                 thr = uint32_t(s.sorted[last] >> 32);
-                // its rank among the tokens that equal it (they lie side by side)
-                if (tid == 0) s.listed = 0;
+                // its rank among the tokens that equal it (they lie side by side); `listed` stands,
+                // other CTAs may still be adding the lengths up
+                if (tid == 0) s.equal = 0;
                 __syncthreads();
                 for (int i = tid; i <= last; i += kSampleThreads)
-                    if (uint32_t(s.sorted[i] >> 32) == thr) atomicAdd(&s.listed, 1u);
+                    if (uint32_t(s.sorted[i] >> 32) == thr) atomicAdd(&s.equal, 1u);
                 __syncthreads();
-                if (tid < C) *cl.map_shared_rank(&s.border, tid) = u64(thr) << 32 | s.listed;
+                if (tid < C) *cl.map_shared_rank(&s.border, tid) = u64(thr) << 32 | s.equal;
             }
             cl.sync();
             thr = uint32_t(s.border >> 32);

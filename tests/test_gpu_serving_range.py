@@ -5,9 +5,9 @@ import numpy as np
 import pytest
 import torch
 
-from emufpga_b200 import kv8
+from emufpga_b200 import kv8, sampling
 from emufpga_b200._lib import SpmError
-from test_gpu_serving import HALF, TYPES, check_append, gen, ints, pool
+from test_gpu_serving import HALF, TYPES, check_append, check_sample, gen, ints, pool
 
 pytestmark = pytest.mark.gpu
 
@@ -155,3 +155,20 @@ def test_append_where_the_scale_grows_by_more_than_a_float_holds(dtype, old, new
     check_append(c, x[0, :4], x[1, :4], [16, 17, 18, 19])
     check_append(c, x[0, 4:], x[1, 4:], [20])
     assert not c.k_codes[1, :, :4].any() and c.k_codes[1, :, 4].any()
+
+
+# --------------------------------------------------------------- sampling --
+@pytest.mark.parametrize("vocab,every", [(5000, 3), (40000, 20), (70000, 40), (151936, 100)])
+def test_sample_of_many_ties_over_all_slices(vocab, every):
+    # 1500 and more equal tokens on the border of top-p, some in every CTA's slice
+    n = 16
+    x = torch.randn(n, vocab, device="cuda", generator=gen(9)) - 40
+    x[:, ::every] = 3.0
+    rng = np.random.default_rng(vocab)
+    p, u = rng.uniform(0.05, 0.99, n), rng.random(n)
+    first = check_sample(x, np.ones(n), [0] * n, p, [0.0] * n, u)
+    f = lambda v: torch.tensor(v, dtype=torch.float32, device="cuda")  # noqa: E731
+    pp, uu = f(p), f(u)
+    for _ in range(100):
+        again = sampling.sample(x, uu, top_p=pp)
+        assert torch.equal(again.token, first.token) and torch.equal(again.kept, first.kept) and torch.equal(again.prob, first.prob)
