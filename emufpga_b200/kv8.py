@@ -65,10 +65,12 @@ def _on(index: int, stream):
 
 
 def check(status: torch.Tensor) -> None:
-    """Raise for a status word that a call has set, and clear it (synchronises)."""
+    """Raise for a status word that a call has set, and clear it.  Waits for every stream of its device."""
+    torch.cuda.synchronize(status.device)
     code = int(status.item())
     if code:
         status.zero_()
+        torch.cuda.synchronize(status.device)  # before a call on any stream sets it again
         raise SpmError(-9 if code in (12, 13) else -8 if code == 17 else -1, STATUS.get(code, f"code {code}"))
 
 
@@ -240,7 +242,7 @@ class Cache:
         return out
 
     def check(self) -> None:
-        """Raise for what the device found wrong in the calls so far (synchronises)."""
+        """Raise for what the device found wrong in the calls so far, on whichever stream (synchronises)."""
         check(self.status)
 
 

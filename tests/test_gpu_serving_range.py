@@ -172,3 +172,23 @@ def test_sample_of_many_ties_over_all_slices(vocab, every):
     for _ in range(100):
         again = sampling.sample(x, uu, top_p=pp)
         assert torch.equal(again.token, first.token) and torch.equal(again.kept, first.kept) and torch.equal(again.prob, first.prob)
+
+
+# ---------------------------------------------------------------- streams --
+def test_check_sees_calls_on_every_stream():
+    c = pool(4, 16, 2, 64)
+    x, bad, none, much = torch.zeros(1, 2, 64, device="cuda"), ints([77]), ints([0]), ints([17])
+    pages = kv8.Pages(1, 1, 1, 16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(50_000_000)
+            c.append(x, x, bad)
+            pages.plan(none, much, 17)
+        with pytest.raises(SpmError):
+            c.check()
+        with pytest.raises(SpmError):
+            pages.check()
+        c.check()
+        pages.check()
