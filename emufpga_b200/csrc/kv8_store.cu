@@ -300,6 +300,7 @@ spm_status spm_kv8_append(const spm_kv8* c, uint32_t dtype, const void* k, int64
         kv8_check(c);
         kv8_check_type(dtype);
         if (tokens < 0) fail(SPM_E_ARG, "negative token count");
+        if (tokens > INT32_MAX - 65536) fail(SPM_E_ARG, "too many tokens for one call");  // (a window's end fits 32 bits)
         if (tokens == 0) return;
         if (!k || !v || !slots) fail(SPM_E_ARG, "null keys, values or slots");
         DeviceScope scope(c->device);

@@ -27,6 +27,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kPlanThreads = 512, kPlanWarps = kPlanThreads / 32;
 constexpr int kPlanRequests = 8192;
+constexpr int kPlanTokens = INT32_MAX - 65536;  // the last turn's index fits 32 bits
 
 struct PlanArgs {
     const int32_t *cached, *fresh, *ended;
@@ -224,6 +225,7 @@ spm_status spm_page_plan(int device, const int32_t* cached, const int32_t* fresh
         if (page_tokens < 16 || page_tokens > 256 || (page_tokens & (page_tokens - 1)))
             fail(SPM_E_ARG, "page_tokens is 16, 32, 64, 128 or 256");
         if (tokens < 0 || pages < 0 || table_width < 0) fail(SPM_E_ARG, "negative size");
+        if (tokens > kPlanTokens) fail(SPM_E_ARG, "a plan takes up to 2^31 - 65537 tokens");
         if (int64_t(table_width) * page_tokens > INT32_MAX || int64_t(pages) * page_tokens > INT32_MAX)
             fail(SPM_E_ARG, "positions and slots are 32-bit: table_width and pages times page_tokens must fit");
         if (!free_count || !free_left || !starts) fail(SPM_E_ARG, "null free_count, free_left or starts");

@@ -490,10 +490,11 @@ enum {
  * may be the same word).  Per request: starts[requests + 1], the first of its
  * tokens in the call, and lens = cached + fresh; per token: its position in its
  * request and its slot, page * page_tokens + offset, -1 behind the last token up
- * to `tokens`.  A row whose request has ended keeps its entries until they are
- * overwritten; one with ended tokens has none cached.  A plan that fails (status: the
- * first of SPM_PAGE_LENGTH, _STACK, _FREE, _TOKENS, _SHARED) leaves table and stack as they were and returns no
- * tokens: starts and lens 0, positions and slots -1. */
+ * to `tokens` (at most 2^31 - 65537).  A row whose request has ended keeps its
+ * entries until they are overwritten; one with ended tokens has none cached.  A
+ * plan that fails (status: the first of SPM_PAGE_LENGTH, _STACK, _FREE, _TOKENS,
+ * _SHARED) leaves table and stack as they were and returns no tokens: starts and
+ * lens 0, positions and slots -1. */
 spm_status spm_page_plan(int device, const int32_t* cached, const int32_t* fresh, const int32_t* ended,
                          int32_t requests, int32_t page_tokens, int32_t* table, int32_t table_width,
                          int32_t* free_pages, int32_t pages, const int32_t* free_count, int32_t* free_left,
