@@ -7,8 +7,9 @@ leaves the device, and a tick can be captured into a CUDA graph.  What only the
 device can see (a length past its table, a page that is not in the pool, an
 empty stack of free pages) goes into a status word; ``check`` reads it and
 raises.  The calls run on the current stream of the tensors' device, or on
-``stream``.  The reference keeps f32 rows of one client
-(spm-kv/src/cache.rs:49-58); see include/spmgpu.h for the definitions.
+``stream``, and have no backward pass (a tensor that requires a gradient is
+refused).  The reference keeps f32 rows of one client (spm-kv/src/cache.rs:49-58);
+see include/spmgpu.h for the definitions.
 """
 from __future__ import annotations
 
@@ -55,6 +56,11 @@ def _cuda(t: torch.Tensor, what: str) -> int:
     if index < 0:
         raise SpmError(-1, f"{what} must be a CUDA tensor")
     return index
+
+
+def _forward_only(t: torch.Tensor, what: str) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise SpmError(-1, f"{what} requires a gradient, and the serving operators have none: call them under torch.no_grad()")
 
 
 def _on(index: int, stream):
@@ -186,6 +192,7 @@ class Cache:
             raise SpmError(-1, f"{what} must be tokens x heads x {self.head_dim} on {self.device}")
         if t.stride(2) != 1 and t.numel():
             raise SpmError(-1, f"{what} must be contiguous along head_dim")
+        _forward_only(t, what)
         return t.data_ptr()
 
     def append(self, k, v, slots, stream=None) -> None:

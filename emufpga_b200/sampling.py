@@ -13,7 +13,7 @@ import numpy as np
 import torch
 
 from ._lib import SpmError, call
-from .kv8 import _cuda, _dtype, _on
+from .kv8 import _cuda, _dtype, _forward_only, _on
 
 
 @dataclasses.dataclass(frozen=True)
@@ -49,6 +49,7 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, stre
     index = _cuda(logits, "logits")
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise SpmError(-1, "logits must be rows x vocab, contiguous along vocab")
+    _forward_only(logits, "logits")
     n, vocab = logits.shape
 
     def per_row(t, what, dtype=torch.float32):

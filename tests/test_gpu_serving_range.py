@@ -192,3 +192,23 @@ def test_check_sees_calls_on_every_stream():
             pages.check()
         c.check()
         pages.check()
+
+
+# -------------------------------------------------------------- gradients --
+def test_tensors_that_require_a_gradient_are_refused():
+    c = pool(4, 16, 2, 64)
+    x = torch.randn(2, 2, 64, device="cuda", generator=gen(2))
+    starts, lens, table, u = ints([0, 1, 2]), ints([16, 5]), ints([[0], [1]]), torch.full((2,), 0.5, device="cuda")
+    calls = {"q": lambda t: c.attention(t, starts, lens, table, 1), "out": lambda t: c.attention(x, starts, lens, table, 1, out=t),
+             "k": lambda t: c.append(t, x, ints([0, 1])), "v": lambda t: c.append(x, t, ints([0, 1])),
+             "logits": lambda t: sampling.sample(t.flatten(1), u).token}
+    for f in calls.values():
+        leaf = x.clone().requires_grad_()
+        with pytest.raises(SpmError, match="gradient"):
+            f(leaf * 1.0)
+        with pytest.raises(SpmError, match="gradient"):
+            f(leaf)
+        with torch.no_grad():
+            got = f(leaf)
+        want = f(x.clone())
+        assert want is None or torch.equal(got, want)
