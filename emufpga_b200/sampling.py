@@ -27,8 +27,8 @@ class Sampling:
     seed: int = 0
 
     def __post_init__(self):
-        if not self.temperature >= 0 or not self.top_k >= 0 or not 0 <= self.top_p or not 0 <= self.min_p <= 1:
-            raise ValueError("temperature, top_k and top_p are not negative, min_p lies in [0, 1]")
+        if not self.temperature >= 0 or not 0 <= self.top_k < 2 ** 31 or not 0 <= self.top_p or not 0 <= self.min_p <= 1:
+            raise ValueError("temperature, top_k and top_p are not negative, top_k is under 2^31, min_p lies in [0, 1]")
 
     def numbers(self) -> np.random.Generator:
         return np.random.default_rng(self.seed)

@@ -2,6 +2,7 @@
 import pytest
 
 from emufpga_b200 import _lib
+from emufpga_b200.sampling import Sampling
 from test_serving_host import A, cache, planned, refused
 
 
@@ -9,3 +10,11 @@ from test_serving_host import A, cache, planned, refused
 def test_a_slot_map_whose_indexes_pass_32_bits_is_refused(tokens):
     planned(tokens=tokens)
     refused("spm_kv8_append", cache(), _lib.F32, A, 64, 64, A, 64, 64, tokens, A, None)
+
+
+@pytest.mark.parametrize("top_k", [2 ** 31, 2 ** 32 + 1])
+def test_a_top_k_past_32_bits_is_refused(top_k):
+    # (a C int32 would hold -2^31, off, and 1, greedy)
+    with pytest.raises(ValueError):
+        Sampling(top_k=top_k)
+    assert Sampling(top_k=2 ** 31 - 1).top_k == 2 ** 31 - 1
