@@ -777,22 +777,43 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     }
 }
 
-template <class T>
-void launch_sample(const SampleArgs& a, int rows, int ctas, size_t smem, cudaStream_t st) {
-    static std::atomic<unsigned long long> done{0}, wide{0};
-    allow_smem(sample_kernel<T>, sizeof(Shared) + kSampleSlice, done);
-    if (ctas > 8) allow_wide_clusters(sample_kernel<T>, wide);
+cudaLaunchConfig_t sample_config(int rows, int ctas, size_t smem, cudaStream_t st, cudaLaunchAttribute* attr) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(rows) * unsigned(ctas));
     cfg.blockDim = dim3(kSampleThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = unsigned(ctas);
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr->id = cudaLaunchAttributeClusterDimension;
+    attr->val.clusterDim.x = unsigned(ctas);
+    attr->val.clusterDim.y = attr->val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    return cfg;
+}
+
+// Whether the current device has room for a cluster of kSampleClusters CTAs with the longest
+// slices (asked for once per device: a part of a GPU may have too few SMs side by side).
+template <class T>
+bool wide_clusters_fit() {
+    static std::atomic<int> known[64] = {};  // 1: no, 2: yes
+    static std::atomic<unsigned long long> wide{0};
+    int d = 0;
+    CUDA_OK(cudaGetDevice(&d));
+    if (d < 64 && known[d]) return known[d] == 2;
+    allow_wide_clusters(sample_kernel<T>, wide);
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = sample_config(1, kSampleClusters, sizeof(Shared) + kSampleSlice, nullptr, &attr);
+    int n = 0;
+    const bool fits = cudaOccupancyMaxActiveClusters(&n, sample_kernel<T>, &cfg) == cudaSuccess && n > 0;
+    if (!fits) cudaGetLastError();
+    if (d < 64) known[d] = fits ? 2 : 1;
+    return fits;
+}
+
+template <class T>
+void launch_sample(const SampleArgs& a, int rows, int ctas, size_t smem, cudaStream_t st) {
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = sample_config(rows, ctas, smem, st, &attr);
     CUDA_OK(cudaLaunchKernelEx(&cfg, sample_kernel<T>, a));
 }
 
@@ -801,11 +822,13 @@ void launch_type(SampleArgs a, int rows, cudaStream_t st) {
     // A row's chain of passes and barriers takes as long as 32768 logits of one CTA (20 of
     // 28 us for one row of 151936 on 16 CTAs), and CTAs beyond two an SM (one, where the
     // slices are long) come in waves: the number of CTAs with the least waves x (chain +
-    // slice), 2048 logits each at least.  16 (not portable, but a B200's groups of SMs hold
-    // them) from 65537 logits on while that leaves an SM to each: 8 rows of 151936 take 38 us
-    // so where clusters of 8 take 44, of 49152 30 and 25, 16 rows 66 and 48.  (1024 threads
-    // instead of 512, one CTA an SM: 32 us instead of 35 for top-p on one row, 66 instead of
-    // 38 on eight.)
+    // slice), 2048 logits each at least.  16 (not portable: where the device holds such a
+    // cluster, as a whole B200 does) from 65537 logits on while that leaves an SM to each:
+    // 8 rows of 151936 take 38 us so where clusters of 8 take 44, of 49152 30 and 25, 16 rows
+    // 66 and 48.  (1024 threads instead of 512, one CTA an SM: 32 us instead of 35 for top-p
+    // on one row, 66 instead of 38 on eight.)
+    static std::atomic<unsigned long long> done{0};
+    allow_smem(sample_kernel<T>, sizeof(Shared) + kSampleSlice, done);
     const int sms = device_sms();
     const int per = 4 * 32;  // four for each warp, of 32 at most
     auto slice_of = [&](int ctas) { return ((a.vocab + ctas - 1) / ctas + per - 1) / per * per; };
@@ -821,7 +844,7 @@ void launch_type(SampleArgs a, int rows, cudaStream_t st) {
         const int64_t cost = (int64_t(rows) * c + at_once - 1) / at_once * (32768 + (held ? 1 : 2) * int64_t(slice_of(c)));
         if (cost <= least) least = cost, ctas = c;
     }
-    if (a.vocab > 65536 && int64_t(rows) * kSampleClusters <= sms) ctas = kSampleClusters;
+    if (a.vocab > 65536 && int64_t(rows) * kSampleClusters <= sms && wide_clusters_fit<T>()) ctas = kSampleClusters;
     a.slice = slice_of(ctas);
     const size_t smem = smem_of(ctas);
     launch_sample<T>(a, rows, ctas, smem, st);
