@@ -5,9 +5,10 @@ import numpy as np
 import pytest
 import torch
 
+import serving_cases as ref
 from emufpga_b200 import kv8, sampling
 from emufpga_b200._lib import SpmError
-from test_gpu_serving import HALF, TYPES, check_append, check_sample, gen, ints, pool
+from test_gpu_serving import HALF, TICKS, TYPES, Serving, check_append, check_sample, gen, ints, pool
 
 pytestmark = pytest.mark.gpu
 
@@ -212,3 +213,33 @@ def test_tensors_that_require_a_gradient_are_refused():
             got = f(leaf)
         want = f(x.clone())
         assert want is None or torch.equal(got, want)
+
+
+# --------------------------------------------------------------- together --
+def test_ticks_attend_to_exactly_what_the_cache_holds():
+    # every tick's slots, stored values, attention and picks against 64-bit forms over the cache's own values
+    s = Serving()
+    held = {}  # slot -> row of k, v
+    for new, ended in TICKS:
+        s.new.copy_(ints(new))
+        s.ended.copy_(ints(ended))
+        s.cached.masked_fill_(s.ended > 0, 0)
+        slots, out, token = s.tick()
+        s.pages.check()
+        s.cache.check()
+        starts, lens = np.concatenate([[0], np.cumsum(new)]).tolist(), s.cached.tolist()
+        held.update({slot: i for i, slot in enumerate(slots.tolist()) if slot >= 0})
+        for (codes, scales), rows in zip(((s.cache.k_codes, s.cache.k_scales), (s.cache.v_codes, s.cache.v_scales)), (s.k, s.v)):
+            for r, n in enumerate(lens):
+                for p in range(n):
+                    slot = s.pages.table[r, p // 16].item() * 16 + p % 16
+                    got = codes[slot // 16, :, slot % 16].double() * scales[slot // 16].double()[:, None]
+                    # a value and its page's later growths: under one step of the scale
+                    assert ((got - rows[held[slot]].double()).abs() <= scales[slot // 16].double()[:, None]).all()
+        c = s.cache
+        want, tol = ref.attention(s.q, starts, lens, s.pages.table, (c.k_codes, c.v_codes), (c.k_scales, c.v_scales), 0.125)
+        assert ((out.double() - want).abs() <= tol).all() and not out[starts[-1]:].any()
+        last = out[(ints(starts[1:]).long() - 1).clamp(min=0)].flatten(1)
+        logits = (last @ s.head.t()).double().cpu().numpy()
+        for r in range(4):
+            assert token[r].item() == ref.pick(logits[r], 1.0, 7, float(np.float32(0.9)), 0.0, s.u[r].item())[0]
