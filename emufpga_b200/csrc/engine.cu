@@ -772,12 +772,6 @@ int run_gemv(const spm_model* m, GemvLaunch L, uint32_t dtype, cudaStream_t st, 
     return grid;
 }
 
-// One decode step (spm-batch/src/step.rs:19-53), one kernel per streamed op:
-//   embed -> per layer [norm+QKV] [attention] [O+residual] [norm+gate/up+SwiGLU]
-//   [down+residual] -> [final norm + LM head] -> argmax -> positions += 1.
-// The RMSNorms are fused into the GEMV that consumes them: the residual-add
-// epilogues (and the embedding) write per-CTA sums of squares, which the next
-// GEMV reduces in a fixed order before normalising its activations on load.
 // An entry point of this library called from another: its message stands.
 void inner(spm_status st) {
     if (st != SPM_OK) fail(st, spm::last_error());
@@ -823,6 +817,12 @@ void paged_attention(spm_session* s, int l, const LayerIdx& L, int row, int requ
                             g.work, g.work_bytes, s->stream));
 }
 
+// One decode step (spm-batch/src/step.rs:19-53), one kernel per streamed op:
+//   embed -> per layer [norm+QKV] [attention] [O+residual] [norm+gate/up+SwiGLU]
+//   [down+residual] -> [final norm + LM head] -> argmax -> positions += 1.
+// The RMSNorms are fused into the GEMV that consumes them: the residual-add
+// epilogues (and the embedding) write per-CTA sums of squares, which the next
+// GEMV reduces in a fixed order before normalising its activations on load.
 void enqueue_step(spm_session* s, int n) {
     spm_model* m = s->m;
     const spm_model_cfg& c = m->cfg;
@@ -1797,7 +1797,6 @@ spm_status spm_session_free_pages(const spm_session* s, int32_t* pages) {
         *pages = s->pg.free;
     });
 }
-
 
 spm_status spm_session_destroy(spm_session* s) {
     return guarded([&] {
