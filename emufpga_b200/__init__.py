@@ -3,7 +3,7 @@
 The compute lives in libspmgpu.so (built in-tree by ``emufpga_b200.build``);
 this package is its Python face.  See include/spmgpu.h for the C ABI.
 ``kv8`` (page tables, the paged 8-bit KV cache and attention over it) and
-``sampling`` work on torch tensors and are imported on first use.
+``sampling`` work on torch tensors and are imported on first use (not by ``import *``).
 """
 import importlib
 
@@ -20,7 +20,7 @@ def __getattr__(name):
 
 
 __all__ = [
-    "configs", "kv8", "sampling", "linear", "qblocks", "spmfile", "sweep", "ternary", "Model", "Session", "SpmError", "Weights", "decode_blocks", "decode_f32",
+    "configs", "linear", "qblocks", "spmfile", "sweep", "ternary", "Model", "Session", "SpmError", "Weights", "decode_blocks", "decode_f32",
     "decode_q2_k", "decode_q5_k", "decode_q6_k", "decode_q8_0", "default_order", "gguf_find", "gguf_probe",
     "image_probe", "order_check", "pack_image", "serve", "streamed", "synth_gguf",
 ]

@@ -1,4 +1,7 @@
 """Calls of the serving operators that the host refuses before any device work (no GPU needed)."""
+import subprocess
+import sys
+
 import pytest
 
 from emufpga_b200 import _lib
@@ -18,3 +21,9 @@ def test_a_top_k_past_32_bits_is_refused(top_k):
     with pytest.raises(ValueError):
         Sampling(top_k=top_k)
     assert Sampling(top_k=2 ** 31 - 1).top_k == 2 ** 31 - 1
+
+
+def test_the_package_does_not_load_torch_by_itself():
+    code = ("from emufpga_b200 import *; import sys; assert 'torch' not in sys.modules; import emufpga_b200 as eb; "
+            "eb.kv8.Cache, eb.sampling.Sampling; assert 'torch' in sys.modules")
+    assert subprocess.run([sys.executable, "-c", code], capture_output=True, timeout=300).returncode == 0
