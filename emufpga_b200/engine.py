@@ -420,7 +420,8 @@ def serve(model: Model, prompts: Sequence[Sequence[int]], steps: int, max_ticks:
 
     `sampling` (a sampling.Sampling for each client, None for a greedy one)
     draws the tokens fed back instead, client i's from its own seed's numbers,
-    one for each token it produces.  `paged`: as for Session."""
+    one for each token it produces.  `paged`: as for Session; ValueError where
+    the pages do not hold every client's last token."""
     longest = max(len(p) for p in prompts)
     context = longest + steps + 1
     total = longest + steps - 1
@@ -428,6 +429,8 @@ def serve(model: Model, prompts: Sequence[Sequence[int]], steps: int, max_ticks:
         total = min(total, max_ticks)
     if sampling is not None and len(sampling) != len(prompts):
         raise ValueError("one Sampling (or None) per prompt")
+    if paged is not None and paged[1] > 0 and len(prompts) * -(-total // paged[1]) > paged[0]:
+        raise ValueError(f"{len(prompts)} clients of {total} tokens need {len(prompts) * -(-total // paged[1])} pages")
     sess = Session(model, len(prompts), context, paged=paged)
     try:
         tokens = [p[0] for p in prompts]

@@ -4,7 +4,7 @@ import sys
 
 import pytest
 
-from emufpga_b200 import _lib
+from emufpga_b200 import _lib, serve
 from emufpga_b200.sampling import Sampling
 from test_serving_host import A, cache, planned, refused
 
@@ -27,3 +27,10 @@ def test_the_package_does_not_load_torch_by_itself():
     code = ("from emufpga_b200 import *; import sys; assert 'torch' not in sys.modules; import emufpga_b200 as eb; "
             "eb.kv8.Cache, eb.sampling.Sampling; assert 'torch' in sys.modules")
     assert subprocess.run([sys.executable, "-c", code], capture_output=True, timeout=300).returncode == 0
+
+
+@pytest.mark.parametrize("prompts,steps,ticks,pages", [([[1] * 5, [2]], 12, None, 1), ([[1] * 5, [2]], 13, None, 3),
+                                                       ([[1], [2], [3]], 100, 33, 8)])
+def test_serving_from_too_few_pages_is_refused_before_any_step(prompts, steps, ticks, pages):
+    with pytest.raises(ValueError):
+        serve(None, prompts, steps, max_ticks=ticks, paged=(pages, 16))
