@@ -419,27 +419,35 @@ __global__ void __launch_bounds__(kDecThreads, kv8_dec_ctas(HD, NT)) kv8_decode_
                         }
                     }
             }
-            // ---- values ----
+            // ---- values: a step's products in an accumulator of their own, added to the
+            // running ones in f32 (the tensor cores truncate, which over many steps is a bias) ----
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                if (tok0 + 16 * b >= k1) break;
+            for (int d = 0; d < KB; d++) {
+                uint32_t x[NB][4];
 #pragma unroll
-                for (int d = 0; d < KB; d++) {
-                    uint32_t x[4];
-                    ldsm4t(x, vb + b * 16 * L::row + L::at(lrow, lchunk + 2 * d));
+                for (int b = 0; b < NB; b++) ldsm4t(x[b], vb + b * 16 * L::row + L::at(lrow, lchunk + 2 * d));
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const uint32_t lo = x[2 * e] ^ 0x80808080u, hi = x[2 * e + 1] ^ 0x80808080u;
+                for (int e = 0; e < 2; e++) {
+                    float y[NT][4];
+#pragma unroll
+                    for (int n = 0; n < NT; n++) y[n][0] = y[n][1] = y[n][2] = y[n][3] = 0.f;
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {  // (behind the last token: weights of 0 for whatever codes)
+                        const uint32_t lo = x[b][2 * e] ^ 0x80808080u, hi = x[b][2 * e + 1] ^ 0x80808080u;
                         const uint32_t a0 = kv8_codes2<0x4240>(lo), a1 = kv8_codes2<0x4341>(lo), a2 = kv8_codes2<0x4240>(hi),
                                        a3 = kv8_codes2<0x4341>(hi);
 #pragma unroll
                         for (int n = 0; n < NT; n++) {
-                            const uint32_t* lo = w[b][n][NP - 1];
-                            if (apart) mma_f16(o[2 * d + e][n], kv8_under(a0), kv8_under(a1), kv8_under(a2), kv8_under(a3), lo[0], lo[1]);
-                            else if (NP == 2) mma_f16(o[2 * d + e][n], a0, a1, a2, a3, lo[0], lo[1]);
-                            mma_f16(o[2 * d + e][n], a0, a1, a2, a3, w[b][n][0][0], w[b][n][0][1]);
+                            const uint32_t* low = w[b][n][NP - 1];
+                            if (apart) mma_f16(y[n], kv8_under(a0), kv8_under(a1), kv8_under(a2), kv8_under(a3), low[0], low[1]);
+                            else if (NP == 2) mma_f16(y[n], a0, a1, a2, a3, low[0], low[1]);
+                            mma_f16(y[n], a0, a1, a2, a3, w[b][n][0][0], w[b][n][0][1]);
                         }
                     }
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) o[2 * d + e][n][c] += y[n][c];
                 }
             }
             __syncwarp();

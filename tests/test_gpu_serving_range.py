@@ -143,6 +143,25 @@ def test_attention_where_pages_differ_widely_in_every_type(dtype, most, kv_heads
         assert (over | under).any()  # (f16: pages of 2^60 take every output past its range)
 
 
+@pytest.mark.parametrize("dim,requests,most,heads,kv_heads", [
+    (64, 64, 1, 8, 2), (128, 64, 1, 8, 2), (128, 32, 2, 16, 2), (192, 32, 1, 4, 2), (256, 32, 2, 8, 2)])
+def test_attention_over_many_keys_has_no_bias(dim, requests, most, heads, kv_heads):
+    # Values of one sign, each CTA with thousands of keys: a sum that truncates loses 2^-24 of itself
+    # at every product.  What is rounded to nearest has no bias; a step's own products (four of 16 keys
+    # each at most) truncate by 2^-24 each on average, the powers of two are within 2^-22.
+    length = 16384
+    c = pool(length // 64, 64, kv_heads, dim, seed=dim)
+    c.v_codes.copy_(c.v_codes.abs().clamp(min=1))
+    c.k_scales.fill_(2.0 ** -7)
+    q = torch.randn(requests * most, heads, dim, device="cuda", generator=gen(dim))
+    scale = float(np.float32(0.08))
+    got = c.attention(q, ints([most * i for i in range(requests + 1)]), ints([length] * requests),
+                      table_of(c).repeat(requests, 1), most, scale=scale)
+    c.check()
+    want = softmax_rows(c, q[:most], length, most, scale)
+    assert abs(((got[:most] - want) / want).mean().item()) <= 4 * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -22
+
+
 # ----------------------------------------------------------------- append --
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("old,new", [(-126, 22), (-126, 23), (-126, 24), (-126, 31), (-126, 120), (-80, 100), (-40, 110), (-30, 119)])
