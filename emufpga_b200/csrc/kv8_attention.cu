@@ -610,7 +610,17 @@ struct Plan {
     uint64_t prefix_bytes, parts_bytes;
 };
 
-Plan plan_of(const spm_kv8* c, int heads, int requests, int most, int width) {
+// Whether a call's kernel of many queries has to add its tiles in f32.  The tensor cores'
+// accumulators truncate: a row's sum loses 2^-23.4 of itself at every product of 16 keys,
+// 3e-9 a key with weights of one part, 6e-9 with two (measured with values of one sign:
+// 2.4e-5 at 4096 keys, 4.3e-4 at 65536).  Never for f32; for 16-bit results up to a fifth
+// of their own rounding, by what the table can hold.
+bool sums_in_f32(const spm_kv8* c, uint32_t dtype, int width) {
+    const int64_t keys = int64_t(width) * c->page_tokens;
+    return dtype == SPM_F32 || keys > (dtype == SPM_F16 ? 8192 : 131072);
+}
+
+Plan plan_of(const spm_kv8* c, int heads, int requests, int most, int width, bool total) {
     Plan p;
     const int sms = 148;  // of a B200; the grid need not match the device's for the result
     const int group = heads / c->kv_heads;
@@ -618,13 +628,15 @@ Plan plan_of(const spm_kv8* c, int heads, int requests, int most, int width) {
     p.nt = rows <= 8 ? 1 : 2;
     p.tiles = int((rows + 8 * p.nt - 1) / (8 * p.nt));
     const int64_t small = int64_t(requests) * c->kv_heads * p.tiles;
-    const int tall = kv8_prompt_rows(c->head_dim);
-    const int64_t large = int64_t(requests) * c->kv_heads * ((rows + tall - 1) / tall);
+    const int tall = kv8_prompt_rows(c->head_dim, total);
+    const int64_t large = int64_t(requests) * c->kv_heads * ((rows + tall - 1) / tall) * (total && c->head_dim > 192 ? 2 : 1);
     // A row tile of 16 costs this kernel as much as one of 128 or 256 costs the kernel of
     // many queries, but shares its keys out over all SMs: 300 such tiles for each wave of
     // the other's CTAs is about where they meet (8 kv heads of 128 in bf16, 1024 / 4096 /
     // 8000 keys: 256 tiles 43 / 95 / 162 us here and 47 / 124 / 221 there, 336 tiles 55 /
-    // 124 / 208 and 47 / 132 / 241, 640 tiles 79 / 209 / 372 and 46 / 124 / 222).
+    // 124 / 208 and 47 / 132 / 241, 640 tiles 79 / 209 / 372 and 46 / 124 / 222; in f32,
+    // which sums apart, 256 tiles 46 / 106 / 180 and 38 / 102 / 184, 320 tiles 57 / 130 / 221
+    // and 38 / 102 / 184; heads of 256, 4096 keys, 256 tiles 193 and 212, 512 tiles 345 and 212).
     // (More requests than a grid has in z stay here.)
     p.prompt = rows > 16 && requests <= 65535 && small > 300 * ((large + sms - 1) / sms);
     if (p.prompt) {
@@ -666,8 +678,11 @@ spm_status spm_kv8_attention_workspace(const spm_kv8* c, int32_t heads, int32_t 
     return guarded([&] {
         if (!bytes) fail(SPM_E_ARG, "null output");
         check_attention(c, heads, requests, most, table_width);
-        const Plan p = plan_of(c, heads, requests, most, table_width);
-        *bytes = p.prefix_bytes + p.parts_bytes;
+        *bytes = 0;
+        for (bool total : {false, true}) {  // (the type is the call's)
+            const Plan p = plan_of(c, heads, requests, most, table_width, total);
+            *bytes = std::max(*bytes, p.prefix_bytes + p.parts_bytes);
+        }
     });
 }
 
@@ -682,7 +697,8 @@ spm_status spm_kv8_attention(const spm_kv8* c, uint32_t dtype, const void* q, in
         if (rows < 0) fail(SPM_E_ARG, "negative row count");
         if (rows == 0 || ((requests == 0 || most == 0) && !clear_rest)) return;
         if (!q || !out || !starts || (requests && !lens) || (requests && table_width && !table)) fail(SPM_E_ARG, "null argument");
-        const Plan p = plan_of(c, heads, requests, most, table_width);
+        const bool total = sums_in_f32(c, dtype, table_width);
+        const Plan p = plan_of(c, heads, requests, most, table_width, total);
         if ((p.prefix_bytes && !workspace) || workspace_bytes < p.prefix_bytes + p.parts_bytes)
             fail(SPM_E_ARG, "the workspace is smaller than spm_kv8_attention_workspace says");
         if (reinterpret_cast<uintptr_t>(workspace) & 15) fail(SPM_E_ARG, "the workspace must be 16-byte aligned");
@@ -694,7 +710,7 @@ spm_status spm_kv8_attention(const spm_kv8* c, uint32_t dtype, const void* q, in
         a.kv_heads = c->kv_heads, a.group = heads / c->kv_heads;
         a.q = q, a.q_token = q_token, a.q_head = q_head, a.dtype = dtype, a.rows = rows;
         a.starts = starts, a.lens = lens, a.requests = requests, a.most = most;
-        a.table = table, a.width = table_width, a.tile_rows = p.prompt ? kv8_prompt_rows(c->head_dim) : 8 * p.nt, a.tiles = p.tiles;
+        a.table = table, a.width = table_width, a.tile_rows = p.prompt ? kv8_prompt_rows(c->head_dim, total) : 8 * p.nt, a.tiles = p.tiles;
         a.unit = kDecWarps * kv8_sub(c->head_dim);
         a.scale_log2 = float(double(scale) * 1.4426950408889634);
         a.out = out, a.o_token = out_token, a.o_head = out_head;
@@ -706,7 +722,7 @@ spm_status spm_kv8_attention(const spm_kv8* c, uint32_t dtype, const void* q, in
         a.o_vec = !((reinterpret_cast<uintptr_t>(out) | uintptr_t(out_token * size) | uintptr_t(out_head * size)) & 15);
         const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
         if (p.prompt) {
-            launch_kv8_prompt(a, c->head_dim, st);
+            launch_kv8_prompt(a, c->head_dim, total, st);
             return;
         }
         switch (c->head_dim) {

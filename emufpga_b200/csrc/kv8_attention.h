@@ -19,8 +19,8 @@ constexpr int kv8_sub(int head_dim) { return head_dim <= 128 ? 32 : 16; }
 // and has no value to speak of) are the result.
 constexpr float kLift = 15.f;
 
-// Rows of a tile of the kernel of many queries.
-constexpr int kv8_prompt_rows(int head_dim) { return head_dim <= 128 ? 256 : 128; }
+// Rows of a tile of the kernel of many queries; `total`: its form that sums in f32.
+constexpr int kv8_prompt_rows(int head_dim, bool total) { return head_dim <= 128 && !total ? 256 : 128; }
 
 struct Kv8Args {
     const int8_t *k_codes, *v_codes;
@@ -45,8 +45,8 @@ struct Kv8Args {
     int32_t* status;
 };
 
-// The kernel of many queries (kv8_prompt.cu): a.tile_rows = kv8_prompt_rows(head_dim), a.tiles to match.
-void launch_kv8_prompt(const Kv8Args& a, int head_dim, cudaStream_t st);
+// The kernel of many queries (kv8_prompt.cu): a.tile_rows = kv8_prompt_rows(head_dim, total), a.tiles to match.
+void launch_kv8_prompt(const Kv8Args& a, int head_dim, bool total, cudaStream_t st);
 
 namespace dev {
 

@@ -28,7 +28,16 @@
 // f32 queries are two fp16 parts (22 bits), and so are the weights of f32 and f16
 // results: one part, 11 bits, would add as much to an f16 result as its own rounding.
 // For a bf16 result, 8 bits, it is enough.  (1024 queries over 4096 keys, 32/8 heads of
-// 128: f16 140 us, f32 146; heads of 64 f16 126 where one part took 107.)
+// 128: f16 140 us; heads of 64 126 where one part took 107.)
+// The tensor cores truncate their accumulators, which over thousands of keys is a bias
+// (sums_in_f32 in kv8_attention.cu says how large).  f32 results, and 16-bit ones over long
+// tables, therefore take the form with TOTAL: the products of a tile go to an
+// accumulator of their own, which the softmax adds to the running one in f32, the
+// reference's move with it.  TMEM holds that for one group of 128 rows, and for 128
+// dimensions of values where head_dim is 256 (two CTAs to a row tile, each with the
+// whole scores).  f32 results are then within 3e-7 at every length; the case above takes
+// 196 us in f32 where one accumulator took 147 and was off by up to 2.4e-5, 512 queries
+// over 8000 keys 184 where it took 264 (twice the CTAs), heads of 256 390 and 236.
 //
 // What bounds it is the softmax: the 16384 exponentials of a 128 x 128 tile take
 // 1024 cycles of the special function unit, as long as its products, and its other
@@ -50,27 +59,30 @@ using namespace dev;
 constexpr int kRows = 128;                             // of a group: the MMA's M
 constexpr float kSlack = 14.f;                         // of the sum's reference, in powers of two
 
-template <int HD, int NQ, int NP>
+// NQ, NP: fp16 parts of a query and of a weight.  TOTAL: every tile's products in an
+// accumulator of their own, added to the running ones in f32.
+template <int HD, int NQ, int NP, bool TOTAL>
 struct PromptShape {
-    static constexpr int G = kv8_prompt_rows(HD) / kRows;
+    static constexpr int G = kv8_prompt_rows(HD, TOTAL) / kRows;
     // converting warps: as many as leave the softmax its registers (80 of 24 warps, 96 of 20)
     static constexpr int fill = G == 2 ? 7 : 11;
     static constexpr int threads = 32 * (8 * G + fill + 1);
     static constexpr int TN = HD <= 128 ? 128 : 64;    // keys of a tile
     static constexpr int BUF = G == 1 ? 2 : 1;         // buffers of S
+    static constexpr int DV = TOTAL && HD > 192 ? 128 : HD;  // value dimensions of a CTA, as many as TMEM holds twice
     static constexpr int atoms = (HD + 63) / 64;       // 64 dimensions, 128 bytes
     static constexpr int qgroup = atoms * kRows * 128; // bytes of a group's part of Q
     static constexpr int qbytes = G * NQ * qgroup;
-    static constexpr int tile = atoms * TN * 128;      // bytes of a tile of K or V
-    static constexpr int room = (227 * 1024 - 8192 - qbytes) / (2 * tile), stages = room > 4 ? 4 : room;
+    static constexpr int ktile = atoms * TN * 128, vtile = (DV + 63) / 64 * TN * 128;  // bytes of a tile of K and of V
+    static constexpr int room = (227 * 1024 - 8192 - qbytes) / (ktile + vtile), stages = room > 4 ? 4 : room;
     static_assert(stages >= 1, "a tile of K and one of V");
     // (at least half of an SM's: a second CTA would wait for the first one's TMEM)
-    static constexpr int need = qbytes + 2 * stages * tile + 1024, smem = need > 120 * 1024 ? need : 120 * 1024;
+    static constexpr int need = qbytes + stages * (ktile + vtile) + 1024, smem = need > 120 * 1024 ? need : 120 * 1024;
     // TMEM columns: the buffers of S of each group, which its P replaces (16 columns
     // of S, 16 keys, hold the 8 columns of their high parts, then of their low ones),
-    // and O
-    static constexpr int s_col = 0, o_col = BUF * G * TN;
-    static_assert(o_col + G * HD <= 512, "TMEM");
+    // the products with V, and the sums of those
+    static constexpr int s_col = 0, o_col = BUF * G * TN, t_col = o_col + G * DV;
+    static_assert(t_col + (TOTAL ? G * DV : 0) <= 512, "TMEM");
 };
 
 struct PromptSync {
@@ -179,20 +191,20 @@ __device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t at, uint32_t next) {
 typedef std::true_type Yes;
 typedef std::false_type No;
 
-// NQ, NP: fp16 parts of a query and of a weight.
-template <int HD, int NQ, int NP>
-__global__ void __launch_bounds__(PromptShape<HD, NQ, NP>::threads, 1) kv8_prompt_kernel(const Kv8Args a) {
-    using S = PromptShape<HD, NQ, NP>;
-    constexpr int TN = S::TN, ST = S::stages, G = S::G, BUF = S::BUF, FT = 32 * S::fill, kSoftWarps = 8 * G;
+template <int HD, int NQ, int NP, bool TOTAL>
+__global__ void __launch_bounds__(PromptShape<HD, NQ, NP, TOTAL>::threads, 1) kv8_prompt_kernel(const Kv8Args a) {
+    using S = PromptShape<HD, NQ, NP, TOTAL>;
+    constexpr int TN = S::TN, ST = S::stages, G = S::G, BUF = S::BUF, DV = S::DV, FT = 32 * S::fill, kSoftWarps = 8 * G;
     extern __shared__ __align__(1024) uint8_t raw[];
     __shared__ PromptSync y;
-    const uint32_t qs = (saddr(raw) + 1023u) & ~1023u, ks = qs + S::qbytes, vs = ks + ST * S::tile;
+    const uint32_t qs = (saddr(raw) + 1023u) & ~1023u, ks = qs + S::qbytes, vs = ks + ST * S::ktile;
     uint8_t* const base = raw + (qs - saddr(raw));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     kv8_clear<HD>(a, (blockIdx.z * (long long)gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x,
                   (long long)gridDim.x * gridDim.y * gridDim.z);
-    // the last rows see the most keys: they go first
-    const int tile = int(gridDim.x) - 1 - int(blockIdx.x), head = blockIdx.y, req = blockIdx.z;
+    // the last rows see the most keys: they go first; a row tile's CTAs side by side
+    constexpr int parts = HD / DV;
+    const int tile = int(gridDim.x - 1 - blockIdx.x) / parts, d0 = DV * int(blockIdx.x % parts), head = blockIdx.y, req = blockIdx.z;
     const int s0 = a.starts[req], e0 = a.starts[req + 1];
     if (s0 < 0 || e0 < s0 || e0 > a.rows || e0 - s0 > a.most) {
         if (tid == 0) flag(a.status, SPM_PAGE_QUERIES);
@@ -242,18 +254,24 @@ __global__ void __launch_bounds__(PromptShape<HD, NQ, NP>::threads, 1) kv8_promp
         // ---- producers: codes of tile j converted while those of j + 1 and the page
         // numbers of j + 2 are on their way ----
         // 16-byte pieces of a token, and of a thread (head_dim 96: the last ones of half the threads)
-        constexpr int SEG = HD / 16, PIECES = TN * SEG, N = (PIECES + FT - 1) / FT;
-        constexpr bool ragged = PIECES % FT != 0;
+        constexpr int KSEG = HD / 16, VSEG = DV / 16, NK = (TN * KSEG + FT - 1) / FT, NV = (TN * VSEG + FT - 1) / FT;
         const int t = tid - 32 * kSoftWarps;
         const int32_t* trow = a.table + size_t(req) * a.width;
-        uint4 k[N], v[N];
-        int page[N];
-        auto find = [&](int j) {
+        uint4 k[NK], v[NV];
+        int page[NK], vpage[NV];  // (the same where a CTA has all dimensions)
+        auto pages_of = [&](int j, auto seg, auto& page) {
+            constexpr int SEG = decltype(seg)::value, N = sizeof(page) / sizeof(int);
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const int tok = j * TN + (t + i * FT) / SEG;
-                page[i] = tok < keys && (!ragged || t + i * FT < PIECES) ? __ldg(trow + (tok >> a.shift)) : -1;
+                page[i] = tok < keys && t + i * FT < TN * SEG ? __ldg(trow + (tok >> a.shift)) : -1;
             }
+        };
+        typedef std::integral_constant<int, KSEG> KSeg;
+        typedef std::integral_constant<int, VSEG> VSeg;
+        auto find = [&](int j) {
+            pages_of(j, KSeg(), page);
+            if constexpr (DV != HD) pages_of(j, VSeg(), vpage);
         };
         // -1 for none, and for a page that is not in the pool
         auto known = [&](int p, int tok) {
@@ -263,21 +281,29 @@ __global__ void __launch_bounds__(PromptShape<HD, NQ, NP>::threads, 1) kv8_promp
             }
             return p;
         };
-        auto load = [&](const int8_t* codes, int j, uint4 (&c)[N]) {
+        auto load = [&](const int8_t* codes, int j, auto seg, const auto& page, auto& c) {
+            constexpr int SEG = decltype(seg)::value, N = sizeof(page) / sizeof(int), PIECES = TN * SEG;
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int e = t + i * FT, r = e / SEG, o = e % SEG, tok = j * TN + r, p = ragged && e >= PIECES ? -1 : known(page[i], tok);
+                const int e = t + i * FT, r = e / SEG, o = e % SEG, tok = j * TN + r;
+                const int p = PIECES % FT != 0 && e >= PIECES ? -1 : known(page[i], tok);
                 c[i] = make_uint4(0, 0, 0, 0);
                 if (p >= 0)
                     c[i] = __ldg(reinterpret_cast<const uint4*>(
                         codes + ((size_t(p) * a.kv_heads + head) * a.page + (tok & (a.page - 1))) * HD + 16 * o));
             }
         };
-        auto store = [&](uint8_t* to, const uint4 (&c)[N]) {
+        auto load_k = [&](int j) { load(a.k_codes, j, KSeg(), page, k); };
+        auto load_v = [&](int j) {
+            if constexpr (DV == HD) load(a.v_codes, j, KSeg(), page, v);
+            else load(a.v_codes + d0, j, VSeg(), vpage, v);
+        };
+        auto store = [&](uint8_t* to, auto seg, const auto& c) {
+            constexpr int SEG = decltype(seg)::value, N = sizeof(c) / sizeof(uint4), PIECES = TN * SEG;
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const int e = t + i * FT, r = e / SEG, o = e % SEG;
-                if (ragged && e >= PIECES) break;
+                if (PIECES % FT != 0 && e >= PIECES) break;
                 uint32_t h[8];
                 const uint32_t w[4] = {c[i].x ^ 0x80808080u, c[i].y ^ 0x80808080u, c[i].z ^ 0x80808080u, c[i].w ^ 0x80808080u};
 #pragma unroll
@@ -304,8 +330,8 @@ __global__ void __launch_bounds__(PromptShape<HD, NQ, NP>::threads, 1) kv8_promp
         };
         if (tiles) {
             find(0);
-            load(a.k_codes, 0, k);
-            load(a.v_codes, 0, v);
+            load_k(0);
+            load_v(0);
             scales(0);
             find(1);
         }
@@ -314,7 +340,7 @@ __global__ void __launch_bounds__(PromptShape<HD, NQ, NP>::threads, 1) kv8_promp
             const int st = j % ST;
             const uint32_t again = uint32_t(j / ST - 1) & 1u;
             if (j >= ST && !wait(&y.k_empty[st], again)) break;
-            store(base + S::qbytes + st * S::tile, k);
+            store(base + S::qbytes + st * S::ktile, KSeg(), k);
             if (t < TN / 16) {
                 y.ks[j & 7][t] = kscale;
                 const float e = kv8_exponent(vscale);
@@ -324,13 +350,13 @@ __global__ void __launch_bounds__(PromptShape<HD, NQ, NP>::threads, 1) kv8_promp
             }
             fence_proxy_async();
             mbar_arrive(&y.k_full[st]);
-            load(a.k_codes, j + 1, k);
+            load_k(j + 1);
             scales(j + 1);
             if (j >= ST && !wait(&y.v_empty[st], again)) break;
-            store(base + S::qbytes + (ST + st) * S::tile, v);
+            store(base + S::qbytes + ST * S::ktile + st * S::vtile, VSeg(), v);
             fence_proxy_async();
             mbar_arrive(&y.v_full[st]);
-            load(a.v_codes, j + 1, v);
+            load_v(j + 1);
             find(j + 2);
         }
     } else if (warp == kMmaWarp) {
@@ -341,9 +367,9 @@ __global__ void __launch_bounds__(PromptShape<HD, NQ, NP>::threads, 1) kv8_promp
         if (lane == 0) {
             constexpr uint32_t f32_out = 1u << 4, m = uint32_t(kRows >> 4) << 24;
             constexpr uint32_t id_s = f32_out | m | uint32_t(TN >> 3) << 17;
-            constexpr uint32_t id_o = f32_out | m | uint32_t(HD >> 3) << 17 | 1u << 16;  // V is MN-major
+            constexpr uint32_t id_o = f32_out | m | uint32_t(DV >> 3) << 17 | 1u << 16;  // V is MN-major
             auto scores = [&](int g, int j) {
-                const uint32_t k = ks + uint32_t(j % ST) * S::tile, q = qs + uint32_t(g * NQ) * S::qgroup;
+                const uint32_t k = ks + uint32_t(j % ST) * S::ktile, q = qs + uint32_t(g * NQ) * S::qgroup;
 #pragma unroll
                 for (int p = NQ - 1; p >= 0; p--)
 #pragma unroll
@@ -371,13 +397,13 @@ __global__ void __launch_bounds__(PromptShape<HD, NQ, NP>::threads, 1) kv8_promp
                     ok = ok && wait(&y.p_ready[g][j % BUF], uint32_t(j / BUF) & 1u);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t v = vs + uint32_t(j % ST) * S::tile;
+                    const uint32_t v = vs + uint32_t(j % ST) * S::vtile;
 #pragma unroll
                     for (int p = NP - 1; p >= 0; p--)
 #pragma unroll
                         for (int kk = 0; kk < TN / 16; kk++)
-                            umma_f16_ts(tmem + S::o_col + g * HD, tmem + S::s_col + (BUF * g + j % BUF) * TN + 16u * kk + 8u * p,
-                                        sw128_mn_desc(v + 2048u * kk, TN * 128), id_o, j != 0 || p != NP - 1 || kk != 0);
+                            umma_f16_ts(tmem + S::o_col + g * DV, tmem + S::s_col + (BUF * g + j % BUF) * TN + 16u * kk + 8u * p,
+                                        sw128_mn_desc(v + 2048u * kk, TN * 128), id_o, (!TOTAL && j != 0) || p != NP - 1 || kk != 0);
                     if (g == groups - 1) umma_commit(&y.v_empty[j % ST]);
                     umma_commit(&y.o_done[g]);
                     if (j + 1 == tiles) umma_commit(&y.o_last[g]);
@@ -434,7 +460,8 @@ __global__ void __launch_bounds__(PromptShape<HD, NQ, NP>::threads, 1) kv8_promp
         // ---- softmax: two threads to a row, TMEM lane of its group, half of a tile's columns each ----
         const int g = warp >> 3, half = warp >> 2 & 1, r = g * kRows + 32 * (warp & 3) + lane;
         const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
-        const uint32_t s0col = tmem + lanes + S::s_col + uint32_t(BUF * g) * TN, o = tmem + lanes + S::o_col + uint32_t(g) * HD;
+        const uint32_t s0col = tmem + lanes + S::s_col + uint32_t(BUF * g) * TN, o = tmem + lanes + S::o_col + uint32_t(g) * DV,
+                       total = tmem + lanes + S::t_col + uint32_t(g) * DV;
         constexpr int HC = TN / 64;  // of the 32 columns at a time
         const float qscale = y.qscale[r];
         const int limit = r < rows ? len - nq + (row0 + r) / a.group + 1 : 0;  // keys that the row sees
@@ -500,13 +527,13 @@ __global__ void __launch_bounds__(PromptShape<HD, NQ, NP>::threads, 1) kv8_promp
             reach = fmaxf(reach, y.reach[j & 1][half ^ 1][r]);
             // a warp's rows together
             const bool moves = reach > ref + kLift || (ref == -INFINITY && reach > ref);
-            if (__any_sync(0xffffffffu, moves)) {
+            if (TOTAL || __any_sync(0xffffffffu, moves)) {
                 const float to = reach - kLift;
                 const float down = moves ? kv8_step(ref, to) : 1.f;
                 if (moves) ref = to;
                 if (j) {
-                    // O is the products' until P(j - 1) V(j - 1) is done (the one before
-                    // is, S(j) waited for it: the parity is that of one phase alone)
+                    // O is the products' until P(j - 1) V(j - 1) is done (the one before is,
+                    // TOTAL or S(j) waited for it: the parity is that of one phase alone)
                     ok = wait(&y.o_done[g], uint32_t(j - 1) & 1u);
                     if (!__all_sync(0xffffffffu, ok)) {
                         ok = false;
@@ -514,12 +541,18 @@ __global__ void __launch_bounds__(PromptShape<HD, NQ, NP>::threads, 1) kv8_promp
                     }
                     tc_fence_after();
 #pragma unroll 1
-                    for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d += 16) {
+                    for (int d = half * (DV / 2); d < (half + 1) * (DV / 2); d += 16) {
                         float x[16];
                         tmem_ld16(o + d, x);
+                        if (TOTAL && j > 1) {  // (P(j) V(j) goes over O once all have sent P(j))
+                            float y[16];
+                            tmem_ld16(total + d, y);
+#pragma unroll
+                            for (int e = 0; e < 16; e++) x[e] += y[e];
+                        }
 #pragma unroll
                         for (int e = 0; e < 16; e++) x[e] *= down;
-                        tmem_st16(o + d, x);
+                        tmem_st16((TOTAL ? total : o) + d, x);
                     }
                 }
             }
@@ -584,12 +617,18 @@ __global__ void __launch_bounds__(PromptShape<HD, NQ, NP>::threads, 1) kv8_promp
                 sum = y.state[1][0][r] * kv8_step(ma, m) + y.state[1][1][r] * kv8_step(mb, m);
             }
             const int qr = row0 + r, qi = qr / a.group, qh = head * a.group + qr % a.group;
-            const int64_t at = int64_t(s0 + qi) * a.o_token + qh * a.o_head;
+            const int64_t at = int64_t(s0 + qi) * a.o_token + qh * a.o_head + d0;
 #pragma unroll 1
-            for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d += 16) {
+            for (int d = half * (DV / 2); d < (half + 1) * (DV / 2); d += 16) {
                 float v[16];
                 if (tiles) {
                     tmem_ld16(o + d, v);
+                    if (TOTAL && tiles > 1) {
+                        float y[16];
+                        tmem_ld16(total + d, y);
+#pragma unroll
+                        for (int e = 0; e < 16; e++) v[e] += y[e];
+                    }
                 } else {
 #pragma unroll
                     for (int e = 0; e < 16; e++) v[e] = 0.f;
@@ -610,34 +649,34 @@ __global__ void __launch_bounds__(PromptShape<HD, NQ, NP>::threads, 1) kv8_promp
     }
 }
 
-template <int HD, int NQ, int NP>
+template <int HD, int NQ, int NP, bool TOTAL>
 void launch(const Kv8Args& a, cudaStream_t st) {
-    constexpr int smem = PromptShape<HD, NQ, NP>::smem;
-    static_assert(smem + int(sizeof(PromptSync)) <= 227 * 1024, "a CTA's shared memory");
+    using S = PromptShape<HD, NQ, NP, TOTAL>;
+    static_assert(S::smem + int(sizeof(PromptSync)) <= 227 * 1024, "a CTA's shared memory");
     static std::atomic<unsigned long long> done{0};
-    allow_smem(kv8_prompt_kernel<HD, NQ, NP>, smem, done);
-    const dim3 grid(unsigned(a.tiles), unsigned(a.kv_heads), unsigned(a.requests));
-    kv8_prompt_kernel<HD, NQ, NP><<<grid, PromptShape<HD, NQ, NP>::threads, smem, st>>>(a);
+    allow_smem(kv8_prompt_kernel<HD, NQ, NP, TOTAL>, S::smem, done);
+    const dim3 grid(unsigned(a.tiles) * (HD / S::DV), unsigned(a.kv_heads), unsigned(a.requests));
+    kv8_prompt_kernel<HD, NQ, NP, TOTAL><<<grid, S::threads, S::smem, st>>>(a);
     CUDA_OK(cudaGetLastError());
 }
 
 template <int HD>
-void launch_parts(const Kv8Args& a, cudaStream_t st) {
+void launch_parts(const Kv8Args& a, bool total, cudaStream_t st) {
     // a 16-bit query is exact in one part (see above for the weights)
-    if (a.dtype == SPM_F32) launch<HD, 2, 2>(a, st);
-    else if (a.dtype == SPM_F16) launch<HD, 1, 2>(a, st);
-    else launch<HD, 1, 1>(a, st);
+    if (a.dtype == SPM_F32) launch<HD, 2, 2, true>(a, st);
+    else if (a.dtype == SPM_F16) total ? launch<HD, 1, 2, true>(a, st) : launch<HD, 1, 2, false>(a, st);
+    else total ? launch<HD, 1, 1, true>(a, st) : launch<HD, 1, 1, false>(a, st);
 }
 
 }  // namespace
 
-void launch_kv8_prompt(const Kv8Args& a, int head_dim, cudaStream_t st) {
+void launch_kv8_prompt(const Kv8Args& a, int head_dim, bool total, cudaStream_t st) {
     switch (head_dim) {
-        case 64: launch_parts<64>(a, st); break;
-        case 96: launch_parts<96>(a, st); break;
-        case 128: launch_parts<128>(a, st); break;
-        case 192: launch_parts<192>(a, st); break;
-        default: launch_parts<256>(a, st); break;
+        case 64: launch_parts<64>(a, total, st); break;
+        case 96: launch_parts<96>(a, total, st); break;
+        case 128: launch_parts<128>(a, total, st); break;
+        case 192: launch_parts<192>(a, total, st); break;
+        default: launch_parts<256>(a, total, st); break;
     }
 }
 

@@ -162,6 +162,31 @@ def test_attention_over_many_keys_has_no_bias(dim, requests, most, heads, kv_hea
     assert abs(((got[:most] - want) / want).mean().item()) <= 4 * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -22
 
 
+@pytest.mark.parametrize("dtype,length,bound", [
+    # f32: a tile's products truncate, eight of 16 keys each (the low parts' are too small to count) by
+    # 2^-24 on average; the powers of two are within 2^-22
+    ("f32", 4096, 2.0 ** -21 + 2.0 ** -22), ("f32", 16384, 2.0 ** -21 + 2.0 ** -22),
+    # 16 bits: a quarter of their rounding where one accumulator is kept, else the mean of so many roundings
+    ("f16", 8192, 2.0 ** -14), ("f16", 16384, 2.0 ** -16), ("f16", 65536, 2.0 ** -16),
+    ("bf16", 16384, 2.0 ** -11), ("bf16", 163840, 2.0 ** -12)])
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+def test_prompt_attention_over_many_keys_has_no_bias(dtype, length, bound, dim):
+    # values of one sign, of a size of its own in each dimension
+    most, heads, kv_heads, last = 600, 16, 4, 24
+    c = pool(length // 64, 64, kv_heads, dim, seed=dim)
+    size = torch.rand(kv_heads, 1, dim, device="cuda", generator=gen(3)) * 0.8 + 0.2
+    c.v_codes.copy_((c.v_codes.abs().clamp(min=1) * size).ceil())
+    c.k_scales.fill_(2.0 ** -7)
+    c.v_scales.fill_(2.0 ** -5)
+    q = torch.randn(most, heads, dim, device="cuda", generator=gen(dim)).to(TYPES[dtype])
+    scale = float(np.float32(0.08))
+    got = c.attention(q, ints([0, most]), ints([length]), table_of(c), most, scale=scale)[-last:]
+    c.check()
+    want = softmax_rows(c, q[-last:], length, last, scale)
+    off = ((got.double() - want) / want)
+    assert abs(off.mean().item()) <= bound and off.abs().max().item() <= HALF[q.dtype] * 1.25 + 2.0 ** -18
+
+
 # ----------------------------------------------------------------- append --
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("old,new", [(-126, 22), (-126, 23), (-126, 24), (-126, 31), (-126, 120), (-80, 100), (-40, 110), (-30, 119)])
