@@ -14,7 +14,7 @@
 // heads of the group), so that one pass over the codes serves every query of a kv
 // head.
 //   Scores: int8 x int8 (m16n8k32).  The codes go in as they lie; a query row is
-//   fixed point to its largest value, 22 bits in three signed 8-bit digits (two, 14
+//   fixed point to its largest value, 23 bits in three signed 8-bit digits (two, 15
 //   bits, would gain 2% of a long decode).  Sums are exact in int32.
 //   Values: fp16 x fp16 (m16n8k16), fp32 sums.  The codes are exact in fp16: byte
 //   permutes make 0x6400 | (code + 128) = 1024 + 128 + code and a subtraction of 1152
@@ -255,8 +255,9 @@ __global__ void __launch_bounds__(kDecThreads, kv8_dec_ctas(HD, NT)) kv8_decode_
 #pragma unroll
             for (int i = 0; i < HD / 32; i++) big = max(big, __float_as_uint(x[y][i]) & 0x7fffffffu);
             big = __reduce_max_sync(0xffffffffu, big);
-            // the largest to 2^21 .. 2^22 (2^13 .. 2^14), or as far up as a power of two reaches
-            const int up = min((PL == 3 ? 21 : 13) + 127 - int(big >> 23), 126);
+            // the largest to 2^22 .. 2^23, a bit less where its top digit would pass 127 (three
+            // digits hold 127 * 65793), or as far up as a power of two reaches
+            const int up = min(22 + 127 - int(big >> 23) - ((big & 0x7fffffu) > 0x7efe00u), 126);
             const float mul = pow2i(up);
             if (lane == 0) qscale[r] = big < 0x7f800000u ? a.scale_log2 * pow2i(-up) : __int_as_float(0x7fffffff);
             int8_t* dst = reinterpret_cast<int8_t*>(sm + L::q) + (r >> 3) * HD * 8;

@@ -143,6 +143,36 @@ def test_attention_where_pages_differ_widely_in_every_type(dtype, most, kv_heads
         assert (over | under).any()  # (f16: pages of 2^60 take every output past its range)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("most", [1, 3])
+@pytest.mark.parametrize("large", [1.25, 1.99, 1.996])
+def test_attention_queries_are_fixed_point_of_23_bits(dim, most, large):
+    # A large element meets a key dimension of zeros: the others' bits are what is left of 23, or of 22
+    # where the three digits do not hold the largest one's.  Two keys of values 127 and -127.
+    rows = 256 * most
+    c = pool(1, 16, 1, dim, fill=False)
+    c.k_codes.copy_(torch.randint(-100, 101, c.k_codes.shape, device="cuda", generator=gen(dim)))
+    c.k_codes[..., 0] = 0
+    c.k_scales.fill_(1.0)
+    c.v_codes[0, 0, 0], c.v_codes[0, 0, 1:most + 1], c.v_codes[0, 0, most + 1:] = 127, -127, 50
+    c.k_codes[0, 0, 2:most + 1] = c.k_codes[0, 0, 1]
+    c.v_scales.fill_(2.0 ** -7)
+    q = torch.randn(rows, 2, dim, device="cuda", generator=gen(most))
+    q[..., 0] = large * 1024
+    scale = float(np.float32(1 / (60 * dim ** 0.5)))
+    starts, lens = ints(range(0, rows + 1, most)), ints([most + 1] * 256)
+    got = c.attention(q, starts, lens, ints([[0]] * 256), most, scale=scale)[::most].double()
+    c.check()
+    # the first row of each request sees two keys
+    k = c.k_codes[0, 0, :2].double()
+    p = torch.sigmoid(q[::most].double() @ (k[0] - k[1]) * scale)
+    unit = 2.0 ** (10 - 22 + (large > 1.992))
+    # d out / d score is 127 / 64 p (1 - p); an element is off by unit / sqrt(12) in the mean square
+    want_rms = (scale * unit / 12 ** 0.5 * (k[0] - k[1]).square().sum().sqrt() * 127 / 64 * p * (1 - p)).square().mean().sqrt()
+    off = (got - (127 / 128 * (2 * p - 1))[..., None]).square().mean().sqrt()
+    assert off <= 1.2 * want_rms + 2.0 ** -22, (off / want_rms).item()
+
+
 @pytest.mark.parametrize("dim,requests,most,heads,kv_heads", [
     (64, 64, 1, 8, 2), (128, 64, 1, 8, 2), (128, 32, 2, 16, 2), (192, 32, 1, 4, 2), (256, 32, 2, 8, 2)])
 def test_attention_over_many_keys_has_no_bias(dim, requests, most, heads, kv_heads):
