@@ -28,9 +28,10 @@
 //   column become rows g and g + 8.
 //
 // What bounds it is the cache's bytes (64 requests of 1000 to 16384 keys, 8 kv heads of
-// 128: 1.16 GB in 215 us, 5.4 TB/s, and 8 us to join the parts), nearly as much the
-// issue of its products; for a few requests the latency of one unit (8 requests of 1200
-// keys: 9.5 and 5 us).  Each warp streams its own 32 tokens (16 where
+// 128: 1.16 GB in 205 us and 9 to join the parts, 5.4 TB/s together, in a short run of
+// calls; 235 to 248 in a long one; f16 225 and f32 237 in a short one), nearly as much
+// the issue of its products; for a few requests the latency of one unit (8 requests of
+// 1200 keys: 11 us).  Each warp streams its own 32 tokens (16 where
 // head_dim is over 128) at a time through a ring in shared memory (16-byte asynchronous copies, no barrier
 // among warps).  Work is cut into units of four such steps of a (row tile, kv head),
 // and every CTA takes an equal run of the units of all requests, so that ragged

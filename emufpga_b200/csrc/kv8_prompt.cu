@@ -22,7 +22,7 @@
 // 4096 keys; a product of 64 columns takes the tensor cores as long as one of 128.)
 // The accumulator's reference lies 2^15, what fp16 holds, under the largest weighted value
 // and moves with it, so that weights keep 11 bits down to 2^-29 of the row's largest
-// (and a step of 2^-40 of it in two parts).  A slack of 2^14 instead, which hardly ever
+// and a step of 2^-39 of it under that, in one part or two.  A slack of 2^14 instead, which hardly ever
 // reads the accumulator back, took 124.7 us where this takes 130.8, and lost every weight
 // under 2^-25 of the largest.  The sum is f32: its reference has that slack.
 // f32 queries are two fp16 parts (22 bits), and so are the weights of f32 and f16

@@ -20,8 +20,8 @@
 // where top-k does not spare them; for few rows the chain of dependent passes and
 // cluster barriers.  A row is one thread-block cluster whose CTAs keep its
 // slices in shared memory, so the logits are read from HBM once and the
-// histograms are added through distributed shared memory.  One row of 49152 takes 18 to 22
-// us, 8 of 151936 with top-p 38, 128 of 151936 in bf16 76 with top-k (0.5 TB/s) and 158
+// histograms are added through distributed shared memory.  One row of 49152 takes 18 to 21
+// us, 8 of 151936 with top-p 39, 128 of 151936 in bf16 86 with top-k (0.45 TB/s) and 160
 // with top-p: about 40 and 170 instructions a logit.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
