@@ -34,8 +34,8 @@
 // tables, therefore take the form with TOTAL: the products of a tile go to an
 // accumulator of their own, which the softmax adds to the running one in f32, the
 // reference's move with it.  TMEM holds that for one group of 128 rows, and for 128
-// dimensions of values where head_dim is 256 (two CTAs to a row tile, each with the
-// whole scores).  f32 results are then within 3e-7 at every length; the case above takes
+// dimensions of values where head_dim is 256 (a cluster of two CTAs to a row tile, each
+// with the whole scores).  f32 results are then within 3e-7 at every length; the case above takes
 // 196 us in f32 where one accumulator took 147 and was off by up to 2.4e-5, 512 queries
 // over 8000 keys 184 where it took 264 (twice the CTAs), heads of 256 390 and 236.
 //
@@ -235,11 +235,14 @@ __global__ void __launch_bounds__(PromptShape<HD, NQ, NP, TOTAL>::threads, 1) kv
         mbar_fence_init();
     }
     constexpr int kMmaWarp = kSoftWarps + S::fill;
-    // Each role does what it can before the first products, then all meet.
+    // Each role does what it can before the first products, then all meet: a row tile's
+    // CTAs too, which read the same queries before either writes its dimensions (out may be q).
     auto together = [&] {
         fence_proxy_async();
         tc_fence_before();
         __syncthreads();
+        if constexpr (parts > 1)
+            asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
         tc_fence_after();
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) {  // false once any wait of the CTA has given up
@@ -656,8 +659,18 @@ void launch(const Kv8Args& a, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
     allow_smem(kv8_prompt_kernel<HD, NQ, NP, TOTAL>, S::smem, done);
     const dim3 grid(unsigned(a.tiles) * (HD / S::DV), unsigned(a.kv_heads), unsigned(a.requests));
-    kv8_prompt_kernel<HD, NQ, NP, TOTAL><<<grid, S::threads, S::smem, st>>>(a);
-    CUDA_OK(cudaGetLastError());
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(S::threads);
+    cfg.dynamicSmemBytes = S::smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];  // a row tile's CTAs are a cluster
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = HD / S::DV;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = HD > S::DV ? 1 : 0;
+    CUDA_OK(cudaLaunchKernelEx(&cfg, kv8_prompt_kernel<HD, NQ, NP, TOTAL>, a));
 }
 
 template <int HD>

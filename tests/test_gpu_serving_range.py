@@ -217,6 +217,25 @@ def test_prompt_attention_over_many_keys_has_no_bias(dtype, length, bound, dim):
     assert abs(off.mean().item()) <= bound and off.abs().max().item() <= HALF[q.dtype] * 1.25 + 2.0 ** -18
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("news,lens,width", [([1, 1, 1], [900, 3, 0], 64), ([700, 33, 300], [3000, 40, 300], 64), ([700], [900], 8300)])
+def test_attention_in_place(dtype, dim, news, lens, width):
+    # the queries' memory receives the result, whatever shares a row's keys or dimensions out; the last: a long table
+    c = pool(60, 64, 4, dim, seed=dim)
+    table = torch.full((len(lens), width), -1, dtype=torch.int32, device="cuda")
+    for r, n in enumerate(lens):
+        table[r, :-(-n // 64)] = torch.arange(-(-n // 64), device="cuda") + r
+    starts, ln = ints(np.concatenate([[0], np.cumsum(news)])), ints(lens)
+    q = torch.randn(sum(news) + 2, 16, dim, device="cuda", generator=gen(dim)).to(TYPES[dtype])
+    want = c.attention(q, starts, ln, table, max(news))
+    for _ in range(20):
+        same = q.clone()
+        assert c.attention(same, starts, ln, table, max(news), out=same) is same
+        assert torch.equal(same[:-2], want[:-2]) and torch.equal(same[-2:], q[-2:])
+    c.check()
+
+
 # ----------------------------------------------------------------- append --
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("old,new", [(-126, 22), (-126, 23), (-126, 24), (-126, 31), (-126, 120), (-80, 100), (-40, 110), (-30, 119)])
