@@ -615,7 +615,7 @@ struct Plan {
 // Whether a call's kernel of many queries has to add its tiles in f32.  The tensor cores'
 // accumulators truncate: a row's sum loses 2^-23.4 of itself at every product of 16 keys,
 // 3e-9 a key with weights of one part, 6e-9 with two (measured with values of one sign:
-// 2.4e-5 at 4096 keys, 4.3e-4 at 65536).  Never for f32; for 16-bit results up to a fifth
+// 2.4e-5 at 4096 keys, 4.3e-4 at 65536).  Never for f32; for 16-bit results up to a tenth
 // of their own rounding, by what the table can hold.
 bool sums_in_f32(const spm_kv8* c, uint32_t dtype, int width) {
     const int64_t keys = int64_t(width) * c->page_tokens;

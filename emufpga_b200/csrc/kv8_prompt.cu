@@ -20,11 +20,12 @@
 // for one group, which has two buffers of S instead.  (Two buffers of 64 keys for
 // two groups too: 176 us where one of 128 took 135, 32 heads of 128, 1024 queries over
 // 4096 keys; a product of 64 columns takes the tensor cores as long as one of 128.)
-// The accumulator's reference lies 2^15, what fp16 holds, under the largest weighted value
-// and moves with it, so that weights keep 11 bits down to 2^-29 of the row's largest
-// and a step of 2^-39 of it under that, in one part or two.  A slack of 2^14 instead, which hardly ever
-// reads the accumulator back, took 124.7 us where this takes 130.8, and lost every weight
-// under 2^-25 of the largest.  The sum is f32: its reference has that slack.
+// The accumulator's reference lies 2^15, what fp16 holds, under the largest weighted
+// value and moves with it, so that weights keep 11 bits down to 2^-29 of the row's
+// largest and a step of 2^-39 of it under that, in one part or two.  A slack of 2^14
+// instead, which hardly ever reads the accumulator back, took 124.7 us where this takes
+// 130.8, and lost every weight under 2^-25 of the largest.  The sum is f32: its reference
+// has that slack.
 // f32 queries are two fp16 parts (22 bits), and so are the weights of f32 and f16
 // results: one part, 11 bits, would add as much to an f16 result as its own rounding.
 // For a bf16 result, 8 bits, it is enough.  (1024 queries over 4096 keys, 32/8 heads of
@@ -35,9 +36,10 @@
 // accumulator of their own, which the softmax adds to the running one in f32, the
 // reference's move with it.  TMEM holds that for one group of 128 rows, and for 128
 // dimensions of values where head_dim is 256 (a cluster of two CTAs to a row tile, each
-// with the whole scores).  f32 results are then within 3e-7 at every length; the case above takes
-// 196 us in f32 where one accumulator took 147 and was off by up to 2.4e-5, 512 queries
-// over 8000 keys 184 where it took 264 (twice the CTAs), heads of 256 390 and 236.
+// with the whole scores).  f32 results are then within 5e-7 at every length; the case
+// above takes 195 us in f32 where one accumulator took 147 and was off by up to 2.4e-5,
+// 512 queries over 8000 keys 185 where it took 264 (twice the CTAs), heads of 256 390
+// and 236.
 //
 // What bounds it is the softmax: the 16384 exponentials of a 128 x 128 tile take
 // 1024 cycles of the special function unit, as long as its products, and its other
@@ -675,7 +677,7 @@ void launch(const Kv8Args& a, cudaStream_t st) {
 
 template <int HD>
 void launch_parts(const Kv8Args& a, bool total, cudaStream_t st) {
-    // a 16-bit query is exact in one part (see above for the weights)
+    // a 16-bit query is one part, to 2^-34 of its largest (see above for the weights)
     if (a.dtype == SPM_F32) launch<HD, 2, 2, true>(a, st);
     else if (a.dtype == SPM_F16) total ? launch<HD, 1, 2, true>(a, st) : launch<HD, 1, 2, false>(a, st);
     else total ? launch<HD, 1, 1, true>(a, st) : launch<HD, 1, 1, false>(a, st);

@@ -196,7 +196,7 @@ def test_attention_over_many_keys_has_no_bias(dim, requests, most, heads, kv_hea
     # f32: a tile's products truncate, eight of 16 keys each (the low parts' are too small to count) by
     # 2^-24 on average; the powers of two are within 2^-22
     ("f32", 4096, 2.0 ** -21 + 2.0 ** -22), ("f32", 16384, 2.0 ** -21 + 2.0 ** -22),
-    # 16 bits: a quarter of their rounding where one accumulator is kept, else the mean of so many roundings
+    # 16 bits: an eighth of their rounding where one accumulator is kept, else the mean of so many roundings
     ("f16", 8192, 2.0 ** -14), ("f16", 16384, 2.0 ** -16), ("f16", 65536, 2.0 ** -16),
     ("bf16", 16384, 2.0 ** -11), ("bf16", 163840, 2.0 ** -12)])
 @pytest.mark.parametrize("dim", [64, 128, 192, 256])
